@@ -57,6 +57,13 @@ enum vq_metric {
     VQ_MANHATTAN = 3    /* src/distances.rs:152 */
 };
 
+/* Types of the elements of the arrays that the calls on scores and log probabilities take. */
+enum vq_type {
+    VQ_F32 = 0,
+    VQ_F16 = 1, /* IEEE binary16 */
+    VQ_BF16 = 2 /* the upper half of a binary32 */
+};
+
 /* ---- context and device memory ------------------------------------------------------- */
 
 int32_t vq_ctx_create(int32_t device, vq_ctx **out);
@@ -415,6 +422,61 @@ int32_t vq_tsvq_decode_f16(vq_ctx *ctx, const vq_tree *tree, const int32_t *d_le
 /* TSVQ::quantize (src/tsvq.rs:231-249) for host rows, as vq_pq_quantize_host.  h_leaf: n leaf indices. */
 int32_t vq_tsvq_quantize_host(vq_ctx *ctx, int32_t metric, const float *h_x, int64_t n, const vq_tree *tree, int32_t *h_leaf,
                               uint16_t *h_out);
+
+/* ---- 8-bit scores and log probabilities of codes ------------------------------------------------ */
+
+/* The soft side of an assignment: where vq_assign gives a row's nearest centroid, these give its score against every
+ * one of k centroids (or any k codes that a model answers with), and what is read from scores.  No counterpart in the
+ * reference.  All four are asynchronous, run on the context's stream and use no buffer of the context except where
+ * stated; sizes of zero rows return VQ_OK and touch nothing; what lies between rows or behind the last one is left as it is.
+ * Any stride and any address that is a multiple of the element's size will do; 8-bit rows are fastest at
+ * 16-byte aligned addresses and strides that are multiples of 16. */
+
+/* Rows to 8-bit integers with a scale each: d_scale[i] = max_t |x[i][t]| / 127, rounded to binary32;
+ * d_q[i][t] = the integer nearest to x[i][t] / d_scale[i] (the exact quotient, ties to even), -127 to 127.
+ * A scale of zero (a row of zeros, or of values so small that the quotient by 127 is): integers 0.  A row that holds an infinity or a
+ * NaN: its scale is NaN, its integers 0, so that its scores are NaN.  dim <= 131071.  The rows of d_q are ld_q bytes apart. */
+int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_t ld, int32_t dim, int8_t *d_q,
+                   int64_t ld_q, float *d_scale);
+
+/* d_out[i*ld_out + j] = (sum_t d_x[i][t] * d_w[j][t]) * d_xs[i] * d_ws[j] + d_bias[j], n rows against k codes: the sum
+ * exact in 32-bit integers, the rest in f32, rounded to out_type.  d_bias may be NULL.  With the bias -|c_j|^2 / 2 of codewords c_j the
+ * order of a row's scores is that of the squared Euclidean distance, nearest first (up to the 8-bit rounding).
+ * dim <= 131071, k <= 2^24; d_x rows are ld_x bytes apart, d_w rows ld_w.  The scores may not overlap an input. */
+int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t n, int64_t ld_x, const int8_t *d_w,
+                     const float *d_ws, int32_t k, int64_t ld_w, int32_t dim, const float *d_bias, int32_t out_type,
+                     void *d_out, int64_t ld_out);
+
+/* What is read from rows of scores s[i][0..k), with probabilities p_j = exp(beta * s_j) / sum:
+ *   d_max[i], d_logsum[i]   m = max_j s_j and L = log sum_j exp(beta * (s_j - m)); log of the whole sum = beta*m + L
+ *   d_logprob[i]   beta * (s_c - m) - L for the code c = d_codes[i * code_stride]
+ *   d_entropy[i]   -sum_j p_j log p_j
+ *   d_top_logprob, d_top_code   n * top: log probabilities and codes of the `top` largest scores, in falling order, of equal
+ *                  scores the lower code first; -inf and code -1 where fewer codes have a score above -inf
+ * Codes have code_bytes = 1, 2 (unsigned) or 4 (signed) bytes, as vq_assign, vq_assign_u16 and vq_tsvq_descend write them; a negative code
+ * is none given: log probability 0; a code of k or above gives NaN.
+ * A score of -inf is a code that cannot be: it has probability zero.  A row of nothing else: m = L = -inf,
+ * log probability -inf, entropy 0.  A row with a NaN or +inf: L, log probability (of a given code), entropy and alternatives
+ * are NaN, with codes -1.  Any of the outputs may be NULL, d_codes and d_logprob only together.
+ * beta > 0 and finite, top <= 32, k <= 2^24.  Sums are held in f32.
+ * Long rows are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context, which
+ * grows with n * k and is kept until the context is destroyed.  So calls may be captured into a graph where an earlier call at this
+ * size or above has run (else VQ_ERR_UNSUPPORTED, and the capture goes on), and such graphs are to run on the context's stream. */
+int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
+                         int32_t code_bytes, const void *d_codes, int64_t code_stride, int32_t top, float *d_logprob,
+                         float *d_max, float *d_logsum, float *d_entropy, float *d_top_logprob, int32_t *d_top_code);
+
+/* The gradient of a loss with respect to the scores, from its gradients with respect to the log probabilities of the codes (d_g_logprob,
+ * may be NULL) and to the entropies (d_g_entropy, may be NULL; not both):
+ *   d_grad[i][j] = beta * (g_lp * ([j = c] - p_j) - g_H * p_j * (log p_j + H))
+ * with m, L and H as vq_code_logprobs left them (d_entropy may be NULL where d_g_entropy is), computed in f32 and rounded
+ * to `type`, the type of the scores and of the gradient.  Probability zero, as which one below 2^-126 may count: gradient zero but for the code's own term.  A negative code takes no part in g_lp's
+ * term; a code of k or above, or a row whose L is NaN, makes the row's gradient NaN; a row of -inf only has gradient
+ * zero.  d_grad may be d_scores itself (same stride); another overlap is refused. */
+int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
+                              int32_t code_bytes, const void *d_codes, int64_t code_stride, const float *d_max,
+                              const float *d_logsum, const float *d_entropy, const float *d_g_logprob,
+                              const float *d_g_entropy, void *d_grad, int64_t ld_grad);
 
 #ifdef __cplusplus
 }

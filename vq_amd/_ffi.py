@@ -16,6 +16,8 @@ ERR_INVALID_ARG, ERR_DIM_MISMATCH, ERR_EMPTY_INPUT = -1, -2, -3
 ERR_UNSUPPORTED, ERR_OOM, ERR_HIP, ERR_RESEED_EXHAUSTED = -4, -5, -6, -7
 
 SQEUCLIDEAN, EUCLIDEAN, COSINE, MANHATTAN = 0, 1, 2, 3
+F32, F16, BF16 = 0, 1, 2
+_TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
 PROF_LBG_ASSIGN, PROF_LBG_UPDATE, PROF_ENCODE, PROF_ASSIGN_KERNEL = 0, 1, 2, 3
 
 # every symbol include/vq_hip.h declares: name -> (restype, argtypes)
@@ -78,6 +80,12 @@ SYMBOLS = {
     "vq_tsvq_decode_f16": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "vq_pq_quantize_host": (_i32, [_vp, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "vq_rvq_quantize_host": (_i32, [_vp, _i32, _vp, _i64, _i32, _i32, _i32, _vp, C.c_float, _vp, _vp]),
+    "vq_rows_i8": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "vq_scores_i8": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _i64]),
+    "vq_code_logprobs": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, C.c_float, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _vp,
+                                _vp, _vp]),
+    "vq_code_logprobs_grad": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _vp, _vp, _vp,
+                                     _vp, _vp, _i64]),
     "vq_tsvq_quantize_host": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _vp]),
 }
 
@@ -444,6 +452,33 @@ class Context:
 
     def tsvq_decode_f16(self, tree, d_leaf, n, d_out):
         self._check(_lib.vq_tsvq_decode_f16(self._h, tree._h, d_leaf.ptr, n, d_out.ptr))
+
+    # -- 8-bit scores and log probabilities of codes -------------------------------------------
+    # types: F32, F16, BF16 or their names "f32", "f16", "bf16"
+    def rows_i8(self, type, d_x, n, ld, dim, d_q, ld_q, d_scale):
+        """Rows to 8-bit integers, the nearest to x / scale, and a scale = max |x| / 127 per row."""
+        self._check(_lib.vq_rows_i8(self._h, _TYPES.get(type, type), _ptr(d_x), n, ld, dim, _ptr(d_q), ld_q, _ptr(d_scale)))
+
+    def scores_i8(self, d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, out_type, d_out, ld_out):
+        """Scores of 8-bit rows against 8-bit codes: (x . w) * xs * ws + bias (bias: None for none)."""
+        self._check(_lib.vq_scores_i8(self._h, _ptr(d_x), _ptr(d_xs), n, ld_x, _ptr(d_w), _ptr(d_ws), k, ld_w, dim,
+                                      _ptr(d_bias), _TYPES.get(out_type, out_type), _ptr(d_out), ld_out))
+
+    def code_logprobs(self, type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, top, d_logprob, d_max,
+                      d_logsum, d_entropy, d_top_logprob=None, d_top_code=None):
+        """Log probability of a code per row, largest score, log of the sum of exponentials relative to it, entropy,
+        and the `top` best codes.  Any output may be None (codes and their log probabilities together)."""
+        self._check(_lib.vq_code_logprobs(self._h, _TYPES.get(type, type), _ptr(d_scores), n, ld, k, beta, code_bytes,
+                                          _ptr(d_codes), code_stride, top, _ptr(d_logprob), _ptr(d_max), _ptr(d_logsum),
+                                          _ptr(d_entropy), _ptr(d_top_logprob), _ptr(d_top_code)))
+
+    def code_logprobs_grad(self, type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, d_max, d_logsum,
+                           d_entropy, d_g_logprob, d_g_entropy, d_grad, ld_grad):
+        """Gradient with respect to the scores, from those with respect to log probabilities and entropies (either may be
+        None) and from what code_logprobs left.  d_grad may be d_scores."""
+        self._check(_lib.vq_code_logprobs_grad(self._h, _TYPES.get(type, type), _ptr(d_scores), n, ld, k, beta, code_bytes,
+                                               _ptr(d_codes), code_stride, _ptr(d_max), _ptr(d_logsum), _ptr(d_entropy),
+                                               _ptr(d_g_logprob), _ptr(d_g_entropy), _ptr(d_grad), ld_grad))
 
 
 def _ptr(a):

@@ -1,0 +1,148 @@
+// What the calls on 8-bit scores and log probabilities of codes take and refuse: rules on sizes, strides and addresses
+// alone, without HIP, so that a CPU test can go through them.
+#pragma once
+#include <cstdint>
+#include <cstdio>
+#include <string>
+
+#include "../../include/vq_hip.h"
+
+namespace vq {
+
+// Components of an 8-bit row: the sum of as many products of two bytes (at most 2^14 each) fits 32 bits.
+constexpr int32_t kMaxDimI8 = 131071;
+constexpr int32_t kMaxTop = 32;           // alternatives of a row
+constexpr int32_t kMaxScoreCodes = 1 << 24;  // codes of a row of scores
+
+// Status and text of a refusal; VQ_OK: the call may run.
+struct Refusal {
+    int32_t status = VQ_OK;
+    std::string text;
+};
+inline Refusal refuse(int32_t status, const std::string &what) { return {status, "Invalid parameter: " + what}; }
+
+inline int type_bytes(int32_t type) { return type == VQ_F32 ? 4 : type == VQ_F16 || type == VQ_BF16 ? 2 : 0; }
+
+// The bytes of n rows of `row` bytes, `ld` bytes apart; [0, 0) for no rows.
+struct Span {
+    uintptr_t lo = 0, hi = 0;
+    Span(const void *p, int64_t n, int64_t ld, int64_t row) {
+        if (p && n > 0) lo = (uintptr_t)p, hi = lo + (uintptr_t)((n - 1) * ld + row);
+    }
+    bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+};
+// n rows of ld elements stay below 2^48 bytes, more than any memory
+inline bool too_long(int64_t n, int64_t ld, int bytes) {
+    return ld > 0 && n > (int64_t)(((uint64_t)1 << 48) / (uint64_t)bytes) / ld;
+}
+inline bool misaligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) != 0; }
+
+inline Refusal check_rows_i8(int32_t type, const void *x, int64_t n, int64_t ld, int32_t dim, const void *q, int64_t ld_q,
+                             const void *scale) {
+    const int e = type_bytes(type);
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(type));
+    if (n < 0 || dim <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative and dim must be greater than 0");
+    if (dim > kMaxDimI8) return refuse(VQ_ERR_UNSUPPORTED, "dim must be at most 131071");
+    if (ld < dim || ld_q < dim) return refuse(VQ_ERR_INVALID_ARG, "a row stride is below dim");
+    if (too_long(n, ld, e) || too_long(n, ld_q, 1)) return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
+    if (n == 0) return {};
+    if (!x || !q || !scale) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(x, e) || misaligned(scale, 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span sx(x, n, ld * e, (int64_t)dim * e), sq(q, n, ld_q, dim), ss(scale, 1, 0, n * 4);
+    if (sx.meets(sq) || sx.meets(ss) || sq.meets(ss)) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+    return {};
+}
+
+inline Refusal check_scores_i8(const void *x, const void *xs, int64_t n, int64_t ld_x, const void *w, const void *ws, int32_t k,
+                               int64_t ld_w, int32_t dim, const void *bias, int32_t out_type, const void *out, int64_t ld_out) {
+    const int e = type_bytes(out_type);
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(out_type));
+    if (n < 0 || dim <= 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative, dim and k must be greater than 0");
+    if (dim > kMaxDimI8) return refuse(VQ_ERR_UNSUPPORTED, "dim must be at most 131071");
+    if (k > kMaxScoreCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 16777216");
+    if (ld_x < dim || ld_w < dim || ld_out < k) return refuse(VQ_ERR_INVALID_ARG, "a row stride is below the row's length");
+    if (too_long(n, ld_x, 1) || too_long(k, ld_w, 1) || too_long(n, ld_out, e))
+        return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
+    if (n == 0) return {};
+    if (!x || !xs || !w || !ws || !out) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(xs, 4) || misaligned(ws, 4) || misaligned(bias, 4) || misaligned(out, e))
+        return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span so(out, n, ld_out * e, (int64_t)k * e);
+    if (so.meets({x, n, ld_x, dim}) || so.meets({w, k, ld_w, dim}) || so.meets({xs, 1, 0, n * 4}) ||
+        so.meets({ws, 1, 0, (int64_t)k * 4}) || so.meets({bias, 1, 0, (int64_t)k * 4}))
+        return refuse(VQ_ERR_INVALID_ARG, "the scores overlap an input");
+    return {};
+}
+
+// The scores, codes and sizes that both calls on log probabilities take.
+inline Refusal check_scored_codes(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t code_bytes,
+                                  const void *codes, int64_t code_stride) {
+    const int e = type_bytes(type);
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(type));
+    if (n < 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative and k must be greater than 0");
+    if (k > kMaxScoreCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 16777216");
+    if (ld < k) return refuse(VQ_ERR_INVALID_ARG, "the row stride is below k");
+    if (too_long(n, ld, e)) return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
+    if (!(beta > 0.0f) || !(beta <= 3.0e38f)) return refuse(VQ_ERR_INVALID_ARG, "beta must be a number greater than 0");
+    if (codes) {
+        if (code_bytes != 1 && code_bytes != 2 && code_bytes != 4) return refuse(VQ_ERR_INVALID_ARG, "codes have 1, 2 or 4 bytes");
+        if (code_stride <= 0 || too_long(n, code_stride, code_bytes)) return refuse(VQ_ERR_INVALID_ARG, "stride of the codes");
+        if (misaligned(codes, code_bytes)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    }
+    if (n == 0) return {};
+    if (!s) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(s, e)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    return {};
+}
+
+inline Refusal check_code_logprobs(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t code_bytes,
+                                   const void *codes, int64_t code_stride, int32_t top, const void *logprob, const void *max,
+                                   const void *logsum, const void *entropy, const void *top_logprob, const void *top_code) {
+    const Refusal r = check_scored_codes(type, s, n, ld, k, beta, code_bytes, codes, code_stride);
+    if (r.status != VQ_OK) return r;
+    if (top < 0) return refuse(VQ_ERR_INVALID_ARG, "top must not be negative");
+    if (top > kMaxTop) return refuse(VQ_ERR_UNSUPPORTED, "top must be at most 32");
+    if (n == 0) return {};
+    if ((codes == nullptr) != (logprob == nullptr)) return refuse(VQ_ERR_INVALID_ARG, "codes and their log probabilities go together");
+    if (top > 0 && (!top_logprob || !top_code)) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    const void *outs[] = {logprob, max, logsum, entropy, top ? top_logprob : nullptr, top ? top_code : nullptr};
+    const int e = type_bytes(type);
+    const Span in[] = {{s, n, ld * e, (int64_t)k * e}, {codes, n, code_stride * code_bytes, code_bytes}};
+    for (int a = 0; a < 6; ++a) {
+        if (misaligned(outs[a], 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+        const Span oa(outs[a], 1, 0, n * 4 * (a < 4 ? 1 : top));
+        for (int b = 0; b < a; ++b)
+            if (oa.meets({outs[b], 1, 0, n * 4 * (b < 4 ? 1 : top)})) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+        for (const Span &i : in)
+            if (oa.meets(i)) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+    }
+    return {};
+}
+
+inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta,
+                                        int32_t code_bytes, const void *codes, int64_t code_stride, const void *max,
+                                        const void *logsum, const void *entropy, const void *g_logprob, const void *g_entropy,
+                                        const void *grad, int64_t ld_grad) {
+    const Refusal r = check_scored_codes(type, s, n, ld, k, beta, code_bytes, codes, code_stride);
+    if (r.status != VQ_OK) return r;
+    const int e = type_bytes(type);
+    if (ld_grad < k || too_long(n, ld_grad, e)) return refuse(VQ_ERR_INVALID_ARG, "stride of the gradient");
+    if (n == 0) return {};
+    if (!max || !logsum || !grad || (!g_logprob && !g_entropy)) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (g_logprob && !codes) return refuse(VQ_ERR_INVALID_ARG, "a gradient of log probabilities without their codes");
+    if (g_entropy && !entropy) return refuse(VQ_ERR_INVALID_ARG, "a gradient of entropies without the entropies");
+    const void *rows[] = {max, logsum, entropy, g_logprob, g_entropy};
+    const Span sg(grad, n, ld_grad * e, (int64_t)k * e);
+    for (const void *p : rows) {
+        if (misaligned(p, 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+        if (sg.meets({p, 1, 0, n * 4})) return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps an input");
+    }
+    if (misaligned(grad, e)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    if (sg.meets({codes, n, code_stride * code_bytes, code_bytes})) return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps an input");
+    // in place, or elsewhere
+    if (!(grad == s && ld_grad == ld) && sg.meets({s, n, ld * e, (int64_t)k * e}))
+        return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps the scores otherwise than in place");
+    return {};
+}
+
+}  // namespace vq

@@ -1,0 +1,104 @@
+// C entry points of the 8-bit scores and the log probabilities of codes.
+#include <algorithm>
+
+#include "ctx.hpp"
+#include "logprobs.hpp"
+#include "score_rules.hpp"
+#include "scores_i8.hpp"
+
+using namespace vqh;
+
+namespace {
+
+int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Refusals and calls without rows end the call; `go` says whether it runs.
+int32_t admit(vq_ctx *ctx, const vq::Refusal &r, int64_t n, bool *go) {
+    *go = false;
+    if (r.status != VQ_OK) return fail(ctx, r.status, "%s", r.text.c_str());
+    if (n == 0) return VQ_OK;
+    VQ_HIP(ctx, hipSetDevice(ctx->device));
+    *go = true;
+    return VQ_OK;
+}
+
+// f(T) with the type of the elements
+template <typename F> void by_type(int32_t type, F f) {
+    if (type == VQ_F32)
+        f(vq::F32());
+    else if (type == VQ_F16)
+        f(vq::F16());
+    else
+        f(vq::BF16());
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_t ld, int32_t dim, int8_t *d_q,
+                   int64_t ld_q, float *d_scale) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_rows_i8(type, d_x, n, ld, dim, d_q, ld_q, d_scale), n, &go));
+    if (!go) return VQ_OK;
+    const vq::RowsI8Args a{d_x, n, ld, dim, d_q, ld_q, d_scale};
+    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_rows_i8<decltype(t)>, dim3((unsigned)std::min<int64_t>(cdiv64(n, 4), 1 << 20)), dim3(256), 0, ctx->stream, a); });
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
+}
+
+int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t n, int64_t ld_x, const int8_t *d_w,
+                     const float *d_ws, int32_t k, int64_t ld_w, int32_t dim, const float *d_bias, int32_t out_type,
+                     void *d_out, int64_t ld_out) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_scores_i8(d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, out_type, d_out, ld_out), n, &go));
+    if (!go) return VQ_OK;
+    vq::ScoresArgs a{d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, d_out, ld_out};
+    const int64_t slice = 65535 * 64;
+    for (int64_t r = 0; r < n; r += slice) {
+        a.n = std::min(n - r, slice);
+        a.x = d_x + r * ld_x;
+        a.xs = d_xs + r;
+        a.out = (char *)d_out + r * ld_out * vq::type_bytes(out_type);
+        by_type(out_type, [&](auto t) {
+            hipLaunchKernelGGL(vq::k_scores_any<decltype(t)>, dim3(cdiv(k, 64), cdiv(a.n, 64)), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
+    return VQ_OK;
+}
+
+int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
+                         int32_t code_bytes, const void *d_codes, int64_t code_stride, int32_t top, float *d_logprob,
+                         float *d_max, float *d_logsum, float *d_entropy, float *d_top_logprob, int32_t *d_top_code) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_logprobs(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, top, d_logprob,
+                                              d_max, d_logsum, d_entropy, d_top_logprob, d_top_code), n, &go));
+    if (!go) return VQ_OK;
+    const vq::LogprobArgs a{d_scores, n, ld, k, beta, d_codes, code_stride, code_bytes, top, d_logprob, d_max, d_logsum, d_entropy,
+                            d_top_logprob, d_top_code};
+    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_logprobs_rows<decltype(t)>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(256), 0, ctx->stream, a); });
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
+}
+
+int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
+                              int32_t code_bytes, const void *d_codes, int64_t code_stride, const float *d_max,
+                              const float *d_logsum, const float *d_entropy, const float *d_g_logprob,
+                              const float *d_g_entropy, void *d_grad, int64_t ld_grad) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_logprobs_grad(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, d_max,
+                                                   d_logsum, d_entropy, d_g_logprob, d_g_entropy, d_grad, ld_grad), n, &go));
+    if (!go) return VQ_OK;
+    const vq::GradArgs a{d_scores, n, ld, k, beta, d_codes, code_stride, code_bytes, d_max, d_logsum, d_entropy, d_g_logprob,
+                         d_g_entropy, d_grad, ld_grad};
+    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_logprobs_grad<decltype(t)>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(256), 0, ctx->stream, a); });
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
+}
+
+}  // extern "C"
