@@ -19,6 +19,7 @@ int scores(i64 x, i64 xs, i64 n, i64 ldx, i64 w, i64 ws, int k, i64 ldw, int dim
     return vq::check_scores_i8(P(x), P(xs), n, ldx, P(w), P(ws), k, ldw, dim, P(b), type, P(out), ldo).status; }
 int logprobs(int type, i64 s, i64 n, i64 ld, int k, float beta, int cb, i64 c, i64 cs, int top, i64 lp, i64 m, i64 l, i64 h, i64 tl, i64 tc) {
     return vq::check_code_logprobs(type, P(s), n, ld, k, beta, cb, P(c), cs, top, P(lp), P(m), P(l), P(h), P(tl), P(tc)).status; }
+int plan(i64 n, int k, i64 *out) { const vq::RowPlan p = vq::plan_rows(n, k); out[0] = p.lanes, out[1] = p.per_lane, out[2] = p.parts, out[3] = p.codes; return 0; }
 int grad(int type, i64 s, i64 n, i64 ld, int k, float beta, int cb, i64 c, i64 cs, i64 m, i64 l, i64 h, i64 gl, i64 gh, i64 g, i64 ldg) {
     return vq::check_code_logprobs_grad(type, P(s), n, ld, k, beta, cb, P(c), cs, P(m), P(l), P(h), P(gl), P(gh), P(g), ldg).status; }
 }
@@ -58,7 +59,7 @@ REFUSED = [
     ("scores", dict(b=5 * A + 2), INVALID), ("scores", dict(out=6 * A + 2), INVALID), ("scores", dict(out=A), INVALID),
     ("scores", dict(out=3 * A + 1000), INVALID), ("scores", dict(out=5 * A), INVALID), ("scores", dict(n=1 << 61), INVALID),
     ("logprobs", dict(k=0), INVALID), ("logprobs", dict(ld=99), INVALID), ("logprobs", dict(beta=0.0), INVALID), ("logprobs", dict(beta=-1.0), INVALID),
-    ("logprobs", dict(beta=float("nan")), INVALID), ("logprobs", dict(beta=float("inf")), INVALID), ("logprobs", dict(cb=3), INVALID),
+    ("logprobs", dict(beta=float("nan")), INVALID), ("logprobs", dict(beta=float("inf")), INVALID), ("logprobs", dict(beta=1e31), INVALID), ("logprobs", dict(beta=1e-31), INVALID), ("logprobs", dict(cb=3), INVALID),
     ("logprobs", dict(cb=8), INVALID), ("logprobs", dict(cs=0), INVALID), ("logprobs", dict(c=2 * A + 2), INVALID), ("logprobs", dict(c=0), INVALID),
     ("logprobs", dict(lp=0), INVALID), ("logprobs", dict(top=-1), INVALID), ("logprobs", dict(top=33), UNSUPPORTED), ("logprobs", dict(tl=0), INVALID),
     ("logprobs", dict(tc=0), INVALID), ("logprobs", dict(s=0), INVALID), ("logprobs", dict(s=A + 1), INVALID), ("logprobs", dict(m=4 * A + 2), INVALID),
@@ -75,7 +76,7 @@ TAKEN = [
     ("scores", {}), ("scores", dict(n=0, x=0, xs=0, w=0, ws=0, out=0)), ("scores", dict(b=0)), ("scores", dict(x=A + 3, ldx=101)), ("scores", dict(type=1, out=6 * A + 2)),
     ("scores", dict(xs=4 * A)),  # inputs may share memory
     ("logprobs", {}), ("logprobs", dict(n=0, s=0, c=0, lp=0, m=0, l=0, h=0, tl=0, tc=0)), ("logprobs", dict(top=0, tl=0, tc=0)), ("logprobs", dict(c=0, lp=0)),
-    ("logprobs", dict(m=0, l=0, h=0)), ("logprobs", dict(cb=1, c=2 * A + 1, cs=16)), ("logprobs", dict(top=32, k=2, ld=2)), ("logprobs", dict(beta=1e-30)),
+    ("logprobs", dict(m=0, l=0, h=0)), ("logprobs", dict(cb=1, c=2 * A + 1, cs=16)), ("logprobs", dict(top=32, k=2, ld=2)), ("logprobs", dict(beta=1.1e-30)),
     ("grad", {}), ("grad", dict(g=A)), ("grad", dict(gl=0, c=0)), ("grad", dict(gh=0, h=0)), ("grad", dict(n=0, s=0, g=0, m=0)),
 ]
 
@@ -88,6 +89,18 @@ def test_refused(lib, call, change, status):
 @pytest.mark.parametrize("call,change", TAKEN)
 def test_taken(lib, call, change):
     assert getattr(lib, call)(*{**CALLS[call], **change}.values()) == 0
+
+
+def test_every_code_of_a_row_has_a_lane(lib):
+    lib.plan.argtypes = [C.c_longlong, C.c_int, C.c_void_p]
+    out = (C.c_longlong * 4)()
+    for k in [1, 2, 3, 7, 8, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 50021, 65536, 262144, 1 << 24]:
+        for n in (1, 2, 3, 15, 16, 17, 64, 255, 1024, 100_000, 1 << 30):
+            lib.plan(n, k, out)
+            lanes, per_lane, parts, codes = out
+            assert codes <= lanes * per_lane and parts * codes >= k and (parts - 1) * codes < k and (parts == 1 or (lanes == 256 and codes % 64 == 0))
+            assert parts <= 64 or k > 1 << 20
+            assert lanes in (1, 4, 16, 64, 256) and per_lane in ((16,) if lanes < 256 else (8, 16, 32, 64))
 
 
 def test_a_missing_context_is_an_error():

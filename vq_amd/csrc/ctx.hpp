@@ -86,6 +86,10 @@ struct vq_ctx {
     // the LBG's assignment, sort keys in and out, the sort's workspace, per-cluster tables, flags
     DevBuf big_chunk, big_win, big_wind, big_best, big_fresh, big_codes, big_keys, big_sorted, big_sort_tmp, big_tables,
         big_flags;
+    // parts of long rows of scores; what it was before it grew stays until the context ends, since captured
+    // graphs may hold its address
+    DevBuf score_parts;
+    std::vector<void *> outgrown;
     // optional per-kernel-class timing (HIP events on the stream)
     bool prof_on = false;
     std::vector<hipEvent_t> prof_pool;
@@ -145,6 +149,23 @@ inline int32_t ensure(vq_ctx *ctx, DevBuf &b, size_t bytes) {
     }
     size_t want = bytes + bytes / 8 + 256;
     VQ_HIP(ctx, hipMalloc(&b.p, want));
+    b.cap = want;
+    return VQ_OK;
+}
+
+// A workspace that captured graphs may hold the address of: it grows by a new allocation, at least twice the last, and the
+// ones before stay.  While the stream is being captured it cannot grow, and the capture goes on.
+inline int32_t ensure_kept(vq_ctx *ctx, DevBuf &b, size_t bytes) {
+    if (bytes <= b.cap) return VQ_OK;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    VQ_HIP(ctx, hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+        return fail(ctx, VQ_ERR_UNSUPPORTED, "a capture of this call needs an earlier call of this size: its workspace cannot grow meanwhile");
+    const size_t want = bytes > 2 * b.cap ? bytes + 256 : 2 * b.cap;
+    void *p = nullptr;
+    VQ_HIP(ctx, hipMalloc(&p, want));
+    if (b.p) ctx->outgrown.push_back(b.p);
+    b.p = p;
     b.cap = want;
     return VQ_OK;
 }

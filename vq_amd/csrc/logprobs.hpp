@@ -55,77 +55,391 @@ __device__ __forceinline__ float key_score(uint64_t key) {
 }
 __device__ __forceinline__ int32_t key_code(uint64_t key) { return (int32_t)~(uint32_t)key; }
 
-// What a row's thread writes: x_c is the score of its code.
-template <typename T>
-__device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, float m, float S, float W) {
-    const bool none = m == kNegInf;
-    const float L = logf(S);
-    if (a.max) a.max[row] = m;
-    if (a.logsum) a.logsum[row] = L;
-    if (a.entropy) a.entropy[row] = none ? 0.0f : L - W / S;
-    if (a.logprob) {
-        const int64_t c = code_at(a.codes, a.code_bytes, row * a.code_stride);
-        float lp = 0.0f;
-        if (c >= a.k)
-            lp = __builtin_nanf("");
-        else if (c >= 0)
-            lp = none ? kNegInf : a.beta * (T::up(((const typename T::Raw *)a.s)[row * a.ld + c]) - m) - L;
-        a.logprob[row] = lp;
+// ---- the codes of a lane ----------------------------------------------------------------------------
+// A row, or a part of it, lies in the registers of LANES lanes for the whole of its pass, so that it is read once: vector u
+// of a lane holds the codes from lo + (u * LANES + lane) * VEC on, 16 bytes of them.  A vector that would pass the end
+// hi is read from hi - VEC on instead, without a branch, and what lies before its own place in it becomes -inf.
+template <typename T, int LANES, int NV> struct Share {
+    typedef typename T::Raw Raw;
+    static constexpr int VEC = 16 / (int)sizeof(Raw), E = NV * VEC;
+    float x[E];
+
+    static __device__ __forceinline__ int base(int u, int lane, int lo, int hi) { return min(lo + (u * LANES + lane) * VEC, hi - VEC); }
+
+    __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
+        struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
+            uint32_t w[4];
+        };
+        Piece raw[NV];
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+            if (u == 0 || lo + u * LANES * VEC < hi) raw[u] = *reinterpret_cast<const Piece *>(s + base(u, lane, lo, hi));
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            if (u > 0 && lo + u * LANES * VEC >= hi) {  // uniform: nothing of the row is left
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) x[u * VEC + v] = kNegInf;
+                continue;
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if constexpr (sizeof(Raw) == 4)
+                    x[u * VEC + v] = __uint_as_float(raw[u].w[v]);
+                else
+                    x[u * VEC + v] = T::up((Raw)(v & 1 ? raw[u].w[v >> 1] >> 16 : raw[u].w[v >> 1] & 0xffffu));
+            }
+            if (lo + (u + 1) * LANES * VEC > hi) {  // uniform: the vectors that are read from elsewhere
+                const int skip = lo + (u * LANES + lane) * VEC - base(u, lane, lo, hi);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) x[u * VEC + v] = v < skip ? kNegInf : x[u * VEC + v];
+            }
+        }
     }
+    __device__ __forceinline__ int code(int e, int lane, int lo, int hi) const { return base(e / VEC, lane, lo, hi) + e % VEC; }
+};
+
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // (a NaN wins)
+
+// Over the lanes of aligned groups of G, for every lane of the group, in an order that is the same in every run.  f's first
+// operand stays where a step brings nothing.
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ uint32_t dpp_keep(uint32_t old, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t row, int t, uint64_t key, float m, float L) {
-    const float v = key_score(key);
-    const bool bad = L != L, none = key == 0 || v == kNegInf;
-    a.top_logprob[row * a.top + t] = bad ? __builtin_nanf("") : none ? kNegInf : a.beta * (v - m) - L;
-    a.top_code[row * a.top + t] = bad || none ? -1 : key_code(key);
+template <int G, typename F> __device__ __forceinline__ uint32_t over_group(uint32_t v, uint32_t none, F f) {
+    if constexpr (G >= 2) v = f(v, dpp_keep<0xB1>(v, v));
+    if constexpr (G >= 4) v = f(v, dpp_keep<0x4E>(v, v));
+    if constexpr (G >= 8) v = f(v, dpp_keep<0x141>(v, v));
+    if constexpr (G >= 16) v = f(v, dpp_keep<0x140>(v, v));
+    static_assert(G <= 16 || G == 64, "rows of 16 lanes, or the wave");
+    if constexpr (G == 64) {
+        v = f(v, dpp_keep<0x142, 0xa>(none, v));  // a row's last lane to the next row
+        v = f(v, dpp_keep<0x143, 0xc>(none, v));  // the lower half's to the upper half
+        v = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    }
+    return v;
+}
+template <int G> __device__ __forceinline__ float group_max(float v) {
+    return __uint_as_float(over_group<G>(__float_as_uint(v), __float_as_uint(kNegInf), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(larger(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+template <int G> __device__ __forceinline__ float group_sum(float v) {
+    return __uint_as_float(over_group<G>(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+template <int G> __device__ __forceinline__ int group_min(int v) {
+    return (int)over_group<G>((uint32_t)v, 0x7fffffffu, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
+}
+// The largest key of the wave.
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+    const auto most = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    const uint32_t hi = over_group<64>((uint32_t)(v >> 32), 0u, most);
+    const uint32_t lo = over_group<64>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u, 0u, most);
+    return (uint64_t)hi << 32 | lo;
 }
 
-// A workgroup per row: the largest score, the sums relative to it, then one round per alternative.
-template <typename T>
-__global__ void __launch_bounds__(256) k_logprobs_rows(LogprobArgs a) {
-    __shared__ float part[3][4];
-    __shared__ uint64_t best[4];
-    const int tid = threadIdx.x, wave = tid >> 6;
-    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-    const typename T::Raw *s = (const typename T::Raw *)a.s + row * a.ld;
-    float m = kNegInf;
-    for (int j = tid; j < a.k; j += 256) m = __builtin_elementwise_maximum(m, T::up(s[j]));
-    for (int o = 32; o; o >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, o));
-    if ((tid & 63) == 0) part[0][wave] = m;
-    __syncthreads();
-    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(part[0][0], part[0][1]),
-                                      __builtin_elementwise_maximum(part[0][2], part[0][3]));
-    const float ms = m == kNegInf ? 0.0f : m;
-    float S = 0.0f, W = 0.0f;
-    for (int j = tid; j < a.k; j += 256) {
-        const float d = a.beta * (T::up(s[j]) - ms), e = expf(d);
-        S += e;
-        W += e == 0.0f ? 0.0f : e * d;
+// Sums of one share relative to the largest score m of its row or part: S = sum 2^d, W = sum 2^d d with
+// d = (x - m) * beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero).
+template <int E> __device__ __forceinline__ void share_sums(const float (&x)[E], float m, float c, float &S, float &W) {
+    S = 0.0f, W = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float d = fmaxf((x[e] - m) * c, -200.0f), p = __builtin_amdgcn_exp2f(d);
+        S += p;
+        W = __builtin_fmaf(p, d, W);
     }
-    for (int o = 32; o; o >>= 1) S += __shfl_xor(S, o), W += __shfl_xor(W, o);
-    if ((tid & 63) == 0) part[1][wave] = S, part[2][wave] = W;
+}
+// m where sums can be taken relative to it; else 0, and the row's results are those of `none` or `bad`
+__device__ __forceinline__ bool is_bad(float m) { return !(m < __builtin_inff()); }
+__device__ __forceinline__ float relative_to(float m) { return m == kNegInf || is_bad(m) ? 0.0f : m; }
+
+struct RowSums {
+    float m, L, H;
+};
+__device__ __forceinline__ RowSums row_sums(float m, float S, float W) {
+    if (is_bad(m)) return {m, __builtin_nanf(""), __builtin_nanf("")};
+    if (m == kNegInf) return {m, kNegInf, 0.0f};
+    const float L = logf(S);
+    return {m, L, L - W / S * kLn2};
+}
+// The log probability of the row's code, whose score was read with the row.
+struct CodeScore {
+    int64_t code = -1;
+    float score = 0.0f;
+    template <typename T> __device__ __forceinline__ void read(const LogprobArgs &a, int64_t row, T) {
+        if (!a.logprob) return;
+        code = code_at(a.codes, a.code_bytes, row * a.code_stride);
+        if (code >= 0 && code < a.k) score = T::up(((const typename T::Raw *)a.s)[row * a.ld + code]);
+    }
+};
+__device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, const RowSums &r, const CodeScore &c) {
+    if (a.max) a.max[row] = r.m;
+    if (a.logsum) a.logsum[row] = r.L;
+    if (a.entropy) a.entropy[row] = r.H;
+    if (a.logprob)
+        a.logprob[row] = c.code < 0 ? 0.0f : c.code >= a.k ? __builtin_nanf("") : r.m == kNegInf ? kNegInf : a.beta * (c.score - r.m) - r.L;
+}
+__device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t row, int t, float v, int code, const RowSums &r) {
+    const bool bad = r.L != r.L, none = v == kNegInf || code < 0;
+    a.top_logprob[row * a.top + t] = bad ? __builtin_nanf("") : none ? kNegInf : a.beta * (v - r.m) - r.L;
+    a.top_code[row * a.top + t] = bad || none ? -1 : code;
+}
+
+// ---- short rows: G lanes each ------------------------------------------------------------------------
+// Up to 16 codes per lane, 64 / G rows per wave: no LDS, no waits.  One round per alternative: the largest score left, the
+// first code that has it, which then leaves.  TINY: rows shorter than a vector, one lane each.
+template <typename T, int G, bool TINY>
+__global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
+    constexpr int NV = TINY ? 1 : (int)sizeof(typename T::Raw);
+    typedef Share<T, G, NV> S16;
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
+    const typename T::Raw *s = (const typename T::Raw *)a.s + row * a.ld;
+    S16 r;
+    if constexpr (TINY) {
+#pragma unroll
+        for (int e = 0; e < S16::E; ++e) r.x[e] = e < a.k ? T::up(s[e]) : kNegInf;
+    } else
+        r.load(s, 0, a.k, lane);
+    CodeScore cs;
+    cs.read(a, row, T());
+    float m = r.x[0];
+#pragma unroll
+    for (int e = 1; e < S16::E; ++e) m = larger(m, r.x[e]);
+    m = group_max<G>(m);
+    float S, W;
+    share_sums(r.x, relative_to(m), a.beta * kLog2e, S, W);
+    S = group_sum<G>(S);
+    W = group_sum<G>(W);
+    const RowSums sums = row_sums(m, S, W);
+    const bool writes = lane == 0 && mine < a.n;
+    if (writes) write_row(a, row, sums, cs);
+    float best = m;
+    for (int t = 0; t < a.top; ++t) {
+        int e0 = -1;
+#pragma unroll
+        for (int e = S16::E - 1; e >= 0; --e) e0 = r.x[e] == best ? e : e0;
+        const int at = e0 < 0 ? 0x7fffffff : TINY ? e0 : r.code(e0, lane, 0, a.k), first = group_min<G>(at);
+        if (writes) write_alternative(a, row, t, best, first == 0x7fffffff ? -1 : first, sums);
+        if (t + 1 == a.top) break;
+        best = kNegInf;
+#pragma unroll
+        for (int e = 0; e < S16::E; ++e) {
+            r.x[e] = e == e0 && at == first ? kNegInf : r.x[e];
+            best = fmaxf(best, r.x[e]);
+        }
+        best = group_max<G>(best);
+    }
+}
+
+// ---- longer rows, in parts: a workgroup each ------------------------------------------------------------
+constexpr int kMostCandidates = 512;
+
+struct PartArgs {
+    LogprobArgs a;
+    int parts, part_codes;  // part q has the codes from q * part_codes on
+    float *sums;     // [n][parts][3]: largest score, S, W
+    uint64_t *keys;  // [n][parts][top], in falling order, 0 behind the last
+};
+
+struct PartLds {
+    float red[4][4];
+    int count;
+    uint64_t key[kMostCandidates];
+    uint64_t best[32];
+};
+
+// The `top` largest of a workgroup's scores, in falling order, into l.best (0 behind the last one above -inf).
+// floor: a score that at least `top` of the scores reach, if there are as many.  What reaches it is listed (in whatever order, the
+// keys are all different) and sorted by counting; a longer list than there is room for, as of a row of equal scores, is not
+// taken: then one round per alternative over the registers, which empties them.
+template <typename S64>
+__device__ __forceinline__ void part_best(S64 &r, const float (&vmax)[S64::E / S64::VEC], float floor, int lo, int hi, int top, PartLds &l) {
+    constexpr int NV = S64::E / S64::VEC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (!__ballot(vmax[u] >= floor && vmax[u] > kNegInf)) continue;
+#pragma unroll
+        for (int v = 0; v < S64::VEC; ++v) {
+            const float y = r.x[u * S64::VEC + v];
+            if (y >= floor && y > kNegInf) {
+                const int at = atomicAdd(&l.count, 1);
+                if (at < kMostCandidates) l.key[at] = rank_key(y, (uint32_t)r.code(u * S64::VEC + v, tid, lo, hi));
+            }
+        }
+    }
+    if (tid < 32) l.best[tid] = 0;
     __syncthreads();
-    S = part[1][0] + part[1][1] + part[1][2] + part[1][3];
-    W = part[2][0] + part[2][1] + part[2][2] + part[2][3];
-    if (tid == 0) write_row<T>(a, row, m, S, W);
-    uint64_t last = ~0ull;
+    const int count = l.count;
+    if (count <= kMostCandidates) {
+        for (int i = tid; i < count; i += 256) {
+            const uint64_t mine = l.key[i];
+            int above = 0;
+            for (int j = 0; j < count; ++j) above += l.key[j] > mine;
+            if (above < top) l.best[above] = mine;
+        }
+        __syncthreads();
+        return;
+    }
+    __syncthreads();  // everyone has read the count and the zeros are there
+    float best = kNegInf;
+#pragma unroll
+    for (int e = 0; e < S64::E; ++e) best = fmaxf(best, r.x[e]);
+    for (int t = 0; t < top; ++t) {
+        best = group_max<64>(best);
+        if (lane == 0) l.red[0][wave] = best;
+        __syncthreads();
+        best = fmaxf(fmaxf(l.red[0][0], l.red[0][1]), fmaxf(l.red[0][2], l.red[0][3]));
+        if (best == kNegInf) break;  // the same in every lane
+        int e0 = -1;
+#pragma unroll
+        for (int e = S64::E - 1; e >= 0; --e) e0 = r.x[e] == best ? e : e0;
+        const int at = e0 < 0 ? 0x7fffffff : r.code(e0, tid, lo, hi);
+        int first = group_min<64>(at);
+        if (lane == 0) l.red[1][wave] = __int_as_float(first);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) first = min(first, __float_as_int(l.red[1][w]));
+        if (tid == 0) l.best[t] = rank_key(best, (uint32_t)first);
+        best = kNegInf;
+#pragma unroll
+        for (int e = 0; e < S64::E; ++e) {
+            r.x[e] = e == e0 && at == first ? kNegInf : r.x[e];
+            best = fmaxf(best, r.x[e]);
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
+    typedef Share<T, 256, NV> S64;
+    constexpr int E = S64::E, VEC = S64::VEC;
+    __shared__ PartLds l;
+    const LogprobArgs &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row = blockIdx.x / (unsigned)p.parts;
+    const int part = (int)(blockIdx.x % (unsigned)p.parts), lo = part * p.part_codes, hi = min(a.k, lo + p.part_codes);
+    S64 r;
+    r.load((const typename T::Raw *)a.s + row * a.ld, lo, hi, tid);
+    CodeScore cs;
+    if (p.parts == 1 && tid == 0) cs.read(a, row, T());
+    float vmax[NV], m;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        vmax[u] = r.x[u * VEC];
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) vmax[u] = larger(vmax[u], r.x[u * VEC + v]);
+        m = u ? larger(m, vmax[u]) : vmax[u];
+    }
+    const float mine = m;
+    m = group_max<64>(m);
+    // The floor of the alternatives: in each of the waves whose lanes all have codes, a share of them, rounded up, of the lanes have a score
+    // that reaches the wave's floor, so `top` scores reach the smallest of these.
+    const int full = max(1, min(4, (hi - lo) / (64 * VEC)));
+    float floor = mine;
+    if (a.top && wave < full) {
+        float left = mine;
+        for (int q = (a.top + full - 1) / full; q; --q) {
+            floor = group_max<64>(left);
+            const unsigned long long who = __ballot(left == floor);
+            if (lane == __ffsll(who) - 1) left = kNegInf;
+        }
+    }
+    if (lane == 0) l.red[0][wave] = m, l.red[1][wave] = floor;
+    if (tid == 0) l.count = 0;
+    __syncthreads();
+    m = larger(larger(l.red[0][0], l.red[0][1]), larger(l.red[0][2], l.red[0][3]));
+    floor = l.red[1][0];
+    for (int w = 1; w < full; ++w) floor = fminf(floor, l.red[1][w]);
+    float S, W;
+    share_sums(r.x, relative_to(m), a.beta * kLog2e, S, W);
+    S = group_sum<64>(S);
+    W = group_sum<64>(W);
+    if (lane == 0) l.red[2][wave] = S, l.red[3][wave] = W;
+    if (a.top && !is_bad(m)) part_best(r, vmax, floor, lo, hi, a.top, l);
+    else if (tid < 32) l.best[tid] = 0;
+    __syncthreads();
+    if (p.parts == 1) {
+        if (wave == 0) {
+            S = l.red[2][0] + l.red[2][1] + l.red[2][2] + l.red[2][3];
+            W = l.red[3][0] + l.red[3][1] + l.red[3][2] + l.red[3][3];
+            const RowSums sums = row_sums(m, S, W);
+            if (lane == 0) write_row(a, row, sums, cs);
+            if (lane < a.top) write_alternative(a, row, lane, key_score(l.best[lane]), l.best[lane] ? key_code(l.best[lane]) : -1, sums);
+        }
+    } else {
+        if (tid < 3) {
+            const float v[2] = {l.red[2][0] + l.red[2][1] + l.red[2][2] + l.red[2][3], l.red[3][0] + l.red[3][1] + l.red[3][2] + l.red[3][3]};
+            p.sums[(int64_t)blockIdx.x * 3 + tid] = tid == 0 ? m : tid == 1 ? v[0] : v[1];
+        }
+        if (tid < a.top) p.keys[(int64_t)blockIdx.x * a.top + tid] = l.best[tid];
+    }
+}
+
+// A wave joins the parts of a row: sums rescaled to the largest score of all, and the alternatives from the heads of the
+// parts' lists.
+template <typename T>
+__global__ void __launch_bounds__(64) k_logprobs_join(PartArgs p) {
+    const LogprobArgs &a = p.a;
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x;
+    const float *sums = p.sums + row * p.parts * 3;
+    CodeScore cs;
+    cs.read(a, row, T());
+    float m = kNegInf;
+    for (int q = lane; q < p.parts; q += 64) m = larger(m, sums[q * 3]);
+    m = group_max<64>(m);
+    float S = 0.0f, W = 0.0f;
+    for (int q = lane; q < p.parts; q += 64) {
+        const float d = fmaxf((sums[q * 3] - relative_to(m)) * (a.beta * kLog2e), -200.0f), f = __builtin_amdgcn_exp2f(d);
+        S = __builtin_fmaf(f, sums[q * 3 + 1], S);
+        W = __builtin_fmaf(f, __builtin_fmaf(sums[q * 3 + 1], d, sums[q * 3 + 2]), W);
+    }
+    S = group_sum<64>(S);
+    W = group_sum<64>(W);
+    const RowSums r = row_sums(m, S, W);
+    if (lane == 0) write_row(a, row, r, cs);
+    // A lane has the list of one part, the largest left in a register and the next behind it, so that the read
+    // of a round's winner is not waited for.
+    if (a.top == 0) return;
+    const int total = p.parts * a.top;
+    const uint64_t *keys = p.keys + row * total;
+    if (p.parts <= 64) {
+        __shared__ uint64_t lists[64 * 32];
+        for (int i = lane; i < total; i += 64) lists[i] = keys[i];
+        __syncthreads();
+        const uint64_t *list = lists + min(lane, p.parts - 1) * a.top;
+        uint64_t head = lane < p.parts ? list[0] : 0, next = lane < p.parts && a.top > 1 ? list[1] : 0, mine = 0;
+        int at = 1;
+        for (int t = 0; t < a.top; ++t) {
+            const uint64_t key = wave_max(head);
+            if (lane == t) mine = key;
+            if (head == key) {
+                head = next;
+                ++at;
+                next = lane < p.parts && at < a.top ? list[at] : 0;
+            }
+        }
+        if (lane < a.top) write_alternative(a, row, lane, key_score(mine), mine ? key_code(mine) : -1, r);
+        return;
+    }
+    uint64_t last = ~0ull;  // more than a million codes: through the lists of a lane's parts in every round
     for (int t = 0; t < a.top; ++t) {
         uint64_t key = 0;
-        for (int j = tid; j < a.k; j += 256) {
-            const uint64_t c = rank_key(T::up(s[j]), (uint32_t)j);
-            key = c < last && c > key ? c : key;
-        }
-        for (int o = 32; o; o >>= 1) {
-            const uint64_t c = __shfl_xor(key, o);
-            key = c > key ? c : key;
-        }
-        if ((tid & 63) == 0) best[wave] = key;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) key = best[w] > key ? best[w] : key;
-        __syncthreads();
+        for (int q = lane; q < p.parts; q += 64)
+            for (int i = 0; i < a.top; ++i) {
+                const uint64_t c = keys[q * a.top + i];
+                if (c < last) {  // the first of this part that is left
+                    key = c > key ? c : key;
+                    break;
+                }
+            }
+        key = wave_max(key);
         last = key;
-        if (tid == 0) write_alternative(a, row, t, key, m, logf(S));
-    }
+        if (lane == 0) write_alternative(a, row, t, key_score(key), key ? key_code(key) : -1, r);
     }
 }
 

@@ -83,7 +83,7 @@ inline Refusal check_scored_codes(int32_t type, const void *s, int64_t n, int64_
     if (k > kMaxScoreCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 16777216");
     if (ld < k) return refuse(VQ_ERR_INVALID_ARG, "the row stride is below k");
     if (too_long(n, ld, e)) return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
-    if (!(beta > 0.0f) || !(beta <= 3.0e38f)) return refuse(VQ_ERR_INVALID_ARG, "beta must be a number greater than 0");
+    if (!(beta >= 1e-30f) || !(beta <= 1e30f)) return refuse(VQ_ERR_INVALID_ARG, "beta must be between 1e-30 and 1e30");
     if (codes) {
         if (code_bytes != 1 && code_bytes != 2 && code_bytes != 4) return refuse(VQ_ERR_INVALID_ARG, "codes have 1, 2 or 4 bytes");
         if (code_stride <= 0 || too_long(n, code_stride, code_bytes)) return refuse(VQ_ERR_INVALID_ARG, "stride of the codes");
@@ -143,6 +143,24 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
     if (!(grad == s && ld_grad == ld) && sg.meets({s, n, ld * e, (int64_t)k * e}))
         return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps the scores otherwise than in place");
     return {};
+}
+
+// How the rows of a call go through the GPU.  Rows of up to 1024 codes have 1, 4, 16 or 64 lanes each, 16 codes per lane (`lanes`).
+// Longer ones have a workgroup of 256 lanes per part, 8 to 64 codes per lane (`per_lane`): as many as it takes for a row to be
+// one part, but no more than leave 1024 workgroups (four per compute unit) to the call, and no fewer than 8; at most 64 parts where
+// 64 codes per lane allow that.  Parts are of equal length, in whole 64 codes (`codes`; the last one is shorter).
+constexpr int kShortCodes = 1024;
+struct RowPlan {
+    int lanes, per_lane;
+    int64_t parts;
+    int32_t codes;
+};
+inline RowPlan plan_rows(int64_t n, int32_t k) {
+    if (k <= kShortCodes) return {k <= 16 ? 1 : k <= 64 ? 4 : k <= 256 ? 16 : 64, 16, 1, k};
+    int e = 64;
+    while (e > 8 && (k <= 128 * e || (n * ((k + 256 * e - 1) / (256 * e)) < 1024 && k <= 128 * e * 64))) e /= 2;
+    const int32_t least = (k + 256 * e - 1) / (256 * e), codes = ((k + least - 1) / least + 63) / 64 * 64;
+    return {256, e, (k + codes - 1) / codes, codes};
 }
 
 }  // namespace vq

@@ -32,6 +32,55 @@ template <typename F> void by_type(int32_t type, F f) {
         f(vq::BF16());
 }
 
+template <typename T, bool TINY, int G> void short_rows(vq_ctx *ctx, const vq::LogprobArgs &a) {
+    hipLaunchKernelGGL((vq::k_logprobs_short<T, G, TINY>), dim3((unsigned)cdiv64(a.n, 256 / G)), dim3(256), 0, ctx->stream, a);
+}
+template <typename T> void row_parts(vq_ctx *ctx, const vq::PartArgs &p, int per_lane) {
+    constexpr int VEC = 16 / (int)sizeof(typename T::Raw);
+    const dim3 grid((unsigned)(p.a.n * p.parts)), wg(256);
+    if (per_lane == 8)
+        hipLaunchKernelGGL((vq::k_logprobs_part<T, 8 / VEC>), grid, wg, 0, ctx->stream, p);
+    else if (per_lane == 16)
+        hipLaunchKernelGGL((vq::k_logprobs_part<T, 16 / VEC>), grid, wg, 0, ctx->stream, p);
+    else if (per_lane == 32)
+        hipLaunchKernelGGL((vq::k_logprobs_part<T, 32 / VEC>), grid, wg, 0, ctx->stream, p);
+    else
+        hipLaunchKernelGGL((vq::k_logprobs_part<T, 64 / VEC>), grid, wg, 0, ctx->stream, p);
+}
+
+int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, const vq::RowPlan &plan) {
+    if (plan.lanes < 256) {
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            if (a.k < 16 / (int)sizeof(typename T::Raw))
+                short_rows<T, true, 1>(ctx, a);
+            else if (plan.lanes == 1)
+                short_rows<T, false, 1>(ctx, a);
+            else if (plan.lanes == 4)
+                short_rows<T, false, 4>(ctx, a);
+            else if (plan.lanes == 16)
+                short_rows<T, false, 16>(ctx, a);
+            else
+                short_rows<T, false, 64>(ctx, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+        return VQ_OK;
+    }
+    vq::PartArgs p{a, (int)plan.parts, plan.codes, nullptr, nullptr};
+    if (plan.parts > 1) {
+        const size_t most = (size_t)a.n * plan.parts;
+        VQ_TRY(ensure_kept(ctx, ctx->score_parts, most * (8 * a.top + 12)));
+        p.keys = (uint64_t *)ctx->score_parts.p;
+        p.sums = (float *)(p.keys + most * a.top);
+    }
+    by_type(type, [&](auto t) {
+        row_parts<decltype(t)>(ctx, p, plan.per_lane);
+        if (plan.parts > 1) hipLaunchKernelGGL(vq::k_logprobs_join<decltype(t)>, dim3((unsigned)a.n), dim3(64), 0, ctx->stream, p);
+    });
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -78,10 +127,18 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
     VQ_TRY(admit(ctx, vq::check_code_logprobs(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, top, d_logprob,
                                               d_max, d_logsum, d_entropy, d_top_logprob, d_top_code), n, &go));
     if (!go) return VQ_OK;
-    const vq::LogprobArgs a{d_scores, n, ld, k, beta, d_codes, code_stride, code_bytes, top, d_logprob, d_max, d_logsum, d_entropy,
-                            d_top_logprob, d_top_code};
-    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_logprobs_rows<decltype(t)>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(256), 0, ctx->stream, a); });
-    VQ_HIP(ctx, hipGetLastError());
+    const vq::RowPlan plan = vq::plan_rows(n, k);
+    // rows per launch: a grid has fewer than 2^32 lanes, and the parts' results at most 64 MiB
+    const int64_t slice = plan.lanes < 256 ? (int64_t)(1 << 23) * (256 / plan.lanes)
+                                           : std::max<int64_t>(1, (plan.parts == 1 ? 1 << 23 : (64 << 20) / (12 + 8 * top)) / plan.parts);
+    const int e = vq::type_bytes(type);
+    for (int64_t r = 0; r < n; r += slice) {
+        vq::LogprobArgs a{(const char *)d_scores + r * ld * e, std::min(slice, n - r), ld, k, beta,
+                          d_codes ? (const char *)d_codes + r * code_stride * code_bytes : nullptr, code_stride, code_bytes, top,
+                          d_logprob ? d_logprob + r : nullptr, d_max ? d_max + r : nullptr, d_logsum ? d_logsum + r : nullptr,
+                          d_entropy ? d_entropy + r : nullptr, top ? d_top_logprob + r * top : nullptr, top ? d_top_code + r * top : nullptr};
+        VQ_TRY(logprobs_slice(ctx, type, a, plan));
+    }
     return VQ_OK;
 }
 
