@@ -458,7 +458,7 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
  * A score of -inf is a code that cannot be: it has probability zero.  A row of nothing else: m = L = -inf,
  * log probability -inf, entropy 0.  A row with a NaN or +inf: L, log probability (of a given code), entropy and alternatives
  * are NaN, with codes -1.  Any of the outputs may be NULL, d_codes and d_logprob only together.
- * beta from 1e-30 to 1e30, top <= 32, k <= 2^24.  Sums are held in f32.
+ * beta from 1e-30 to 1e30, top <= 32, k <= 2^20.  Sums are held in f32.
  * Long rows are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context, which
  * grows with n * k and is kept until the context is destroyed.  So calls may be captured into a graph where an earlier call at this
  * size or above has run (else VQ_ERR_UNSUPPORTED, and the capture goes on), and such graphs are to run on the context's stream. */

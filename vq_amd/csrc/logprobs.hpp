@@ -139,29 +139,45 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
-// Sums of one share relative to the largest score m of its row or part: S = sum 2^d, W = sum 2^d d with
-// d = (x - m) * beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero).
-template <int E> __device__ __forceinline__ void share_sums(const float (&x)[E], float m, float c, float &S, float &W) {
-    S = 0.0f, W = 0.0f;
+// Sums of the scores of a lane relative to the largest score m of their row or part: S = sum 2^d, W = sum 2^d d with
+// d = (x - m) * c, c = beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero).  One fused operation per
+// exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
+// them, and taken out of the joined sums (away).  From |M| = 10^6 on, where r may be more than 1/16, exponents are formed from x - m.
+struct Sums {
+    float m, S = 0.0f, W = 0.0f, r = 0.0f;
+    template <int E> __device__ __forceinline__ Sums(const float (&x)[E], float most, float c) : m(most) {
+        const float from = is_bad(m) || m == kNegInf ? 0.0f : m, M = from * c;  // (such rows' sums are not looked at)
+        if (__ballot(fabsf(M) >= 1e6f) == 0) {
+            r = __builtin_fmaf(from, c, -M);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float d = fmaxf((x[e] - m) * c, -200.0f), p = __builtin_amdgcn_exp2f(d);
+            for (int e = 0; e < E; ++e) add(__builtin_fmaf(x[e], c, -M));
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) add((x[e] - from) * c);
+        }
+    }
+    __device__ __forceinline__ Sums(float most, float sum, float weighted) : m(most), S(sum), W(weighted) {}
+    __device__ __forceinline__ void add(float exponent) {
+        const float d = fmaxf(exponent, -200.0f), p = __builtin_amdgcn_exp2f(d);
         S += p;
         W = __builtin_fmaf(p, d, W);
     }
-}
-// m where sums can be taken relative to it; else 0, and the row's results are those of `none` or `bad`
-__device__ __forceinline__ bool is_bad(float m) { return !(m < __builtin_inff()); }
-__device__ __forceinline__ float relative_to(float m) { return m == kNegInf || is_bad(m) ? 0.0f : m; }
+    __device__ __forceinline__ void away() {
+        const float f = __builtin_amdgcn_exp2f(-r);
+        W = f * __builtin_fmaf(-r, S, W);
+        S *= f;
+    }
+    static __device__ __forceinline__ bool is_bad(float m) { return !(m < __builtin_inff()); }
+};
 
 struct RowSums {
     float m, L, H;
 };
-__device__ __forceinline__ RowSums row_sums(float m, float S, float W) {
-    if (is_bad(m)) return {m, __builtin_nanf(""), __builtin_nanf("")};
-    if (m == kNegInf) return {m, kNegInf, 0.0f};
-    const float L = logf(S);
-    return {m, L, L - W / S * kLn2};
+__device__ __forceinline__ RowSums row_sums(const Sums &s) {
+    if (Sums::is_bad(s.m)) return {s.m, __builtin_nanf(""), __builtin_nanf("")};
+    if (s.m == kNegInf) return {s.m, kNegInf, 0.0f};
+    const float L = logf(s.S);
+    return {s.m, L, L - s.W / s.S * kLn2};
 }
 // The log probability of the row's code, whose score was read with the row.
 struct CodeScore {
@@ -208,11 +224,11 @@ __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
 #pragma unroll
     for (int e = 1; e < S16::E; ++e) m = larger(m, r.x[e]);
     m = group_max<G>(m);
-    float S, W;
-    share_sums(r.x, relative_to(m), a.beta * kLog2e, S, W);
-    S = group_sum<G>(S);
-    W = group_sum<G>(W);
-    const RowSums sums = row_sums(m, S, W);
+    Sums sum(r.x, m, a.beta * kLog2e);
+    sum.S = group_sum<G>(sum.S);
+    sum.W = group_sum<G>(sum.W);
+    sum.away();
+    const RowSums sums = row_sums(sum);
     const bool writes = lane == 0 && mine < a.n;
     if (writes) write_row(a, row, sums, cs);
     float best = m;
@@ -233,6 +249,24 @@ __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
     }
 }
 
+__device__ __forceinline__ void wave_sync() {  // a wave's reads and writes of LDS stay in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// How many of the keys in LDS are above one; zeros up to a whole eight of them lie behind the last.
+__device__ __forceinline__ int keys_above(const uint64_t *key, int count, uint64_t mine) {
+    int above = 0;
+    for (int j = 0; j < count; j += 8) {
+        uint64_t o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) o[u] = key[j + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) above += o[u] > mine;
+    }
+    return above;
+}
+
 // ---- longer rows, in parts: a workgroup each ------------------------------------------------------------
 constexpr int kMostCandidates = 512;
 
@@ -246,7 +280,7 @@ struct PartArgs {
 struct PartLds {
     float red[4][4];
     int count;
-    uint64_t key[kMostCandidates];
+    uint64_t key[kMostCandidates + 8];
     uint64_t best[32];
 };
 
@@ -274,10 +308,11 @@ __device__ __forceinline__ void part_best(S64 &r, const float (&vmax)[S64::E / S
     __syncthreads();
     const int count = l.count;
     if (count <= kMostCandidates) {
+        if (tid < 8) l.key[count + tid] = 0;  // (up to a whole eight)
+        __syncthreads();
         for (int i = tid; i < count; i += 256) {
             const uint64_t mine = l.key[i];
-            int above = 0;
-            for (int j = 0; j < count; ++j) above += l.key[j] > mine;
+            const int above = keys_above(l.key, count, mine);
             if (above < top) l.best[above] = mine;
         }
         __syncthreads();
@@ -354,93 +389,92 @@ __global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
     m = larger(larger(l.red[0][0], l.red[0][1]), larger(l.red[0][2], l.red[0][3]));
     floor = l.red[1][0];
     for (int w = 1; w < full; ++w) floor = fminf(floor, l.red[1][w]);
-    float S, W;
-    share_sums(r.x, relative_to(m), a.beta * kLog2e, S, W);
-    S = group_sum<64>(S);
-    W = group_sum<64>(W);
-    if (lane == 0) l.red[2][wave] = S, l.red[3][wave] = W;
-    if (a.top && !is_bad(m)) part_best(r, vmax, floor, lo, hi, a.top, l);
+    Sums sum(r.x, m, a.beta * kLog2e);
+    sum.S = group_sum<64>(sum.S);
+    sum.W = group_sum<64>(sum.W);
+    if (lane == 0) l.red[2][wave] = sum.S, l.red[3][wave] = sum.W;
+    if (a.top && !Sums::is_bad(m)) part_best(r, vmax, floor, lo, hi, a.top, l);
     else if (tid < 32) l.best[tid] = 0;
     __syncthreads();
+    if (wave) return;
+    sum.S = l.red[2][0] + l.red[2][1] + l.red[2][2] + l.red[2][3];
+    sum.W = l.red[3][0] + l.red[3][1] + l.red[3][2] + l.red[3][3];
+    sum.away();
     if (p.parts == 1) {
-        if (wave == 0) {
-            S = l.red[2][0] + l.red[2][1] + l.red[2][2] + l.red[2][3];
-            W = l.red[3][0] + l.red[3][1] + l.red[3][2] + l.red[3][3];
-            const RowSums sums = row_sums(m, S, W);
-            if (lane == 0) write_row(a, row, sums, cs);
-            if (lane < a.top) write_alternative(a, row, lane, key_score(l.best[lane]), l.best[lane] ? key_code(l.best[lane]) : -1, sums);
-        }
+        const RowSums sums = row_sums(sum);
+        if (lane == 0) write_row(a, row, sums, cs);
+        if (lane < a.top) write_alternative(a, row, lane, key_score(l.best[lane]), l.best[lane] ? key_code(l.best[lane]) : -1, sums);
     } else {
-        if (tid < 3) {
-            const float v[2] = {l.red[2][0] + l.red[2][1] + l.red[2][2] + l.red[2][3], l.red[3][0] + l.red[3][1] + l.red[3][2] + l.red[3][3]};
-            p.sums[(int64_t)blockIdx.x * 3 + tid] = tid == 0 ? m : tid == 1 ? v[0] : v[1];
-        }
-        if (tid < a.top) p.keys[(int64_t)blockIdx.x * a.top + tid] = l.best[tid];
+        const int64_t at = blockIdx.x;
+        if (lane == 0) p.sums[at * 3] = sum.m, p.sums[at * 3 + 1] = sum.S, p.sums[at * 3 + 2] = sum.W;
+        if (lane < a.top) p.keys[at * a.top + lane] = l.best[lane];
     }
 }
 
-// A wave joins the parts of a row: sums rescaled to the largest score of all, and the alternatives from the heads of the
-// parts' lists.
+// A wave joins the parts of a row: sums rescaled to the largest score of all, and the alternatives from the parts' lists.
+// With j = (top - 1) / parts, rounded down, `top` keys or more reach the q-th largest of the lists' keys number j where
+// q * (j + 1) >= top: what reaches that floor, a few at the head of every list, is gathered and sorted by counting.  (One
+// round of the whole wave per alternative took 0.2 us each: a row of 32 parts, 20 alternatives 8.0 us, 4.5 so.)
 template <typename T>
-__global__ void __launch_bounds__(64) k_logprobs_join(PartArgs p) {
+__global__ void __launch_bounds__(256) k_logprobs_join(PartArgs p) {
+    extern __shared__ uint64_t join_lds[];
     const LogprobArgs &a = p.a;
-    const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x;
-    const float *sums = p.sums + row * p.parts * 3;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top = a.top, parts = p.parts;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+    if (row >= a.n) return;  // (no barriers below)
     CodeScore cs;
     cs.read(a, row, T());
-    float m = kNegInf;
-    for (int q = lane; q < p.parts; q += 64) m = larger(m, sums[q * 3]);
-    m = group_max<64>(m);
-    float S = 0.0f, W = 0.0f;
-    for (int q = lane; q < p.parts; q += 64) {
-        const float d = fmaxf((sums[q * 3] - relative_to(m)) * (a.beta * kLog2e), -200.0f), f = __builtin_amdgcn_exp2f(d);
-        S = __builtin_fmaf(f, sums[q * 3 + 1], S);
-        W = __builtin_fmaf(f, __builtin_fmaf(sums[q * 3 + 1], d, sums[q * 3 + 2]), W);
-    }
-    S = group_sum<64>(S);
-    W = group_sum<64>(W);
-    const RowSums r = row_sums(m, S, W);
-    if (lane == 0) write_row(a, row, r, cs);
-    // A lane has the list of one part, the largest left in a register and the next behind it, so that the read
-    // of a round's winner is not waited for.
-    if (a.top == 0) return;
-    const int total = p.parts * a.top;
+    const int total = parts * top;
     const uint64_t *keys = p.keys + row * total;
-    if (p.parts <= 64) {
-        __shared__ uint64_t lists[64 * 32];
-        for (int i = lane; i < total; i += 64) lists[i] = keys[i];
-        __syncthreads();
-        const uint64_t *list = lists + min(lane, p.parts - 1) * a.top;
-        uint64_t head = lane < p.parts ? list[0] : 0, next = lane < p.parts && a.top > 1 ? list[1] : 0, mine = 0;
-        int at = 1;
-        for (int t = 0; t < a.top; ++t) {
-            const uint64_t key = wave_max(head);
-            if (lane == t) mine = key;
-            if (head == key) {
-                head = next;
-                ++at;
-                next = lane < p.parts && at < a.top ? list[at] : 0;
-            }
-        }
-        if (lane < a.top) write_alternative(a, row, lane, key_score(mine), mine ? key_code(mine) : -1, r);
-        return;
+    uint64_t *lists = join_lds + wave * (2 * total + 8), *found = lists + total;
+    for (int i = lane; i < total; i += 512) {
+        uint64_t k[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) k[u] = i + 64 * u < total ? keys[i + 64 * u] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i + 64 * u < total) lists[i + 64 * u] = k[u];
     }
-    uint64_t last = ~0ull;  // more than a million codes: through the lists of a lane's parts in every round
-    for (int t = 0; t < a.top; ++t) {
-        uint64_t key = 0;
-        for (int q = lane; q < p.parts; q += 64)
-            for (int i = 0; i < a.top; ++i) {
-                const uint64_t c = keys[q * a.top + i];
-                if (c < last) {  // the first of this part that is left
-                    key = c > key ? c : key;
-                    break;
-                }
-            }
-        key = wave_max(key);
-        last = key;
-        if (lane == 0) write_alternative(a, row, t, key_score(key), key ? key_code(key) : -1, r);
+    const float *sums = p.sums + (row * parts + min(lane, parts - 1)) * 3, c = a.beta * kLog2e;
+    const float pm = sums[0], pS = lane < parts ? sums[1] : 0.0f, pW = lane < parts ? sums[2] : 0.0f, m = group_max<64>(pm);
+    const float d = fmaxf((pm - (Sums::is_bad(m) || m == kNegInf ? 0.0f : m)) * c, -200.0f), f = __builtin_amdgcn_exp2f(d);
+    const RowSums r = row_sums({m, group_sum<64>(f * pS), group_sum<64>(f * __builtin_fmaf(pS, d, pW))});
+    if (lane == 0) write_row(a, row, r, cs);
+    if (top == 0) return;
+    wave_sync();
+    const uint64_t *list = lists + min(lane, parts - 1) * top;
+    const int j = (top - 1) / parts, q = (top + j) / (j + 1);
+    const uint64_t probe = lane < parts ? list[j] : 0;
+    int above = 0;
+    for (int o = 0; o < parts; ++o) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(probe >> 32), o) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)probe, o);
+        above += other > probe;
     }
+    // (keys are different but for those that are 0: where fewer than q are not, the floor is 1)
+    const unsigned long long who = __ballot(lane < parts && probe != 0 && above == q - 1);
+    const int at = who ? __ffsll(who) - 1 : 0;
+    const uint64_t floor = !who ? 1 : (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(probe >> 32), at) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)probe, at);
+    int count = 0;
+    uint64_t next = lane < parts ? list[0] : 0;
+    for (int i = 1;; ++i) {
+        const unsigned long long more = __ballot(next >= floor);
+        if (!more) break;
+        if (next >= floor) found[count + __popcll(more & ((1ull << lane) - 1))] = next;
+        count += __popcll(more);
+        next = next >= floor && i < top ? list[i] : 0;
+    }
+    if (lane < 8) found[count + lane] = 0;
+    if (lane < top) lists[lane] = 0;  // (the best of all; the lists have been read)
+    wave_sync();
+    for (int i = lane; i < count; i += 64) {
+        const uint64_t mine = found[i];
+        const int rank = keys_above(found, count, mine);
+        if (rank < top) lists[rank] = mine;
+    }
+    wave_sync();
+    if (lane < top) write_alternative(a, row, lane, key_score(lists[lane]), lists[lane] ? key_code(lists[lane]) : -1, r);
 }
 
 struct GradArgs {

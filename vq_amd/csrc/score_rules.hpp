@@ -1,6 +1,7 @@
 // What the calls on 8-bit scores and log probabilities of codes take and refuse: rules on sizes, strides and addresses
 // alone, without HIP, so that a CPU test can go through them.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <string>
@@ -12,7 +13,8 @@ namespace vq {
 // Components of an 8-bit row: the sum of as many products of two bytes (at most 2^14 each) fits 32 bits.
 constexpr int32_t kMaxDimI8 = 131071;
 constexpr int32_t kMaxTop = 32;           // alternatives of a row
-constexpr int32_t kMaxScoreCodes = 1 << 24;  // codes of a row of scores
+constexpr int32_t kMaxScoreCodes = 1 << 24;  // codes that rows are scored against
+constexpr int32_t kMaxRowCodes = 1 << 20;    // codes of a row of scores whose probabilities are asked for
 
 // Status and text of a refusal; VQ_OK: the call may run.
 struct Refusal {
@@ -80,7 +82,7 @@ inline Refusal check_scored_codes(int32_t type, const void *s, int64_t n, int64_
     const int e = type_bytes(type);
     if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(type));
     if (n < 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative and k must be greater than 0");
-    if (k > kMaxScoreCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 16777216");
+    if (k > kMaxRowCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 1048576");
     if (ld < k) return refuse(VQ_ERR_INVALID_ARG, "the row stride is below k");
     if (too_long(n, ld, e)) return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
     if (!(beta >= 1e-30f) || !(beta <= 1e30f)) return refuse(VQ_ERR_INVALID_ARG, "beta must be between 1e-30 and 1e30");
@@ -147,18 +149,18 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
 
 // How the rows of a call go through the GPU.  Rows of up to 1024 codes have 1, 4, 16 or 64 lanes each, 16 codes per lane (`lanes`).
 // Longer ones have a workgroup of 256 lanes per part, 8 to 64 codes per lane (`per_lane`): as many as it takes for a row to be
-// one part, but no more than leave 1024 workgroups (four per compute unit) to the call, and no fewer than 8; at most 64 parts where
-// 64 codes per lane allow that.  Parts are of equal length, in whole 64 codes (`codes`; the last one is shorter).
-constexpr int kShortCodes = 1024;
+// one part, but no more than leave WORKGROUPS workgroups to the call, and no fewer than 8; at most 64 parts.  Parts are of equal
+// length, in whole 64 codes (`codes`; the last one is shorter).
+constexpr int kShortCodes = 1024, kMostParts = 64;
+static_assert(kMaxRowCodes <= kMostParts * 64 * 256, "64 codes per lane hold every row");
 struct RowPlan {
     int lanes, per_lane;
-    int64_t parts;
-    int32_t codes;
+    int32_t parts, codes;
 };
 inline RowPlan plan_rows(int64_t n, int32_t k) {
     if (k <= kShortCodes) return {k <= 16 ? 1 : k <= 64 ? 4 : k <= 256 ? 16 : 64, 16, 1, k};
     int e = 64;
-    while (e > 8 && (k <= 128 * e || (n * ((k + 256 * e - 1) / (256 * e)) < 1024 && k <= 128 * e * 64))) e /= 2;
+    while (e > 8 && (k <= 128 * e || (n * ((k + 256 * e - 1) / (256 * e)) < 4096 && k <= 128 * e * kMostParts))) e /= 2;
     const int32_t least = (k + 256 * e - 1) / (256 * e), codes = ((k + least - 1) / least + 63) / 64 * 64;
     return {256, e, (k + codes - 1) / codes, codes};
 }

@@ -75,7 +75,11 @@ int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, cons
     }
     by_type(type, [&](auto t) {
         row_parts<decltype(t)>(ctx, p, plan.per_lane);
-        if (plan.parts > 1) hipLaunchKernelGGL(vq::k_logprobs_join<decltype(t)>, dim3((unsigned)a.n), dim3(64), 0, ctx->stream, p);
+        if (plan.parts > 1) {
+            const int rows = plan.parts <= 8 ? 4 : 1;  // per workgroup: at most 32.5 KB of lists
+            hipLaunchKernelGGL(vq::k_logprobs_join<decltype(t)>, dim3((unsigned)cdiv64(a.n, rows)), dim3(64 * rows),
+                               rows * 8 * (2 * plan.parts * a.top + 8), ctx->stream, p);
+        }
     });
     VQ_HIP(ctx, hipGetLastError());
     return VQ_OK;
