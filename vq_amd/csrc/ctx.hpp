@@ -90,6 +90,7 @@ struct vq_ctx {
     // graphs may hold its address
     DevBuf score_parts;
     std::vector<void *> outgrown;
+    uint32_t scores_lds_set = 0;  // dynamic-LDS limit granted to the tiles of scores, a bit per instance
     // optional per-kernel-class timing (HIP events on the stream)
     bool prof_on = false;
     std::vector<hipEvent_t> prof_pool;

@@ -165,4 +165,19 @@ inline RowPlan plan_rows(int64_t n, int32_t k) {
     return {256, e, (k + codes - 1) / codes, codes};
 }
 
+// Scores: 8-bit rows at aligned addresses and strides go through tiles of 256 x 256, 128 x 128 or 64 x 64 rows and codes, the largest that
+// leave 256 of them (one per compute unit) to the call; others through k_scores_any (0).
+// Places within a tile's rows are counted in 32 bits: strides up to 2^22.
+constexpr int64_t kMaxTileStride = 1 << 22;
+inline int score_tile(int64_t n, int32_t k, bool aligned) {
+    if (!aligned) return 0;
+    for (int t : {256, 128})
+        if (((n + t - 1) / t) * ((k + t - 1) / t) >= 256) return t;
+    return 64;
+}
+// Rows of a launch: fewer than 2^22 tiles of 64 x 64, and no more tiles of rows than a grid's second dimension holds.
+inline int64_t score_rows_of_a_launch(int32_t k) {
+    return 64 * std::min<int64_t>(65535, std::max<int64_t>(1, (1 << 22) / ((k + 63) / 64)));
+}
+
 }  // namespace vq

@@ -115,4 +115,171 @@ __global__ void __launch_bounds__(256) k_scores_any(ScoresArgs a) {
     }
 }
 
+// ---- tiles ----------------------------------------------------------------------------------------------
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+
+// A tile's place: workgroup i runs on XCD i % 8, and every XCD gets a run of consecutive tiles, column by column through panels
+// of four tiles of rows, so that what its compute units read at a time comes from its own L2.
+struct TilePlace {
+    int64_t r;
+    int c;
+};
+__device__ __forceinline__ TilePlace tile_place(uint32_t id, uint32_t row_tiles, uint32_t code_tiles) {
+    const uint32_t all = row_tiles * code_tiles, q = all / 8, rest = all % 8, xcd = id % 8;
+    const uint32_t at = xcd * q + min(xcd, rest) + id / 8, panel = at / (4 * code_tiles), in = at - panel * 4 * code_tiles;
+    const uint32_t high = min(4u, row_tiles - panel * 4);
+    return {(int64_t)(panel * 4 + in % high), (int)(in / high)};
+}
+
+// 16 bytes per lane from base + offset to LDS, in the order of the lanes; zeros from `bytes` on, which the hardware checks.
+// `base`, `bytes` and `to` are the same in every lane.
+__device__ __forceinline__ void copy_to_lds(const int8_t *base, int bytes, char *to, int offset) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass does not know the type of a buffer)
+    __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, offset, 0, 0, 0);
+#endif
+}
+
+// Everyone's copies into LDS are there, and what everyone read from it.
+__device__ __forceinline__ void step_barrier() {
+    asm volatile("" ::: "memory");  // (the compiler moves no access across)
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// TR rows x TC codes by WR x WC waves, each TR / WR rows x TC / WC codes in blocks of 32 x 32.  The operands come in steps of 128
+// components straight into LDS, the next step's on their way while a step is worked on; one barrier per step.  A row of a step
+// is 128 bytes there, its eight 16-byte pieces in an order that depends on the row, so that the reads of a fragment (32 rows at the
+// same place) meet all banks; since the copies fill LDS in the order of the lanes, each lane fetches the piece that belongs at its place.
+// Buffer addresses are checked by the hardware: rows behind the last read as zeros.  Every row's bytes behind component `dim`
+// are somebody's data: they are cleared in the rows of x before the last step is worked on, and count for nothing in w then.
+// The codes are the first operand: a lane ends with runs of four codes of a row, scales them, and the tile leaves through LDS in whole lines.
+// Aligned rows only (address and stride multiples of 16).
+template <typename OutT, int TR, int TC, int WR, int WC>
+__global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint32_t row_tiles, uint32_t code_tiles) {
+    constexpr int NW = WR * WC, R = TR / WR / 32, C = TC / WC / 32, XI = TR / 8 / NW, WI = TC / 8 / NW, STAGE = (TR + TC) * 128;
+    static_assert(XI * 8 * NW == TR && WI * 8 * NW == TC && R * 32 * WR == TR && C * 32 * WC == TC, "whole blocks");
+    typedef typename OutT::Raw Raw;
+    extern __shared__ __attribute__((aligned(1024))) char tile_lds[];
+    float *lws = reinterpret_cast<float *>(tile_lds + 2 * STAGE), *lbias = lws + TC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WC, wc = wave % WC;
+    const TilePlace place = tile_place(blockIdx.x, row_tiles, code_tiles);
+    const int64_t row0 = place.r * TR;
+    const int code0 = place.c * TC, rows = (int)min((int64_t)TR, a.n - row0), codes = min(TC, a.k - code0);
+    const int steps = (a.dim + 127) / 128, dim16 = (a.dim + 15) & ~15;
+    const int8_t *px = a.x + row0 * a.ld_x, *pw = a.w + (int64_t)code0 * a.ld_w;
+    const int ldx = (int)a.ld_x, ldw = (int)a.ld_w, left_x = (rows - 1) * ldx + dim16, left_w = (codes - 1) * ldw + dim16;
+    const int l8 = lane >> 3;
+    const int swz = l8, chunk = ((lane & 7) ^ swz) * 16;
+    int vx[XI], vw[WI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) vx[i] = ((wave * XI + i) * 8 + l8) * ldx + chunk;
+#pragma unroll
+    for (int i = 0; i < WI; ++i) vw[i] = ((wave * WI + i) * 8 + l8) * ldw + chunk;
+    const auto bring = [&](int step, int buf) {
+        char *to = tile_lds + buf * STAGE;
+#pragma unroll
+        for (int i = 0; i < XI; ++i)
+            copy_to_lds(px + step * 128, left_x - step * 128, to + (wave * XI + i) * 1024, vx[i]);
+#pragma unroll
+        for (int i = 0; i < WI; ++i)
+            copy_to_lds(pw + step * 128, left_w - step * 128, to + TR * 128 + (wave * WI + i) * 1024, vw[i]);
+    };
+    bring(0, 0);
+    for (int j = tid; j < TC; j += 64 * NW) {
+        lws[j] = j < codes ? a.ws[code0 + j] : 0.0f;
+        lbias[j] = a.bias && j < codes ? a.bias[code0 + j] : 0.0f;
+    }
+    i32x16 acc[R][C];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[r][c][i] = 0;
+    const int l32 = lane & 31, h = lane >> 5;
+    int off[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + (((2 * s + h) ^ (l32 & 7)) * 16);
+    for (int step = 0; step < steps; ++step) {
+        const int buf = step & 1;
+        step_barrier();
+        if (step + 1 < steps) bring(step + 1, buf ^ 1);
+        char *at = tile_lds + buf * STAGE;
+        if (step + 1 == steps && (a.dim & 127)) {  // uniform
+            const int t0 = a.dim & 127;
+            for (int i = tid; i < TR * 8; i += 64 * NW) {
+                const int row = i >> 3, p = (i & 7) * 16;  // the piece of components p to p + 15
+                if (p + 16 > t0) {
+                    i32x4 *v = reinterpret_cast<i32x4 *>(at + row * 128 + ((i & 7) ^ (row & 7)) * 16);
+                    i32x4 x = *v;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int keep = min(max(t0 - p - 4 * q, 0), 4);
+                        x[q] = keep == 4 ? x[q] : x[q] & ((1 << (8 * keep)) - 1);
+                    }
+                    *v = x;
+                }
+            }
+            __syncthreads();
+        }
+        const char *ax = at + wr * (R * 32 * 128), *aw = at + TR * 128 + wc * (C * 32 * 128);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            i32x4 fx[R], fw[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) fw[c] = *reinterpret_cast<const i32x4 *>(aw + c * 4096 + off[s]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) fx[r] = *reinterpret_cast<const i32x4 *>(ax + r * 4096 + off[s]);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c], fx[r], acc[r][c], 0, 0, 0);
+        }
+    }
+    step_barrier();  // LDS is free
+    constexpr int LINE = C * 32 * (int)sizeof(Raw), PITCH = LINE + 16, PIECES = LINE / 16;
+    static_assert(NW * 32 * PITCH <= 2 * STAGE, "a block of rows per wave fits");
+    char *mine = tile_lds + wave * (32 * PITCH);
+    const int wcode = code0 + wc * (C * 32);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t brow = row0 + wr * (R * 32) + r * 32;
+        const float xs = a.xs[min(brow + l32, a.n - 1)];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int j = wc * (C * 32) + c * 32 + q * 8 + h * 4;
+                const f32x4 s4 = *reinterpret_cast<const f32x4 *>(lws + j), b4 = *reinterpret_cast<const f32x4 *>(lbias + j);
+                struct __attribute__((aligned(4 * sizeof(Raw)))) {
+                    Raw v[4];
+                } o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o.v[i] = OutT::down((float)acc[r][c][q * 4 + i] * xs * s4[i] + b4[i]);
+                __builtin_memcpy(mine + l32 * PITCH + (c * 32 + q * 8 + h * 4) * sizeof(Raw), &o, sizeof(o));
+            }
+        wave_sync();
+#pragma unroll
+        for (int i = lane; i < 32 * PIECES; i += 64) {
+            const int row = i / PIECES, piece = i % PIECES, code = wcode + piece * (16 / (int)sizeof(Raw));
+            struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
+                uint32_t w[4];
+            };
+            const i32x4 v = *reinterpret_cast<const i32x4 *>(mine + row * PITCH + piece * 16);
+            if (brow + row < a.n && code < a.k) {
+                Raw *to = (Raw *)a.out + (brow + row) * a.ld_out + code;
+                if (code + 16 / (int)sizeof(Raw) <= a.k)
+                    *reinterpret_cast<Piece *>(to) = __builtin_bit_cast(Piece, v);
+                else
+                    for (int e = 0; e < 16 / (int)sizeof(Raw); ++e)
+                        if (code + e < a.k) to[e] = reinterpret_cast<const Raw *>(mine + row * PITCH + piece * 16)[e];
+            }
+        }
+        wave_sync();
+    }
+}
+constexpr int tile_lds_bytes(int tr, int tc) { return 2 * (tr + tc) * 128 + tc * 8; }
+
 }  // namespace vq

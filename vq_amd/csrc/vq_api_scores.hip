@@ -32,6 +32,32 @@ template <typename F> void by_type(int32_t type, F f) {
         f(vq::BF16());
 }
 
+// One launch of tiles; the limit of the LDS above 64 KB is asked for once per context and instance.
+template <typename T, int TR, int TC, int WR, int WC> int32_t score_tiles(vq_ctx *ctx, const vq::ScoresArgs &a, int bit) {
+    constexpr int lds = vq::tile_lds_bytes(TR, TC);
+    const auto kernel = vq::k_scores_tile<T, TR, TC, WR, WC>;
+    if (lds > 65536 && !(ctx->scores_lds_set >> bit & 1)) {
+        VQ_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        ctx->scores_lds_set |= 1u << bit;
+    }
+    const uint32_t rt = (uint32_t)cdiv64(a.n, TR), ct = (uint32_t)cdiv64(a.k, TC);
+    hipLaunchKernelGGL(kernel, dim3(rt * ct), dim3(64 * WR * WC), lds, ctx->stream, a, rt, ct);
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
+}
+
+template <typename T> int32_t scores_slice(vq_ctx *ctx, const vq::ScoresArgs &a, int type, int way) {
+    switch (way) {
+    case 256: return score_tiles<T, 256, 256, 2, 4>(ctx, a, type * 4);
+    case 128: return score_tiles<T, 128, 128, 2, 2>(ctx, a, type * 4 + 1);
+    case 64: return score_tiles<T, 64, 64, 2, 2>(ctx, a, type * 4 + 2);
+    default:
+        hipLaunchKernelGGL(vq::k_scores_any<T>, dim3(cdiv(a.k, 64), cdiv(a.n, 64)), dim3(256), 0, ctx->stream, a);
+        VQ_HIP(ctx, hipGetLastError());
+        return VQ_OK;
+    }
+}
+
 template <typename T, bool TINY, int G> void short_rows(vq_ctx *ctx, const vq::LogprobArgs &a) {
     hipLaunchKernelGGL((vq::k_logprobs_short<T, G, TINY>), dim3((unsigned)cdiv64(a.n, 256 / G)), dim3(256), 0, ctx->stream, a);
 }
@@ -108,17 +134,19 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
     bool go;
     VQ_TRY(admit(ctx, vq::check_scores_i8(d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, out_type, d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
+    const bool aligned = !vq::misaligned(d_x, 16) && !vq::misaligned(d_w, 16) && ld_x % 16 == 0 && ld_w % 16 == 0 && ld_x <= vq::kMaxTileStride &&
+                         ld_w <= vq::kMaxTileStride;
     vq::ScoresArgs a{d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, d_out, ld_out};
-    const int64_t slice = 65535 * 64;
+    const int64_t slice = vq::score_rows_of_a_launch(k);
     for (int64_t r = 0; r < n; r += slice) {
         a.n = std::min(n - r, slice);
         a.x = d_x + r * ld_x;
         a.xs = d_xs + r;
         a.out = (char *)d_out + r * ld_out * vq::type_bytes(out_type);
-        by_type(out_type, [&](auto t) {
-            hipLaunchKernelGGL(vq::k_scores_any<decltype(t)>, dim3(cdiv(k, 64), cdiv(a.n, 64)), dim3(256), 0, ctx->stream, a);
-        });
-        VQ_HIP(ctx, hipGetLastError());
+        const int way = vq::score_tile(a.n, k, aligned);
+        int32_t rc = VQ_OK;
+        by_type(out_type, [&](auto t) { rc = scores_slice<decltype(t)>(ctx, a, out_type, way); });
+        VQ_TRY(rc);
     }
     return VQ_OK;
 }
