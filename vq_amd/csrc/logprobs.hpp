@@ -62,18 +62,30 @@ __device__ __forceinline__ int32_t key_code(uint64_t key) { return (int32_t)~(ui
 template <typename T, int LANES, int NV> struct Share {
     typedef typename T::Raw Raw;
     static constexpr int VEC = 16 / (int)sizeof(Raw), E = NV * VEC;
+    struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
+        uint32_t w[4];
+    };
+    Piece raw[NV];
     float x[E];
 
     static __device__ __forceinline__ int base(int u, int lane, int lo, int hi) { return min(lo + (u * LANES + lane) * VEC, hi - VEC); }
 
-    __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
-        struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
-            uint32_t w[4];
-        };
-        Piece raw[NV];
+    __device__ __forceinline__ void fetch(const Raw *s, int lo, int hi, int lane) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
             if (u == 0 || lo + u * LANES * VEC < hi) raw[u] = *reinterpret_cast<const Piece *>(s + base(u, lane, lo, hi));
+    }
+    static __device__ __forceinline__ void values(const Piece &piece, float *to) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            if constexpr (sizeof(Raw) == 4)
+                to[v] = __uint_as_float(piece.w[v]);
+            else
+                to[v] = T::up((Raw)(v & 1 ? piece.w[v >> 1] >> 16 : piece.w[v >> 1] & 0xffffu));
+        }
+    }
+    __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
+        fetch(s, lo, hi, lane);
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             if (u > 0 && lo + u * LANES * VEC >= hi) {  // uniform: nothing of the row is left
@@ -81,13 +93,7 @@ template <typename T, int LANES, int NV> struct Share {
                 for (int v = 0; v < VEC; ++v) x[u * VEC + v] = kNegInf;
                 continue;
             }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                if constexpr (sizeof(Raw) == 4)
-                    x[u * VEC + v] = __uint_as_float(raw[u].w[v]);
-                else
-                    x[u * VEC + v] = T::up((Raw)(v & 1 ? raw[u].w[v >> 1] >> 16 : raw[u].w[v >> 1] & 0xffffu));
-            }
+            values(raw[u], x + u * VEC);
             if (lo + (u + 1) * LANES * VEC > hi) {  // uniform: the vectors that are read from elsewhere
                 const int skip = lo + (u * LANES + lane) * VEC - base(u, lane, lo, hi);
 #pragma unroll
@@ -490,29 +496,80 @@ struct GradArgs {
     int64_t ld_grad;
 };
 
-// The gradient of one score: lp = log p, one: whether this is the row's code.
-__device__ __forceinline__ float grad_one(float lp, bool one, float beta, float gl, float gh, float H) {
-    const float p = expf(lp), t = p == 0.0f ? 0.0f : p * (gl + gh * (lp + H));
-    return beta * ((one ? gl : 0.0f) - t);
+// 2^d with d = (x - m) * c - L2 is the probability (c = beta * log2 e, L2 = L * log2 e), d * ln 2 its logarithm; both held above 2^-200,
+// which is zero in f32, and zero times a number a zero.  A and B hold the factors: beta * (g_lp + g_H * (log p + H)) = A * d + B.
+// A lane has NV vectors of a row, G lanes a row or (G = 256, blockIdx.y) a piece of one; its code's own term is added where one of its
+// vectors holds the code.  A vector that would pass the row's end is read from elsewhere (Share) but only its own values are
+// written, one by one, so that the gradient may take the scores' place.
+template <typename T, int G, int NV>
+__global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
+    typedef Share<T, G, NV> S;
+    typedef typename T::Raw Raw;
+    constexpr int VEC = S::VEC;
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
+    const int lo = G == 256 ? (int)blockIdx.y * (G * S::E) : 0, hi = a.k;
+    S r;
+    r.fetch((const Raw *)a.s + row * a.ld, lo, hi, lane);
+    Raw *to = (Raw *)a.grad + row * a.ld_grad;
+    const float m = a.max[row], L = a.logsum[row], gh = a.g_entropy ? a.g_entropy[row] : 0.0f, H = a.g_entropy ? a.entropy[row] : 0.0f;
+    int64_t code = -1;
+    float gl = 0.0f;
+    if (a.g_logprob) {
+        code = code_at(a.codes, a.code_bytes, row * a.code_stride);
+        if (code >= 0) gl = a.g_logprob[row];
+    }
+    const bool none = m == kNegInf, bad = L != L || code >= a.k;
+    const float from = none ? 0.0f : m, c = a.beta * kLog2e, L2 = none ? 0.0f : L * kLog2e, own = a.beta * gl;
+    const float A = none ? 0.0f : a.beta * gh * kLn2, B = bad ? __builtin_nanf("") : none ? 0.0f : a.beta * __builtin_fmaf(gh, H, gl);
+    if (none) code = -1;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (u > 0 && lo + u * G * VEC >= hi) break;  // uniform
+        const int at = lo + (u * G + lane) * VEC, base = S::base(u, lane, lo, hi);
+        float x[VEC];
+        S::values(r.raw[u], x);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float d = fmaxf(__builtin_fmaf(x[v] - from, c, -L2), -200.0f);
+            x[v] = __builtin_amdgcn_exp2f(d) * -__builtin_fmaf(d, A, B);
+        }
+        const int64_t hit = code - base;
+        if (hit >= 0 && hit < VEC) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) x[v] = v == hit ? x[v] + own : x[v];
+        }
+        typename S::Piece o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if constexpr (sizeof(Raw) == 4)
+                o.w[q] = __float_as_uint(x[q]);
+            else
+                o.w[q] = (uint32_t)T::down(x[2 * q]) | (uint32_t)T::down(x[2 * q + 1]) << 16;
+        }
+        if (mine >= a.n || at >= hi) continue;
+        if (base == at)
+            *reinterpret_cast<typename S::Piece *>(to + at) = o;
+        else
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                if (base + v >= at) to[base + v] = T::down(x[v]);
+    }
 }
 
+// Rows shorter than a vector: a lane each.
 template <typename T>
-__global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
-    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+__global__ void __launch_bounds__(256) k_logprobs_grad_tiny(GradArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= a.n) return;
     const typename T::Raw *s = (const typename T::Raw *)a.s + row * a.ld;
-    typename T::Raw *g = (typename T::Raw *)a.grad + row * a.ld_grad;
-    const float m = a.max[row], L = a.logsum[row];
-    const bool none = m == kNegInf;
-    const float ms = none ? 0.0f : m, gh = a.g_entropy ? a.g_entropy[row] : 0.0f, H = a.g_entropy ? a.entropy[row] : 0.0f;
-    float gl = 0.0f;
-    int64_t c = -1;
-    if (a.g_logprob) {
-        c = code_at(a.codes, a.code_bytes, row * a.code_stride);
-        gl = c >= a.k ? __builtin_nanf("") : c < 0 ? 0.0f : a.g_logprob[row];
-    }
-    for (int j = threadIdx.x; j < a.k; j += 256)
-        g[j] = T::down(none ? 0.0f : L != L || gl != gl ? __builtin_nanf("")
-                                                          : grad_one(a.beta * (T::up(s[j]) - ms) - L, j == c, a.beta, gl, gh, H));
+    const float m = a.max[row], L = a.logsum[row], gh = a.g_entropy ? a.g_entropy[row] : 0.0f, H = a.g_entropy ? a.entropy[row] : 0.0f;
+    const int64_t code = a.g_logprob ? code_at(a.codes, a.code_bytes, row * a.code_stride) : -1;
+    const float gl = code >= 0 ? a.g_logprob[row] : 0.0f;
+    for (int j = 0; j < a.k; ++j) {
+        const float lp = fmaxf(a.beta * (T::up(s[j]) - m) - L, -140.0f);
+        const float g = a.beta * ((j == code ? gl : 0.0f) - __builtin_amdgcn_exp2f(lp * kLog2e) * (gl + gh * (lp + H)));
+        ((typename T::Raw *)a.grad)[row * a.ld_grad + j] = T::down(m == kNegInf ? 0.0f : L != L || code >= a.k ? __builtin_nanf("") : g);
     }
 }
 

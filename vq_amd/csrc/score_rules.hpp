@@ -180,4 +180,15 @@ inline int64_t score_rows_of_a_launch(int32_t k) {
     return 64 * std::min<int64_t>(65535, std::max<int64_t>(1, (1 << 22) / ((k + 63) / 64)));
 }
 
+// Lanes and vectors of 16 bytes per lane that hold a row of `length` values in registers: 16 or 64 lanes with one vector, 64 with four, a
+// workgroup with eight; lanes 0: none does.
+struct LanePlan {
+    int lanes, vectors;
+};
+inline LanePlan plan_lanes(int32_t length, int bytes) {
+    const int vec = 16 / bytes;
+    if (length < vec || length > 2048 * vec) return {0, 0};
+    return length <= 16 * vec ? LanePlan{16, 1} : length <= 64 * vec ? LanePlan{64, 1} : length <= 256 * vec ? LanePlan{64, 4} : LanePlan{256, 8};
+}
+
 }  // namespace vq

@@ -11,15 +11,27 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // x / scale to the nearest integer, ties to even, from the exact quotient: the rounded product with the reciprocal is
 // at most one off, and the distance r = x - q * scale to it is exact in f32 (a multiple of the last bit of
-// `scale`, or of x where that is finer and q <= 1, of less than 2^24 of them).
-__device__ __forceinline__ int nearest_i8(float x, float scale, float inv) {
-    float q = __builtin_rintf(x * inv);
-    const float r = __builtin_fmaf(-q, scale, x), half = 0.5f * scale;
-    const bool odd = ((int)q & 1) != 0;
-    if (r > half || (r == half && odd)) q += 1.0f;
-    if (r < -half || (r == -half && odd)) q -= 1.0f;
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+// `scale`, or of x where that is finer and q <= 1, of less than 2^24 of them), so r says which way to go.
+__device__ __forceinline__ int nearest_i8(float x, float scale, float inv, float half) {
+    const float q = __builtin_rintf(x * inv), r = __builtin_fmaf(-q, scale, x), far = fabsf(r);
+    const int i = (int)q, there = i + (r < 0.0f ? -1 : 1);
+    return max(-127, min(127, far > half || (far == half && (i & 1)) ? there : i));
 }
+
+// The scale of a row from its largest magnitude, given as the bits of a number (an infinity is above every
+// number and a NaN above it).
+struct RowScale {
+    float scale, up, sc, inv, half;
+    __device__ __forceinline__ explicit RowScale(uint32_t most) {
+        scale = most >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(most) / 127.0f;
+        up = scale < 0x1p-100f ? 0x1p60f : 1.0f;  // small scales: both sides of the quotient times 2^60, exactly, so that the reciprocal is finite
+        sc = scale * up;
+        inv = 1.0f / sc;
+        half = 0.5f * sc;
+    }
+    __device__ __forceinline__ int of(float x) const { return nearest_i8(x * up, sc, inv, half); }
+    __device__ __forceinline__ bool usable() const { return scale > 0.0f; }
+};
 
 struct RowsI8Args {
     const void *x;
@@ -30,22 +42,71 @@ struct RowsI8Args {
     float *scale;
 };
 
-// A wave per row.
-template <typename T>
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// G lanes per row, which lies in their registers between the search for its largest magnitude and the quotients.  The vectors at
+// its end overlap (Share) where its length is no multiple of theirs: what they share, both write alike.
+template <typename T, int G, int NV>
 __global__ void __launch_bounds__(256) k_rows_i8(RowsI8Args a) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.n; row += (int64_t)gridDim.x * 4) {
+    typedef Share<T, G, NV> S;
+    constexpr int VEC = S::VEC;
+    const int lane = threadIdx.x & (G - 1);
+    const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
+    S r;
+    r.fetch((const typename T::Raw *)a.x + row * a.ld, 0, a.dim, lane);
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (u > 0 && u * G * VEC >= a.dim) break;  // uniform
+        S::values(r.raw[u], r.x + u * VEC);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) m = max(m, magnitude(r.x[u * VEC + v]));
+    }
+    const auto most = [](uint32_t p, uint32_t q) { return p > q ? p : q; };
+    m = over_group<(G > 64 ? 64 : G)>(m, 0u, most);
+    if constexpr (G == 256) {
+        __shared__ uint32_t part[4];
+        if ((lane & 63) == 0) part[lane >> 6] = m;
+        __syncthreads();
+        m = most(most(part[0], part[1]), most(part[2], part[3]));
+    }
+    const RowScale s(m);
+    if (mine >= a.n) return;
+    if (lane == 0) a.scale[row] = s.scale;
+    int8_t *q = a.q + row * a.ld_q;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (u > 0 && u * G * VEC >= a.dim) break;
+        struct __attribute__((packed, aligned(1))) Bytes {
+            uint32_t w[VEC / 4];
+        } o;
+#pragma unroll
+        for (int w = 0; w < VEC / 4; ++w) {
+            o.w[w] = 0;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o.w[w] |= ((uint32_t)s.of(r.x[u * VEC + w * 4 + v]) & 0xffu) << (8 * v);
+            if (!s.usable()) o.w[w] = 0;
+        }
+        *reinterpret_cast<Bytes *>(q + S::base(u, lane, 0, a.dim)) = o;
+    }
+}
+
+// Rows longer than registers hold, or shorter than a vector: a workgroup per row, which is read twice.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_i8_any(RowsI8Args a) {
+    __shared__ uint32_t part[4];
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
         const typename T::Raw *x = (const typename T::Raw *)a.x + row * a.ld;
-        uint32_t m = 0;  // magnitudes as integers: an infinity is above every number and a NaN above it
-        for (int t = lane; t < a.dim; t += 64) m = max(m, __float_as_uint(T::up(x[t])) & 0x7fffffffu);
-        for (int o = 32; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-        const bool bad = m >= 0x7f800000u;
-        const float scale = bad ? __builtin_nanf("") : __uint_as_float(m) / 127.0f;
-        // small scales: both sides of the quotient times 2^60, exactly, so that the reciprocal is finite
-        const float up = scale < 0x1p-100f ? 0x1p60f : 1.0f, sc = scale * up, inv = 1.0f / sc;
-        for (int t = lane; t < a.dim; t += 64)
-            a.q[row * a.ld_q + t] = (int8_t)(scale > 0.0f ? nearest_i8(T::up(x[t]) * up, sc, inv) : 0);
-        if (lane == 0) a.scale[row] = scale;
+        uint32_t m = 0;
+        for (int t = threadIdx.x; t < a.dim; t += 256) m = max(m, magnitude(T::up(x[t])));
+        const auto most = [](uint32_t p, uint32_t q) { return p > q ? p : q; };
+        m = over_group<64>(m, 0u, most);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+        __syncthreads();
+        const RowScale s(most(most(part[0], part[1]), most(part[2], part[3])));
+        for (int t = threadIdx.x; t < a.dim; t += 256) a.q[row * a.ld_q + t] = (int8_t)(s.usable() ? s.of(T::up(x[t])) : 0);
+        if (threadIdx.x == 0) a.scale[row] = s.scale;
+        __syncthreads();
     }
 }
 

@@ -121,9 +121,27 @@ int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_
     bool go;
     VQ_TRY(admit(ctx, vq::check_rows_i8(type, d_x, n, ld, dim, d_q, ld_q, d_scale), n, &go));
     if (!go) return VQ_OK;
-    const vq::RowsI8Args a{d_x, n, ld, dim, d_q, ld_q, d_scale};
-    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_rows_i8<decltype(t)>, dim3((unsigned)std::min<int64_t>(cdiv64(n, 4), 1 << 20)), dim3(256), 0, ctx->stream, a); });
-    VQ_HIP(ctx, hipGetLastError());
+    const int e = vq::type_bytes(type);
+    const vq::LanePlan plan = vq::plan_lanes(dim, e);
+    const int64_t slice = (int64_t)1 << 23;  // rows per launch: a grid has fewer than 2^32 lanes
+    for (int64_t r = 0; r < n; r += slice) {
+        const vq::RowsI8Args a{(const char *)d_x + r * ld * e, std::min(slice, n - r), ld, dim, d_q + r * ld_q, ld_q, d_scale + r};
+        const auto grid = [&](int lanes) { return dim3((unsigned)cdiv64(a.n, 256 / lanes)); };
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            if (plan.lanes == 16)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 16, 1>), grid(16), dim3(256), 0, ctx->stream, a);
+            else if (plan.lanes == 64 && plan.vectors == 1)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 64, 1>), grid(64), dim3(256), 0, ctx->stream, a);
+            else if (plan.lanes == 64)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 64, 4>), grid(64), dim3(256), 0, ctx->stream, a);
+            else if (plan.lanes == 256)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 256, 8>), grid(256), dim3(256), 0, ctx->stream, a);
+            else
+                hipLaunchKernelGGL(vq::k_rows_i8_any<T>, dim3((unsigned)std::min<int64_t>(a.n, 1 << 20)), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
     return VQ_OK;
 }
 
@@ -183,10 +201,26 @@ int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, i
     VQ_TRY(admit(ctx, vq::check_code_logprobs_grad(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, d_max,
                                                    d_logsum, d_entropy, d_g_logprob, d_g_entropy, d_grad, ld_grad), n, &go));
     if (!go) return VQ_OK;
-    const vq::GradArgs a{d_scores, n, ld, k, beta, d_codes, code_stride, code_bytes, d_max, d_logsum, d_entropy, d_g_logprob,
-                         d_g_entropy, d_grad, ld_grad};
-    by_type(type, [&](auto t) { hipLaunchKernelGGL(vq::k_logprobs_grad<decltype(t)>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(256), 0, ctx->stream, a); });
-    VQ_HIP(ctx, hipGetLastError());
+    const int e = vq::type_bytes(type), vec = 16 / e;
+    const int64_t slice = (int64_t)1 << 23;  // rows per launch: a grid has fewer than 2^32 lanes
+    for (int64_t r = 0; r < n; r += slice) {
+        const auto at = [&](const float *p) { return p ? p + r : nullptr; };
+        const vq::GradArgs a{(const char *)d_scores + r * ld * e, std::min(slice, n - r), ld, k, beta,
+                             d_codes ? (const char *)d_codes + r * code_stride * code_bytes : nullptr, code_stride, code_bytes,
+                             at(d_max), at(d_logsum), at(d_entropy), at(d_g_logprob), at(d_g_entropy), (char *)d_grad + r * ld_grad * e, ld_grad};
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            if (k < vec)
+                hipLaunchKernelGGL(vq::k_logprobs_grad_tiny<T>, dim3((unsigned)cdiv64(a.n, 256)), dim3(256), 0, ctx->stream, a);
+            else if (k <= 64 * vec)
+                hipLaunchKernelGGL((vq::k_logprobs_grad<T, 16, 4>), dim3((unsigned)cdiv64(a.n, 16)), dim3(256), 0, ctx->stream, a);
+            else if (k <= 256 * vec)
+                hipLaunchKernelGGL((vq::k_logprobs_grad<T, 64, 4>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
+            else
+                hipLaunchKernelGGL((vq::k_logprobs_grad<T, 256, 4>), dim3((unsigned)a.n, (unsigned)cdiv64(k, 1024 * vec)), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
     return VQ_OK;
 }
 
