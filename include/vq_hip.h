@@ -429,8 +429,7 @@ int32_t vq_tsvq_quantize_host(vq_ctx *ctx, int32_t metric, const float *h_x, int
  * one of k centroids (or any k codes that a model answers with), and what is read from scores.  No counterpart in the
  * reference.  All four are asynchronous, run on the context's stream and use no buffer of the context except where
  * stated; sizes of zero rows return VQ_OK and touch nothing; what lies between rows or behind the last one is left as it is.
- * Any stride and any address that is a multiple of the element's size will do; 8-bit rows are fastest at
- * 16-byte aligned addresses and strides that are multiples of 16. */
+ * Any stride and any address that is a multiple of the element's size will do. */
 
 /* Rows to 8-bit integers with a scale each: d_scale[i] = max_t |x[i][t]| / 127, rounded to binary32;
  * d_q[i][t] = the integer nearest to x[i][t] / d_scale[i] (the exact quotient, ties to even), -127 to 127.
@@ -442,7 +441,10 @@ int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_
 /* d_out[i*ld_out + j] = (sum_t d_x[i][t] * d_w[j][t]) * d_xs[i] * d_ws[j] + d_bias[j], n rows against k codes: the sum
  * exact in 32-bit integers, the rest in f32, rounded to out_type.  d_bias may be NULL.  With the bias -|c_j|^2 / 2 of codewords c_j the
  * order of a row's scores is that of the squared Euclidean distance, nearest first (up to the 8-bit rounding).
- * dim <= 131071, k <= 2^24; d_x rows are ld_x bytes apart, d_w rows ld_w.  The scores may not overlap an input. */
+ * dim <= 131071, k <= 2^24; d_x rows are ld_x bytes apart, d_w rows ld_w.  The scores may not overlap an input.
+ * Fastest where addresses and strides of d_x and d_w are multiples of 16.  The last row is then read up to the next multiple of 16 bytes; what
+ * lies behind component dim counts for nothing.  Large calls on other rows copy them to aligned ones in a buffer of the context, which
+ * grows and is kept like that of vq_code_logprobs below, and captures need an earlier call alike. */
 int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t n, int64_t ld_x, const int8_t *d_w,
                      const float *d_ws, int32_t k, int64_t ld_w, int32_t dim, const float *d_bias, int32_t out_type,
                      void *d_out, int64_t ld_out);

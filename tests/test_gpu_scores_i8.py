@@ -121,6 +121,12 @@ def test_scores_any_place(ctx, kind, n, dim, k):
     _scores(ctx, rng, n, dim, k, kind, ldx=16, ldw=5, ldo=3, offset=5)
 
 
+@pytest.mark.parametrize("ldx,ldw,offset", [(1, 0, 0), (-1037 % 16, 3, 0), (0, -1037 % 16, 0), (-1037 % 16, -1037 % 16, 4), (7, 9, 1)])
+def test_scores_copied_to_aligned_rows(ctx, ldx, ldw, offset):
+    """More than 2^28 to multiply: rows, codes or both at strides or addresses that are not aligned."""
+    _scores(ctx, np.random.default_rng(6), 520, 1037, 530, "f32", ldx=ldx, ldw=ldw, offset=offset)
+
+
 @pytest.mark.parametrize("n,dim,k", [(1, 131071, 5), (20, 131071, 20), (200, 131071, 130)])
 def test_scores_longest_rows(ctx, n, dim, k):
     """The largest sums there are: 131,071 products of -128 with itself, 1023 below 2^31."""

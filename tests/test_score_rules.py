@@ -20,6 +20,10 @@ int scores(i64 x, i64 xs, i64 n, i64 ldx, i64 w, i64 ws, int k, i64 ldw, int dim
 int logprobs(int type, i64 s, i64 n, i64 ld, int k, float beta, int cb, i64 c, i64 cs, int top, i64 lp, i64 m, i64 l, i64 h, i64 tl, i64 tc) {
     return vq::check_code_logprobs(type, P(s), n, ld, k, beta, cb, P(c), cs, top, P(lp), P(m), P(l), P(h), P(tl), P(tc)).status; }
 int plan(i64 n, int k, i64 *out) { const vq::RowPlan p = vq::plan_rows(n, k); out[0] = p.lanes, out[1] = p.per_lane, out[2] = p.parts, out[3] = p.codes; return 0; }
+int way(i64 n, int k, int dim) { return vq::score_way(n, k, dim); }
+i64 launch_rows(int k) { return vq::score_rows_of_a_launch(k); }
+int pack(i64 n, int k, int dim) { return vq::score_pack(n, k, dim); }
+int lanes(int length, int bytes) { const vq::LanePlan p = vq::plan_lanes(length, bytes); return p.lanes * p.vectors * 16 / bytes; }
 int grad(int type, i64 s, i64 n, i64 ld, int k, float beta, int cb, i64 c, i64 cs, i64 m, i64 l, i64 h, i64 gl, i64 gh, i64 g, i64 ldg) {
     return vq::check_code_logprobs_grad(type, P(s), n, ld, k, beta, cb, P(c), cs, P(m), P(l), P(h), P(gl), P(gh), P(g), ldg).status; }
 }
@@ -101,6 +105,36 @@ def test_every_code_of_a_row_has_a_lane(lib):
             assert codes <= lanes * per_lane and parts * codes >= k and (parts - 1) * codes < k and (parts == 1 or (lanes == 256 and codes % 64 == 0))
             assert parts <= 64
             assert lanes in (1, 4, 16, 64, 256) and per_lane in ((16,) if lanes < 256 else (8, 16, 32, 64))
+
+
+def test_tiles_fit_their_launches(lib):
+    """Rows and codes of a workgroup, and its lanes, by way: a grid has fewer than 2^32 lanes and at most 65,535 workgroups in its
+    second dimension, which k_scores_any and FEW use for the rows."""
+    lib.way.argtypes, lib.launch_rows.argtypes, lib.launch_rows.restype = [C.c_longlong, C.c_int, C.c_int], [C.c_int], C.c_longlong
+    lib.pack.argtypes = [C.c_longlong, C.c_int, C.c_int]
+    size = [(16, 16, 256), (64, 64, 256), (64, 64, 256), (64, 128, 512), (128, 128, 512), (256, 256, 512), (128, 128, 512)]
+    seen = set()
+    for k in [1, 2, 16, 24, 64, 65, 127, 128, 129, 256, 777, 1024, 4096, 65536, 262144, 1 << 24]:
+        most = lib.launch_rows(k)
+        assert most >= 64 and most % 64 == 0 and most // 64 <= 65535 and most // 64 * -(-k // 64) * 256 < 1 << 32
+        for n in [1, 2, 16, 17, 64, 65, 128, 129, 300, 1000, 4099, 16384, 100_000, most - 1, most]:
+            for dim in (1, 128, 8192, 131071):
+                if n <= most:
+                    w = lib.way(n, k, dim)
+                    rows, codes, wg = size[w]
+                    tiles = -(-n // rows) * -(-k // codes)
+                    assert tiles * wg < 1 << 32 and (w or -(-n // 16) <= 65535)
+                    seen.add(w)
+                if lib.pack(n, k, dim):
+                    assert k * (dim + 15) <= (1 << 30) + 15 * k and n * k * dim >= 1 << 28
+    assert seen == set(range(7))
+
+
+def test_rows_in_registers(lib):
+    for size in (2, 4):
+        for length in [1, 3, 4, 7, 8, 64, 65, 128, 129, 512, 513, 1024, 1025, 2048, 2049, 8192, 8193, 16384, 16385, 131071]:
+            held = lib.lanes(length, size)
+            assert held >= length if 16 // size <= length <= 2048 * 16 // size else held == 0
 
 
 def test_a_missing_context_is_an_error():

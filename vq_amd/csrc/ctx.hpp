@@ -86,9 +86,9 @@ struct vq_ctx {
     // the LBG's assignment, sort keys in and out, the sort's workspace, per-cluster tables, flags
     DevBuf big_chunk, big_win, big_wind, big_best, big_fresh, big_codes, big_keys, big_sorted, big_sort_tmp, big_tables,
         big_flags;
-    // parts of long rows of scores; what it was before it grew stays until the context ends, since captured
-    // graphs may hold its address
-    DevBuf score_parts;
+    // parts of long rows of scores, and aligned copies of 8-bit rows; what they were before they grew stays until the
+    // context ends, since captured graphs may hold the addresses
+    DevBuf score_parts, score_packed;
     std::vector<void *> outgrown;
     uint32_t scores_lds_set = 0;  // dynamic-LDS limit granted to the tiles of scores, a bit per instance
     // optional per-kernel-class timing (HIP events on the stream)

@@ -357,7 +357,7 @@ __device__ __forceinline__ void part_best(S64 &r, const float (&vmax)[S64::E / S
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
     typedef Share<T, 256, NV> S64;
-    constexpr int E = S64::E, VEC = S64::VEC;
+    constexpr int VEC = S64::VEC;
     __shared__ PartLds l;
     const LogprobArgs &a = p.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;

@@ -165,15 +165,40 @@ inline RowPlan plan_rows(int64_t n, int32_t k) {
     return {256, e, (k + codes - 1) / codes, codes};
 }
 
-// Scores: 8-bit rows at aligned addresses and strides go through tiles of 256 x 256, 128 x 128 or 64 x 64 rows and codes, the largest that
-// leave 256 of them (one per compute unit) to the call; others through k_scores_any (0).
+// How scores of aligned 8-bit rows are made (microseconds at n x dim x k, bf16 results, of the kernels compared):
+//   FEW        16 x 16 per workgroup, the components shared out among its waves: up to 32 tiles of 64 x 64, or 16 rows and 256 of them
+//              (32 x 4096 x 1024 6.0, T64 9.1; 14 x 3136 x 9152 8.4 and 9.3; 600 x 6000 x 600 25 and 17)
+//   T64        64 x 64, 256 components per barrier, four steps in flight: one workgroup per compute unit at most
+//              (1024 x 4096 x 1024 10.7, T64_MANY 17.6, T128 18.5)
+//   T64_MANY   64 x 64, 128 components per barrier, two steps: several workgroups per compute unit, where 128 codes would be half
+//              empty (84,654 x 188 x 24 8.7, T64_128 11.4, T128_MANY 10.8)
+//   T64_128    64 rows x 128 codes, three steps: where they leave a compute unit one workgroup (1200 x 2000 x 1200 10.1, T64 14.6,
+//              T128 13.5), and up to 64 rows (64 x 1280 x 65,536 19.8, T64_MANY 22.9, T128_MANY 21.3)
+//   T128       128 x 128, four steps: one workgroup per compute unit (4099 x 1000 x 777 11.4, T64_MANY 13.1, T128_MANY 12.0)
+//   T256       256 x 256: two per compute unit and more than 256 components, or one and many steps (8192 x 8192 x 8192 469,
+//              T128_MANY 536; 4096 x 4096 x 4096 66 and 79; 100,000 x 384 x 1024 107 and 116)
+//   T128_MANY  128 x 128, two steps, several workgroups per compute unit: the others (1247 x 27 x 16,682 16.4, T256 20.4;
+//              1M x 128 x 256 173 and 179; 100,000 x 128 x 256 20.6 and 24.1)
 // Places within a tile's rows are counted in 32 bits: strides up to 2^22.
+enum ScoreWay { FEW, T64, T64_MANY, T64_128, T128, T256, T128_MANY };
 constexpr int64_t kMaxTileStride = 1 << 22;
-inline int score_tile(int64_t n, int32_t k, bool aligned) {
-    if (!aligned) return 0;
-    for (int t : {256, 128})
-        if (((n + t - 1) / t) * ((k + t - 1) / t) >= 256) return t;
-    return 64;
+inline ScoreWay score_way(int64_t n, int32_t k, int32_t dim) {
+    const auto tiles = [&](int r, int c) { return ((n + r - 1) / r) * ((k + c - 1) / c); };
+    if (tiles(64, 64) <= 32 || (n <= 16 && tiles(64, 64) <= 256)) return FEW;
+    if (tiles(64, 64) <= 256) return T64;
+    if (k <= 64) return T64_MANY;
+    if (n <= 64 || tiles(64, 128) <= 256) return T64_128;
+    if (tiles(128, 128) <= 256) return T128;
+    if (n > 128 && ((tiles(256, 256) >= 512 && dim > 256) || (tiles(256, 256) >= 256 && dim >= 1024))) return T256;
+    return T128_MANY;
+}
+// Rows at other addresses or strides: through k_scores_any, which takes them as they are; where there is more than 2^28 to
+// multiply and 32 rows and codes or more, they are copied to aligned rows first (4096 x 4099 x 4096 at a stride of 4099 282 us, 90 so),
+// up to 1 GiB of codes, and of rows as many at a time as make 512 MiB.
+constexpr int64_t kPackRows = 512 << 20, kPackCodes = 1 << 30;
+inline int64_t packed_stride(int32_t dim) { return (dim + 15) / 16 * 16; }
+inline bool score_pack(int64_t n, int32_t k, int32_t dim) {
+    return n >= 32 && k >= 32 && k * packed_stride(dim) <= kPackCodes && (double)n * k * dim >= 0x1p28;
 }
 // Rows of a launch: fewer than 2^22 tiles of 64 x 64, and no more tiles of rows than a grid's second dimension holds.
 inline int64_t score_rows_of_a_launch(int32_t k) {

@@ -2,6 +2,8 @@
 //
 // This translation unit must be compiled with -ffp-contract=off.
 #pragma once
+#include <algorithm>
+
 #include "logprobs.hpp"
 
 namespace vq {
@@ -125,16 +127,22 @@ struct ScoresArgs {
 };
 
 // 16 bytes of a row from component t on, zeros beyond the row; any alignment.
+struct __attribute__((packed, aligned(1))) Bytes16 {
+    i32x4 v;
+};
 __device__ __forceinline__ i32x4 piece16(const int8_t *row, int t, int dim) {
-    if (t + 16 <= dim && (((uintptr_t)(row + t)) & 15) == 0) return *reinterpret_cast<const i32x4 *>(row + t);
-    union {
-        i32x4 v;
-        int8_t b[16];
-    } u;
-    u.v = i32x4{0, 0, 0, 0};
+    if (t + 16 <= dim) return reinterpret_cast<const Bytes16 *>(row + t)->v;
+    i32x4 v = {0, 0, 0, 0};
+#pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (t + i < dim) u.b[i] = row[t + i];
-    return u.v;
+        if (t + i < dim) v[i >> 2] |= (int32_t)((uint32_t)(uint8_t)row[t + i] << (8 * (i & 3)));
+    return v;
+}
+
+// Rows to rows of whole 16 bytes, zeros behind their components: a piece per lane.
+__global__ void __launch_bounds__(256) k_pack_i8(const int8_t *__restrict__ x, int64_t n, int64_t ld, int dim, int8_t *__restrict__ to) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per_row = (dim + 15) / 16, row = at / per_row;
+    if (row < n) reinterpret_cast<i32x4 *>(to)[at] = piece16(x + row * ld, (int)(at - row * per_row) * 16, dim);
 }
 
 // 64 rows x 64 codes per workgroup, operands staged through LDS in steps of 64 components, for any stride and
@@ -201,13 +209,19 @@ __device__ __forceinline__ void copy_to_lds(const int8_t *base, int bytes, char 
 #endif
 }
 
-// Everyone's copies into LDS are there, and what everyone read from it.
-__device__ __forceinline__ void step_barrier() {
+// Everyone's copies into LDS but for each wave's last LEFT are there, and what everyone read from it.
+template <int LEFT> __device__ __forceinline__ void step_barrier() {
+    static_assert(LEFT < 64, "the counter has six bits");
     asm volatile("" ::: "memory");  // (the compiler moves no access across)
-    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (LEFT & 15) | (LEFT >> 4) << 14);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+
+// Where in its 128 bytes a row has a piece of 16 (and which piece lies at a place): 16 rows' same pieces, two rows to a line of the 64 banks,
+// meet every bank once.  (By the row's lowest three bits, two and two in the same banks, half of the time in LDS was lost: 104M of
+// 212M cycles over the compute units at 16,384 x 8192 against 8192 codes, now 3M of 111M.)
+__device__ __forceinline__ int piece_place(int row, int piece) { return (piece ^ (row >> 1 & 7)) * 16; }
 
 // TR rows x TC codes by WR x WC waves, each TR / WR rows x TC / WC codes in blocks of 32 x 32.  The operands come in steps of 128
 // components straight into LDS, the next step's on their way while a step is worked on; one barrier per step.  A row of a step
@@ -217,41 +231,51 @@ __device__ __forceinline__ void step_barrier() {
 // are somebody's data: they are cleared in the rows of x before the last step is worked on, and count for nothing in w then.
 // The codes are the first operand: a lane ends with runs of four codes of a row, scales them, and the tile leaves through LDS in whole lines.
 // Aligned rows only (address and stride multiples of 16).
-template <typename OutT, int TR, int TC, int WR, int WC>
-__global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint32_t row_tiles, uint32_t code_tiles) {
-    constexpr int NW = WR * WC, R = TR / WR / 32, C = TC / WC / 32, XI = TR / 8 / NW, WI = TC / 8 / NW, STAGE = (TR + TC) * 128;
+template <typename OutT, int TR, int TC, int WR, int WC, int KS, int STAGES>
+__global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint32_t row_tiles, uint32_t code_tiles, int lds_bytes) {
+    constexpr int NW = WR * WC, R = TR / WR / 32, C = TC / WC / 32, XI = TR / 8 / NW, WI = TC / 8 / NW, HALF = (TR + TC) * 128, STAGE = KS * HALF, STEP = KS * 128;
     static_assert(XI * 8 * NW == TR && WI * 8 * NW == TC && R * 32 * WR == TR && C * 32 * WC == TC, "whole blocks");
     typedef typename OutT::Raw Raw;
     extern __shared__ __attribute__((aligned(1024))) char tile_lds[];
-    float *lws = reinterpret_cast<float *>(tile_lds + 2 * STAGE), *lbias = lws + TC;
+    constexpr int LINE = C * 32 * (int)sizeof(Raw), PITCH = LINE + 16, PIECES = LINE / 16;  // of a block of rows on its way out
+    float *lws = reinterpret_cast<float *>(tile_lds + lds_bytes), *lbias = lws + TC;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / WC, wc = wave % WC;
     const TilePlace place = tile_place(blockIdx.x, row_tiles, code_tiles);
     const int64_t row0 = place.r * TR;
     const int code0 = place.c * TC, rows = (int)min((int64_t)TR, a.n - row0), codes = min(TC, a.k - code0);
-    const int steps = (a.dim + 127) / 128, dim16 = (a.dim + 15) & ~15;
+    const int steps = (a.dim + STEP - 1) / STEP, dim16 = (a.dim + 15) & ~15;
     const int8_t *px = a.x + row0 * a.ld_x, *pw = a.w + (int64_t)code0 * a.ld_w;
     const int ldx = (int)a.ld_x, ldw = (int)a.ld_w, left_x = (rows - 1) * ldx + dim16, left_w = (codes - 1) * ldw + dim16;
-    const int l8 = lane >> 3;
-    const int swz = l8, chunk = ((lane & 7) ^ swz) * 16;
     int vx[XI], vw[WI];
 #pragma unroll
-    for (int i = 0; i < XI; ++i) vx[i] = ((wave * XI + i) * 8 + l8) * ldx + chunk;
+    for (int i = 0; i < XI; ++i) {
+        const int row = (wave * XI + i) * 8 + (lane >> 3);
+        vx[i] = row * ldx + piece_place(row, lane & 7);
+    }
 #pragma unroll
-    for (int i = 0; i < WI; ++i) vw[i] = ((wave * WI + i) * 8 + l8) * ldw + chunk;
+    for (int i = 0; i < WI; ++i) {
+        const int row = (wave * WI + i) * 8 + (lane >> 3);
+        vw[i] = row * ldw + piece_place(row, lane & 7);
+    }
     const auto bring = [&](int step, int buf) {
-        char *to = tile_lds + buf * STAGE;
 #pragma unroll
-        for (int i = 0; i < XI; ++i)
-            copy_to_lds(px + step * 128, left_x - step * 128, to + (wave * XI + i) * 1024, vx[i]);
+        for (int kb = 0; kb < KS; ++kb) {
+            const int at = step * STEP + kb * 128;
+            char *to = tile_lds + buf * STAGE + kb * HALF;
+            const bool any = KS == 1 || at < dim16;  // else nothing is read, and LDS gets zeros
 #pragma unroll
-        for (int i = 0; i < WI; ++i)
-            copy_to_lds(pw + step * 128, left_w - step * 128, to + TR * 128 + (wave * WI + i) * 1024, vw[i]);
+            for (int i = 0; i < XI; ++i) copy_to_lds(px + at, any ? left_x - at : 0, to + (wave * XI + i) * 1024, vx[i]);
+#pragma unroll
+            for (int i = 0; i < WI; ++i) copy_to_lds(pw + at, any ? left_w - at : 0, to + TR * 128 + (wave * WI + i) * 1024, vw[i]);
+        }
     };
-    bring(0, 0);
     for (int j = tid; j < TC; j += 64 * NW) {
         lws[j] = j < codes ? a.ws[code0 + j] : 0.0f;
         lbias[j] = a.bias && j < codes ? a.bias[code0 + j] : 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (i < steps) bring(i, i);
     i32x16 acc[R][C];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -262,22 +286,25 @@ __global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint
     const int l32 = lane & 31, h = lane >> 5;
     int off[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + (((2 * s + h) ^ (l32 & 7)) * 16);
+    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + piece_place(l32, 2 * s + h);
+    int buf = 0;  // step % STAGES
     for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1;
-        step_barrier();
-        if (step + 1 < steps) bring(step + 1, buf ^ 1);
+        if (step + STAGES - 1 <= steps)
+            step_barrier<(STAGES - 2) * KS * (XI + WI)>();
+        else
+            step_barrier<0>();
+        if (step + STAGES - 1 < steps) bring(step + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);  // where the step before lay
         char *at = tile_lds + buf * STAGE;
-        if (step + 1 == steps && (a.dim & 127)) {  // uniform
-            const int t0 = a.dim & 127;
-            for (int i = tid; i < TR * 8; i += 64 * NW) {
-                const int row = i >> 3, p = (i & 7) * 16;  // the piece of components p to p + 15
-                if (p + 16 > t0) {
-                    i32x4 *v = reinterpret_cast<i32x4 *>(at + row * 128 + ((i & 7) ^ (row & 7)) * 16);
+        buf = buf + 1 == STAGES ? 0 : buf + 1;
+        if (step + 1 == steps && a.dim % STEP) {  // uniform
+            for (int i = tid; i < KS * TR * 8; i += 64 * NW) {
+                const int kb = i / (TR * 8), row = i / 8 % TR, p = step * STEP + kb * 128 + (i & 7) * 16;  // the piece of components p to p + 15
+                if (p + 16 > a.dim) {
+                    i32x4 *v = reinterpret_cast<i32x4 *>(at + kb * HALF + row * 128 + piece_place(row, i & 7));
                     i32x4 x = *v;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int keep = min(max(t0 - p - 4 * q, 0), 4);
+                        const int keep = min(max(a.dim - p - 4 * q, 0), 4);
                         x[q] = keep == 4 ? x[q] : x[q] & ((1 << (8 * keep)) - 1);
                     }
                     *v = x;
@@ -286,23 +313,32 @@ __global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint
             __syncthreads();
         }
         const char *ax = at + wr * (R * 32 * 128), *aw = at + TR * 128 + wc * (C * 32 * 128);
+        i32x4 fx[2][R], fw[2][C];  // of a quarter of the step, and of the next
+        const auto read = [&](int s) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            i32x4 fx[R], fw[C];
+            for (int c = 0; c < C; ++c) fw[s & 1][c] = *reinterpret_cast<const i32x4 *>(aw + (s >> 2) * HALF + c * 4096 + off[s & 3]);
 #pragma unroll
-            for (int c = 0; c < C; ++c) fw[c] = *reinterpret_cast<const i32x4 *>(aw + c * 4096 + off[s]);
+            for (int r = 0; r < R; ++r) fx[s & 1][r] = *reinterpret_cast<const i32x4 *>(ax + (s >> 2) * HALF + r * 4096 + off[s & 3]);
+        };
+        read(0);
 #pragma unroll
-            for (int r = 0; r < R; ++r) fx[r] = *reinterpret_cast<const i32x4 *>(ax + r * 4096 + off[s]);
+        for (int s = 0; s < 4 * KS; ++s) {
+            if (s + 1 < 4 * KS) read(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int c = 0; c < C; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c], fx[r], acc[r][c], 0, 0, 0);
+                for (int c = 0; c < C; ++c)
+                    acc[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s & 1][c], fx[s & 1][r], acc[r][c], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    step_barrier();  // LDS is free
-    constexpr int LINE = C * 32 * (int)sizeof(Raw), PITCH = LINE + 16, PIECES = LINE / 16;
-    static_assert(NW * 32 * PITCH <= 2 * STAGE, "a block of rows per wave fits");
+    step_barrier<0>();  // LDS is free
     char *mine = tile_lds + wave * (32 * PITCH);
+    // Whole lines of 128 bytes pass the caches (16,384 x 512 x 16,384 to f32 367 -> 285 us, 100,000 x 384 x 1024 142 -> 103); parts of
+    // lines would each cost memory a line (1M x 128 x 256 to bf16 with 64 bytes per wave and row 172 -> 190, 3000 x 300 x 3000, whose
+    // rows end inside lines, 15.7 -> 19.8).
+    const bool past = ((uintptr_t)a.out & 127) == 0 && a.ld_out % (128 / (int)sizeof(Raw)) == 0;
     const int wcode = code0 + wc * (C * 32);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -331,16 +367,105 @@ __global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint
             const i32x4 v = *reinterpret_cast<const i32x4 *>(mine + row * PITCH + piece * 16);
             if (brow + row < a.n && code < a.k) {
                 Raw *to = (Raw *)a.out + (brow + row) * a.ld_out + code;
-                if (code + 16 / (int)sizeof(Raw) <= a.k)
-                    *reinterpret_cast<Piece *>(to) = __builtin_bit_cast(Piece, v);
-                else
-                    for (int e = 0; e < 16 / (int)sizeof(Raw); ++e)
+                if (code + 16 / (int)sizeof(Raw) > a.k)
+                    for (int e = 0; e < 16 / (int)sizeof(Raw); ++e) {
                         if (code + e < a.k) to[e] = reinterpret_cast<const Raw *>(mine + row * PITCH + piece * 16)[e];
+                    }
+                else if (LINE >= 128 && past)
+                    __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>(to));
+                else
+                    *reinterpret_cast<Piece *>(to) = __builtin_bit_cast(Piece, v);
             }
         }
         wave_sync();
     }
 }
-constexpr int tile_lds_bytes(int tr, int tc) { return 2 * (tr + tc) * 128 + tc * 8; }
+// LDS of a workgroup below its codes' scales and biases (8 bytes each): the steps in flight, or a block of rows per wave on its way
+// out.  Short rows have fewer steps than are provided for; more workgroups share a compute unit then.
+inline int tile_lds_bytes(int tr, int tc, int waves, int waves_c, int ks, int stages, int dim, int bytes) {
+    const int steps = std::min(stages, (dim + ks * 128 - 1) / (ks * 128));
+    return std::max(steps * ks * (tr + tc) * 128, waves * 32 * (tc / waves_c * bytes + 16));
+}
+
+// ---- few tiles: the components shared out among the waves -------------------------------------------------
+// A workgroup makes RB * 16 rows x CB * 16 codes, each of its KW waves from every KW-th run of 128 components, straight from memory into the
+// operands' registers, the next run on its way; the waves' sums meet in LDS.  16 rows of 64 consecutive bytes per read.  Rows and
+// codes behind the last are read as the last; components behind `dim` count as zero in x.  Aligned rows only.
+template <typename OutT, int RB, int CB, int KW>
+__global__ void __launch_bounds__(64 * KW) k_scores_few(ScoresArgs a) {
+    constexpr int TR = RB * 16, TC = CB * 16, PITCH = TC + 4;
+    typedef typename OutT::Raw Raw;
+    __shared__ __attribute__((aligned(16))) int32_t sums[KW][TR][PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, h = lane >> 4;
+    const int64_t row0 = (int64_t)blockIdx.y * TR;
+    const int code0 = blockIdx.x * TC;
+    const int8_t *px[RB], *pw[CB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) px[r] = a.x + min(row0 + r * 16 + l16, a.n - 1) * a.ld_x;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) pw[c] = a.w + (int64_t)min(code0 + c * 16 + l16, a.k - 1) * a.ld_w;
+    i32x4 acc[RB][CB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[r][c] = i32x4{0, 0, 0, 0};
+    struct Run {
+        i32x4 x[RB][2], w[CB][2];
+    };
+    const auto bring = [&](Run &f, int t0) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int t = t0 + s * 64 + h * 16, at = t < a.dim ? t : 0;  // (what is behind the row counts for nothing)
+#pragma unroll
+            for (int c = 0; c < CB; ++c) f.w[c][s] = *reinterpret_cast<const i32x4 *>(pw[c] + at);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) f.x[r][s] = *reinterpret_cast<const i32x4 *>(px[r] + at);
+        }
+    };
+    const auto use = [&](Run &f, int t0) {
+        if (t0 + 128 > a.dim) {  // uniform
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int keep = min(max(a.dim - (t0 + s * 64 + h * 16 + 4 * q), 0), 4);
+                    const int mask = keep == 4 ? -1 : (1 << (8 * keep)) - 1;
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) f.x[r][s][q] &= mask;
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int c = 0; c < CB; ++c) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[c][s], f.x[r][s], acc[r][c], 0, 0, 0);
+    };
+    Run f[2];
+    int t = wave * 128;
+    if (t < a.dim) bring(f[0], t);
+    for (; t < a.dim; t += KW * 256) {
+        if (t + KW * 128 < a.dim) bring(f[1], t + KW * 128);
+        use(f[0], t);
+        if (t + KW * 256 < a.dim) bring(f[0], t + KW * 256);
+        if (t + KW * 128 < a.dim) use(f[1], t + KW * 128);
+    }
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int c = 0; c < CB; ++c) *reinterpret_cast<i32x4 *>(&sums[wave][r * 16 + l16][c * 16 + h * 4]) = acc[r][c];
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < TR * TC; i += 64 * KW) {
+        const int row = i / TC, j = i % TC;
+        int32_t sum = 0;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) sum += sums[w][row][j];
+        if (row0 + row < a.n && code0 + j < a.k) {
+            const float y = (float)sum * a.xs[row0 + row] * a.ws[code0 + j];
+            ((Raw *)a.out)[(row0 + row) * a.ld_out + code0 + j] = OutT::down(a.bias ? y + a.bias[code0 + j] : y);
+        }
+    }
+}
 
 }  // namespace vq

@@ -33,29 +33,51 @@ template <typename F> void by_type(int32_t type, F f) {
 }
 
 // One launch of tiles; the limit of the LDS above 64 KB is asked for once per context and instance.
-template <typename T, int TR, int TC, int WR, int WC> int32_t score_tiles(vq_ctx *ctx, const vq::ScoresArgs &a, int bit) {
-    constexpr int lds = vq::tile_lds_bytes(TR, TC);
-    const auto kernel = vq::k_scores_tile<T, TR, TC, WR, WC>;
-    if (lds > 65536 && !(ctx->scores_lds_set >> bit & 1)) {
-        VQ_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+template <typename T, int TR, int TC, int WR, int WC, int KS, int STAGES> int32_t score_tiles(vq_ctx *ctx, const vq::ScoresArgs &a, int bit) {
+    static_assert(WR * WC * 32 * (TC / WC * (int)sizeof(typename T::Raw) + 16) <= STAGES * KS * (TR + TC) * 128, "blocks on their way out fit into the steps' LDS");
+    const int lds = vq::tile_lds_bytes(TR, TC, WR * WC, WC, KS, STAGES, a.dim, (int)sizeof(typename T::Raw));
+    const auto kernel = vq::k_scores_tile<T, TR, TC, WR, WC, KS, STAGES>;
+    if (lds + TC * 8 > 65536 && !(ctx->scores_lds_set >> bit & 1)) {
+        VQ_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        STAGES * KS * (TR + TC) * 128 + TC * 8));
         ctx->scores_lds_set |= 1u << bit;
     }
     const uint32_t rt = (uint32_t)cdiv64(a.n, TR), ct = (uint32_t)cdiv64(a.k, TC);
-    hipLaunchKernelGGL(kernel, dim3(rt * ct), dim3(64 * WR * WC), lds, ctx->stream, a, rt, ct);
+    hipLaunchKernelGGL(kernel, dim3(rt * ct), dim3(64 * WR * WC), lds + TC * 8, ctx->stream, a, rt, ct, lds);
     VQ_HIP(ctx, hipGetLastError());
     return VQ_OK;
 }
 
-template <typename T> int32_t scores_slice(vq_ctx *ctx, const vq::ScoresArgs &a, int type, int way) {
-    switch (way) {
-    case 256: return score_tiles<T, 256, 256, 2, 4>(ctx, a, type * 4);
-    case 128: return score_tiles<T, 128, 128, 2, 2>(ctx, a, type * 4 + 1);
-    case 64: return score_tiles<T, 64, 64, 2, 2>(ctx, a, type * 4 + 2);
-    default:
+// aligned: addresses and strides are multiples of 16, and the strides at most kMaxTileStride.
+template <typename T> int32_t scores_slice(vq_ctx *ctx, const vq::ScoresArgs &a, int type, bool aligned) {
+    if (!aligned) {
         hipLaunchKernelGGL(vq::k_scores_any<T>, dim3(cdiv(a.k, 64), cdiv(a.n, 64)), dim3(256), 0, ctx->stream, a);
         VQ_HIP(ctx, hipGetLastError());
         return VQ_OK;
     }
+    const vq::ScoreWay way = vq::score_way(a.n, a.k, a.dim);
+    const int bit = type * 8 + way;
+    constexpr int WC = sizeof(typename T::Raw) == 4 ? 4 : 2;  // waves side by side: a wave's codes of a row are 128 bytes of results
+    switch (way) {
+    case vq::FEW:
+        hipLaunchKernelGGL((vq::k_scores_few<T, 1, 1, 4>), dim3(cdiv(a.k, 16), cdiv(a.n, 16)), dim3(256), 0, ctx->stream, a);
+        VQ_HIP(ctx, hipGetLastError());
+        return VQ_OK;
+    case vq::T64: return score_tiles<T, 64, 64, 2, 2, 2, 4>(ctx, a, bit);
+    case vq::T64_MANY: return score_tiles<T, 64, 64, 2, 2, 1, 2>(ctx, a, bit);
+    case vq::T64_128: return score_tiles<T, 64, 128, 2, WC, 1, 3>(ctx, a, bit);
+    case vq::T128: return score_tiles<T, 128, 128, 8 / WC, WC, 1, 4>(ctx, a, bit);
+    case vq::T256: return score_tiles<T, 256, 256, 2, 4, 1, 2>(ctx, a, bit);
+    default: return score_tiles<T, 128, 128, 8 / WC, WC, 1, 2>(ctx, a, bit);
+    }
+}
+
+// n 8-bit rows to aligned ones.
+int32_t pack_i8(vq_ctx *ctx, const int8_t *x, int64_t n, int64_t ld, int32_t dim, int8_t *to) {
+    const int64_t pieces = n * (vq::packed_stride(dim) / 16);
+    hipLaunchKernelGGL(vq::k_pack_i8, dim3((unsigned)cdiv64(pieces, 256)), dim3(256), 0, ctx->stream, x, n, ld, dim, to);
+    VQ_HIP(ctx, hipGetLastError());
+    return VQ_OK;
 }
 
 template <typename T, bool TINY, int G> void short_rows(vq_ctx *ctx, const vq::LogprobArgs &a) {
@@ -152,18 +174,34 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
     bool go;
     VQ_TRY(admit(ctx, vq::check_scores_i8(d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, out_type, d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
-    const bool aligned = !vq::misaligned(d_x, 16) && !vq::misaligned(d_w, 16) && ld_x % 16 == 0 && ld_w % 16 == 0 && ld_x <= vq::kMaxTileStride &&
-                         ld_w <= vq::kMaxTileStride;
+    const auto fit = [](const void *p, int64_t ld) { return !vq::misaligned(p, 16) && ld % 16 == 0 && ld <= vq::kMaxTileStride; };
+    bool ready_x = fit(d_x, ld_x), ready_w = fit(d_w, ld_w);
     vq::ScoresArgs a{d_x, d_xs, n, ld_x, d_w, d_ws, k, ld_w, dim, d_bias, d_out, ld_out};
-    const int64_t slice = vq::score_rows_of_a_launch(k);
+    int64_t slice = vq::score_rows_of_a_launch(k);
+    int8_t *packed_x = nullptr;
+    if (!(ready_x && ready_w) && vq::score_pack(n, k, dim)) {
+        const int64_t ld = vq::packed_stride(dim);
+        if (!ready_x) slice = std::min(slice, std::max<int64_t>(64, vq::kPackRows / ld / 64 * 64));
+        const int64_t rows = ready_x ? 0 : std::min(n, slice);
+        VQ_TRY(ensure_kept(ctx, ctx->score_packed, (size_t)((rows + (ready_w ? 0 : k)) * ld)));
+        int8_t *to = (int8_t *)ctx->score_packed.p;
+        if (!ready_w) {
+            VQ_TRY(pack_i8(ctx, d_w, k, ld_w, dim, to));
+            a.w = to, a.ld_w = ld, ready_w = true;
+        }
+        if (!ready_x) packed_x = to + (a.w == to ? k * ld : 0), a.ld_x = ld, ready_x = true;
+    }
     for (int64_t r = 0; r < n; r += slice) {
         a.n = std::min(n - r, slice);
         a.x = d_x + r * ld_x;
         a.xs = d_xs + r;
         a.out = (char *)d_out + r * ld_out * vq::type_bytes(out_type);
-        const int way = vq::score_tile(a.n, k, aligned);
+        if (packed_x) {
+            VQ_TRY(pack_i8(ctx, a.x, a.n, ld_x, dim, packed_x));
+            a.x = packed_x;
+        }
         int32_t rc = VQ_OK;
-        by_type(out_type, [&](auto t) { rc = scores_slice<decltype(t)>(ctx, a, out_type, way); });
+        by_type(out_type, [&](auto t) { rc = scores_slice<decltype(t)>(ctx, a, out_type, ready_x && ready_w); });
         VQ_TRY(rc);
     }
     return VQ_OK;
