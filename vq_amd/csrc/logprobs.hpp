@@ -114,7 +114,9 @@ template <typename T, int LANES, int NV> struct Share {
     __device__ __forceinline__ int code(int e, int lane, int lo, int hi) const { return base(e / VEC, lane, lo, hi) + e % VEC; }
 };
 
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // (a NaN wins)
+// The larger one: of a number and a NaN the number (a NaN in a row shows in its sums), and the NaN.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ float larger_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // Over the lanes of aligned groups of G, for every lane of the group, in an order that is the same in every run.  f's first
 // operand stays where a step brings nothing.
@@ -156,7 +158,8 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 }
 
 // Sums of the scores of a lane relative to the largest score m of their row or part: S = sum 2^d, W = sum 2^d d with
-// d = (x - m) * c, c = beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero).  One fused operation per
+// d = (x - m) * c, c = beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero) but for a NaN, which makes the
+// sums NaN: m is the largest number of the row.  One fused operation per
 // exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
 // them, and taken out of the joined sums (away).  From |M| = 10^6 on, where r may be more than 1/16, exponents are formed from x - m.
 struct Sums {
@@ -174,7 +177,7 @@ struct Sums {
     }
     __device__ __forceinline__ Sums(float most, float sum, float weighted) : m(most), S(sum), W(weighted) {}
     __device__ __forceinline__ void add(float exponent) {
-        const float d = fmaxf(exponent, -200.0f), p = __builtin_amdgcn_exp2f(d);
+        const float d = larger_or_nan(exponent, -200.0f), p = __builtin_amdgcn_exp2f(d);
         S += p;
         W = __builtin_fmaf(p, d, W);
     }
@@ -190,10 +193,11 @@ struct RowSums {
     float m, L, H;
 };
 __device__ __forceinline__ RowSums row_sums(const Sums &s) {
+    if (s.S != s.S) return {s.S, s.S, s.S};
     if (Sums::is_bad(s.m)) return {s.m, __builtin_nanf(""), __builtin_nanf("")};
     if (s.m == kNegInf) return {s.m, kNegInf, 0.0f};
-    const float L = logf(s.S);
-    return {s.m, L, L - s.W / s.S * kLn2};
+    const float L = __builtin_amdgcn_logf(s.S) * kLn2;  // (log2; S is about 1 or above)
+    return {s.m, L, __builtin_fmaf(-s.W * __builtin_amdgcn_rcpf(s.S), kLn2, L)};
 }
 // The log probability of the row's code, whose score was read with the row.
 struct CodeScore {
@@ -219,26 +223,27 @@ __device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t 
 }
 
 // ---- short rows: G lanes each ------------------------------------------------------------------------
-// Up to 16 codes per lane, 64 / G rows per wave: no LDS, no waits.  One round per alternative: the largest score left, the
-// first code that has it, which then leaves.  TINY: rows shorter than a vector, one lane each.
-template <typename T, int G, bool TINY>
+// Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  One round per alternative: the largest score left, the
+// first code that has it, which then leaves.  Bound by its instructions as much as by memory, so a row of 256 has 8 lanes rather than
+// 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives SHORT16 -> SHORT8 us).
+// TINY: rows shorter than a vector, one lane each.
+template <typename T, int G, int E, bool TINY>
 __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
-    constexpr int NV = TINY ? 1 : (int)sizeof(typename T::Raw);
-    typedef Share<T, G, NV> S16;
+    typedef Share<T, G, TINY ? 1 : E * (int)sizeof(typename T::Raw) / 16> SE;
     const int lane = threadIdx.x & (G - 1);
     const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
     const typename T::Raw *s = (const typename T::Raw *)a.s + row * a.ld;
-    S16 r;
+    SE r;
     if constexpr (TINY) {
 #pragma unroll
-        for (int e = 0; e < S16::E; ++e) r.x[e] = e < a.k ? T::up(s[e]) : kNegInf;
+        for (int e = 0; e < SE::E; ++e) r.x[e] = e < a.k ? T::up(s[e]) : kNegInf;
     } else
         r.load(s, 0, a.k, lane);
     CodeScore cs;
     cs.read(a, row, T());
     float m = r.x[0];
 #pragma unroll
-    for (int e = 1; e < S16::E; ++e) m = larger(m, r.x[e]);
+    for (int e = 1; e < SE::E; ++e) m = larger(m, r.x[e]);
     m = group_max<G>(m);
     Sums sum(r.x, m, a.beta * kLog2e);
     sum.S = group_sum<G>(sum.S);
@@ -251,15 +256,16 @@ __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
     for (int t = 0; t < a.top; ++t) {
         int e0 = -1;
 #pragma unroll
-        for (int e = S16::E - 1; e >= 0; --e) e0 = r.x[e] == best ? e : e0;
+        for (int e = SE::E - 1; e >= 0; --e) e0 = r.x[e] == best ? e : e0;
         const int at = e0 < 0 ? 0x7fffffff : TINY ? e0 : r.code(e0, lane, 0, a.k), first = group_min<G>(at);
         if (writes) write_alternative(a, row, t, best, first == 0x7fffffff ? -1 : first, sums);
         if (t + 1 == a.top) break;
+        const int gone = at == first ? e0 : -1;
         best = kNegInf;
 #pragma unroll
-        for (int e = 0; e < S16::E; ++e) {
-            r.x[e] = e == e0 && at == first ? kNegInf : r.x[e];
-            best = fmaxf(best, r.x[e]);
+        for (int e = 0; e < SE::E; ++e) {
+            r.x[e] = e == gone ? kNegInf : r.x[e];
+            best = larger(best, r.x[e]);
         }
         best = group_max<G>(best);
     }
@@ -310,11 +316,11 @@ __device__ __forceinline__ void part_best(S64 &r, const float (&vmax)[S64::E / S
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-        if (!__ballot(vmax[u] >= floor && vmax[u] > kNegInf)) continue;
+        if (!__ballot(vmax[u] >= floor)) continue;
 #pragma unroll
         for (int v = 0; v < S64::VEC; ++v) {
             const float y = r.x[u * S64::VEC + v];
-            if (y >= floor && y > kNegInf) {
+            if (y >= floor) {
                 const int at = atomicAdd(&l.count, 1);
                 if (at < kMostCandidates) l.key[at] = rank_key(y, (uint32_t)r.code(u * S64::VEC + v, tid, lo, hi));
             }
@@ -405,6 +411,7 @@ __global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
     m = larger(larger(l.red[0][0], l.red[0][1]), larger(l.red[0][2], l.red[0][3]));
     floor = l.red[1][0];
     for (int w = 1; w < full; ++w) floor = fminf(floor, l.red[1][w]);
+    floor = fmaxf(floor, -3.402823466e38f);  // -inf is none of them
     Sums sum(r.x, m, a.beta * kLog2e);
     sum.S = group_sum<64>(sum.S);
     sum.W = group_sum<64>(sum.W);
@@ -453,7 +460,8 @@ __global__ void __launch_bounds__(256) k_logprobs_join(PartArgs p) {
     }
     const float *sums = p.sums + (row * parts + min(lane, parts - 1)) * 3, c = a.beta * kLog2e;
     const float pm = sums[0], pS = lane < parts ? sums[1] : 0.0f, pW = lane < parts ? sums[2] : 0.0f, m = group_max<64>(pm);
-    const float d = fmaxf((pm - (Sums::is_bad(m) || m == kNegInf ? 0.0f : m)) * c, -200.0f), f = __builtin_amdgcn_exp2f(d);
+    const float d = fmaxf((pm - (Sums::is_bad(m) || m == kNegInf ? 0.0f : m)) * c, -200.0f);
+    const float f = lane < parts ? __builtin_amdgcn_exp2f(d) : 0.0f;
     const RowSums r = row_sums({m, group_sum<64>(f * pS), group_sum<64>(f * __builtin_fmaf(pS, d, pW))});
     if (lane == 0) write_row(a, row, r, cs);
     if (top == 0) return;

@@ -147,7 +147,8 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
     return {};
 }
 
-// How the rows of a call go through the GPU.  Rows of up to 1024 codes have 1, 4, 16 or 64 lanes each, 16 codes per lane (`lanes`).
+// How the rows of a call go through the GPU.  Rows of up to 1024 codes have 1, 4, 8 or 64 lanes each, 16 codes per lane, 32 where
+// there are 8 (`lanes`, `per_lane`).
 // Longer ones have a workgroup of 256 lanes per part, 8 to 64 codes per lane (`per_lane`): as many as it takes for a row to be
 // one part, but no more than leave WORKGROUPS workgroups to the call, and no fewer than 8; at most 64 parts.  Parts are of equal
 // length, in whole 64 codes (`codes`; the last one is shorter).
@@ -158,7 +159,7 @@ struct RowPlan {
     int32_t parts, codes;
 };
 inline RowPlan plan_rows(int64_t n, int32_t k) {
-    if (k <= kShortCodes) return {k <= 16 ? 1 : k <= 64 ? 4 : k <= 256 ? 16 : 64, 16, 1, k};
+    if (k <= kShortCodes) return {k <= 16 ? 1 : k <= 64 ? 4 : k <= 256 ? 8 : 64, k > 64 && k <= 256 ? 32 : 16, 1, k};
     int e = 64;
     while (e > 8 && (k <= 128 * e || (n * ((k + 256 * e - 1) / (256 * e)) < 4096 && k <= 128 * e * kMostParts))) e /= 2;
     const int32_t least = (k + 256 * e - 1) / (256 * e), codes = ((k + least - 1) / least + 63) / 64 * 64;

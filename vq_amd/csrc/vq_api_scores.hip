@@ -80,8 +80,8 @@ int32_t pack_i8(vq_ctx *ctx, const int8_t *x, int64_t n, int64_t ld, int32_t dim
     return VQ_OK;
 }
 
-template <typename T, bool TINY, int G> void short_rows(vq_ctx *ctx, const vq::LogprobArgs &a) {
-    hipLaunchKernelGGL((vq::k_logprobs_short<T, G, TINY>), dim3((unsigned)cdiv64(a.n, 256 / G)), dim3(256), 0, ctx->stream, a);
+template <typename T, bool TINY, int G, int E> void short_rows(vq_ctx *ctx, const vq::LogprobArgs &a) {
+    hipLaunchKernelGGL((vq::k_logprobs_short<T, G, E, TINY>), dim3((unsigned)cdiv64(a.n, 256 / G)), dim3(256), 0, ctx->stream, a);
 }
 template <typename T> void row_parts(vq_ctx *ctx, const vq::PartArgs &p, int per_lane) {
     constexpr int VEC = 16 / (int)sizeof(typename T::Raw);
@@ -101,15 +101,15 @@ int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, cons
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
             if (a.k < 16 / (int)sizeof(typename T::Raw))
-                short_rows<T, true, 1>(ctx, a);
+                short_rows<T, true, 1, 16>(ctx, a);
             else if (plan.lanes == 1)
-                short_rows<T, false, 1>(ctx, a);
+                short_rows<T, false, 1, 16>(ctx, a);
             else if (plan.lanes == 4)
-                short_rows<T, false, 4>(ctx, a);
-            else if (plan.lanes == 16)
-                short_rows<T, false, 16>(ctx, a);
+                short_rows<T, false, 4, 16>(ctx, a);
+            else if (plan.lanes == 8)
+                short_rows<T, false, 8, 32>(ctx, a);
             else
-                short_rows<T, false, 64>(ctx, a);
+                short_rows<T, false, 64, 16>(ctx, a);
         });
         VQ_HIP(ctx, hipGetLastError());
         return VQ_OK;
