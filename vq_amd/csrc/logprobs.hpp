@@ -95,16 +95,19 @@ template <typename T, int LANES, int NV> struct Share {
         }
     }
     __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
-        fetch<false>(s, lo, hi, lane);
+        if (lo + LANES * E <= hi) {  // uniform: whole vectors all of them
+#pragma unroll
+            for (int u = 0; u < NV; ++u) raw[u] = *reinterpret_cast<const Piece *>(s + lo + (u * LANES + lane) * VEC);
+#pragma unroll
+            for (int u = 0; u < NV; ++u) values(raw[u], x + u * VEC);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) raw[u] = *reinterpret_cast<const Piece *>(s + base(u, lane, lo, hi));
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            if (u > 0 && lo + u * LANES * VEC >= hi) {  // uniform: nothing of the row is left
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) x[u * VEC + v] = kNegInf;
-                continue;
-            }
             values(raw[u], x + u * VEC);
-            if (lo + (u + 1) * LANES * VEC > hi) {  // uniform: the vectors that are read from elsewhere
+            if (lo + (u + 1) * LANES * VEC > hi) {  // uniform: the vectors that are read from elsewhere, or have nothing of the row
                 const int skip = lo + (u * LANES + lane) * VEC - base(u, lane, lo, hi);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) x[u * VEC + v] = v < skip ? kNegInf : x[u * VEC + v];
@@ -123,11 +126,14 @@ __device__ __forceinline__ float larger_or_nan(float a, float b) { return __buil
 template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ uint32_t dpp_keep(uint32_t old, uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
 }
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_all(uint32_t v) {  // every lane of a row brings something
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
 template <int G, typename F> __device__ __forceinline__ uint32_t over_group(uint32_t v, uint32_t none, F f) {
-    if constexpr (G >= 2) v = f(v, dpp_keep<0xB1>(v, v));
-    if constexpr (G >= 4) v = f(v, dpp_keep<0x4E>(v, v));
-    if constexpr (G >= 8) v = f(v, dpp_keep<0x141>(v, v));
-    if constexpr (G >= 16) v = f(v, dpp_keep<0x140>(v, v));
+    if constexpr (G >= 2) v = f(v, dpp_all<0xB1>(v));
+    if constexpr (G >= 4) v = f(v, dpp_all<0x4E>(v));
+    if constexpr (G >= 8) v = f(v, dpp_all<0x141>(v));
+    if constexpr (G >= 16) v = f(v, dpp_all<0x140>(v));
     static_assert(G <= 16 || G == 64, "rows of 16 lanes, or the wave");
     if constexpr (G == 64) {
         v = f(v, dpp_keep<0x142, 0xa>(none, v));  // a row's last lane to the next row
@@ -225,7 +231,7 @@ __device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t 
 // ---- short rows: G lanes each ------------------------------------------------------------------------
 // Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  One round per alternative: the largest score left, the
 // first code that has it, which then leaves.  Bound by its instructions as much as by memory, so a row of 256 has 8 lanes rather than
-// 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives SHORT16 -> SHORT8 us).
+// 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives 215 -> 190 us).
 // TINY: rows shorter than a vector, one lane each.
 template <typename T, int G, int E, bool TINY>
 __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
@@ -371,7 +377,7 @@ __device__ __forceinline__ void part_best(S64 &r, const float (&vmax)[S64::E / S
 }
 
 template <typename T, int NV>
-__global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
+__global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <= 32 ? 8 : 4) k_logprobs_part(PartArgs p) {
     typedef Share<T, 256, NV> S64;
     constexpr int VEC = S64::VEC;
     __shared__ PartLds l;
@@ -434,6 +440,8 @@ __global__ void __launch_bounds__(256) k_logprobs_part(PartArgs p) {
     }
 }
 
+// (Joining in the part that is done last, which takes stores and loads past the caches and a counter, saves nothing for one row,
+// 10.0 and 9.9 us, and costs 8192 rows of 65,536 203 -> 235.)
 // A wave joins the parts of a row: sums rescaled to the largest score of all, and the alternatives from the parts' lists.
 // With j = (top - 1) / parts, rounded down, `top` keys or more reach the q-th largest of the lists' keys number j where
 // q * (j + 1) >= top: what reaches that floor, a few at the head of every list, is gathered and sorted by counting.  (One
