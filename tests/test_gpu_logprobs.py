@@ -141,7 +141,7 @@ def test_tops(ctx, kind, top, n, k):
 
 
 @pytest.mark.parametrize("kind", R.TYPES)
-@pytest.mark.parametrize("k", [5, 33, 256, 300, 1024, 3000, 20000, 70001])
+@pytest.mark.parametrize("k", [5, 33, 256, 300, 700, 1024, 3000, 20000, 70001])
 def test_orders_and_ties(ctx, kind, k):
     """Rows in which the alternatives are hard to come by: rising, falling, all the same, few different values, the best ones
     side by side in one thread's share, all but a few impossible, the last code the best."""
@@ -153,6 +153,23 @@ def test_orders_and_ties(ctx, kind, k):
                   np.where(np.arange(k) % 256 == 17, 4.0, rng.standard_normal(k)), np.full(k, -np.inf), np.where(np.arange(k) % 64 < 4, 3.0, 1.0)])
     for top in (1, 4, 32):
         Call(ctx, R.pack(x, kind), kind, 1.0, rng.integers(0, k, len(x)), top=top).check()
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", [1025, 1600, 2048, 2049, 3001, 4096])
+def test_many_rows_of_a_wave(ctx, kind, k):
+    """Enough rows for a wave each: ties, masks, rows with nothing left and rows of equal scores among them."""
+    n = 4099
+    rng = np.random.default_rng(k)
+    x = rng.integers(-8, 9, (n, k)) * 0.5 if k % 2 else _rows(rng, n, k)
+    x = x.astype(np.float32)
+    x[::7] = np.where(rng.random((len(x[::7]), k)) < 0.5, -np.inf, x[::7])
+    x[3::11] = 1.25
+    x[5] = -np.inf
+    x[6, :k - 3] = -np.inf
+    x[8, k // 2] = np.nan
+    codes = rng.integers(-1, k + 1, n)
+    Call(ctx, R.pack(x, kind), kind, 0.9, codes, top=7 if k % 3 else 32).check()
 
 
 @pytest.mark.parametrize("kind", R.TYPES)

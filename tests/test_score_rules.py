@@ -104,7 +104,7 @@ def test_every_code_of_a_row_has_a_lane(lib):
             lanes, per_lane, parts, codes = out
             assert codes <= lanes * per_lane and parts * codes >= k and (parts - 1) * codes < k and (parts == 1 or (lanes == 256 and codes % 64 == 0))
             assert parts <= 64 and (parts == 1 or codes == lanes * per_lane)
-            assert lanes in (1, 4, 8, 64, 256) and per_lane in ({8: (32,)}.get(lanes, (16,)) if lanes < 256 else (8, 16, 32, 64))
+            assert per_lane in {1: (16,), 4: (16,), 8: (32,), 64: (16, 32, 64), 256: (32, 64)}[lanes]
 
 
 def test_tiles_fit_their_launches(lib):

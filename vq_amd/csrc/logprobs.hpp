@@ -222,15 +222,56 @@ __device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, con
     if (a.logprob)
         a.logprob[row] = c.code < 0 ? 0.0f : c.code >= a.k ? __builtin_nanf("") : r.m == kNegInf ? kNegInf : a.beta * (c.score - r.m) - r.L;
 }
-__device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t row, int t, float v, int code, const RowSums &r) {
-    const bool bad = r.L != r.L, none = v == kNegInf || code < 0;
-    a.top_logprob[row * a.top + t] = bad ? __builtin_nanf("") : none ? kNegInf : a.beta * (v - r.m) - r.L;
-    a.top_code[row * a.top + t] = bad || none ? -1 : code;
+// An alternative as it is written: its log probability and its code.
+struct Alternative {
+    float lp = 0.0f;
+    int32_t code = -1;
+    __device__ __forceinline__ void set(const LogprobArgs &a, float v, int c, const RowSums &r) {
+        const bool bad = r.L != r.L, none = v == kNegInf || c < 0;
+        lp = bad ? __builtin_nanf("") : none ? kNegInf : a.beta * (v - r.m) - r.L;
+        code = bad || none ? -1 : c;
+    }
+    __device__ __forceinline__ void write(const LogprobArgs &a, int64_t row, int t) const {
+        a.top_logprob[row * a.top + t] = lp;
+        a.top_code[row * a.top + t] = code;
+    }
+};
+__device__ __forceinline__ void write_alternative(const LogprobArgs &a, int64_t row, int t, uint64_t key, const RowSums &r) {
+    Alternative o;
+    o.set(a, key_score(key), key ? key_code(key) : -1, r);
+    o.write(a, row, t);
+}
+
+// One round per alternative over the scores of G lanes, which it empties: the largest score left, the first code that has
+// it, which then leaves.  Lane t % G keeps alternative t, and the lanes write G of them at a time.  code_of(e): the code of a lane's score e.
+template <int G, int E, typename F>
+__device__ __forceinline__ void best_by_rounds(const LogprobArgs &a, int64_t row, bool writes, float (&x)[E], const RowSums &r, int lane, F code_of) {
+    float best = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) best = larger(best, x[e]);
+    best = group_max<G>(best);
+    Alternative o;
+    for (int t = 0; t < a.top; ++t) {
+        int e0 = -1;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) e0 = x[e] == best ? e : e0;
+        const int at = e0 < 0 ? 0x7fffffff : code_of(e0), first = group_min<G>(at);
+        if ((t & (G - 1)) == lane) o.set(a, best, first == 0x7fffffff ? -1 : first, r);
+        if (((t & (G - 1)) == G - 1 || t + 1 == a.top) && lane <= (t & (G - 1)) && writes) o.write(a, row, (t & ~(G - 1)) + lane);
+        if (t + 1 == a.top) break;
+        const int gone = at == first ? e0 : -1;
+        best = kNegInf;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = e == gone ? kNegInf : x[e];
+            best = larger(best, x[e]);
+        }
+        best = group_max<G>(best);
+    }
 }
 
 // ---- short rows: G lanes each ------------------------------------------------------------------------
-// Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  One round per alternative: the largest score left, the
-// first code that has it, which then leaves.  Bound by its instructions as much as by memory, so a row of 256 has 8 lanes rather than
+// Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  Bound by its instructions as much as by memory, so a row of 256 has 8 lanes rather than
 // 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives 215 -> 190 us).
 // TINY: rows shorter than a vector, one lane each.
 template <typename T, int G, int E, bool TINY>
@@ -256,25 +297,9 @@ __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
     sum.W = group_sum<G>(sum.W);
     sum.away();
     const RowSums sums = row_sums(sum);
-    const bool writes = lane == 0 && mine < a.n;
-    if (writes) write_row(a, row, sums, cs);
-    float best = m;
-    for (int t = 0; t < a.top; ++t) {
-        int e0 = -1;
-#pragma unroll
-        for (int e = SE::E - 1; e >= 0; --e) e0 = r.x[e] == best ? e : e0;
-        const int at = e0 < 0 ? 0x7fffffff : TINY ? e0 : r.code(e0, lane, 0, a.k), first = group_min<G>(at);
-        if (writes) write_alternative(a, row, t, best, first == 0x7fffffff ? -1 : first, sums);
-        if (t + 1 == a.top) break;
-        const int gone = at == first ? e0 : -1;
-        best = kNegInf;
-#pragma unroll
-        for (int e = 0; e < SE::E; ++e) {
-            r.x[e] = e == gone ? kNegInf : r.x[e];
-            best = larger(best, r.x[e]);
-        }
-        best = group_max<G>(best);
-    }
+    const bool writes = mine < a.n;
+    if (writes && lane == 0) write_row(a, row, sums, cs);
+    if (a.top) best_by_rounds<G>(a, row, writes, r.x, sums, lane, [&](int e) { return TINY ? e : r.code(e, lane, 0, a.k); });
 }
 
 __device__ __forceinline__ void wave_sync() {  // a wave's reads and writes of LDS stay in order
@@ -293,6 +318,66 @@ __device__ __forceinline__ int keys_above(const uint64_t *key, int count, uint64
         for (int u = 0; u < 8; ++u) above += o[u] > mine;
     }
     return above;
+}
+
+// ---- rows of a wave -------------------------------------------------------------------------------------
+// E codes per lane, a row per wave.  The alternatives come from a list of the scores that reach a floor, the top-th largest of the
+// lanes' largest ones; the list is sorted by counting.  A list that does not fit, as of a row of equal scores, is not taken: then by rounds.
+constexpr int kWaveList = 128;
+
+template <typename T, int E>
+__global__ void __launch_bounds__(256, E == 16 ? 8 : E == 32 ? 6 : 4) k_logprobs_wave(LogprobArgs a) {
+    typedef Share<T, 64, E * (int)sizeof(typename T::Raw) / 16> SE;
+    __shared__ uint64_t lists[4][kWaveList + 8 + 32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top = a.top;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.n) return;  // (no barriers below)
+    SE r;
+    r.load((const typename T::Raw *)a.s + row * a.ld, 0, a.k, lane);
+    CodeScore cs;
+    cs.read(a, row, T());
+    float most = r.x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) most = larger(most, r.x[e]);
+    const float m = group_max<64>(most);
+    Sums sum(r.x, m, a.beta * kLog2e);
+    sum.S = group_sum<64>(sum.S);
+    sum.W = group_sum<64>(sum.W);
+    sum.away();
+    const RowSums sums = row_sums(sum);
+    if (lane == 0) write_row(a, row, sums, cs);
+    if (top == 0) return;
+    float floor = most, left = most;
+    for (int t = 0; t < top; ++t) {
+        floor = group_max<64>(left);
+        const unsigned long long who = __ballot(left == floor);
+        if (lane == __ffsll(who) - 1) left = kNegInf;
+    }
+    floor = fmaxf(floor, -3.402823466e38f);  // -inf is none of them
+    uint64_t *list = lists[wave], *best = list + kWaveList + 8;
+    int count = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const unsigned long long who = __ballot(r.x[e] >= floor);
+        if (!who) continue;
+        const int at = count + __popcll(who & ((1ull << lane) - 1));
+        if (r.x[e] >= floor && at < kWaveList) list[at] = rank_key(r.x[e], (uint32_t)r.code(e, lane, 0, a.k));
+        count += __popcll(who);
+    }
+    if (count > kWaveList) {  // uniform
+        best_by_rounds<64>(a, row, true, r.x, sums, lane, [&](int e) { return r.code(e, lane, 0, a.k); });
+        return;
+    }
+    if (lane < 8) list[count + lane] = 0;
+    if (lane < 32) best[lane] = 0;
+    wave_sync();
+    for (int i = lane; i < count; i += 64) {
+        const uint64_t mine = list[i];
+        const int rank = keys_above(list, count, mine);
+        if (rank < top) best[rank] = mine;
+    }
+    wave_sync();
+    if (lane < top) write_alternative(a, row, lane, best[lane], sums);
 }
 
 // ---- longer rows, in parts: a workgroup each ------------------------------------------------------------
@@ -432,7 +517,7 @@ __global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <=
     if (p.parts == 1) {
         const RowSums sums = row_sums(sum);
         if (lane == 0) write_row(a, row, sums, cs);
-        if (lane < a.top) write_alternative(a, row, lane, key_score(l.best[lane]), l.best[lane] ? key_code(l.best[lane]) : -1, sums);
+        if (lane < a.top) write_alternative(a, row, lane, l.best[lane], sums);
     } else {
         const int64_t at = blockIdx.x;
         if (lane == 0) p.sums[at * 3] = sum.m, p.sums[at * 3 + 1] = sum.S, p.sums[at * 3 + 2] = sum.W;
@@ -506,7 +591,7 @@ __global__ void __launch_bounds__(256) k_logprobs_join(PartArgs p) {
         if (rank < top) lists[rank] = mine;
     }
     wave_sync();
-    if (lane < top) write_alternative(a, row, lane, key_score(lists[lane]), lists[lane] ? key_code(lists[lane]) : -1, r);
+    if (lane < top) write_alternative(a, row, lane, lists[lane], r);
 }
 
 struct GradArgs {

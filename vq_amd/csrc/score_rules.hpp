@@ -147,21 +147,22 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
     return {};
 }
 
-// How the rows of a call go through the GPU.  Rows of up to 1024 codes have 1, 4, 8 or 64 lanes each, 16 codes per lane, 32 where
-// there are 8 (`lanes`, `per_lane`).
-// Longer ones have a workgroup of 256 lanes per part, 8 to 64 codes per lane (`per_lane`): as many as it takes for a row to be
-// one part, but no more than leave 4096 workgroups to the call, and no fewer than 8; at most 64 parts.  Parts have all the codes that
-// their lanes hold (`codes`), the last one what is left (777 x 50,021, f16: 27.1 us; parts of equal length 27.6, 1024 workgroups 28.6).
-constexpr int kShortCodes = 1024, kMostParts = 64;
-static_assert(kMaxRowCodes <= kMostParts * 64 * 256, "64 codes per lane hold every row");
+// How the rows of a call go through the GPU (`lanes` of a row, `per_lane` codes each).  Rows of up to 256 codes have 1, 4 or 8 lanes, of up to 4096
+// a wave with 16, 32 or 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2; 10,000 x 2000, 13.4 and 22.6; 100,000 x
+// 2000, 20 alternatives, 168 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
+// 10.8).  Longer ones go in parts of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough (one row of 65,536, f32, 20
+// alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6).
+constexpr int kMostParts = 64;
 struct RowPlan {
     int lanes, per_lane;
     int32_t parts, codes;
 };
+static_assert(kMaxRowCodes <= kMostParts * 64 * 256, "64 codes per lane hold every row");
 inline RowPlan plan_rows(int64_t n, int32_t k) {
-    if (k <= kShortCodes) return {k <= 16 ? 1 : k <= 64 ? 4 : k <= 256 ? 8 : 64, k > 64 && k <= 256 ? 32 : 16, 1, k};
-    int e = 64;
-    while (e > 8 && (k <= 128 * e || (n * ((k + 256 * e - 1) / (256 * e)) < 4096 && k <= 128 * e * kMostParts))) e /= 2;
+    if (k <= 256) return {k <= 16 ? 1 : k <= 64 ? 4 : 8, k <= 64 ? 16 : 32, 1, k};
+    if (k <= 4096) return {64, k <= 1024 ? 16 : k <= 2048 ? 32 : 64, 1, k};
+    const int64_t whole = (k + 16383) / 16384;
+    const int e = k <= 8192 || (k > 16384 && n * whole < 4096 && k <= kMostParts * 8192) ? 32 : 64;
     return {256, e, (k + 256 * e - 1) / (256 * e), 256 * e};
 }
 

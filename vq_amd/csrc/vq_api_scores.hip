@@ -86,11 +86,7 @@ template <typename T, bool TINY, int G, int E> void short_rows(vq_ctx *ctx, cons
 template <typename T> void row_parts(vq_ctx *ctx, const vq::PartArgs &p, int per_lane) {
     constexpr int VEC = 16 / (int)sizeof(typename T::Raw);
     const dim3 grid((unsigned)(p.a.n * p.parts)), wg(256);
-    if (per_lane == 8)
-        hipLaunchKernelGGL((vq::k_logprobs_part<T, 8 / VEC>), grid, wg, 0, ctx->stream, p);
-    else if (per_lane == 16)
-        hipLaunchKernelGGL((vq::k_logprobs_part<T, 16 / VEC>), grid, wg, 0, ctx->stream, p);
-    else if (per_lane == 32)
+    if (per_lane == 32)
         hipLaunchKernelGGL((vq::k_logprobs_part<T, 32 / VEC>), grid, wg, 0, ctx->stream, p);
     else
         hipLaunchKernelGGL((vq::k_logprobs_part<T, 64 / VEC>), grid, wg, 0, ctx->stream, p);
@@ -108,8 +104,12 @@ int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, cons
                 short_rows<T, false, 4, 16>(ctx, a);
             else if (plan.lanes == 8)
                 short_rows<T, false, 8, 32>(ctx, a);
+            else if (plan.per_lane == 16)
+                hipLaunchKernelGGL((vq::k_logprobs_wave<T, 16>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
+            else if (plan.per_lane == 32)
+                hipLaunchKernelGGL((vq::k_logprobs_wave<T, 32>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
             else
-                short_rows<T, false, 64, 16>(ctx, a);
+                hipLaunchKernelGGL((vq::k_logprobs_wave<T, 64>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
         });
         VQ_HIP(ctx, hipGetLastError());
         return VQ_OK;
