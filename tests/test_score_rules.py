@@ -19,7 +19,7 @@ int scores(i64 x, i64 xs, i64 n, i64 ldx, i64 w, i64 ws, int k, i64 ldw, int dim
     return vq::check_scores_i8(P(x), P(xs), n, ldx, P(w), P(ws), k, ldw, dim, P(b), type, P(out), ldo).status; }
 int logprobs(int type, i64 s, i64 n, i64 ld, int k, float beta, int cb, i64 c, i64 cs, int top, i64 lp, i64 m, i64 l, i64 h, i64 tl, i64 tc) {
     return vq::check_code_logprobs(type, P(s), n, ld, k, beta, cb, P(c), cs, top, P(lp), P(m), P(l), P(h), P(tl), P(tc)).status; }
-int plan(i64 n, int k, i64 *out) { const vq::RowPlan p = vq::plan_rows(n, k); out[0] = p.lanes, out[1] = p.per_lane, out[2] = p.parts, out[3] = p.codes; return 0; }
+int plan(i64 n, int k, int top, i64 *out) { const vq::RowPlan p = vq::plan_rows(n, k, top); out[0] = p.lanes, out[1] = p.per_lane, out[2] = p.parts, out[3] = p.codes; return 0; }
 int way(i64 n, int k, int dim) { return vq::score_way(n, k, dim); }
 i64 launch_rows(int k) { return vq::score_rows_of_a_launch(k); }
 int pack(i64 n, int k, int dim) { return vq::score_pack(n, k, dim); }
@@ -96,15 +96,17 @@ def test_taken(lib, call, change):
 
 
 def test_every_code_of_a_row_has_a_lane(lib):
-    lib.plan.argtypes = [C.c_longlong, C.c_int, C.c_void_p]
+    lib.plan.argtypes = [C.c_longlong, C.c_int, C.c_int, C.c_void_p]
     out = (C.c_longlong * 4)()
     for k in [1, 2, 3, 7, 8, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 50021, 65536, 262144, 1000003, 1 << 20]:
         for n in (1, 2, 3, 15, 16, 17, 64, 255, 1024, 100_000, 1 << 30):
-            lib.plan(n, k, out)
-            lanes, per_lane, parts, codes = out
-            assert codes <= lanes * per_lane and parts * codes >= k and (parts - 1) * codes < k and (parts == 1 or (lanes == 256 and codes % 64 == 0))
-            assert parts <= 64 and (parts == 1 or codes == lanes * per_lane)
-            assert per_lane in {1: (16,), 4: (16,), 8: (32,), 64: (16, 32, 64), 256: (32, 64)}[lanes]
+            for top in (0, 2, 8, 32):
+                lib.plan(n, k, top, out)
+                lanes, per_lane, parts, codes = out
+                assert codes <= lanes * per_lane and parts * codes >= k and (parts - 1) * codes < k and (parts == 1 or (lanes == 256 and codes % 64 == 0))
+                assert parts <= 64 and (parts == 1 or codes == lanes * per_lane)
+                assert per_lane in {1: (16,), 4: (16,), 8: (32,), 64: (8, 16, 32, 64), 256: (32, 64)}[lanes]
+                assert lanes < 64 or k >= 8  # a vector of 16 bytes at least
 
 
 def test_tiles_fit_their_launches(lib):

@@ -326,7 +326,7 @@ __device__ __forceinline__ int keys_above(const uint64_t *key, int count, uint64
 constexpr int kWaveList = 128;
 
 template <typename T, int E>
-__global__ void __launch_bounds__(256, E == 16 ? 8 : E == 32 ? 6 : 4) k_logprobs_wave(LogprobArgs a) {
+__global__ void __launch_bounds__(256, E <= 16 ? 8 : E == 32 ? 6 : 4) k_logprobs_wave(LogprobArgs a) {
     typedef Share<T, 64, E * (int)sizeof(typename T::Raw) / 16> SE;
     __shared__ uint64_t lists[4][kWaveList + 8 + 32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top = a.top;
@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(256, E == 16 ? 8 : E == 32 ? 6 : 4) k_logprobs
     const RowSums sums = row_sums(sum);
     if (lane == 0) write_row(a, row, sums, cs);
     if (top == 0) return;
-    float floor = most, left = most;
-    for (int t = 0; t < top; ++t) {
+    float floor = a.k <= kWaveList ? kNegInf : most, left = most;  // (short rows: all of them)
+    for (int t = 0; t < top && a.k > kWaveList; ++t) {
         floor = group_max<64>(left);
         const unsigned long long who = __ballot(left == floor);
         if (lane == __ffsll(who) - 1) left = kNegInf;

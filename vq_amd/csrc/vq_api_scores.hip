@@ -104,6 +104,8 @@ int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, cons
                 short_rows<T, false, 4, 16>(ctx, a);
             else if (plan.lanes == 8)
                 short_rows<T, false, 8, 32>(ctx, a);
+            else if (plan.per_lane == 8)
+                hipLaunchKernelGGL((vq::k_logprobs_wave<T, 8>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
             else if (plan.per_lane == 16)
                 hipLaunchKernelGGL((vq::k_logprobs_wave<T, 16>), dim3((unsigned)cdiv64(a.n, 4)), dim3(256), 0, ctx->stream, a);
             else if (plan.per_lane == 32)
@@ -215,7 +217,7 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
     VQ_TRY(admit(ctx, vq::check_code_logprobs(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, top, d_logprob,
                                               d_max, d_logsum, d_entropy, d_top_logprob, d_top_code), n, &go));
     if (!go) return VQ_OK;
-    const vq::RowPlan plan = vq::plan_rows(n, k);
+    const vq::RowPlan plan = vq::plan_rows(n, k, top);
     // rows per launch: a grid has fewer than 2^32 lanes, and the parts' results at most 64 MiB
     const int64_t slice = plan.lanes < 256 ? (int64_t)(1 << 23) * (256 / plan.lanes)
                                            : std::max<int64_t>(1, (plan.parts == 1 ? 1 << 23 : (64 << 20) / (12 + 8 * top)) / plan.parts);
