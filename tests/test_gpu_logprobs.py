@@ -352,6 +352,35 @@ def test_graph(ctx):
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
 
 
+def test_capture_before_the_workspace_is_there():
+    """A call whose workspace would have to grow is refused while the stream is captured; the capture goes on with a call
+    that needs none, and the refused call runs afterwards."""
+    import vq_amd
+    hip, lib = C.CDLL("libamdhip64.so"), vq_amd._ffi.lib()
+    c = vq_amd.Context(0)
+    stream = C.c_void_p(lib.vq_ctx_stream(c._h))
+    x, lp = c.to_device(np.linspace(0, 5, 70000, dtype=np.float32)), c.empty(2, np.float32)
+    codes = c.to_device(np.full(1, 7, np.int32))
+    graph, run = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    with pytest.raises(vq_amd.VqError) as e:
+        c.code_logprobs("f32", x, 1, 70000, 70000, 1.0, 4, codes, 1, 0, lp, None, None, None)
+    assert e.value.code == vq_amd._ffi.ERR_UNSUPPORTED and "capture" in str(e.value)
+    c.code_logprobs("f32", x, 1, 70000, 100, 1.0, 4, codes, 1, 0, lp, None, None, None)
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, 0) == 0
+    for _ in range(3):
+        assert hip.hipGraphLaunch(run, stream) == 0
+        c.sync()
+        st = R.statistics(x.download()[None, :100].astype(np.float64), 1.0)
+        assert abs(lp.download()[0] - st["lp"][0, 7]) < 1e-5
+        c.code_logprobs("f32", x, 1, 70000, 70000, 1.0, 4, codes, 1, 0, lp, None, None, None)
+        st = R.statistics(x.download()[None].astype(np.float64), 1.0)
+        assert abs(lp.download()[0] - st["lp"][0, 7]) < 1e-4
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    c.close()
+
+
 def test_refusals_leave_the_context_usable(ctx):
     import vq_amd
     x, codes, lp = ctx.to_device(np.zeros((2, 8), np.float32)), ctx.to_device(np.zeros(2, np.int32)), ctx.empty(2, np.float32)

@@ -154,23 +154,6 @@ inline int32_t ensure(vq_ctx *ctx, DevBuf &b, size_t bytes) {
     return VQ_OK;
 }
 
-// A workspace that captured graphs may hold the address of: it grows by a new allocation, at least twice the last, and the
-// ones before stay.  While the stream is being captured it cannot grow, and the capture goes on.
-inline int32_t ensure_kept(vq_ctx *ctx, DevBuf &b, size_t bytes) {
-    if (bytes <= b.cap) return VQ_OK;
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    VQ_HIP(ctx, hipStreamIsCapturing(ctx->stream, &st));
-    if (st != hipStreamCaptureStatusNone)
-        return fail(ctx, VQ_ERR_UNSUPPORTED, "a capture of this call needs an earlier call of this size: its workspace cannot grow meanwhile");
-    const size_t want = bytes > 2 * b.cap ? bytes + 256 : 2 * b.cap;
-    void *p = nullptr;
-    VQ_HIP(ctx, hipMalloc(&p, want));
-    if (b.p) ctx->outgrown.push_back(b.p);
-    b.p = p;
-    b.cap = want;
-    return VQ_OK;
-}
-
 // Gives a workspace buffer back once nothing on the context's streams uses it.
 inline int32_t release(vq_ctx *ctx, DevBuf &b) {
     if (!b.p) return VQ_OK;

@@ -66,24 +66,18 @@ template <typename T, int LANES, int NV> struct Share {
     struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
         uint32_t w[4];
     };
-    typedef AnyWords Words;
     Piece raw[NV];
     float x[E];
 
     static __device__ __forceinline__ int base(int u, int lane, int lo, int hi) { return min(lo + (u * LANES + lane) * VEC, hi - VEC); }
 
-    // ONCE: nobody is expected to read the row after this; it passes the caches (rows to 8 bits and their scores, 1M x 128 x 256 306 -> 274 us,
-    // gradients of 8192 x 65,536 401 -> 389; short rows' log probabilities 215 -> 219, they do not)
-    template <bool ONCE> __device__ __forceinline__ void fetch(const Raw *s, int lo, int hi, int lane) {
+    // The reads of a row that nobody is expected to read after this: they pass the caches (rows to 8 bits and their scores, 1M x 128 x 256
+    // 306 -> 274 us, gradients of 8192 x 65,536 401 -> 389; short rows' log probabilities 215 -> 219, they go by load).
+    __device__ __forceinline__ void fetch_once(const Raw *s, int lo, int hi, int lane) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
-            if (u == 0 || lo + u * LANES * VEC < hi) {
-                const Raw *at = s + base(u, lane, lo, hi);
-                if constexpr (ONCE)
-                    raw[u] = __builtin_bit_cast(Piece, __builtin_nontemporal_load(reinterpret_cast<const Words *>(at)));
-                else
-                    raw[u] = *reinterpret_cast<const Piece *>(at);
-            }
+            if (u == 0 || lo + u * LANES * VEC < hi)
+                raw[u] = __builtin_bit_cast(Piece, __builtin_nontemporal_load(reinterpret_cast<const AnyWords *>(s + base(u, lane, lo, hi))));
     }
     static __device__ __forceinline__ void values(const Piece &piece, float *to) {
 #pragma unroll
@@ -155,18 +149,9 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
 template <int G> __device__ __forceinline__ int group_min(int v) {
     return (int)over_group<G>((uint32_t)v, 0x7fffffffu, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
 }
-// The largest key of the wave.
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-    const auto most = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    const uint32_t hi = over_group<64>((uint32_t)(v >> 32), 0u, most);
-    const uint32_t lo = over_group<64>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u, 0u, most);
-    return (uint64_t)hi << 32 | lo;
-}
-
 // Sums of the scores of a lane relative to the largest score m of their row or part: S = sum 2^d, W = sum 2^d d with
 // d = (x - m) * c, c = beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero) but for a NaN, which makes the
-// sums NaN: m is the largest number of the row.  One fused operation per
-// exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
+// sums NaN: m is the largest number of the row.  One fused operation per exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
 // them, and taken out of the joined sums (away).  From |M| = 10^6 on, where r may be more than 1/16, exponents are formed from x - m.
 struct Sums {
     float m, S = 0.0f, W = 0.0f, r = 0.0f;
@@ -271,8 +256,8 @@ __device__ __forceinline__ void best_by_rounds(const LogprobArgs &a, int64_t row
 }
 
 // ---- short rows: G lanes each ------------------------------------------------------------------------
-// Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  Bound by its instructions as much as by memory, so a row of 256 has 8 lanes rather than
-// 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives 215 -> 190 us).
+// Up to 16 codes per lane, or 32, 64 / G rows per wave: no LDS, no waits.  Bound by its instructions as much as by memory, so a
+// row of 256 has 8 lanes rather than 16, and what every row costs is shared by eight of them (a million rows of 256 scores, two alternatives 215 -> 190 us).
 // TINY: rows shorter than a vector, one lane each.
 template <typename T, int G, int E, bool TINY>
 __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
@@ -525,12 +510,12 @@ __global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <=
     }
 }
 
-// (Joining in the part that is done last, which takes stores and loads past the caches and a counter, saves nothing for one row,
-// 10.0 and 9.9 us, and costs 8192 rows of 65,536 203 -> 235.)
 // A wave joins the parts of a row: sums rescaled to the largest score of all, and the alternatives from the parts' lists.
 // With j = (top - 1) / parts, rounded down, `top` keys or more reach the q-th largest of the lists' keys number j where
 // q * (j + 1) >= top: what reaches that floor, a few at the head of every list, is gathered and sorted by counting.  (One
-// round of the whole wave per alternative took 0.2 us each: a row of 32 parts, 20 alternatives 8.0 us, 4.5 so.)
+// round of the whole wave per alternative took 0.2 us each: a row of 32 parts, 20 alternatives 8.0 us, 4.5 so.)  A launch of its
+// own: joining in the part that is done last, which takes a counter, stores and loads past the caches, saves nothing for one row
+// (10.0 and 9.9 us) and costs 8192 rows of 65,536 203 -> 235.
 template <typename T>
 __global__ void __launch_bounds__(256) k_logprobs_join(PartArgs p) {
     extern __shared__ uint64_t join_lds[];
@@ -621,7 +606,7 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
     const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
     const int lo = G == 256 ? (int)blockIdx.y * (G * S::E) : 0, hi = a.k;
     S r;
-    r.template fetch<true>((const Raw *)a.s + row * a.ld, lo, hi, lane);
+    r.fetch_once((const Raw *)a.s + row * a.ld, lo, hi, lane);
     Raw *to = (Raw *)a.grad + row * a.ld_grad;
     const float m = a.max[row], L = a.logsum[row], gh = a.g_entropy ? a.g_entropy[row] : 0.0f, H = a.g_entropy ? a.entropy[row] : 0.0f;
     int64_t code = -1;
@@ -661,7 +646,7 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
         }
         if (mine >= a.n || at >= hi) continue;
         if (base == at && past)
-            __builtin_nontemporal_store(__builtin_bit_cast(typename S::Words, o), reinterpret_cast<typename S::Words *>(to + at));
+            __builtin_nontemporal_store(__builtin_bit_cast(AnyWords, o), reinterpret_cast<AnyWords *>(to + at));
         else if (base == at)
             *reinterpret_cast<typename S::Piece *>(to + at) = o;
         else

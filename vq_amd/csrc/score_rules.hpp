@@ -3,8 +3,6 @@
 #pragma once
 #include <algorithm>
 #include <cstdint>
-#include <cstdio>
-#include <string>
 
 #include "../../include/vq_hip.h"
 
@@ -19,9 +17,9 @@ constexpr int32_t kMaxRowCodes = 1 << 20;    // codes of a row of scores whose p
 // Status and text of a refusal; VQ_OK: the call may run.
 struct Refusal {
     int32_t status = VQ_OK;
-    std::string text;
+    const char *text = "";
 };
-inline Refusal refuse(int32_t status, const std::string &what) { return {status, "Invalid parameter: " + what}; }
+inline Refusal refuse(int32_t status, const char *what) { return {status, what}; }
 
 inline int type_bytes(int32_t type) { return type == VQ_F32 ? 4 : type == VQ_F16 || type == VQ_BF16 ? 2 : 0; }
 
@@ -42,7 +40,7 @@ inline bool misaligned(const void *p, int bytes) { return ((uintptr_t)p & (uintp
 inline Refusal check_rows_i8(int32_t type, const void *x, int64_t n, int64_t ld, int32_t dim, const void *q, int64_t ld_q,
                              const void *scale) {
     const int e = type_bytes(type);
-    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(type));
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "no such type");
     if (n < 0 || dim <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative and dim must be greater than 0");
     if (dim > kMaxDimI8) return refuse(VQ_ERR_UNSUPPORTED, "dim must be at most 131071");
     if (ld < dim || ld_q < dim) return refuse(VQ_ERR_INVALID_ARG, "a row stride is below dim");
@@ -58,7 +56,7 @@ inline Refusal check_rows_i8(int32_t type, const void *x, int64_t n, int64_t ld,
 inline Refusal check_scores_i8(const void *x, const void *xs, int64_t n, int64_t ld_x, const void *w, const void *ws, int32_t k,
                                int64_t ld_w, int32_t dim, const void *bias, int32_t out_type, const void *out, int64_t ld_out) {
     const int e = type_bytes(out_type);
-    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(out_type));
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "no such type");
     if (n < 0 || dim <= 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative, dim and k must be greater than 0");
     if (dim > kMaxDimI8) return refuse(VQ_ERR_UNSUPPORTED, "dim must be at most 131071");
     if (k > kMaxScoreCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 16777216");
@@ -80,7 +78,7 @@ inline Refusal check_scores_i8(const void *x, const void *xs, int64_t n, int64_t
 inline Refusal check_scored_codes(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t code_bytes,
                                   const void *codes, int64_t code_stride) {
     const int e = type_bytes(type);
-    if (!e) return refuse(VQ_ERR_INVALID_ARG, "type " + std::to_string(type));
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "no such type");
     if (n < 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative and k must be greater than 0");
     if (k > kMaxRowCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 1048576");
     if (ld < k) return refuse(VQ_ERR_INVALID_ARG, "the row stride is below k");
@@ -149,9 +147,8 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
 
 // How the rows of a call go through the GPU (`lanes` of a row, `per_lane` codes each).  Rows of up to 256 codes have 1, 4 or 8 lanes, a wave where
 // there are no more than 16,384 of them and 8 alternatives or more (309 x 20, f16, 32 alternatives 5.0 us, 18.4 in 4 lanes; 8000 x 256, f32, 20: 12.9
-// and 19.0, 5: 7.3 and 6.5); of up to 4096
-// a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2; 10,000 x 2000, 13.4 and 22.6; 100,000 x
-// 2000, 20 alternatives, 168 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
+// and 19.0, 5: 7.3 and 6.5); of up to 4096 a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2;
+// 10,000 x 2000, 13.4 and 22.6; 100,000 x 2000, 20 alternatives, 168 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
 // 10.8).  Longer ones go in parts of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough (one row of 65,536, f32, 20
 // alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6).
 constexpr int kMostParts = 64;

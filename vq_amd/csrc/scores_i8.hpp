@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) k_rows_i8(RowsI8Args a) {
     const int lane = threadIdx.x & (G - 1);
     const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, row = min(mine, a.n - 1);
     S r;
-    r.template fetch<true>((const typename T::Raw *)a.x + row * a.ld, 0, a.dim, lane);
+    r.fetch_once((const typename T::Raw *)a.x + row * a.ld, 0, a.dim, lane);
     uint32_t m = 0;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
