@@ -206,15 +206,19 @@ inline int64_t score_rows_of_a_launch(int32_t k) {
     return 64 * std::min<int64_t>(65535, std::max<int64_t>(1, (1 << 22) / ((k + 63) / 64)));
 }
 
-// Lanes and vectors of 16 bytes per lane that hold a row of `length` values in registers: 16 or 64 lanes with one vector, 64 with four, a
-// workgroup with eight; lanes 0: none does.
+// Lanes and vectors of 16 bytes per lane that hold a row of `length` values in registers: 4 lanes with one vector or four, 8 with four, 64 with
+// one or four, a workgroup with eight; lanes 0: none does.  Short rows have few lanes, so that a wave shares what a row costs beside its values,
+// two divisions most of all, among 16 or 8 of them (1M rows of 128 f32 102 us with 8 lanes, 202 with 64; of 24 bf16 23 with 4, 71 with 16).
 struct LanePlan {
     int lanes, vectors;
 };
 inline LanePlan plan_lanes(int32_t length, int bytes) {
     const int vec = 16 / bytes;
     if (length < vec || length > 2048 * vec) return {0, 0};
-    return length <= 16 * vec ? LanePlan{16, 1} : length <= 64 * vec ? LanePlan{64, 1} : length <= 256 * vec ? LanePlan{64, 4} : LanePlan{256, 8};
+    if (length <= 16 * vec) return {4, length <= 4 * vec ? 1 : 4};
+    if (length <= 32 * vec) return {8, 4};
+    if (length <= 256 * vec) return {64, length <= 64 * vec ? 1 : 4};
+    return {256, 8};
 }
 
 }  // namespace vq

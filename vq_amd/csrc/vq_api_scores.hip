@@ -175,8 +175,12 @@ int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_
         const auto grid = [&](int lanes) { return dim3((unsigned)cdiv64(a.n, 256 / lanes)); };
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
-            if (plan.lanes == 16)
-                hipLaunchKernelGGL((vq::k_rows_i8<T, 16, 1>), grid(16), dim3(256), 0, ctx->stream, a);
+            if (plan.lanes == 4 && plan.vectors == 1)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 4, 1>), grid(4), dim3(256), 0, ctx->stream, a);
+            else if (plan.lanes == 4)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 4, 4>), grid(4), dim3(256), 0, ctx->stream, a);
+            else if (plan.lanes == 8)
+                hipLaunchKernelGGL((vq::k_rows_i8<T, 8, 4>), grid(8), dim3(256), 0, ctx->stream, a);
             else if (plan.lanes == 64 && plan.vectors == 1)
                 hipLaunchKernelGGL((vq::k_rows_i8<T, 64, 1>), grid(64), dim3(256), 0, ctx->stream, a);
             else if (plan.lanes == 64)
@@ -274,6 +278,8 @@ int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, i
             typedef decltype(t) T;
             if (k < vec)
                 hipLaunchKernelGGL(vq::k_logprobs_grad_tiny<T>, dim3((unsigned)cdiv64(a.n, 256)), dim3(256), 0, ctx->stream, a);
+            else if (k <= 16 * vec)
+                hipLaunchKernelGGL((vq::k_logprobs_grad<T, 4, 4>), dim3((unsigned)cdiv64(a.n, 64)), dim3(256), 0, ctx->stream, a);
             else if (k <= 64 * vec)
                 hipLaunchKernelGGL((vq::k_logprobs_grad<T, 16, 4>), dim3((unsigned)cdiv64(a.n, 16)), dim3(256), 0, ctx->stream, a);
             else if (k <= 256 * vec)
