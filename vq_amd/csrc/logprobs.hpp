@@ -292,6 +292,16 @@ __device__ __forceinline__ void wave_sync() {  // a wave's reads and writes of L
     __builtin_amdgcn_wave_barrier();
 }
 
+// The q-th largest of the lanes' values, of which `most` is the largest.
+__device__ __forceinline__ float lane_floor(float value, float most, int q, int lane) {
+    while (--q > 0) {
+        const unsigned long long who = __ballot(value == most);
+        if (lane == __ffsll(who) - 1) value = kNegInf;
+        most = group_max<64>(value);
+    }
+    return most;
+}
+
 // How many of the keys in LDS are above one; zeros up to a whole eight of them lie behind the last.
 __device__ __forceinline__ int keys_above(const uint64_t *key, int count, uint64_t mine) {
     int above = 0;
@@ -332,12 +342,7 @@ __global__ void __launch_bounds__(256, E <= 16 ? 8 : E == 32 ? 6 : 4) k_logprobs
     const RowSums sums = row_sums(sum);
     if (lane == 0) write_row(a, row, sums, cs);
     if (top == 0) return;
-    float floor = a.k <= kWaveList ? kNegInf : most, left = most;  // (short rows: all of them)
-    for (int t = 0; t < top && a.k > kWaveList; ++t) {
-        floor = group_max<64>(left);
-        const unsigned long long who = __ballot(left == floor);
-        if (lane == __ffsll(who) - 1) left = kNegInf;
-    }
+    float floor = a.k <= kWaveList ? kNegInf : lane_floor(most, m, top, lane);  // (short rows: all of them)
     floor = fmaxf(floor, -3.402823466e38f);  // -inf is none of them
     uint64_t *list = lists[wave], *best = list + kWaveList + 8;
     int count = 0;
@@ -472,15 +477,8 @@ __global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <=
     // The floor of the alternatives: in each of the waves whose lanes all have codes, a share of them, rounded up, of the lanes have a score
     // that reaches the wave's floor, so `top` scores reach the smallest of these.
     const int full = max(1, min(4, (hi - lo) / (64 * VEC)));
-    float floor = mine;
-    if (a.top && wave < full) {
-        float left = mine;
-        for (int q = (a.top + full - 1) / full; q; --q) {
-            floor = group_max<64>(left);
-            const unsigned long long who = __ballot(left == floor);
-            if (lane == __ffsll(who) - 1) left = kNegInf;
-        }
-    }
+    float floor = m;
+    if (a.top && wave < full) floor = lane_floor(mine, m, (a.top + full - 1) / full, lane);
     if (lane == 0) l.red[0][wave] = m, l.red[1][wave] = floor;
     if (tid == 0) l.count = 0;
     __syncthreads();
