@@ -150,7 +150,7 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
 // and 19.0, 5: 7.3 and 6.5); of up to 4096 a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2;
 // 10,000 x 2000, 13.4 and 22.6; 100,000 x 2000, 20 alternatives, 168 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
 // 10.8).  Longer ones go in parts of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough (one row of 65,536, f32, 20
-// alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6).
+// alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6; 26.3 since then).
 constexpr int kMostParts = 64;
 struct RowPlan {
     int lanes, per_lane;
