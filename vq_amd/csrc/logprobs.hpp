@@ -292,8 +292,19 @@ __device__ __forceinline__ void wave_sync() {  // a wave's reads and writes of L
     __builtin_amdgcn_wave_barrier();
 }
 
-// The q-th largest of the lanes' values, of which `most` is the largest.
-__device__ __forceinline__ float lane_floor(float value, float most, int q, int lane) {
+// A value that q of the lanes' values reach, of which `most` is the largest: the q-th largest of them, in a round per value up to eight,
+// beyond that the bits of its rank from the highest down to bit LOW, a compare and a count of lanes each.
+template <int LOW> __device__ __forceinline__ float lane_floor(float value, float most, int q, int lane) {
+    if (q > 8) {  // uniform
+        const uint32_t mine = (uint32_t)(rank_key(larger(value, kNegInf), 0) >> 32);
+        uint32_t at = 0;
+#pragma unroll
+        for (int bit = 31; bit >= LOW; --bit) {
+            const uint32_t next = at | 1u << bit;
+            if (__popcll(__ballot(mine >= next)) >= q) at = next;
+        }
+        return larger(key_score((uint64_t)at << 32), kNegInf);  // (below the rank of -inf lie NaNs)
+    }
     while (--q > 0) {
         const unsigned long long who = __ballot(value == most);
         if (lane == __ffsll(who) - 1) value = kNegInf;
@@ -342,7 +353,7 @@ __global__ void __launch_bounds__(256, E <= 16 ? 8 : E == 32 ? 6 : 4) k_logprobs
     const RowSums sums = row_sums(sum);
     if (lane == 0) write_row(a, row, sums, cs);
     if (top == 0) return;
-    float floor = a.k <= kWaveList ? kNegInf : lane_floor(most, m, top, lane);  // (short rows: all of them)
+    float floor = a.k <= kWaveList ? kNegInf : lane_floor<sizeof(typename T::Raw) == 2 ? 16 : 8>(most, m, top, lane);  // (short rows: all of them)
     floor = fmaxf(floor, -3.402823466e38f);  // -inf is none of them
     uint64_t *list = lists[wave], *best = list + kWaveList + 8;
     int count = 0;
@@ -478,7 +489,7 @@ __global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <=
     // that reaches the wave's floor, so `top` scores reach the smallest of these.
     const int full = max(1, min(4, (hi - lo) / (64 * VEC)));
     float floor = m;
-    if (a.top && wave < full) floor = lane_floor(mine, m, (a.top + full - 1) / full, lane);
+    if (a.top && wave < full) floor = lane_floor<sizeof(typename T::Raw) == 2 ? 16 : 8>(mine, m, (a.top + full - 1) / full, lane);
     if (lane == 0) l.red[0][wave] = m, l.red[1][wave] = floor;
     if (tid == 0) l.count = 0;
     __syncthreads();
