@@ -156,6 +156,35 @@ def test_orders_and_ties(ctx, kind, k):
 
 
 @pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("n,k,top", [(30, 256, 32), (30, 200, 9), (30, 300, 32), (30, 513, 17), (30, 1100, 32), (30, 4096, 9), (30, 16500, 32), (30, 33000, 12),
+                                     (16500, 132, 16), (16500, 256, 20), (16400, 256, 32), (16400, 129, 31)])
+def test_floor_of_many_alternatives(ctx, kind, n, k, top):
+    """More than eight alternatives per wave: scores alike in their leading bits, below zero, around zero and subnormal, fewer of
+    them above -inf than asked for, in few threads, with NaN or +inf; and many short rows."""
+    rng = np.random.default_rng([n, k, top])
+    x = _rows(rng, n, k).astype(np.float32)
+    near = rng.integers(0, 400, k)
+    x[0] = np.float32(1.0) + near.astype(np.float32) * np.float32(2.0 ** -23)
+    x[1] = -(np.float32(1.0) + near.astype(np.float32) * np.float32(2.0 ** -23))
+    x[2] = -np.abs(x[2]) - 100
+    x[3] = (near - 200) * 2.0 ** -149
+    x[4] = np.where(near % 2 == 0, 0.0, -0.0)
+    x[5] = np.where(np.arange(k) < top - 1, x[5], -np.inf)
+    x[6] = np.where(np.arange(k) >= k - top, x[6], -np.inf)
+    x[7] = np.where(np.arange(k) % 8 == 0, -3.0, -np.inf)
+    x[8], x[8, ::8] = -5.0, np.nan
+    x[9, k - 1] = np.inf
+    x[10] = np.where(np.arange(k) // 8 < 9, 50.0 + x[10], -50.0)
+    x[11] = 2.0 ** rng.integers(-30, 15, k)
+    x[12] = -x[11]
+    x[13] = -65504.0
+    x[14] = -np.inf
+    x[15] = np.where(np.arange(k) == k // 2, x[15], -np.inf)
+    x[16] = np.nan
+    Call(ctx, R.pack(x, kind), kind, 1.0, rng.integers(-1, k + 1, n), top=top, pad=n % 4).check()
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
 @pytest.mark.parametrize("k", [1025, 1600, 2048, 2049, 3001, 4096])
 def test_many_rows_of_a_wave(ctx, kind, k):
     """Enough rows for a wave each: ties, masks, rows with nothing left and rows of equal scores among them."""

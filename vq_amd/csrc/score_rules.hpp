@@ -146,9 +146,10 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
 }
 
 // How the rows of a call go through the GPU (`lanes` of a row, `per_lane` codes each).  Rows of up to 256 codes have 1, 4 or 8 lanes, a wave where
-// there are no more than 16,384 of them and 8 alternatives or more (309 x 20, f16, 32 alternatives 5.0 us, 18.4 in 4 lanes; 8000 x 256, f32, 20: 12.9
-// and 19.0, 5: 7.3 and 6.5); of up to 4096 a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2;
-// 10,000 x 2000, 13.4 and 22.6; 100,000 x 2000, 20 alternatives, 168 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
+// there are no more than 16,384 of them and 8 alternatives or more (2000 x 24, f32, 32 alternatives 5.4 us, 14.3 in 4 lanes; x 256, 20: 5.5 and 18.8,
+// 2: the same), or more than 128 codes and 16 alternatives or more, for which five lanes more than those hold codes (200,000 x 256, f32, 20:
+// 104 and 143, 32: 113 and 220, 12: 100 and 90; x 128, 32: 238 and 219; bf16, 20: 115 and 143, 32, which all 32 lanes have to give: 309 and 221); of up to 4096 a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2;
+// 10,000 x 2000, 13.4 and 22.6; 100,000 x 2000, 20 alternatives, 107 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
 // 10.8).  Longer ones go in parts of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough (one row of 65,536, f32, 20
 // alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6; 26.3 since then).
 constexpr int kMostParts = 64;
@@ -157,8 +158,9 @@ struct RowPlan {
     int32_t parts, codes;
 };
 static_assert(kMaxRowCodes <= kMostParts * 64 * 256, "64 codes per lane hold every row");
-inline RowPlan plan_rows(int64_t n, int32_t k, int32_t top) {
-    if (k <= 512 && k >= 8 && (k > 256 || (top >= 8 && n <= 16384))) return {64, 8, 1, k};
+inline RowPlan plan_rows(int64_t n, int32_t k, int32_t top, int bytes = 4) {
+    const bool many = (n <= 16384 && top >= 8) || (k > 128 && top >= 16 && k * bytes / 16 >= top + 5);
+    if (k <= 512 && k >= 8 && (k > 256 || many)) return {64, 8, 1, k};
     if (k <= 256) return {k <= 16 ? 1 : k <= 64 ? 4 : 8, k <= 64 ? 16 : 32, 1, k};
     if (k <= 4096) return {64, k <= 1024 ? 16 : k <= 2048 ? 32 : 64, 1, k};
     const int64_t whole = (k + 16383) / 16384;

@@ -243,7 +243,7 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
     VQ_TRY(admit(ctx, vq::check_code_logprobs(type, d_scores, n, ld, k, beta, code_bytes, d_codes, code_stride, top, d_logprob,
                                               d_max, d_logsum, d_entropy, d_top_logprob, d_top_code), n, &go));
     if (!go) return VQ_OK;
-    const vq::RowPlan plan = vq::plan_rows(n, k, top);
+    const vq::RowPlan plan = vq::plan_rows(n, k, top, vq::type_bytes(type));
     // rows per launch: a grid has fewer than 2^32 lanes, and the parts' results at most 64 MiB
     const int64_t slice = plan.lanes < 256 ? (int64_t)(1 << 23) * (256 / plan.lanes)
                                            : std::max<int64_t>(1, (plan.parts == 1 ? 1 << 23 : (64 << 20) / (12 + 8 * top)) / plan.parts);
