@@ -474,8 +474,8 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
  *   d_grad[i][j] = beta * (g_lp * ([j = c] - p_j) - g_H * p_j * (log p_j + H))
  * with m, L and H as vq_code_logprobs left them (d_entropy may be NULL where d_g_entropy is), computed in f32 and rounded
  * to `type`, the type of the scores and of the gradient.  Probability zero, as which one below 2^-126 may count: gradient zero but for the code's own term.  A negative code takes no part in g_lp's
- * term; a code of k or above, or a row whose L is NaN, makes the row's gradient NaN; a row of -inf only has gradient
- * zero.  d_grad may be d_scores itself (same stride); another overlap is refused. */
+ * term; a row of -inf only has gradient zero, whatever its code; a code of k or above, or a row whose L is NaN, makes any other row's
+ * gradient NaN.  d_grad may be d_scores itself (same stride); another overlap is refused. */
 int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
                               int32_t code_bytes, const void *d_codes, int64_t code_stride, const float *d_max,
                               const float *d_logsum, const float *d_entropy, const float *d_g_logprob,

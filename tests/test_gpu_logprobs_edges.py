@@ -1,0 +1,34 @@
+"""GPU: log probabilities of codes and their gradient at the edges of what the header promises, for every way a row goes
+through the GPU, against plain forms in 64 bits (scores_ref.py)."""
+import numpy as np
+import pytest
+
+import scores_ref as R
+from test_gpu_logprobs import Call, _rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import vq_amd
+    c = vq_amd.Context(0)
+    yield c
+    c.close()
+
+
+# rows of a lane (below a vector of 16 bytes, and not), of 4 and 8 lanes, of a wave, of a workgroup, in parts
+LENGTHS = [2, 3, 6, 12, 40, 200, 300, 900, 3000, 6000, 20000, 50001]
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", LENGTHS)
+def test_gradient_of_rows_without_a_code_that_can_be(ctx, kind, k):
+    """A row of -inf only has gradient zero, a code of k or above among them; such a code makes any other row's gradient NaN."""
+    rng = np.random.default_rng(k)
+    x = _rows(rng, 6, k)
+    x[1], x[2], x[4] = -np.inf, -np.inf, -np.inf
+    c = Call(ctx, R.pack(x, kind), kind, 1.0, np.array([0, k, k - 1, k, -1, k + 100]), top=2).check()
+    got = c.grad(rng.standard_normal(6), rng.standard_normal(6))
+    assert (got[[1, 2, 4]] == 0).all() and np.isnan(got[[3, 5]]).all() and np.isfinite(got[0]).all()
+    c.grad(rng.standard_normal(6), None)

@@ -626,8 +626,8 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
     }
     const bool none = m == kNegInf, bad = L != L || code >= a.k;
     const float from = none ? 0.0f : m, c = a.beta * kLog2e, L2 = none ? 0.0f : L * kLog2e, own = a.beta * gl;
-    const float A = none ? 0.0f : a.beta * gh * kLn2, B = bad ? __builtin_nanf("") : none ? 0.0f : a.beta * __builtin_fmaf(gh, H, gl);
-    if (none) code = -1;
+    const float A = none ? 0.0f : a.beta * gh * kLn2, B = none ? 0.0f : bad ? __builtin_nanf("") : a.beta * __builtin_fmaf(gh, H, gl);
+    if (none) code = -1;  // (before all else: such a row's gradient is zero, whatever its code)
     const bool past = ((uintptr_t)a.grad & 127) == 0 && a.ld_grad % (128 / (int)sizeof(Raw)) == 0;  // whole lines pass the caches (412 -> 401 us)
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
