@@ -32,3 +32,22 @@ def test_gradient_of_rows_without_a_code_that_can_be(ctx, kind, k):
     got = c.grad(rng.standard_normal(6), rng.standard_normal(6))
     assert (got[[1, 2, 4]] == 0).all() and np.isnan(got[[3, 5]]).all() and np.isfinite(got[0]).all()
     c.grad(rng.standard_normal(6), None)
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", [1] + LENGTHS)
+def test_no_probability_above_one(ctx, kind, k):
+    """Rows that one code decides, at scores of many sizes: no log probability is above zero, no entropy and no L below."""
+    rng = np.random.default_rng(k)
+    n = 400 if k < 5000 else 60
+    x = rng.uniform(-30, 30, (n, 1)) * 2.0 ** rng.integers(-3, 6, (n, 1)) - 2000.0 * rng.integers(1, 4, (n, k))
+    best = rng.integers(0, k, n)
+    x[np.arange(n), best] = rng.uniform(-30, 30, n) * 2.0 ** rng.integers(-3, 6, n)
+    for beta in (1.0, 0.375, 11.0):
+        c = Call(ctx, R.pack(x, kind), kind, beta, best, top=2).check()
+        lp, m, L, H = (o.download()[:n] for o in c.out)
+        assert (lp <= 0).all(), (lp.max(), (lp > 0).sum())
+        assert (L >= 0).all() and (H >= 0).all(), (L.min(), H.min())
+        assert (c.top_lp.download()[:n] <= 0).all()
+        with np.errstate(divide="ignore"):
+            assert not np.isnan(np.log1p(-np.exp(lp))).any()

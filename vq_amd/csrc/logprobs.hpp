@@ -187,8 +187,10 @@ __device__ __forceinline__ RowSums row_sums(const Sums &s) {
     if (s.S != s.S) return {s.S, s.S, s.S};
     if (Sums::is_bad(s.m)) return {s.m, __builtin_nanf(""), __builtin_nanf("")};
     if (s.m == kNegInf) return {s.m, kNegInf, 0.0f};
-    const float L = __builtin_amdgcn_logf(s.S) * kLn2;  // (log2; S is about 1 or above)
-    return {s.m, L, __builtin_fmaf(-s.W * __builtin_amdgcn_rcpf(s.S), kLn2, L)};
+    // S is 1 or above, the largest score's own term, and -W zero or above; rounding may leave either a bit short, so L and H are held at 0:
+    // no log probability is above zero and no entropy below
+    const float L = fmaxf(__builtin_amdgcn_logf(s.S) * kLn2, 0.0f);  // (log2)
+    return {s.m, L, fmaxf(__builtin_fmaf(-s.W * __builtin_amdgcn_rcpf(s.S), kLn2, L), 0.0f)};
 }
 // The log probability of the row's code, whose score was read with the row.
 struct CodeScore {
