@@ -51,3 +51,22 @@ def test_no_probability_above_one(ctx, kind, k):
         assert (c.top_lp.download()[:n] <= 0).all()
         with np.errstate(divide="ignore"):
             assert not np.isnan(np.log1p(-np.exp(lp))).any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("k", LENGTHS[1:])
+def test_scores_further_apart_than_a_number(ctx, kind, k):
+    """Scores whose difference is beyond binary32: their log probability, beta times it, is within for a beta below 1."""
+    rng = np.random.default_rng(k)
+    x = np.full((5, k), -np.inf)
+    x[:, 0], x[:, k - 1] = 3e38, -3e38
+    x[1, k // 2] = -2.5e38
+    x[2] = rng.uniform(-3e38, 3e38, k)
+    x[2, 0], x[2, k - 1] = 3.3e38, -3.3e38
+    x[3, 0] = 1.0
+    x[4, k // 2] = 3e38
+    for beta in (0.5, 2.0 ** -10, 2.0 ** -60, 2.0 ** -99, 3.0):
+        c = Call(ctx, R.pack(x, kind), kind, beta, np.array([k - 1, k - 1, k - 1, k - 1, k - 1]), top=4).check()
+        lp = c.out[0].download()[:5]
+        assert np.isfinite(lp).all() or beta == 3.0
+        c.grad(rng.standard_normal(5), rng.standard_normal(5))

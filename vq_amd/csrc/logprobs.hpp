@@ -202,12 +202,18 @@ struct CodeScore {
         if (code >= 0 && code < a.k) score = T::up(((const typename T::Raw *)a.s)[row * a.ld + code]);
     }
 };
+// beta * (s - m) - L for a score s of a row: halves where the difference is beyond f32, as of scores of +-3e38, which a beta below 1
+// brings back.
+__device__ __forceinline__ float log_probability(float beta, float s, const RowSums &r) {
+    const float d = s - r.m;
+    return (d == kNegInf ? beta * (0.5f * s - 0.5f * r.m) * 2.0f : beta * d) - r.L;
+}
 __device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, const RowSums &r, const CodeScore &c) {
     if (a.max) a.max[row] = r.m;
     if (a.logsum) a.logsum[row] = r.L;
     if (a.entropy) a.entropy[row] = r.H;
     if (a.logprob)
-        a.logprob[row] = c.code < 0 ? 0.0f : c.code >= a.k ? __builtin_nanf("") : r.m == kNegInf ? kNegInf : a.beta * (c.score - r.m) - r.L;
+        a.logprob[row] = c.code < 0 ? 0.0f : c.code >= a.k ? __builtin_nanf("") : r.m == kNegInf ? kNegInf : log_probability(a.beta, c.score, r);
 }
 // An alternative as it is written: its log probability and its code.
 struct Alternative {
@@ -215,7 +221,7 @@ struct Alternative {
     int32_t code = -1;
     __device__ __forceinline__ void set(const LogprobArgs &a, float v, int c, const RowSums &r) {
         const bool bad = r.L != r.L, none = v == kNegInf || c < 0;
-        lp = bad ? __builtin_nanf("") : none ? kNegInf : a.beta * (v - r.m) - r.L;
+        lp = bad ? __builtin_nanf("") : none ? kNegInf : log_probability(a.beta, v, r);
         code = bad || none ? -1 : c;
     }
     __device__ __forceinline__ void write(const LogprobArgs &a, int64_t row, int t) const {
