@@ -53,6 +53,26 @@ def test_no_probability_above_one(ctx, kind, k):
             assert not np.isnan(np.log1p(-np.exp(lp))).any()
 
 
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", [2, 6, 12, 40, 100, 250])
+def test_a_row_does_not_depend_on_its_neighbours(ctx, kind, k):
+    """Rows of several to a wave: the same bits whatever scores the other rows hold."""
+    rng = np.random.default_rng(k)
+    n = 192
+    x = _rows(rng, n, k, 8.0) + rng.uniform(-300, 300, (n, 1))
+    codes = rng.integers(0, k, n)
+
+    def outputs(v):
+        c = Call(ctx, R.pack(v, kind), kind, 0.875, codes, top=2).check()
+        return [o.download()[:n] for o in (*c.out, c.top_lp, c.top_code)]
+    first = outputs(x)
+    for far in (3e4, 6e4 if kind == "f16" else 5e6, -6e4 if kind == "f16" else 3e38, -np.inf, np.nan):
+        y = x.copy()
+        y[1::2] = y[1::2] * 0.01 + far if abs(far) < 1e30 else far
+        for a, b in zip(first, outputs(y)):
+            assert np.array_equal(a[::2].view(np.uint32), b[::2].view(np.uint32))
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("k", LENGTHS[1:])
 def test_scores_further_apart_than_a_number(ctx, kind, k):
