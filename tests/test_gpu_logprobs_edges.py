@@ -90,3 +90,29 @@ def test_scores_further_apart_than_a_number(ctx, kind, k):
         lp = c.out[0].download()[:5]
         assert np.isfinite(lp).all() or beta == 3.0
         c.grad(rng.standard_normal(5), rng.standard_normal(5))
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", LENGTHS)
+def test_gradient_where_the_probability_is_zero(ctx, kind, k):
+    """Zero there, but for the code's own term, whatever the loss's gradients are, infinities among them."""
+    rng = np.random.default_rng(k)
+    n = 6
+    x = _rows(rng, n, k)
+    gone = rng.random((n, k)) < 0.5
+    gone[:, 0], gone[:, k - 1] = False, True
+    x[gone] = -np.inf
+    gl, gh = rng.standard_normal(n), rng.standard_normal(n)
+    gl[1], gl[2], gh[3], gh[4] = np.inf, -np.inf, 3e38, -np.inf
+    codes = np.array([0, 0, -1, 0, 0, k - 1])
+    c = Call(ctx, R.pack(x, kind), kind, 2.0, codes, top=1).check()
+    dgl, dgh = ctx.to_device(gl.astype(np.float32)), ctx.to_device(gh.astype(np.float32))
+    out = ctx.to_device(R.pack(np.full((n, k), 5.0), kind))
+    ctx.code_logprobs_grad(kind, c.ptr, n, k, k, 2.0, 4, c.dcodes, 1, c.out[1], c.out[2], c.out[3], dgl, dgh, out, k)
+    got = R.unpack(out.download(), kind)
+    own = np.zeros((n, k), bool)
+    own[5, k - 1] = True
+    assert (got[gone & ~own] == 0).all()
+    want = 2.0 * np.float64(np.float32(gl[5]))
+    assert abs(got[5, k - 1] - want) <= (R.HALF_STEP[kind] + R.U24) * 1.01 * abs(want)
+    assert not np.isfinite(got[1, 0]) and np.isfinite(got[0]).all()

@@ -618,7 +618,8 @@ struct GradArgs {
 };
 
 // 2^d with d = (x - m) * c - L2 is the probability (c = beta * log2 e, L2 = L * log2 e), d * ln 2 its logarithm; both held above 2^-200,
-// which is zero in f32, and zero times a number a zero.  A and B hold the factors: beta * (g_lp + g_H * (log p + H)) = A * d + B.
+// which is zero in f32.  A and B hold the factors: beta * (g_lp + g_H * (log p + H)) = A * d + B; where one of them is beyond f32, a
+// probability of zero still makes a gradient of zero (a compare and a choice per value: 1M rows of 64 bf16 57.3 -> 58.3 us, longer rows alike).
 // A lane has NV vectors of a row, G lanes a row or (G = 256, blockIdx.y) a piece of one; its code's own term is added where one of its
 // vectors holds the code.  A vector that would pass the row's end is read from elsewhere (Share) but only its own values are
 // written, one by one, so that the gradient may take the scores' place.
@@ -643,6 +644,7 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
     const bool none = m == kNegInf, bad = L != L || code >= a.k;
     const float from = none ? 0.0f : m, c = a.beta * kLog2e, L2 = none ? 0.0f : L * kLog2e, own = a.beta * gl;
     const float A = none ? 0.0f : a.beta * gh * kLn2, B = none ? 0.0f : bad ? __builtin_nanf("") : a.beta * __builtin_fmaf(gh, H, gl);
+    const float gone = bad && !none ? B : 0.0f;  // the gradient where the probability is zero, also times an infinite factor
     if (none) code = -1;  // (before all else: such a row's gradient is zero, whatever its code)
     const bool past = ((uintptr_t)a.grad & 127) == 0 && a.ld_grad % (128 / (int)sizeof(Raw)) == 0;  // whole lines pass the caches (412 -> 401 us)
 #pragma unroll
@@ -654,7 +656,8 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(GradArgs a) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const float d = fmaxf(__builtin_fmaf(x[v] - from, c, -L2), -200.0f);
-            x[v] = __builtin_amdgcn_exp2f(d) * -__builtin_fmaf(d, A, B);
+            const float p = __builtin_amdgcn_exp2f(d);
+            x[v] = p == 0.0f ? gone : p * -__builtin_fmaf(d, A, B);
         }
         const int64_t hit = code - base;
         if (hit >= 0 && hit < VEC) {
@@ -692,7 +695,8 @@ __global__ void __launch_bounds__(256) k_logprobs_grad_tiny(GradArgs a) {
     const float gl = code >= 0 ? a.g_logprob[row] : 0.0f;
     for (int j = 0; j < a.k; ++j) {
         const float lp = fmaxf(a.beta * (T::up(s[j]) - m) - L, -140.0f);
-        const float g = a.beta * ((j == code ? gl : 0.0f) - __builtin_amdgcn_exp2f(lp * kLog2e) * (gl + gh * (lp + H)));
+        const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+        const float g = a.beta * ((j == code ? gl : 0.0f) - (p == 0.0f ? 0.0f : p * (gl + gh * (lp + H))));
         ((typename T::Raw *)a.grad)[row * a.ld_grad + j] = T::down(m == kNegInf ? 0.0f : L != L || code >= a.k ? __builtin_nanf("") : g);
     }
 }
