@@ -439,7 +439,7 @@ int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_
                    int64_t ld_q, float *d_scale);
 
 /* d_out[i*ld_out + j] = (sum_t d_x[i][t] * d_w[j][t]) * d_xs[i] * d_ws[j] + d_bias[j], n rows against k codes: the sum
- * exact in 32-bit integers, the rest in f32, rounded to out_type.  d_bias may be NULL.  With the bias -|c_j|^2 / 2 of codewords c_j the
+ * exact in 32-bit integers, the rest in f32, rounded to out_type.  d_bias may be NULL: nothing is added.  With the bias -|c_j|^2 / 2 of codewords c_j the
  * order of a row's scores is that of the squared Euclidean distance, nearest first (up to the 8-bit rounding).
  * dim <= 131071, k <= 2^24; d_x rows are ld_x bytes apart, d_w rows ld_w.  The scores may not overlap an input.
  * Fastest where addresses and strides of d_x and d_w are multiples of 16.  The last row is then read up to the next multiple of 16 bytes; what

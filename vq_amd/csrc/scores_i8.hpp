@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(64 * WR * WC) k_scores_tile(ScoresArgs a, uint
     };
     for (int j = tid; j < TC; j += 64 * NW) {
         lws[j] = j < codes ? a.ws[code0 + j] : 0.0f;
-        lbias[j] = a.bias && j < codes ? a.bias[code0 + j] : 0.0f;
+        lbias[j] = a.bias && j < codes ? a.bias[code0 + j] : -0.0f;  // (adding -0 changes nothing, not even a zero's sign)
     }
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
