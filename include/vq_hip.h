@@ -444,7 +444,7 @@ int32_t vq_rows_i8(vq_ctx *ctx, int32_t type, const void *d_x, int64_t n, int64_
  * dim <= 131071, k <= 2^24; d_x rows are ld_x bytes apart, d_w rows ld_w.  The scores may not overlap an input.
  * Fastest where addresses and strides of d_x and d_w are multiples of 16.  The last row is then read up to the next multiple of 16 bytes; what
  * lies behind component dim counts for nothing.  Large calls on other rows copy them to aligned ones in a buffer of the context, which
- * grows and is kept like that of vq_code_logprobs below, and captures need the same call before alike. */
+ * grows and is kept like that of vq_code_logprobs below: a capture needs the same call before, or one of more rows against the same codes. */
 int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t n, int64_t ld_x, const int8_t *d_w,
                      const float *d_ws, int32_t k, int64_t ld_w, int32_t dim, const float *d_bias, int32_t out_type,
                      void *d_out, int64_t ld_out);
@@ -461,10 +461,10 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
  * log probability -inf, entropy 0.  A row with a NaN or +inf: L, log probability (of a given code), entropy and alternatives
  * are NaN, with codes -1.  Any of the outputs may be NULL, d_codes and d_logprob only together.
  * beta from 1e-30 to 1e30, top <= 32, k <= 2^20.  Sums are held in f32.
- * Rows above 16,384 codes are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context, which
- * grows with n * k and is kept until the context is destroyed.  So such a call may be captured into a graph where the same call has run
- * before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the capture goes on), and such graphs are to run on the
- * context's stream. */
+ * Rows above 16,384 codes are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context of up to 64 MiB, which
+ * grows with n, k and top and is kept until the context is destroyed.  So such a call may be captured into a graph where the same call, or one
+ * that is smaller in none of the three, has run before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the
+ * capture goes on), and such graphs are to run on the context's stream. */
 int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
                          int32_t code_bytes, const void *d_codes, int64_t code_stride, int32_t top, float *d_logprob,
                          float *d_max, float *d_logsum, float *d_entropy, float *d_top_logprob, int32_t *d_top_code);

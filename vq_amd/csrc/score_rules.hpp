@@ -168,6 +168,23 @@ inline RowPlan plan_rows(int64_t n, int32_t k, int32_t top, int bytes = 4) {
     return {256, e, (k + 256 * e - 1) / (256 * e), 256 * e};
 }
 
+// Rows of a launch: a grid has fewer than 2^32 lanes, and the parts' results (sums and lists) take at most 64 MiB.
+constexpr int64_t kPartBytes = 64 << 20;
+inline int64_t part_bytes(int32_t top) { return 12 + 8 * top; }
+inline int64_t logprob_rows_of_a_launch(const RowPlan &plan, int32_t top) {
+    if (plan.lanes < 256) return (int64_t)(1 << 23) * (256 / plan.lanes);
+    return std::max<int64_t>(1, (plan.parts == 1 ? 1 << 23 : kPartBytes / part_bytes(top)) / plan.parts);
+}
+// Bytes of the parts' results that a call provides for: no fewer than its plan takes, and no fewer than any call of no more rows, codes
+// and alternatives does, so that one of those may follow in a capture.  (A plan itself halves its parts' length, and so doubles their number,
+// where rows or codes get fewer: 1024 rows of 65,536 codes have 4 parts each, 1023 have 8.)
+inline int64_t part_workspace(int64_t n, int32_t k, int32_t top) {
+    if (k <= 16384) return 0;
+    const int64_t whole = (k + 16383) / 16384, halves = std::min<int64_t>(kMostParts, (k + 8191) / 8192);
+    const int64_t most = kPartBytes / part_bytes(top) + 1, rows = std::min(n, most);  // (products stay small)
+    return std::min(kPartBytes, std::max(rows * whole, std::min<int64_t>(rows * halves, 2 * 4095)) * part_bytes(top));
+}
+
 // How scores of aligned 8-bit rows are made (microseconds at n x dim x k, bf16 results, of the kernels compared):
 //   FEW        16 x 16 per workgroup, the components shared out among its waves: up to 32 tiles of 64 x 64, or 16 rows and 256 of them
 //              (32 x 4096 x 1024 6.0, T64 9.1; 14 x 3136 x 9152 8.4 and 9.3; 600 x 6000 x 600 25 and 17)

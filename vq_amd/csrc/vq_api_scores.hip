@@ -140,10 +140,8 @@ int32_t logprobs_slice(vq_ctx *ctx, int32_t type, const vq::LogprobArgs &a, cons
     }
     vq::PartArgs p{a, (int)plan.parts, plan.codes, nullptr, nullptr};
     if (plan.parts > 1) {
-        const size_t most = (size_t)a.n * plan.parts;
-        VQ_TRY(ensure_kept(ctx, ctx->score_parts, most * (8 * a.top + 12)));
-        p.keys = (uint64_t *)ctx->score_parts.p;
-        p.sums = (float *)(p.keys + most * a.top);
+        p.keys = (uint64_t *)ctx->score_parts.p;  // (the call has provided it)
+        p.sums = (float *)(p.keys + (size_t)a.n * plan.parts * a.top);
     }
     by_type(type, [&](auto t) {
         row_parts<decltype(t)>(ctx, p, plan.per_lane);
@@ -244,9 +242,8 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
                                               d_max, d_logsum, d_entropy, d_top_logprob, d_top_code), n, &go));
     if (!go) return VQ_OK;
     const vq::RowPlan plan = vq::plan_rows(n, k, top, vq::type_bytes(type));
-    // rows per launch: a grid has fewer than 2^32 lanes, and the parts' results at most 64 MiB
-    const int64_t slice = plan.lanes < 256 ? (int64_t)(1 << 23) * (256 / plan.lanes)
-                                           : std::max<int64_t>(1, (plan.parts == 1 ? 1 << 23 : (64 << 20) / (12 + 8 * top)) / plan.parts);
+    const int64_t slice = vq::logprob_rows_of_a_launch(plan, top);
+    if (plan.parts > 1) VQ_TRY(ensure_kept(ctx, ctx->score_parts, (size_t)vq::part_workspace(n, k, top)));
     const int e = vq::type_bytes(type);
     for (int64_t r = 0; r < n; r += slice) {
         vq::LogprobArgs a{(const char *)d_scores + r * ld * e, std::min(slice, n - r), ld, k, beta,
