@@ -461,7 +461,7 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
  * log probability -inf, entropy 0.  A row with a NaN or +inf: L, log probability (of a given code), entropy and alternatives
  * are NaN, with codes -1.  Any of the outputs may be NULL, d_codes and d_logprob only together.
  * beta from 1e-30 to 1e30, top <= 32, k <= 2^20.  Sums are held in f32.
- * Rows above 16,384 codes are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context of up to 64 MiB, which
+ * Rows above 16,384 codes are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context, which
  * grows with n, k and top and is kept until the context is destroyed.  So such a call may be captured into a graph where the same call, or one
  * that is smaller in none of the three, has run before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the
  * capture goes on), and such graphs are to run on the context's stream. */

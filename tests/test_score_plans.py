@@ -40,6 +40,28 @@ def lib(tmp_path_factory):
     return lib
 
 
+@pytest.mark.parametrize("bytes_", [2, 4])
+def test_every_code_of_a_row_has_a_lane(lib, bytes_):
+    """By the size of an element: every code has a register, and where lanes read whole vectors a row has one."""
+    out = (C.c_longlong * 4)()
+    for k in LENGTHS:
+        for n in ROWS:
+            for top in TOPS:
+                lib.plan(n, k, top, bytes_, out)
+                lanes, per_lane, parts, codes = out
+                assert parts * codes >= k and (parts - 1) * codes < k and codes <= lanes * per_lane
+                assert parts <= 64 and (parts == 1 or (lanes == 256 and codes == lanes * per_lane))
+                assert per_lane in {1: (16,), 4: (16,), 8: (32,), 64: (8, 16, 32, 64), 256: (32, 64)}[lanes]
+                assert k >= 16 // bytes_ or lanes == 1
+
+
+def test_sizes_of_the_tests_reach_every_way(lib):
+    assert set(SIZES) == set(range(7))
+    for way, sizes in SIZES.items():
+        for n, dim, k in sizes:
+            assert lib.way(n, k, dim) == way, (n, dim, k)
+
+
 def test_a_smaller_call_needs_no_more(lib):
     """The workspace of a call holds what its plan takes, and what any call takes that is larger in none of rows, codes and
     alternatives."""
