@@ -210,11 +210,10 @@ struct CodeScore {
         if (code >= 0 && code < a.k) score = T::up(((const typename T::Raw *)a.s)[row * a.ld + code]);
     }
 };
-// beta * (s - m) - L for a score s of a row: halves where the difference is beyond f32, as of scores of +-3e38, which a beta below 1
-// brings back.
+// beta * (s - m) - L for a score s of a row, by half the difference: scores of +-3e38 are further apart than f32 reaches, and a beta
+// below 1 brings them back.
 __device__ __forceinline__ float log_probability(float beta, float s, const RowSums &r) {
-    const float d = s - r.m;
-    return (d == kNegInf ? beta * (0.5f * s - 0.5f * r.m) * 2.0f : beta * d) - r.L;
+    return 2.0f * beta * __builtin_fmaf(0.5f, s, -0.5f * r.m) - r.L;
 }
 __device__ __forceinline__ void write_row(const LogprobArgs &a, int64_t row, const RowSums &r, const CodeScore &c) {
     if (a.max) a.max[row] = r.m;
