@@ -154,25 +154,20 @@ template <int G> __device__ __forceinline__ int group_min(int v) {
 // sums NaN: m is the largest number of the row.  One fused operation per exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
 // them, and taken out of the joined sums (away).  From |M| = 10^6 on, where r may be more than 1/16, exponents are formed from x - m.
 struct Sums {
-    float m, S, W, r = 0.0f;
-    // MIXED: the lanes have several rows' scores, and what the other rows hold does not change a row's sums.
-    template <bool MIXED, int E> static __device__ __forceinline__ Sums of(const float (&x)[E], float most, float c) {
-        Sums s(most, 0.0f, 0.0f);
-        const float from = is_bad(most) || most == kNegInf ? 0.0f : most, M = from * c;  // (such rows' sums are not looked at)
-        const bool far = fabsf(M) >= 1e6f;
-        if (__ballot(far) == 0) {
-            s.r = __builtin_fmaf(from, c, -M);
+    float m, S = 0.0f, W = 0.0f, r = 0.0f;
+    template <int E> __device__ __forceinline__ Sums(const float (&x)[E], float most, float c) : m(most) {
+        const float from = is_bad(m) || m == kNegInf ? 0.0f : m, M = from * c;  // (such rows' sums are not looked at)
+        if (__ballot(fabsf(M) >= 1e6f) == 0) {
+            r = __builtin_fmaf(from, c, -M);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s.add(__builtin_fmaf(x[e], c, -M));
-        } else if constexpr (MIXED) {
-            s.r = far ? 0.0f : __builtin_fmaf(from, c, -M);
+            for (int e = 0; e < E; ++e) add(__builtin_fmaf(x[e], c, -M));
+        } else {  // each row of the wave in its own way, so that its bits do not depend on what the others hold
+            const bool far = fabsf(M) >= 1e6f;
+            const float off = far ? from : 0.0f, by = far ? 0.0f : M;
+            r = far ? 0.0f : __builtin_fmaf(from, c, -M);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s.add(far ? (x[e] - from) * c : __builtin_fmaf(x[e], c, -M));
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) s.add((x[e] - from) * c);
+            for (int e = 0; e < E; ++e) add(__builtin_fmaf(x[e] - off, c, -by));
         }
-        return s;
     }
     __device__ __forceinline__ Sums(float most, float sum, float weighted) : m(most), S(sum), W(weighted) {}
     __device__ __forceinline__ void add(float exponent) {
@@ -292,7 +287,7 @@ __global__ void __launch_bounds__(256) k_logprobs_short(LogprobArgs a) {
 #pragma unroll
     for (int e = 1; e < SE::E; ++e) m = larger(m, r.x[e]);
     m = group_max<G>(m);
-    Sums sum = Sums::of<(G < 64)>(r.x, m, a.beta * kLog2e);
+    Sums sum(r.x, m, a.beta * kLog2e);
     sum.S = group_sum<G>(sum.S);
     sum.W = group_sum<G>(sum.W);
     sum.away();
@@ -361,7 +356,7 @@ __global__ void __launch_bounds__(256, E <= 16 ? 8 : E == 32 ? 6 : 4) k_logprobs
 #pragma unroll
     for (int e = 1; e < E; ++e) most = larger(most, r.x[e]);
     const float m = group_max<64>(most);
-    Sums sum = Sums::of<false>(r.x, m, a.beta * kLog2e);
+    Sums sum(r.x, m, a.beta * kLog2e);
     sum.S = group_sum<64>(sum.S);
     sum.W = group_sum<64>(sum.W);
     sum.away();
@@ -512,7 +507,7 @@ __global__ void __launch_bounds__(256, 16 / (int)sizeof(typename T::Raw) * NV <=
     floor = l.red[1][0];
     for (int w = 1; w < full; ++w) floor = fminf(floor, l.red[1][w]);
     floor = fmaxf(floor, -3.402823466e38f);  // -inf is none of them
-    Sums sum = Sums::of<false>(r.x, m, a.beta * kLog2e);
+    Sums sum(r.x, m, a.beta * kLog2e);
     sum.S = group_sum<64>(sum.S);
     sum.W = group_sum<64>(sum.W);
     if (lane == 0) l.red[2][wave] = sum.S, l.red[3][wave] = sum.W;
