@@ -459,7 +459,9 @@ int32_t vq_scores_i8(vq_ctx *ctx, const int8_t *d_x, const float *d_xs, int64_t 
  * is none given: log probability 0; a code of k or above gives NaN.
  * A score of -inf is a code that cannot be: it has probability zero.  A row of nothing else: m = L = -inf,
  * log probability -inf, entropy 0.  A row with a NaN or +inf: L, log probability (of a given code), entropy and alternatives
- * are NaN, with codes -1.  Any of the outputs may be NULL, d_codes and d_logprob only together.
+ * are NaN, with codes -1; m is +inf, or NaN with a NaN in the row.  No log probability is above zero, no entropy below, and
+ * no L but that of a row of nothing else.  Any of the
+ * outputs may be NULL, d_codes and d_logprob only together.
  * beta from 1e-30 to 1e30, top <= 32, k <= 2^20.  Sums are held in f32.
  * Rows above 16,384 codes are cut into parts that workgroups of their own take; the parts' results lie in a buffer of the context, which
  * grows with n, k and top and is kept until the context is destroyed.  So such a call may be captured into a graph where the same call, or one
@@ -474,8 +476,8 @@ int32_t vq_code_logprobs(vq_ctx *ctx, int32_t type, const void *d_scores, int64_
  *   d_grad[i][j] = beta * (g_lp * ([j = c] - p_j) - g_H * p_j * (log p_j + H))
  * with m, L and H as vq_code_logprobs left them (d_entropy may be NULL where d_g_entropy is), computed in f32 and rounded
  * to `type`, the type of the scores and of the gradient.  Probability zero, as which one below 2^-126 may count: gradient zero but for the code's own term.  A negative code takes no part in g_lp's
- * term; a row of -inf only has gradient zero, whatever its code; a code of k or above, or a row whose L is NaN, makes any other row's
- * gradient NaN.  d_grad may be d_scores itself (same stride); another overlap is refused. */
+ * term; a row of -inf only has gradient zero, whatever its code; a code of k or above, where d_g_logprob is given, or a row
+ * whose L is NaN makes any other row's gradient NaN.  d_grad may be d_scores itself (same stride); another overlap is refused. */
 int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta,
                               int32_t code_bytes, const void *d_codes, int64_t code_stride, const float *d_max,
                               const float *d_logsum, const float *d_entropy, const float *d_g_logprob,

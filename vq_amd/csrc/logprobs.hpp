@@ -152,7 +152,7 @@ template <int G> __device__ __forceinline__ int group_min(int v) {
 // Sums of the scores of a lane relative to the largest score m of their row or part: S = sum 2^d, W = sum 2^d d with
 // d = (x - m) * c, c = beta * log2 e, held above -200 (2^-200 is zero in f32, and zero times it a zero) but for a NaN, which makes the
 // sums NaN: m is the largest number of the row.  One fused operation per exponent, x * c - M with M = m * c rounded; what M is off by, r = m * c - M, is exact and the same for all of
-// them, and taken out of the joined sums (away).  From |M| = 10^6 on, where r may be more than 1/16, exponents are formed from x - m.
+// them, and taken out of the joined sums (away).  Below |M| = 10^6 r is at most 1/32; from there on exponents are formed from x - m.
 struct Sums {
     float m, S = 0.0f, W = 0.0f, r = 0.0f;
     template <int E> __device__ __forceinline__ Sums(const float (&x)[E], float most, float c) : m(most) {

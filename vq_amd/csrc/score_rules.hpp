@@ -145,13 +145,20 @@ inline Refusal check_code_logprobs_grad(int32_t type, const void *s, int64_t n, 
     return {};
 }
 
-// How the rows of a call go through the GPU (`lanes` of a row, `per_lane` codes each).  Rows of up to 256 codes have 1, 4 or 8 lanes, a wave where
-// there are no more than 16,384 of them and 8 alternatives or more (2000 x 24, f32, 32 alternatives 5.4 us, 14.3 in 4 lanes; x 256, 20: 5.5 and 18.8,
-// 2: the same), or more than 128 codes and 16 alternatives or more, for which five lanes more than those hold codes (200,000 x 256, f32, 20:
-// 104 and 143, 32: 113 and 220, 12: 100 and 90; x 128, 32: 238 and 219; bf16, 20: 115 and 143, 32, which all 32 lanes have to give: 309 and 221); of up to 4096 a wave with 8 to 64 codes per lane (600 x 4000, bf16, 5 alternatives: 6.3 us, in parts 10.2;
-// 10,000 x 2000, 13.4 and 22.6; 100,000 x 2000, 20 alternatives, 107 and 283).  Of up to 16,384 a workgroup of 256 lanes with 32 or 64 (8 x 8192, f32, 20 alternatives: 6.3 us, in eight parts
-// 10.8).  Longer ones go in parts of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough (one row of 65,536, f32, 20
-// alternatives: 10.6 us, 12.1 in parts of 16,384, 10.4 of 2048; 300 x 32,000, bf16: 7.7, 8.7, 9.4; 777 x 50,021, f16, 27.1, parts of equal length 27.6; 26.3 since then).
+// How the rows of a call go through the GPU: `lanes` of a row, `per_lane` codes each (microseconds of the ways compared, calls in a row):
+//   1, 4, 8 lanes  rows of up to 256 codes, several to a wave: the alternatives one after another (200,000 x 256, f32, 12 alternatives
+//                  92, a wave each 107; 2000 x 256, 2 alternatives 5.4 and 5.5)
+//   a wave, 8      up to 512 codes; of shorter rows those with many alternatives, which a wave lists and sorts at once: up to 16,384 rows with 8
+//                  or more (2000 x 24, f32, 32 alternatives 5.3, in 4 lanes 18; x 256, 20: 5.4, in 8 lanes 19; the line is low for the
+//                  most rows and the fewest alternatives, 16,384 x 24, f16, 8: 11.3 and 6.4), and above 128 codes those with 16 or more for
+//                  which five lanes more than these hold codes (200,000 x 256, f32, 20: 112 and 145, 16: 110 and 119; x 128, 32: 240 and
+//                  222; bf16, x 256, 20: 119 and 143, 32, which all the 32 lanes with codes would have to give: 310 and 220)
+//   a wave         up to 4096 codes, 16 to 64 per lane (600 x 4000, bf16, 5 alternatives 6.1, a workgroup each 6.7; 10,000 x 2000, 5:
+//                  15 and 32; 100,000 x 2000, 20: 109 and 360)
+//   a workgroup    up to 16,384 codes, 32 or 64 per lane (8 x 16,384, f32, 20 alternatives 7.7, in two parts 11.7)
+//   parts          longer rows: of 16,384 codes, or of 8192 where those would be fewer than 4096 workgroups and 64 parts are enough
+//                  (777 x 50,021, f16, 5 alternatives 26.5 in parts of 8192, 28.3; 300 x 32,000, bf16, 8: 13.9 and 15.2; 8192 x 65,536, 8:
+//                  214 and 198; about 1000 x 65,536 33.2 and 32.6)
 constexpr int kMostParts = 64;
 struct RowPlan {
     int lanes, per_lane;
@@ -213,8 +220,10 @@ inline ScoreWay score_way(int64_t n, int32_t k, int32_t dim) {
     return T128_MANY;
 }
 // Rows at other addresses or strides: through k_scores_any, which takes them as they are; where there is more than 2^28 to
-// multiply and 32 rows and codes or more, they are copied to aligned rows first (4096 x 4099 x 4096 at a stride of 4099 282 us, 90 so),
-// up to 1 GiB of codes, and of rows as many at a time as make 512 MiB.
+// multiply and 32 rows and codes or more, they are copied to aligned rows first (4096 x 4099 x 4096 at a stride of 4099 282 us, 90 so; about
+// 2^28: 256 x 1000 x 1000 at 1001 14.3 and 11.6, 512 x 100 x 5000 at 101 10.5 and 10.9), up to 1 GiB of codes, and of rows as many at a time
+// as make 512 MiB.  The line at 32 is not where the two meet: of 1 to 31 rows at a stride of 1000 against 65,536 aligned codes the copy would
+// take 2 to 3 us off 18 to 20, while 32 and 64 such rows against as many codes at that stride take 44, as they are 20 and 26.
 constexpr int64_t kPackRows = 512 << 20, kPackCodes = 1 << 30;
 inline int64_t packed_stride(int32_t dim) { return (dim + 15) / 16 * 16; }
 inline bool score_pack(int64_t n, int32_t k, int32_t dim) {
