@@ -287,7 +287,7 @@ def _plain_distill(s):
         loss = torch.where(q > 0, q * (lq - mine), 0.0).sum(1)
         if c["rest"]:
             loss = loss + torch.where(r > 0, r * (r.log() - logrest), 0.0)
-        out = [loss, m, logsum, logrest]
+        out = [loss, m, logsum] + [logrest] * c["rest"]
         if not c["grad"]:
             return tuple(out)
     p = (x - m.masked_fill(none, 0.0)[:, None]).mul_(beta).sub_(logsum.masked_fill(none, 0.0)[:, None])
@@ -368,13 +368,13 @@ def run(state):
     if op == "distill":
         with_grad = c["grad"]
         ctx.code_distill(c["type"], s["scores"].data_ptr(), n, s["ld"], k, c["beta"], c["top"], s["lp"].data_ptr(), s["code"].data_ptr(), c["top"],
-                         c["rest"], s["loss"].data_ptr(), s["max"].data_ptr(), s["logsum"].data_ptr(), s["logrest"].data_ptr(),
+                         c["rest"], s["loss"].data_ptr(), s["max"].data_ptr(), s["logsum"].data_ptr(), s["logrest"].data_ptr() if c["rest"] else None,
                          s["g"].data_ptr() if with_grad else None, s["grad"].data_ptr() if with_grad else None, s["ld"])
-        got = s["loss"], s["max"], s["logsum"], s["logrest"]
+        got = (s["loss"], s["max"], s["logsum"]) + ((s["logrest"],) if c["rest"] else ())
         return got + (s["grad"],) if with_grad else got
     if op == "back":
         ctx.code_distill_grad(c["type"], s["scores"].data_ptr(), n, s["ld"], k, c["beta"], c["top"], s["lp"].data_ptr(), s["code"].data_ptr(), c["top"],
-                              c["rest"], s["max"].data_ptr(), s["logsum"].data_ptr(), s["logrest"].data_ptr(), s["g"].data_ptr(),
+                              c["rest"], s["max"].data_ptr(), s["logsum"].data_ptr(), s["logrest"].data_ptr() if c["rest"] else None, s["g"].data_ptr(),
                               s["grad"].data_ptr(), s["ld"])
         return s["grad"]
     ctx.code_verify(c["type"], s["target"].data_ptr(), s["ld"], c["beta"], s["draft"].data_ptr() if s["draft"] is not None else None, s["ld"],
@@ -398,7 +398,7 @@ def work(case):
     if op == "verify":
         rows = n * (c["draft"] + 1) + (0 if c["greedy"] else n * c["draft"])
         return {"bytes": float(rows * k * e + n * (c["draft"] * (c["codes"] + 8) + 16)), "flops": 4.0 * rows * k}
-    lists = n * (c["top"] * 8 + 20)
+    lists = n * (c["top"] * 8 + 16 + 4 * c["rest"])
     if op == "back":
         return {"bytes": float(2 * n * k * e + lists), "flops": 4.0 * n * k}
     return {"bytes": float((2 if c["grad"] else 1) * n * k * e + lists), "flops": (8.0 if c["grad"] else 4.0) * n * k}
@@ -456,7 +456,7 @@ def _exact_rows(c, x, lp, code, g, stats):
         loss = (torch.special.xlogy(q, q) - torch.where(q > 0, q * logp.gather(1, idx), torch.zeros_like(q))).sum(1)
         loss = loss + torch.special.xlogy(r, r) - torch.where(r > 0, r * logrest, torch.zeros_like(r))
         m = x.double().max(1).values
-        out = [loss, m, torch.where(dead, lse, lse - m * c["beta"]), logrest]
+        out = [loss, m, torch.where(dead, lse, lse - m * c["beta"])] + [logrest] * c["rest"]
         if not c["grad"]:
             return out
     p = logp.exp()
