@@ -483,6 +483,84 @@ int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, i
                               const float *d_logsum, const float *d_entropy, const float *d_g_logprob,
                               const float *d_g_entropy, void *d_grad, int64_t ld_grad);
 
+/* ---- models over codes --------------------------------------------------------------------------- */
+
+/* What a model over codes reads (vq_code_embed), learns from (vq_code_embed_grad, vq_code_distill) and answers with (vq_code_verify).  No
+ * counterpart in the reference.  All are asynchronous and run on the context's stream; strides are in elements; any stride and any address
+ * that is a multiple of the element's size will do; what lies between rows or behind the last one is left as it is.  vq_code_embed_grad,
+ * vq_code_verify and, for rows above 16,384 codes, vq_code_distill use a buffer of the context, which grows with each of their sizes and is
+ * kept until the context is destroyed: such a call may be captured into a graph where the same call, or one that is smaller in no size,
+ * has run before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the capture goes on).  Graphs
+ * captured from one context share that buffer and are to run on its stream, one after another. */
+
+/* d_out[i] = scale * sum_s d_table[s * k + d_codes[i * code_stride + s]], n rows of dim from the m stages' tables of k rows each (m = 1: a
+ * lookup), summed in f32 in the order of the stages and rounded to out_type.  Codes have code_bytes = 1, 2 (unsigned) or 4 (signed) bytes, as
+ * vq_assign, vq_assign_u16, vq_rvq_encode and vq_tsvq_descend write them; a negative code is none: it adds nothing; a code of k or above
+ * makes its row NaN.  k and dim <= 2^20, m <= 64.  The output may not overlap an input. */
+int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k, int64_t ld_table, int32_t dim, int32_t m,
+                      int32_t code_bytes, const void *d_codes, int64_t n, int64_t code_stride, float scale, int32_t out_type,
+                      void *d_out, int64_t ld_out);
+
+/* The gradient of the tables from that of the rows, d_g (n rows of dim):
+ *   d_grad[s * k + j] = scale * (sum of d_g[i] over the positions i whose code of stage s is j)
+ * or that added to what d_grad holds (accumulate = 1).  Sums are held in f32, in an order that depends on the codes alone: the same call gives
+ * the same bits.  All m * k rows are written, codes without a position with zeros, except that with accumulate rows without a position
+ * are not touched; n = 0 writes zeros, too.  A code that is negative, or k or above, takes no part.  n * m <= 2^30.
+ * d_grad may not overlap an input. */
+int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n, int64_t ld_g, int32_t dim, int32_t m,
+                           int32_t code_bytes, const void *d_codes, int64_t code_stride, float scale, int32_t k, int32_t accumulate,
+                           int32_t grad_type, void *d_grad, int64_t ld_grad);
+
+/* Rows of scores against a teacher's best alternatives: codes and log probabilities, `top` per row, ld_teacher apart, as vq_code_logprobs
+ * writes them (d_top_code, d_top_logprob) for the teacher's own scores.  With p_j = exp(beta * s_j) / sum and the teacher's q_t:
+ *   d_loss[i] = sum_t q_t (log q_t - log p_{c_t})  [+ r (log r - log R)]
+ *   rest = 0   q_t = the alternatives' probabilities over their sum
+ *   rest = 1   q_t = the probabilities as they are; what they leave, r = max(0, 1 - sum_t q_t), is one more class beside them, against
+ *              R, the probability of all codes that are no alternative (no such term where no other code can be: its scores are all -inf)
+ *   d_max, d_logsum   m and L as vq_code_logprobs writes them
+ *   d_logrest         log R; -inf where no other code can be
+ * An entry with a negative code, or with the log probability -inf, is no alternative; one whose probability is below 2^-149 counts as zero in
+ * the loss.  Of entries with the same code each counts.  A row without any alternative: loss and gradient 0, whatever its scores.  An alternative of
+ * k or above, or a log probability that is NaN or +inf: loss and gradient NaN.  Rows of -inf only, with a NaN or with +inf:
+ * m and L as vq_code_logprobs has them, log R -inf or NaN, the loss +inf (against a teacher with alternatives) or NaN.
+ * d_g_loss and d_grad, together or not at all: the gradient by the scores in the same call,
+ *   d_grad[i][j] = d_g_loss[i] * beta * (Q p_j - q_j), or, for rest = 1 and codes that are no alternative, d_g_loss[i] * beta * (Q R - r) p_j / R
+ * with Q = sum_t q_t + r, rounded to `type`; a row of -inf only has gradient zero; a probability of zero, as which one below 2^-126 may count,
+ * makes the p_j's terms zero.  d_grad may be d_scores itself (same stride); another overlap is refused.
+ * Of d_loss, d_max, d_logsum and d_logrest any may be NULL.  beta from 1e-30 to 1e30, top <= 64, k <= 2^20.  Sums are held in f32, the
+ * teacher's in f64. */
+int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta, int32_t top,
+                        const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest, float *d_loss,
+                        float *d_max, float *d_logsum, float *d_logrest, const float *d_g_loss, void *d_grad, int64_t ld_grad);
+
+/* That gradient alone, from what vq_code_distill left: d_max, d_logsum and, for rest = 1, d_logrest (else it may be NULL).  d_grad may be
+ * d_scores itself (same stride); another overlap is refused. */
+int32_t vq_code_distill_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta, int32_t top,
+                             const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest,
+                             const float *d_max, const float *d_logsum, const float *d_logrest, const float *d_g_loss, void *d_grad,
+                             int64_t ld_grad);
+
+/* Drafted codes of n sequences against the probabilities of a model's scores, and the code that comes next, from given random numbers.
+ *   d_target   n * (draft + 1) rows of k scores, ld_target apart: row b * (draft + 1) + d has those of position d of sequence b, whose
+ *              probabilities are p = softmax(beta * row)
+ *   d_draft    n * draft rows, ld_draft apart, of the scores that the drafts were drawn from, q = softmax(beta_draft * row); or NULL: a
+ *              draft that was not drawn, q = 1 for its code (beta_draft and ld_draft are not looked at)
+ *   d_codes    draft codes per sequence, code_stride apart; a negative one ends the sequence's drafts
+ *   d_uniform  draft + 1 numbers from [0, 1) per sequence, ld_uniform apart
+ * Drafted code c of position d stays where the ones before it do and d_uniform[d] * q_c < p_c.  Of the first that does not stay the position
+ * gets a code drawn from max(p - q, 0) (from p, should nothing be left of that); where all stay the position behind the last gets one from p: the
+ * first code at which the sum of the weights up to it is above d_uniform[draft] times the sum of all (the last code with a weight, should
+ * there be none).  Exponentials and sums are held in f64.
+ *   d_accepted[b]                  how many drafted codes stay
+ *   d_out[b * ld_out + 0..draft]   these, the next code, -1 behind it
+ * A position whose row, or whose draft's row, has no score above -inf, a NaN or +inf, or whose drafted code is k or above, is answered
+ * with -1, and the drafts from there on do not stay.  draft = 0 draws one code per row.  draft <= 63, k <= 2^20, the betas from 1e-30
+ * to 1e30.  An output may not overlap another array. */
+int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t ld_target, float beta, const void *d_draft,
+                       int64_t ld_draft, float beta_draft, int64_t n, int32_t draft, int32_t k, int32_t code_bytes,
+                       const void *d_codes, int64_t code_stride, const float *d_uniform, int64_t ld_uniform, int32_t *d_accepted,
+                       int32_t *d_out, int64_t ld_out);
+
 #ifdef __cplusplus
 }
 #endif

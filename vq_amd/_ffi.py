@@ -86,6 +86,14 @@ SYMBOLS = {
                                 _vp, _vp]),
     "vq_code_logprobs_grad": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _vp, _vp, _vp,
                                      _vp, _vp, _i64]),
+    "vq_code_embed": (_i32, [_vp, _i32, _vp, _i32, _i64, _i32, _i32, _i32, _vp, _i64, _i64, C.c_float, _i32, _vp, _i64]),
+    "vq_code_embed_grad": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64, C.c_float, _i32, _i32, _i32, _vp, _i64]),
+    "vq_code_distill": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, C.c_float, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _i64]),
+    "vq_code_distill_grad": (_i32, [_vp, _i32, _vp, _i64, _i64, _i32, C.c_float, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp,
+                                    _i64]),
+    "vq_code_verify": (_i32, [_vp, _i32, _vp, _i64, C.c_float, _vp, _i64, C.c_float, _i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp,
+                              _vp, _i64]),
     "vq_tsvq_quantize_host": (_i32, [_vp, _i32, _vp, _i64, _vp, _vp, _vp]),
 }
 
@@ -479,6 +487,43 @@ class Context:
         self._check(_lib.vq_code_logprobs_grad(self._h, _TYPES.get(type, type), _ptr(d_scores), n, ld, k, beta, code_bytes,
                                                _ptr(d_codes), code_stride, _ptr(d_max), _ptr(d_logsum), _ptr(d_entropy),
                                                _ptr(d_g_logprob), _ptr(d_g_entropy), _ptr(d_grad), ld_grad))
+
+    # -- models over codes ---------------------------------------------------------------------
+    def code_embed(self, type, d_table, k, ld_table, dim, m, code_bytes, d_codes, n, code_stride, scale, out_type, d_out, ld_out):
+        """Rows of the m stages' tables that the codes name, summed, times scale."""
+        self._check(_lib.vq_code_embed(self._h, _TYPES.get(type, type), _ptr(d_table), k, ld_table, dim, m, code_bytes,
+                                       _ptr(d_codes), n, code_stride, scale, _TYPES.get(out_type, out_type), _ptr(d_out), ld_out))
+
+    def code_embed_grad(self, type, d_g, n, ld_g, dim, m, code_bytes, d_codes, code_stride, scale, k, accumulate, grad_type, d_grad,
+                        ld_grad):
+        """Gradient of the tables from that of the rows; accumulate: added to what d_grad holds."""
+        self._check(_lib.vq_code_embed_grad(self._h, _TYPES.get(type, type), _ptr(d_g), n, ld_g, dim, m, code_bytes,
+                                            _ptr(d_codes), code_stride, scale, k, int(accumulate),
+                                            _TYPES.get(grad_type, grad_type), _ptr(d_grad), ld_grad))
+
+    def code_distill(self, type, d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, d_loss, d_max,
+                     d_logsum, d_logrest, d_g_loss=None, d_grad=None, ld_grad=0):
+        """Loss of rows of scores against a teacher's alternatives (rest: what they leave is one more class), and, with the
+        losses' gradients, the gradient of the scores.  Any output may be None.  d_grad may be d_scores."""
+        self._check(_lib.vq_code_distill(self._h, _TYPES.get(type, type), _ptr(d_scores), n, ld, k, beta, top,
+                                         _ptr(d_teacher_logprob), _ptr(d_teacher_code), ld_teacher, int(rest), _ptr(d_loss),
+                                         _ptr(d_max), _ptr(d_logsum), _ptr(d_logrest), _ptr(d_g_loss), _ptr(d_grad), ld_grad))
+
+    def code_distill_grad(self, type, d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, d_max,
+                          d_logsum, d_logrest, d_g_loss, d_grad, ld_grad):
+        """That gradient alone, from what code_distill left.  d_grad may be d_scores."""
+        self._check(_lib.vq_code_distill_grad(self._h, _TYPES.get(type, type), _ptr(d_scores), n, ld, k, beta, top,
+                                              _ptr(d_teacher_logprob), _ptr(d_teacher_code), ld_teacher, int(rest),
+                                              _ptr(d_max), _ptr(d_logsum), _ptr(d_logrest), _ptr(d_g_loss), _ptr(d_grad),
+                                              ld_grad))
+
+    def code_verify(self, type, d_target, ld_target, beta, d_draft, ld_draft, beta_draft, n, draft, k, code_bytes, d_codes,
+                    code_stride, d_uniform, ld_uniform, d_accepted, d_out, ld_out):
+        """Which drafted codes stay, and the code that comes next, from given random numbers (d_draft: None where the drafts
+        have no scores)."""
+        self._check(_lib.vq_code_verify(self._h, _TYPES.get(type, type), _ptr(d_target), ld_target, beta, _ptr(d_draft),
+                                        ld_draft, beta_draft, n, draft, k, code_bytes, _ptr(d_codes), code_stride,
+                                        _ptr(d_uniform), ld_uniform, _ptr(d_accepted), _ptr(d_out), ld_out))
 
 
 def _ptr(a):

@@ -1,0 +1,234 @@
+// What the calls of models over codes (tables of vectors, distillation, verification of drafts) take and refuse, and how their
+// work is shared out: rules on sizes, strides and addresses alone, without HIP, so that a CPU test can go through them.
+#pragma once
+#include "score_rules.hpp"
+
+namespace vq {
+
+constexpr int32_t kMaxStages = 64;      // codes of a position
+constexpr int32_t kMaxEmbedDim = 1 << 20;
+constexpr int32_t kMaxTeacher = 64;     // a teacher's alternatives of a row: a lane each
+constexpr int32_t kMaxDraft = 63;       // drafted codes of a sequence: with the code that comes next a lane each
+
+inline Refusal check_code_array(const void *codes, int32_t code_bytes, int64_t n, int64_t code_stride, int32_t row) {
+    if (code_bytes != 1 && code_bytes != 2 && code_bytes != 4) return refuse(VQ_ERR_INVALID_ARG, "codes have 1, 2 or 4 bytes");
+    if (code_stride < row || too_long(n, code_stride, code_bytes)) return refuse(VQ_ERR_INVALID_ARG, "stride of the codes");
+    if (misaligned(codes, code_bytes)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    return {};
+}
+
+// Sizes of a table and of the rows that are read from it or summed into it.
+inline Refusal check_table(int32_t type, int32_t out_type, int64_t n, int32_t k, int32_t dim, int32_t m, int64_t ld_table, int64_t ld_rows,
+                           int table_bytes, int row_bytes, float scale) {
+    if (!type_bytes(type) || !type_bytes(out_type)) return refuse(VQ_ERR_INVALID_ARG, "no such type");
+    if (n < 0 || k <= 0 || dim <= 0 || m <= 0) return refuse(VQ_ERR_INVALID_ARG, "n must not be negative, k, dim and m must be greater than 0");
+    if (k > kMaxRowCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 1048576");
+    if (dim > kMaxEmbedDim) return refuse(VQ_ERR_UNSUPPORTED, "dim must be at most 1048576");
+    if (m > kMaxStages) return refuse(VQ_ERR_UNSUPPORTED, "m must be at most 64");
+    if (ld_table < dim || ld_rows < dim) return refuse(VQ_ERR_INVALID_ARG, "a row stride is below dim");
+    if (too_long((int64_t)m * k, ld_table, table_bytes) || too_long(n, ld_rows, row_bytes))
+        return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
+    if (!(scale >= -3.402823466e38f && scale <= 3.402823466e38f)) return refuse(VQ_ERR_INVALID_ARG, "scale must be finite");
+    return {};
+}
+
+inline Refusal check_code_embed(int32_t type, const void *table, int32_t k, int64_t ld_table, int32_t dim, int32_t m, int32_t code_bytes,
+                                const void *codes, int64_t n, int64_t code_stride, float scale, int32_t out_type, const void *out, int64_t ld_out) {
+    const int e = type_bytes(type), o = type_bytes(out_type);
+    Refusal r = check_table(type, out_type, n, k, dim, m, ld_table, ld_out, e, o, scale);
+    if (r.status == VQ_OK) r = check_code_array(codes, code_bytes, n, code_stride, m);
+    if (r.status != VQ_OK || n == 0) return r;
+    if (!table || !codes || !out) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(table, e) || misaligned(out, o)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span so(out, n, ld_out * o, (int64_t)dim * o);
+    if (so.meets({table, (int64_t)m * k, ld_table * e, (int64_t)dim * e}) || so.meets({codes, n, code_stride * code_bytes, (int64_t)m * code_bytes}))
+        return refuse(VQ_ERR_INVALID_ARG, "the output overlaps an input");
+    return {};
+}
+
+inline Refusal check_code_embed_grad(int32_t type, const void *g, int64_t n, int64_t ld_g, int32_t dim, int32_t m, int32_t code_bytes,
+                                     const void *codes, int64_t code_stride, float scale, int32_t k, int32_t accumulate, int32_t grad_type,
+                                     const void *grad, int64_t ld_grad) {
+    const int e = type_bytes(type), o = type_bytes(grad_type);
+    Refusal r = check_table(type, grad_type, n, k, dim, m, ld_grad, ld_g, o, e, scale);
+    if (r.status == VQ_OK) r = check_code_array(codes, code_bytes, n, code_stride, m);
+    if (r.status != VQ_OK) return r;
+    if (n > ((int64_t)1 << 30) / m) return refuse(VQ_ERR_UNSUPPORTED, "n * m must be at most 2^30");
+    if (accumulate != 0 && accumulate != 1) return refuse(VQ_ERR_INVALID_ARG, "accumulate is 0 or 1");
+    if (n == 0 && accumulate) return {};
+    if (!grad || (n > 0 && (!g || !codes))) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(g, e) || misaligned(grad, o)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span so(grad, (int64_t)m * k, ld_grad * o, (int64_t)dim * o);
+    if (so.meets({g, n, ld_g * e, (int64_t)dim * e}) || so.meets({codes, n, code_stride * code_bytes, (int64_t)m * code_bytes}))
+        return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps an input");
+    return {};
+}
+
+// What both calls on a teacher's alternatives take.
+inline Refusal check_teacher(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t top, const void *lp,
+                             const void *code, int64_t ld_teacher, int32_t rest) {
+    const Refusal r = check_scored_codes(type, s, n, ld, k, beta, 4, nullptr, 1);
+    if (r.status != VQ_OK) return r;
+    if (top <= 0) return refuse(VQ_ERR_INVALID_ARG, "top must be greater than 0");
+    if (top > kMaxTeacher) return refuse(VQ_ERR_UNSUPPORTED, "top must be at most 64");
+    if (ld_teacher < top || too_long(n, ld_teacher, 4)) return refuse(VQ_ERR_INVALID_ARG, "stride of the teacher's alternatives");
+    if (rest != 0 && rest != 1) return refuse(VQ_ERR_INVALID_ARG, "rest is 0 or 1");
+    if (n == 0) return {};
+    if (!lp || !code) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(lp, 4) || misaligned(code, 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    return {};
+}
+// The gradient of the scores: in place, or apart from all that is read (and, in the same call, from what else is written).
+inline Refusal check_score_grad(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, int32_t top, const void *lp, const void *code,
+                                int64_t ld_teacher, const void *g, const void *grad, int64_t ld_grad) {
+    const int e = type_bytes(type);
+    if (ld_grad < k || too_long(n, ld_grad, e)) return refuse(VQ_ERR_INVALID_ARG, "stride of the gradient");
+    if (n == 0) return {};
+    if (!g || !grad) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(g, 4) || misaligned(grad, e)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span sg(grad, n, ld_grad * e, (int64_t)k * e);
+    if (sg.meets({lp, n, ld_teacher * 4, top * 4}) || sg.meets({code, n, ld_teacher * 4, top * 4}) || sg.meets({g, 1, 0, n * 4}))
+        return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps an input");
+    if (!(grad == s && ld_grad == ld) && sg.meets({s, n, ld * e, (int64_t)k * e}))
+        return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps the scores otherwise than in place");
+    return {};
+}
+
+inline Refusal check_code_distill(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t top, const void *lp,
+                                  const void *code, int64_t ld_teacher, int32_t rest, const void *loss, const void *max, const void *logsum,
+                                  const void *logrest, const void *g, const void *grad, int64_t ld_grad) {
+    Refusal r = check_teacher(type, s, n, ld, k, beta, top, lp, code, ld_teacher, rest);
+    if (r.status != VQ_OK) return r;
+    if ((g == nullptr) != (grad == nullptr)) return refuse(VQ_ERR_INVALID_ARG, "a gradient and the gradients of the losses go together");
+    if (grad) r = check_score_grad(type, s, n, ld, k, top, lp, code, ld_teacher, g, grad, ld_grad);
+    if (r.status != VQ_OK || n == 0) return r;
+    const int e = type_bytes(type);
+    const void *outs[] = {loss, max, logsum, logrest};
+    const Span in[] = {{s, n, ld * e, (int64_t)k * e}, {lp, n, ld_teacher * 4, top * 4}, {code, n, ld_teacher * 4, top * 4}, {g, 1, 0, n * 4},
+                       {grad, n, ld_grad * e, (int64_t)k * e}};
+    for (int a = 0; a < 4; ++a) {
+        if (misaligned(outs[a], 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+        const Span oa(outs[a], 1, 0, n * 4);
+        for (int b = 0; b < a; ++b)
+            if (oa.meets({outs[b], 1, 0, n * 4})) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+        for (const Span &i : in)
+            if (oa.meets(i)) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+    }
+    return {};
+}
+
+inline Refusal check_code_distill_grad(int32_t type, const void *s, int64_t n, int64_t ld, int32_t k, float beta, int32_t top, const void *lp,
+                                       const void *code, int64_t ld_teacher, int32_t rest, const void *max, const void *logsum,
+                                       const void *logrest, const void *g, const void *grad, int64_t ld_grad) {
+    Refusal r = check_teacher(type, s, n, ld, k, beta, top, lp, code, ld_teacher, rest);
+    if (r.status == VQ_OK) r = check_score_grad(type, s, n, ld, k, top, lp, code, ld_teacher, g, grad, ld_grad);
+    if (r.status != VQ_OK || n == 0) return r;
+    if (!max || !logsum || (rest && !logrest)) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    const int e = type_bytes(type);
+    const Span sg(grad, n, ld_grad * e, (int64_t)k * e);
+    for (const void *p : {max, logsum, rest ? logrest : nullptr}) {
+        if (misaligned(p, 4)) return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+        if (sg.meets({p, 1, 0, n * 4})) return refuse(VQ_ERR_INVALID_ARG, "the gradient overlaps an input");
+    }
+    return {};
+}
+
+inline Refusal check_code_verify(int32_t type, const void *target, int64_t ld_target, float beta, const void *drafts, int64_t ld_draft,
+                                 float beta_draft, int64_t n, int32_t draft, int32_t k, int32_t code_bytes, const void *codes, int64_t code_stride,
+                                 const void *uniform, int64_t ld_uniform, const void *accepted, const void *out, int64_t ld_out) {
+    const int e = type_bytes(type);
+    if (!e) return refuse(VQ_ERR_INVALID_ARG, "no such type");
+    if (n < 0 || draft < 0 || k <= 0) return refuse(VQ_ERR_INVALID_ARG, "n and draft must not be negative and k must be greater than 0");
+    if (k > kMaxRowCodes) return refuse(VQ_ERR_UNSUPPORTED, "k must be at most 1048576");
+    if (draft > kMaxDraft) return refuse(VQ_ERR_UNSUPPORTED, "draft must be at most 63");
+    if (n > (int64_t)1 << 30) return refuse(VQ_ERR_UNSUPPORTED, "n must be at most 2^30");
+    if (ld_target < k || (drafts && ld_draft < k)) return refuse(VQ_ERR_INVALID_ARG, "the row stride is below k");
+    if (too_long(n * (draft + 1), ld_target, e) || (drafts && too_long(n * (draft + 1), ld_draft, e)))
+        return refuse(VQ_ERR_INVALID_ARG, "rows and stride overflow");
+    if (!(beta >= 1e-30f) || !(beta <= 1e30f)) return refuse(VQ_ERR_INVALID_ARG, "beta must be between 1e-30 and 1e30");
+    if (drafts && (!(beta_draft >= 1e-30f) || !(beta_draft <= 1e30f)))
+        return refuse(VQ_ERR_INVALID_ARG, "beta of the drafts must be between 1e-30 and 1e30");
+    if (draft > 0) {
+        const Refusal r = check_code_array(codes, code_bytes, n, code_stride, draft);
+        if (r.status != VQ_OK) return r;
+    }
+    if (ld_uniform < draft + 1 || ld_out < draft + 1 || too_long(n, ld_uniform, 4) || too_long(n, ld_out, 4))
+        return refuse(VQ_ERR_INVALID_ARG, "stride of the random numbers or of the output");
+    if (n == 0) return {};
+    if (!target || !uniform || !accepted || !out || (draft > 0 && !codes)) return refuse(VQ_ERR_INVALID_ARG, "null pointer");
+    if (misaligned(target, e) || misaligned(drafts, e) || misaligned(uniform, 4) || misaligned(accepted, 4) || misaligned(out, 4))
+        return refuse(VQ_ERR_INVALID_ARG, "misaligned pointer");
+    const Span in[] = {{target, n * (draft + 1), ld_target * e, (int64_t)k * e}, {drafts, n * draft, ld_draft * e, (int64_t)k * e},
+                       {draft > 0 ? codes : nullptr, n, code_stride * code_bytes, (int64_t)draft * code_bytes}, {uniform, n, ld_uniform * 4, (draft + 1) * 4}};
+    const Span sa(accepted, 1, 0, n * 4), so(out, n, ld_out * 4, (draft + 1) * 4);
+    if (sa.meets(so)) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+    for (const Span &i : in)
+        if (sa.meets(i) || so.meets(i)) return refuse(VQ_ERR_INVALID_ARG, "an output overlaps another array");
+    return {};
+}
+
+// ---- sums by code ------------------------------------------------------------------------------------
+// The positions of each stage in the order of their codes, as a list of n positions with the codes beside it, and where each code's
+// positions begin: k + 1 numbers.  A workgroup lists the codes of one bucket.
+constexpr int kBucketMost = 512;
+inline int32_t bucket_codes(int32_t k) { return std::min<int32_t>(kBucketMost, (k + 255) / 256); }
+// A code of more positions than this is summed in pieces of as many positions of the list, whose sums are joined afterwards.
+constexpr int kLongCode = 1024;
+inline int64_t embed_chunks(int64_t n) { return n > kLongCode ? (n + kLongCode - 1) / kLongCode : 0; }
+// Bytes of a call's workspace, in the order in which they lie there; each grows with each size.
+struct EmbedWork {
+    int64_t start, rows, codes, partial, bytes;
+};
+inline EmbedWork embed_work(int64_t n, int32_t k, int32_t dim, int32_t m) {
+    const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+    EmbedWork w;
+    w.start = 0;
+    w.rows = up((int64_t)m * (k + 1) * 4);
+    w.codes = w.rows + up(m * n * 4);
+    w.partial = w.codes + up(m * n * 4);
+    w.bytes = w.partial + up(m * embed_chunks(n) * 2 * ((dim + 15) / 16 * 16) * 4);
+    return w;
+}
+
+// ---- rows of scores against a teacher ------------------------------------------------------------------
+// How a row of k scores goes through the GPU: by `waves` waves that hold it whole, 64 * per_lane codes each, or (waves 0) in parts of
+// 256 * per_lane codes, a workgroup each.
+struct DistillPlan {
+    int waves, per_lane;
+    int32_t parts;
+};
+inline DistillPlan plan_distill(int64_t n, int32_t k, bool grad) {
+    if (k <= 4096) return {1, k <= 512 ? 8 : k <= 1024 ? 16 : k <= 2048 ? 32 : 64, 1};
+    if (k <= 16384) return {4, k <= 8192 ? 32 : 64, 1};
+    if (grad && k <= 65536 && n >= 64) return {16, k <= 32768 ? 32 : 64, 1};
+    const int64_t whole = (k + 16383) / 16384;
+    const int e = n * whole < 4096 && k <= kMostParts * 8192 ? 32 : 64;
+    return {0, e, (k + 256 * e - 1) / (256 * e)};
+}
+// Rows of a launch (a grid has fewer than 2^32 lanes) and bytes of the parts' results, which lie beside one another for a launch's rows.
+// (and, behind them, three numbers per row for the gradient)
+constexpr int kDistillPartBytes = 8;
+inline int64_t distill_rows_of_a_launch(const DistillPlan &p) {
+    return p.waves == 1 ? (int64_t)1 << 25 : p.waves ? ((int64_t)1 << 24) / (p.waves * 2) : std::max<int64_t>(1, (kPartBytes / kDistillPartBytes) / p.parts);
+}
+inline int64_t distill_work(int64_t n, int32_t k) {
+    if (k <= 16384) return 0;
+    const int64_t most = (k + 8191) / 8192;  // (no plan cuts a row into more)
+    return std::min<int64_t>(2 * kPartBytes, std::min(n, kPartBytes) * (most * kDistillPartBytes + 12));
+}
+
+// ---- drafts --------------------------------------------------------------------------------------------
+// Rows of scores are cut into parts of 4096 codes; a sequence has draft + 1 rows of its own and as many of its drafts'.
+constexpr int kVerifyPart = 4096;
+inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyPart; }
+// Per row and part a maximum and a sum in 64 bits; per sequence and part a sum more.
+inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8); }
+static_assert(kMaxRowCodes / kVerifyPart * ((2 * kMaxDraft + 1) * 16 + 8) <= kPartBytes * 4, "one sequence fits");
+inline int64_t verify_sequences_of_a_launch(int32_t draft, int32_t k) {
+    return std::max<int64_t>(1, std::min((kPartBytes * 4) / verify_bytes_of_a_sequence(draft, k), ((int64_t)1 << 23) / (verify_parts(k) * (2 * draft + 1))));
+}
+inline int64_t verify_work(int64_t n, int32_t draft, int32_t k) {
+    return std::min(std::min(n, kPartBytes) * verify_bytes_of_a_sequence(draft, k), kPartBytes * 4);  // (at least one sequence's)
+}
+
+}  // namespace vq

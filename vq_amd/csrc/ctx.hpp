@@ -89,6 +89,7 @@ struct vq_ctx {
     // parts of long rows of scores, and aligned copies of 8-bit rows; what they were before they grew stays until the
     // context ends, since captured graphs may hold the addresses
     DevBuf score_parts, score_packed;
+    DevBuf code_work;            // lists of positions by code, parts of rows against a teacher or of drafts; kept like these two
     std::vector<void *> outgrown;
     uint32_t scores_lds_set = 0;  // dynamic-LDS limit granted to the tiles of scores, a bit per instance
     // optional per-kernel-class timing (HIP events on the stream)

@@ -1,0 +1,221 @@
+// C entry points of models over codes: tables of vectors, distillation, verification of drafts.
+#include "code_distill.hpp"
+#include "code_embed.hpp"
+#include "code_rules.hpp"
+#include "code_verify.hpp"
+#include "score_calls.hpp"
+
+using namespace vqh;
+
+namespace {
+
+// f(T, O) with the types of two arrays
+template <typename F> void by_types(int32_t type, int32_t other, F f) {
+    by_type(type, [&](auto t) { by_type(other, [&](auto o) { f(t, o); }); });
+}
+
+// The alternatives' rows of a launch, from row r on.
+vq::DistillArgs distill_slice(const vq::DistillArgs &a, int64_t r, int64_t rows, int e) {
+    vq::DistillArgs s = a;
+    const auto at = [&](float *p) { return p ? p + r : nullptr; };
+    s.s = (const char *)a.s + r * a.ld * e;
+    s.n = std::min(rows, a.n - r);
+    s.lp = a.lp + r * a.ld_teacher;
+    s.code = a.code + r * a.ld_teacher;
+    s.loss = at(a.loss), s.max = at(a.max), s.logsum = at(a.logsum), s.logrest = at(a.logrest);
+    s.g = a.g ? a.g + r : nullptr;
+    s.grad = a.grad ? (char *)a.grad + r * a.ld_grad * e : nullptr;
+    return s;
+}
+
+int32_t distill_grad(vq_ctx *ctx, int32_t type, const vq::DistillArgs &all) {
+    const int64_t slice = (int64_t)1 << 22;  // rows per launch: a grid has fewer than 2^32 lanes
+    for (int64_t r = 0; r < all.n; r += slice) {
+        const vq::DistillArgs a = distill_slice(all, r, slice, vq::type_bytes(type));
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            constexpr int VEC = 16 / (int)sizeof(typename T::Raw);
+            const auto waves = dim3((unsigned)cdiv64(a.n, 4));
+            if (a.k <= 512)
+                hipLaunchKernelGGL((vq::k_distill_grad<T, 1, 8 / VEC>), waves, dim3(256), 0, ctx->stream, a);
+            else if (a.k <= 1024)
+                hipLaunchKernelGGL((vq::k_distill_grad<T, 1, 16 / VEC>), waves, dim3(256), 0, ctx->stream, a);
+            else if (a.k <= 2048)
+                hipLaunchKernelGGL((vq::k_distill_grad<T, 1, 32 / VEC>), waves, dim3(256), 0, ctx->stream, a);
+            else
+                hipLaunchKernelGGL((vq::k_distill_grad<T, 4, 32 / VEC>), dim3((unsigned)a.n, (unsigned)cdiv(a.k, 256 * 32)), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
+    return VQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k, int64_t ld_table, int32_t dim, int32_t m,
+                      int32_t code_bytes, const void *d_codes, int64_t n, int64_t code_stride, float scale, int32_t out_type,
+                      void *d_out, int64_t ld_out) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_embed(type, d_table, k, ld_table, dim, m, code_bytes, d_codes, n, code_stride, scale, out_type,
+                                           d_out, ld_out), n, &go));
+    if (!go) return VQ_OK;
+    const int pieces = cdiv(dim, 16 / vq::type_bytes(type));
+    int shift = 0;
+    while (shift < 8 && 1 << shift < pieces) ++shift;
+    const unsigned across = cdiv(pieces, 1 << shift);
+    const int64_t slice = std::max<int64_t>(256, ((int64_t)1 << 31) / ((int64_t)across << shift));  // a grid has fewer than 2^32 lanes
+    for (int64_t r = 0; r < n; r += slice) {
+        const vq::EmbedArgs a{d_table, ld_table, k, dim, m, (const char *)d_codes + r * code_stride * code_bytes, code_bytes, std::min(slice, n - r),
+                              code_stride, scale, (char *)d_out + r * ld_out * vq::type_bytes(out_type), ld_out};
+        by_types(type, out_type, [&](auto t, auto o) {
+            hipLaunchKernelGGL((vq::k_code_embed<decltype(t), decltype(o)>), dim3((unsigned)cdiv64(a.n, 256 >> shift), across), dim3(256), 0,
+                               ctx->stream, a, shift);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
+    return VQ_OK;
+}
+
+int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n, int64_t ld_g, int32_t dim, int32_t m,
+                           int32_t code_bytes, const void *d_codes, int64_t code_stride, float scale, int32_t k, int32_t accumulate,
+                           int32_t grad_type, void *d_grad, int64_t ld_grad) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    // (without rows the gradient is still written)
+    VQ_TRY(admit(ctx, vq::check_code_embed_grad(type, d_g, n, ld_g, dim, m, code_bytes, d_codes, code_stride, scale, k, accumulate,
+                                                grad_type, d_grad, ld_grad), accumulate ? n : 1, &go));
+    if (!go) return VQ_OK;
+    const vq::EmbedWork work = vq::embed_work(n, k, dim, m);
+    VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)work.bytes));
+    char *w = (char *)ctx->code_work.p;
+    const vq::ListArgs l{d_codes, code_bytes, code_stride, (int)n, k, vq::bucket_codes(k), (int32_t *)(w + work.start), (int32_t *)(w + work.rows),
+                         (int32_t *)(w + work.codes)};
+    hipLaunchKernelGGL(vq::k_code_lists<16>, dim3(cdiv(k, l.width), m), dim3(1024), 0, ctx->stream, l);
+    VQ_HIP(ctx, hipGetLastError());
+    const int keys = 4;
+    const vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, l.start, l.rows, l.row_codes, (float *)(w + work.partial),
+                        (int)vq::embed_chunks(n), (dim + 15) / 16 * 16, keys, (int)cdiv(k, 16 * keys)};
+    const unsigned columns = 16 * 16 / vq::type_bytes(type);
+    by_types(type, grad_type, [&](auto t, auto o) {
+        hipLaunchKernelGGL((vq::k_embed_sums<decltype(t), decltype(o)>), dim3(a.groups + a.chunks, cdiv(dim, columns), m), dim3(256), 0, ctx->stream, a);
+    });
+    VQ_HIP(ctx, hipGetLastError());
+    if (a.chunks) {
+        by_type(grad_type, [&](auto o) {
+            hipLaunchKernelGGL(vq::k_embed_join<decltype(o)>, dim3(a.chunks, cdiv(dim, 64), m), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
+    return VQ_OK;
+}
+
+int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta, int32_t top,
+                        const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest, float *d_loss,
+                        float *d_max, float *d_logsum, float *d_logrest, const float *d_g_loss, void *d_grad, int64_t ld_grad) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_distill(type, d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest,
+                                             d_loss, d_max, d_logsum, d_logrest, d_g_loss, d_grad, ld_grad), n, &go));
+    if (!go) return VQ_OK;
+    const vq::DistillPlan plan = vq::plan_distill(n, k, d_grad != nullptr);
+    vq::DistillArgs all{d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, rest || d_logrest, d_loss, d_max, d_logsum,
+                        d_logrest, d_g_loss, d_grad, ld_grad, plan.parts, nullptr};
+    float *stats = nullptr;
+    const int64_t slice = vq::distill_rows_of_a_launch(plan);
+    if (plan.waves == 0) {
+        // the gradient of a row in parts is a call of its own, from the sums that the caller need not have asked for
+        VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::distill_work(n, k)));
+        all.sums = (float *)ctx->code_work.p;
+        stats = all.sums + std::min(slice, n) * plan.parts * 2;
+    }
+    for (int64_t r = 0; r < n; r += slice) {
+        vq::DistillArgs a = distill_slice(all, r, slice, vq::type_bytes(type));
+        if (plan.waves == 0 && a.grad) {
+            if (!a.max) a.max = stats;
+            if (!a.logsum) a.logsum = stats + std::min(slice, n);
+            if (!a.logrest && rest) a.logrest = stats + 2 * std::min(slice, n);
+        }
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            constexpr int VEC = 16 / (int)sizeof(typename T::Raw);
+            const dim3 waves((unsigned)cdiv64(a.n, 4)), rows((unsigned)a.n), wg(256);
+            if (plan.waves == 1 && plan.per_lane == 8)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 1, 8 / VEC>), waves, wg, 0, ctx->stream, a);
+            else if (plan.waves == 1 && plan.per_lane == 16)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 1, 16 / VEC>), waves, wg, 0, ctx->stream, a);
+            else if (plan.waves == 1 && plan.per_lane == 32)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 1, 32 / VEC>), waves, wg, 0, ctx->stream, a);
+            else if (plan.waves == 1)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 1, 64 / VEC>), waves, wg, 0, ctx->stream, a);
+            else if (plan.waves == 4 && plan.per_lane == 32)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 4, 32 / VEC>), rows, wg, 0, ctx->stream, a);
+            else if (plan.waves == 4)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 4, 64 / VEC>), rows, wg, 0, ctx->stream, a);
+            else if (plan.waves == 16 && plan.per_lane == 32)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 16, 32 / VEC>), rows, dim3(1024), 0, ctx->stream, a);
+            else if (plan.waves == 16)
+                hipLaunchKernelGGL((vq::k_distill_row<T, 16, 64 / VEC>), rows, dim3(1024), 0, ctx->stream, a);
+            else {
+                const dim3 parts((unsigned)(a.n * plan.parts));
+                if (plan.per_lane == 32)
+                    hipLaunchKernelGGL((vq::k_distill_part<T, 32 / VEC>), parts, wg, 0, ctx->stream, a);
+                else
+                    hipLaunchKernelGGL((vq::k_distill_part<T, 64 / VEC>), parts, wg, 0, ctx->stream, a);
+                hipLaunchKernelGGL(vq::k_distill_join<T>, waves, wg, 0, ctx->stream, a);
+            }
+        });
+        VQ_HIP(ctx, hipGetLastError());
+        if (plan.waves == 0 && a.grad) VQ_TRY(distill_grad(ctx, type, a));
+    }
+    return VQ_OK;
+}
+
+int32_t vq_code_distill_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta, int32_t top,
+                             const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest,
+                             const float *d_max, const float *d_logsum, const float *d_logrest, const float *d_g_loss, void *d_grad,
+                             int64_t ld_grad) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_distill_grad(type, d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher,
+                                                  rest, d_max, d_logsum, d_logrest, d_g_loss, d_grad, ld_grad), n, &go));
+    if (!go) return VQ_OK;
+    const vq::DistillArgs a{d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, rest, nullptr, const_cast<float *>(d_max),
+                            const_cast<float *>(d_logsum), const_cast<float *>(d_logrest), d_g_loss, d_grad, ld_grad, 1, nullptr};
+    return distill_grad(ctx, type, a);
+}
+
+int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t ld_target, float beta, const void *d_draft,
+                       int64_t ld_draft, float beta_draft, int64_t n, int32_t draft, int32_t k, int32_t code_bytes,
+                       const void *d_codes, int64_t code_stride, const float *d_uniform, int64_t ld_uniform, int32_t *d_accepted,
+                       int32_t *d_out, int64_t ld_out) {
+    if (!ctx) return VQ_ERR_INVALID_ARG;
+    bool go;
+    VQ_TRY(admit(ctx, vq::check_code_verify(type, d_target, ld_target, beta, d_draft, ld_draft, beta_draft, n, draft, k, code_bytes,
+                                            d_codes, code_stride, d_uniform, ld_uniform, d_accepted, d_out, ld_out), n, &go));
+    if (!go) return VQ_OK;
+    const int e = vq::type_bytes(type), parts = vq::verify_parts(k);
+    const int64_t slice = vq::verify_sequences_of_a_launch(draft, k);
+    VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
+    const void *drafts = draft > 0 ? d_draft : nullptr;
+    for (int64_t b = 0; b < n; b += slice) {
+        const int64_t here = std::min(slice, n - b), rows = here * (draft + 1 + (drafts ? draft : 0));
+        double *most = (double *)ctx->code_work.p, *sum = most + rows * parts;
+        const vq::VerifyArgs a{(const char *)d_target + b * (draft + 1) * ld_target * e, drafts ? (const char *)drafts + b * draft * ld_draft * e : nullptr,
+                               ld_target, ld_draft, beta * vq::kLog2e64, beta_draft * vq::kLog2e64, (int)here, draft, k, parts,
+                               draft ? (const char *)d_codes + b * code_stride * code_bytes : nullptr, code_bytes, code_stride,
+                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, sum + rows * parts};
+        by_type(type, [&](auto t) {
+            typedef decltype(t) T;
+            hipLaunchKernelGGL(vq::k_verify_part<T>, dim3((unsigned)(rows * parts)), dim3(256), 0, ctx->stream, a);
+            if (drafts) hipLaunchKernelGGL(vq::k_verify_left<T>, dim3((unsigned)(here * parts)), dim3(256), 0, ctx->stream, a);
+            hipLaunchKernelGGL(vq::k_verify_pick<T>, dim3((unsigned)here), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
+    return VQ_OK;
+}
+
+}  // extern "C"
