@@ -7,11 +7,18 @@
 
 namespace vq {
 
-// V values of a row from `s` on, as floats; `left` of them are the row's, the others 0.
+// V values of a row from `s` on; `left` of them are the row's, the others 0.  (Held in words: an array of 16-bit values is loaded one by one.)
 template <typename T, int V> struct Values {
     typedef typename T::Raw Raw;
+    static constexpr int WORDS = V * (int)sizeof(Raw) / 4;
     struct __attribute__((packed, aligned(sizeof(Raw)))) Piece {
-        Raw v[V];
+        uint32_t w[WORDS];
+        __device__ __forceinline__ float at(int v) const {
+            if constexpr (sizeof(Raw) == 4)
+                return __uint_as_float(w[v]);
+            else
+                return T::up((Raw)(v & 1 ? w[v >> 1] >> 16 : w[v >> 1] & 0xffffu));
+        }
     };
     static __device__ __forceinline__ Piece fetch(const Raw *s, int left) {
         Piece p;
@@ -19,20 +26,33 @@ template <typename T, int V> struct Values {
             p = *reinterpret_cast<const Piece *>(s);
         } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) p.v[v] = v < left ? s[v] : (Raw)0;
+            for (int q = 0; q < WORDS; ++q) p.w[q] = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v < left) {
+                    if constexpr (sizeof(Raw) == 4)
+                        p.w[v] = __builtin_bit_cast(uint32_t, s[v]);
+                    else
+                        p.w[v >> 1] |= (uint32_t)s[v] << (v & 1) * 16;
+                }
         }
         return p;
     }
     static __device__ __forceinline__ void store(Raw *to, const float (&x)[V], int left) {
-        Piece p;
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.v[v] = T::down(x[v]);
         if (left >= V) {
+            Piece p;
+#pragma unroll
+            for (int q = 0; q < WORDS; ++q) {
+                if constexpr (sizeof(Raw) == 4)
+                    p.w[q] = __builtin_bit_cast(uint32_t, T::down(x[q]));
+                else
+                    p.w[q] = (uint32_t)T::down(x[2 * q]) | (uint32_t)T::down(x[2 * q + 1]) << 16;
+            }
             *reinterpret_cast<Piece *>(to) = p;
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (v < left) to[v] = p.v[v];
+                if (v < left) to[v] = T::down(x[v]);
         }
     }
 };
@@ -49,16 +69,19 @@ struct EmbedArgs {
     int64_t ld_out;
 };
 
-// out[i] = scale * sum over the stages s, in their order, of table[s * k + code]: 1 << shift lanes of a row, 16 bytes of the table each,
-// rows side by side in a workgroup, a row's further pieces by blockIdx.y.
+// out[i] = scale * sum over the stages s, in their order, of table[s * k + code].  The columns are cut into `slices` (of `pieces` vectors of 16 bytes of
+// the table each): workgroup b has slice b % slices, so that with eight of them every XCD reads its own eighth of the tables' columns,
+// which its L2 may hold.  1 << shift lanes of a row, rows side by side in a workgroup, a slice's further pieces by blockIdx.y.
 template <typename T, typename O>
-__global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift) {
+__global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift, int slices, int pieces) {
     typedef typename T::Raw Raw;
-    constexpr int V = 16 / (int)sizeof(Raw), AHEAD = 4;
+    constexpr int V = 16 / (int)sizeof(Raw), AHEAD = 8;
     typedef Values<T, V> In;
-    const int64_t row = (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
-    const int at = ((blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1))) * V, left = a.dim - at;
-    if (row >= a.n || left <= 0) return;
+    const int slice = blockIdx.x % (unsigned)slices;
+    const int64_t row = (int64_t)(blockIdx.x / (unsigned)slices) * (256 >> shift) + (threadIdx.x >> shift);
+    const int piece = (blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1));
+    const int at = (slice * pieces + piece) * V, left = a.dim - at;
+    if (row >= a.n || left <= 0 || piece >= pieces) return;
     const Raw *table = (const Raw *)a.table + at;
     float sum[V];
 #pragma unroll
@@ -78,7 +101,7 @@ __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift) {
         for (int j = 0; j < AHEAD; ++j)
             if (has[j]) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[v] += T::up(p[j].v[v]);
+                for (int v = 0; v < V; ++v) sum[v] += p[j].at(v);
             }
     }
 #pragma unroll
@@ -89,26 +112,30 @@ __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift) {
 // ---- the positions by code ---------------------------------------------------------------------------
 struct ListArgs {
     const void *codes;
-    int code_bytes;
     int64_t code_stride;
     int n, k, width;  // codes of a bucket
-    int32_t *start, *rows, *row_codes;
+    int share, shares;  // positions of a share of the list, and how many there are
+    int32_t *start, *rows, *edges;  // edges: the code of each kLongCode-th position of the list
+    int32_t *counts, *below;  // of several shares: [stage][share][code], [stage][share][bucket]
 };
 
-// A workgroup lists the positions of its bucket of codes, blockIdx.x, in stage blockIdx.y: every workgroup reads all codes of the stage, counts those
-// below its bucket, whose number is where its list begins, and those in it, by wave and code; each wave has a run of the positions, so that
-// the order within a code is that of the positions.
-template <int WAVES>
+// A workgroup has a bucket of codes (blockIdx.x), a share of the positions (blockIdx.y) and a stage (blockIdx.z); it reads all codes of its
+// share, counts those below its bucket, whose number is where its part of the list begins, and those in it, by wave and code.  Each wave has a
+// run of the positions, so that the order within a code is that of the positions.  With one share it goes on and writes its part of the
+// list; of several shares the counts are added up first, by the launch after (PLACE).
+template <int WAVES, int BYTES, bool COUNT, bool PLACE>
 __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
-    __shared__ int hist[WAVES][kBucketMost];
+    extern __shared__ int hist[];  // [wave][code of the bucket]
     __shared__ int below_of[WAVES], total_of[WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), stage = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), stage = blockIdx.z, share = blockIdx.y, buckets = gridDim.x;
     const int lo = blockIdx.x * a.width, width = min(a.width, a.k - lo);
-    const int share = (a.n + 64 * WAVES - 1) / (64 * WAVES) * 64, from = min(a.n, wave * share), to = min(a.n, from + share);
-    for (int i = tid; i < WAVES * kBucketMost; i += 64 * WAVES) hist[i / kBucketMost][i % kBucketMost] = 0;
+    const int first = (int)min((int64_t)a.n, (int64_t)share * a.share), end = (int)min((int64_t)a.n, (int64_t)first + a.share);
+    const int run = ((end - first) + 64 * WAVES - 1) / (64 * WAVES) * 64, from = min(end, first + wave * run), to = min(end, from + run);
+    int *mine = hist + wave * a.width;
+    for (int i = tid; i < WAVES * a.width; i += 64 * WAVES) hist[i] = 0;
     __syncthreads();
     constexpr int AHEAD = 8;
-    const auto code_of = [&](int i) { return i < to ? (uint32_t)code_at(a.codes, a.code_bytes, (int64_t)i * a.code_stride + stage) : 0xffffffffu; };
+    const auto code_of = [&](int i) { return i < to ? (uint32_t)code_at(a.codes, BYTES, (int64_t)i * a.code_stride + stage) : 0xffffffffu; };
     int below = 0;
     for (int i = from + lane; i - lane < to; i += 64 * AHEAD) {
         uint32_t c[AHEAD];
@@ -117,64 +144,108 @@ __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             below += c[j] < (uint32_t)lo;
-            if (c[j] - (uint32_t)lo < (uint32_t)width) atomicAdd(&hist[wave][c[j] - lo], 1);
+            if (c[j] - (uint32_t)lo < (uint32_t)width) atomicAdd(&mine[c[j] - lo], 1);
         }
     }
     below = (int)over_group<64>((uint32_t)below, 0u, [](uint32_t x, uint32_t y) { return x + y; });
     if (lane == 0) below_of[wave] = below;
     __syncthreads();
-    int base = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) base += below_of[w];
-    // where each code's list begins, and in it each wave's share; a lane per code
-    int mine = 0;
-    if (tid < width) {
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) mine += hist[w][tid];
-    }
-    int before = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(before, d);
-        if (lane >= d) before += o;
-    }
-    if (lane == 63) total_of[wave] = before;
-    __syncthreads();
-    int at = base + before - mine;
-    for (int w = 0; w < wave; ++w) at += total_of[w];
-    int32_t *start = a.start + (int64_t)stage * (a.k + 1);
-    if (tid < width) {
-        start[lo + tid] = at;
-        if (lo + tid == a.k - 1) start[a.k] = at + mine;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const int here = hist[w][tid];
-            hist[w][tid] = at;
-            at += here;
+    int32_t *counts = a.counts + (int64_t)stage * a.shares * a.k, *belows = a.below + (int64_t)stage * a.shares * buckets;
+    if constexpr (!PLACE) {
+        for (int i = tid; i < width; i += 64 * WAVES) {
+            int sum = 0;
+            for (int w = 0; w < WAVES; ++w) sum += hist[w * a.width + i];
+            counts[(int64_t)share * a.k + lo + i] = sum;
         }
+        if (tid == 0) {
+            int sum = 0;
+            for (int w = 0; w < WAVES; ++w) sum += below_of[w];
+            belows[share * buckets + blockIdx.x] = sum;
+        }
+        return;
     }
-    __syncthreads();
-    int32_t *rows = a.rows + (int64_t)stage * a.n, *row_codes = a.row_codes + (int64_t)stage * a.n;
+    int base = 0;
+    if constexpr (COUNT) {
+        for (int w = 0; w < WAVES; ++w) base += below_of[w];
+    } else {
+        for (int s = tid; s < a.shares; s += 64 * WAVES) base += belows[s * buckets + blockIdx.x];
+        base = (int)over_group<64>((uint32_t)base, 0u, [](uint32_t x, uint32_t y) { return x + y; });
+        if (lane == 0) total_of[wave] = base;
+        __syncthreads();
+        base = 0;
+        for (int w = 0; w < WAVES; ++w) base += total_of[w];
+        __syncthreads();
+    }
+    // where each code's list begins, in it this share's part, and in that each wave's; a lane per code, 64 * WAVES codes at a time
+    int32_t *start = a.start + (int64_t)stage * (a.k + 1);
+    for (int c0 = 0; c0 < width; c0 += 64 * WAVES) {
+        const int c = c0 + tid;
+        int all = 0, ahead = 0;  // of the code: positions in all shares, in the shares before this one
+        if (c < width) {
+            if constexpr (COUNT) {
+                for (int w = 0; w < WAVES; ++w) all += hist[w * a.width + c];
+            } else {
+                for (int s = 0; s < a.shares; s += 16) {
+                    int here[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) here[j] = s + j < a.shares ? counts[(int64_t)(s + j) * a.k + lo + c] : 0;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) all += here[j], ahead += s + j < share ? here[j] : 0;
+                }
+            }
+        }
+        int upto = all;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        if (lane == 63) total_of[wave] = upto;
+        __syncthreads();
+        int at = base + upto - all, next = base;
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) at += total_of[w];
+            next += total_of[w];
+        }
+        if (c < width) {
+            if (share == 0) {
+                start[lo + c] = at;
+                if (lo + c == a.k - 1) start[a.k] = at + all;
+            }
+            at += ahead;
+            for (int w = 0; w < WAVES; ++w) {
+                const int here = hist[w * a.width + c];
+                hist[w * a.width + c] = at;
+                at += here;
+            }
+        }
+        base = next;
+        __syncthreads();
+    }
+    int32_t *rows = a.rows + (int64_t)stage * a.n, *edges = a.edges + (int64_t)stage * embed_edges(a.n);
     for (int i = from + lane; i - lane < to; i += 64 * AHEAD) {
         uint32_t c[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) c[j] = code_of(i + 64 * j) - (uint32_t)lo;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            unsigned long long left = __ballot(c[j] < (uint32_t)width);
-            while (left) {  // uniform: the codes among these 64 positions, one after another
-                const uint32_t code = (uint32_t)__builtin_amdgcn_readlane((int)c[j], __ffsll(left) - 1);
-                const unsigned long long same = __ballot(c[j] == code);
-                const int first = hist[wave][code];
-                wave_sync();
-                if (c[j] == code) {
-                    const int place = first + __popcll(same & ((1ull << lane) - 1));
-                    rows[place] = i + 64 * j;
-                    row_codes[place] = lo + (int)code;
-                }
-                if (lane == 0) hist[wave][code] = first + __popcll(same);
-                wave_sync();
-                left &= ~same;
+            const bool own = c[j] < (uint32_t)width;
+            const unsigned long long who = __ballot(own);
+            if (!who) continue;  // uniform
+            // the lanes with the same code: bit by bit of it
+            unsigned long long same = who;
+            for (int bit = 1; bit < a.width; bit <<= 1) {
+                const unsigned long long set = __ballot((c[j] & bit) != 0);
+                same &= c[j] & bit ? set : ~set;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            const int place = own ? mine[c[j]] + rank : 0;
+            wave_sync();
+            if (own && rank == 0) mine[c[j]] = place + __popcll(same);
+            wave_sync();
+            if (own) {
+                rows[place] = i + 64 * j;
+                if (place % kLongCode == 0) edges[place / kLongCode] = lo + (int)c[j];
             }
         }
     }
@@ -189,52 +260,97 @@ struct SumArgs {
     int accumulate;
     void *grad;
     int64_t ld_grad;
-    const int32_t *start, *rows, *row_codes;
+    const int32_t *start, *rows, *edges;
     float *partial;  // [stage][chunk][2][padded dim]
-    int chunks, padded, keys, groups;  // codes of 16 lanes one after another; workgroups of codes
+    int chunks, padded, codes, groups, across, first;  // codes of a workgroup; workgroups of codes; of columns, and the first of these
 };
 
+constexpr int kGroupCodes = 128;  // codes of a workgroup at most
 constexpr int kOwnMembers = 32;  // a code of more positions is summed by the whole workgroup
 
-// V columns of the members number a, a + step, ... below b of a list, summed in that order.
+// Adds V columns of the members number a, a + step, ... below b of a list, in that order.
 template <typename T, int V>
 __device__ __forceinline__ void sum_members(const SumArgs &s, const int32_t *rows, int a, int b, int step, int at, int left, float (&sum)[V]) {
     typedef typename T::Raw Raw;
     typedef Values<T, V> In;
     constexpr int AHEAD = 8;
-#pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] = 0.0f;
     const Raw *g = (const Raw *)s.g + at;
     for (int p = a; p < b; p += AHEAD * step) {
+        // (behind the last member the last one again, which is not added: loads under a condition would wait for one another)
+        int row[AHEAD];
         typename In::Piece x[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (p + j * step < b) x[j] = In::fetch(g + (int64_t)rows[p + j * step] * s.ld, left);
+        for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld, left);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (p + j * step < b) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[v] += T::up(x[j].v[v]);
+                for (int v = 0; v < V; ++v) sum[v] += x[j].at(v);
             }
     }
 }
 
+// Rows without members, most of a large table's, of 64 codes and up to 16 KB of their columns: whole lines that pass the caches.  These
+// workgroups come last: zeros written beside the reads of the sums made both slower (16,384 x 1280 bf16 to 65,536 f32 rows 100 us, apart
+// ZZ us).
+constexpr int kZeroCodes = 64, kZeroBytes = 16384;
+template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs &a, unsigned id, int stage, int *list, int *count) {
+    typedef typename O::Raw Out;
+    constexpr int VO = 16 / (int)sizeof(Out), PIECE = kZeroBytes / (int)sizeof(Out);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned pieces = (unsigned)(a.dim + PIECE - 1) / PIECE;
+    const int64_t code = (int64_t)(id / pieces) * kZeroCodes + tid;
+    const int column = (int)(id % pieces) * PIECE, end = min(a.dim, column + PIECE);
+    const int32_t *start = a.start + (int64_t)stage * (a.k + 1);
+    if (wave == 0) {
+        const bool empty = code < a.k && start[code] == start[code + 1];
+        const unsigned long long who = __ballot(empty);
+        if (empty) list[__popcll(who & ((1ull << lane) - 1))] = (int)code;
+        if (lane == 0) *count = __popcll(who);
+    }
+    __syncthreads();
+    const bool past = ((uintptr_t)a.grad & 15) == 0 && a.ld_grad % VO == 0 && a.dim % VO == 0;  // whole pieces of 16 aligned bytes
+    for (int i = wave; i < *count; i += 4) {
+        Out *to = (Out *)a.grad + ((int64_t)stage * a.k + list[i]) * a.ld_grad;
+        for (int c = column + lane * VO; c < end; c += 64 * VO) {
+            if (past) {
+                typedef uint32_t Four __attribute__((ext_vector_type(4)));
+                __builtin_nontemporal_store(Four{0, 0, 0, 0}, reinterpret_cast<Four *>(to + c));
+            } else {
+                const float zeros[VO] = {};
+                Values<O, VO>::store(to + c, zeros, end - c);
+            }
+        }
+    }
+}
+
 // Rows of the gradient: 16 lanes sum V columns each of a code's members.  The first a.groups workgroups take codes, those behind them the
-// chunks of the list that belong to codes of more than kLongCode members.  blockIdx.y: pieces of 16 * V columns, blockIdx.z: stages.
+// chunks of the list that belong to codes of more than kLongCode members; a.across workgroups side by side have the columns,
+// 16 * V each; the last ones write the rows without members.  blockIdx.z: stages.
 template <typename T, typename O>
 __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     typedef typename T::Raw Raw;
     typedef typename O::Raw Out;
-    constexpr int V = 16 / (int)sizeof(Raw), COLUMNS = 16 * V;
+    constexpr int V = 16 / (int)sizeof(Raw), COLUMNS = 16 * V, VO = 16 / (int)sizeof(Out);
     __shared__ float red[16][COLUMNS];
-    __shared__ int longer[16 * 8], count;
-    const int tid = threadIdx.x, sub = tid >> 4, column = blockIdx.y * COLUMNS, at = column + (tid & 15) * V, left = a.dim - at, stage = blockIdx.z;
+    __shared__ int begin[kGroupCodes], behind[kGroupCodes], count[2];
+    __shared__ uint8_t which[2][kGroupCodes];
+    const int tid = threadIdx.x, sub = tid >> 4, column = (a.first + blockIdx.x % (unsigned)a.across) * COLUMNS, at = column + (tid & 15) * V, left = a.dim - at, stage = blockIdx.z;
+    if (blockIdx.x >= (unsigned)(a.groups + a.chunks) * (unsigned)a.across) {
+        write_zeros<O>(a, blockIdx.x - (unsigned)(a.groups + a.chunks) * (unsigned)a.across, stage, begin, &count[0]);
+        return;
+    }
+    const int group = blockIdx.x / (unsigned)a.across;
     const int32_t *start = a.start + (int64_t)stage * (a.k + 1), *rows = a.rows + (int64_t)stage * a.n;
     Out *grad = (Out *)a.grad + (int64_t)stage * a.k * a.ld_grad;
     float sum[V];
     // all 16 groups of lanes sum members [from, to); the sums of COLUMNS columns are in the first lanes then
     const auto together = [&](int from, int to) {
         if (left > 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[v] = 0.0f;
             sum_members<T, V>(a, rows, from + sub, to, 16, at, left, sum);
 #pragma unroll
             for (int v = 0; v < V; ++v) red[sub][(tid & 15) * V + v] = sum[v];
@@ -248,11 +364,13 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
         __syncthreads();
         return total;
     };
-    if ((int)blockIdx.x >= a.groups) {
-        const int chunk = blockIdx.x - a.groups, all = start[a.k], first = chunk * kLongCode, last = min(all, first + kLongCode) - 1;
+    if (group >= a.groups) {
+        const int chunk = group - a.groups, all = start[a.k], first = chunk * kLongCode, last = min(all, first + kLongCode) - 1;
         if (first > last) return;
-        const int32_t *row_codes = a.row_codes + (int64_t)stage * a.n;
-        const int c0 = row_codes[first], c1 = row_codes[last];
+        // the codes of the chunk's first position and, where another one's list goes on behind the chunk, of that (no other list that
+        // begins in the chunk is long)
+        const int32_t *edges = a.edges + (int64_t)stage * embed_edges(a.n);
+        const int c0 = edges[chunk], then = last + 1 < all ? edges[chunk + 1] : c0, c1 = start[then] <= last ? then : c0;
         for (int slot = 0; slot < 2; ++slot) {
             const int c = slot ? c1 : c0;
             if (slot && c1 == c0) break;
@@ -263,36 +381,88 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
         }
         return;
     }
-    if (tid == 0) count = 0;
+    // the workgroup's codes by the number of their members: a group of lanes each, or the whole workgroup
+    const int64_t from = (int64_t)group * a.codes;
+    if (tid < 2) count[tid] = 0;
     __syncthreads();
-    for (int q = 0; q < a.keys; ++q) {
-        const int64_t code = (int64_t)blockIdx.x * 16 * a.keys + q * 16 + sub;
-        if (code >= a.k) continue;
-        const int s0 = start[code], s1 = start[code + 1];
-        if (s1 - s0 > kOwnMembers) {
-            if ((tid & 15) == 0 && s1 - s0 <= kLongCode) longer[atomicAdd(&count, 1)] = (int)code;
-            continue;
+    if (tid < a.codes && from + tid < a.k) {
+        const int s0 = start[from + tid], s1 = start[from + tid + 1], members = s1 - s0;
+        begin[tid] = s0;
+        behind[tid] = s1;
+        if (members > 0 && members <= kLongCode) {
+            const int kind = members <= kOwnMembers ? 0 : 1;
+            which[kind][atomicAdd(&count[kind], 1)] = (uint8_t)tid;  // (in whatever order: each is a sum of its own)
         }
-        if (left <= 0 || (a.accumulate && s0 == s1)) continue;
-        sum_members<T, V>(a, rows, s0, s1, 1, at, left, sum);
-        Out *to = grad + code * a.ld_grad + at;
-        if (a.accumulate) {
-            const typename Values<O, V>::Piece old = Values<O, V>::fetch(to, left);
-#pragma unroll
-            for (int v = 0; v < V; ++v) sum[v] = __builtin_fmaf(a.scale, sum[v], O::up(old.v[v]));
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) sum[v] *= a.scale;
-        }
-        Values<O, V>::store(to, sum, left);
     }
     __syncthreads();
-    const int n_longer = count;
+    // codes of few members, a group of lanes each: the first two members of four codes at a time, since most have no more
+    constexpr int SIDE = 4, EARLY = 2;
+    for (int i = sub; i < count[0]; i += 16 * SIDE) {
+        typename Values<T, V>::Piece x[SIDE][EARLY];
+        int row[SIDE][EARLY];
+#pragma unroll
+        for (int u = 0; u < SIDE; ++u) {  // (beyond the last code or member the last one again)
+            const int j = which[0][min(i + 16 * u, count[0] - 1)], s0 = begin[j], s1 = behind[j];
+#pragma unroll
+            for (int e = 0; e < EARLY; ++e) row[u][e] = rows[min(s0 + e, s1 - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < SIDE; ++u)
+#pragma unroll
+            for (int e = 0; e < EARLY; ++e) x[u][e] = Values<T, V>::fetch((const Raw *)a.g + at + (int64_t)row[u][e] * a.ld, left);
+#pragma unroll
+        for (int u = 0; u < SIDE; ++u) {
+            if (i + 16 * u >= count[0]) break;
+            const int j = which[0][i + 16 * u], s0 = begin[j], s1 = behind[j];
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[v] = x[u][0].at(v);
+            if (s0 + 1 < s1) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) sum[v] += x[u][1].at(v);
+            }
+            if (s0 + EARLY < s1 && left > 0) sum_members<T, V>(a, rows, s0 + EARLY, s1, 1, at, left, sum);
+            // the lanes' 16 bytes of results side by side
+            Out *to = grad + (from + j) * a.ld_grad + column;
+            const auto finish = [&](float (&y)[VO], int col) {
+                const int rest = a.dim - column - col;
+                if (rest <= 0) return;
+                if (a.accumulate) {
+                    const typename Values<O, VO>::Piece old = Values<O, VO>::fetch(to + col, rest);
+#pragma unroll
+                    for (int v = 0; v < VO; ++v) y[v] = __builtin_fmaf(a.scale, y[v], old.at(v));
+                } else {
+#pragma unroll
+                    for (int v = 0; v < VO; ++v) y[v] *= a.scale;
+                }
+                Values<O, VO>::store(to + col, y, rest);
+            };
+            if constexpr (VO == V) {
+                finish(sum, (tid & 15) * V);
+            } else {
+                wave_sync();
+#pragma unroll
+                for (int v = 0; v < V; ++v) red[sub][(tid & 15) * V + v] = sum[v];
+                wave_sync();
+#pragma unroll
+                for (int c = 0; c < COLUMNS; c += 16 * VO) {
+                    const int col = c + (tid & 15) * VO;
+                    if (col < COLUMNS) {
+                        float y[VO];
+#pragma unroll
+                        for (int v = 0; v < VO; ++v) y[v] = red[sub][col + v];
+                        finish(y, col);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int n_longer = count[1];
     for (int i = 0; i < n_longer; ++i) {
-        const int code = longer[i];
-        const float total = together(start[code], start[code + 1]);
+        const int j = which[1][i];
+        const float total = together(begin[j], behind[j]);
         if (tid < COLUMNS && column + tid < a.dim) {
-            Out *to = grad + (int64_t)code * a.ld_grad + column + tid;
+            Out *to = grad + (from + j) * a.ld_grad + column + tid;
             *to = O::down(a.accumulate ? __builtin_fmaf(a.scale, total, O::up(*to)) : a.scale * total);
         }
     }
@@ -305,17 +475,17 @@ __global__ void __launch_bounds__(256) k_embed_join(SumArgs a) {
     typedef typename O::Raw Out;
     __shared__ float red[16][64];
     const int tid = threadIdx.x, sub = tid >> 4, column = blockIdx.y * 64, at = column + (tid & 15) * 4, stage = blockIdx.z, chunk = blockIdx.x;
-    const int32_t *start = a.start + (int64_t)stage * (a.k + 1), *row_codes = a.row_codes + (int64_t)stage * a.n;
-    const int all = start[a.k], first = chunk * kLongCode, last = min(all, first + kLongCode) - 1;
-    if (first > last) return;
-    const int code = row_codes[last], s0 = start[code], s1 = start[code + 1];
-    if (s1 - s0 <= kLongCode || s0 < first) return;
+    const int32_t *start = a.start + (int64_t)stage * (a.k + 1), *edges = a.edges + (int64_t)stage * embed_edges(a.n);
+    const int all = start[a.k], first = chunk * kLongCode, last = first + kLongCode - 1;
+    if (last + 1 >= all) return;  // (a long list that begins in a chunk goes on behind it)
+    const int code = edges[chunk + 1], s0 = start[code], s1 = start[code + 1];
+    if (s1 - s0 <= kLongCode || s0 < first || s0 > last) return;
     const int end = (s1 - 1) / kLongCode;  // the last chunk with members of this code
     const float *partial = a.partial + (int64_t)stage * a.chunks * 2 * a.padded;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at < a.dim) {
         for (int c = chunk + sub; c <= end; c += 16) {
-            const int slot = c == chunk && row_codes[first] != code ? 1 : 0;
+            const int slot = c == chunk && s0 != first ? 1 : 0;
             const float4 x = *reinterpret_cast<const float4 *>(partial + ((int64_t)c * 2 + slot) * a.padded + at);
             sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
         }

@@ -167,25 +167,49 @@ inline Refusal check_code_verify(int32_t type, const void *target, int64_t ld_ta
     return {};
 }
 
+// ---- rows of a table -----------------------------------------------------------------------------------
+// Slices of the columns of a lookup: eight, an XCD's each, where rows of the tables are read many times (twice at least, on average) and a slice has
+// 128 bytes of a row or more; otherwise one.
+inline int embed_slices(int64_t n, int32_t k, int32_t m, int vectors) { return n >= 2 * (int64_t)k && vectors >= 64 && (int64_t)k * m * vectors * 16 > 2 << 20 ? 8 : 1; }
+
 // ---- sums by code ------------------------------------------------------------------------------------
-// The positions of each stage in the order of their codes, as a list of n positions with the codes beside it, and where each code's
-// positions begin: k + 1 numbers.  A workgroup lists the codes of one bucket.
-constexpr int kBucketMost = 512;
-inline int32_t bucket_codes(int32_t k) { return std::min<int32_t>(kBucketMost, (k + 255) / 256); }
+// The positions of each stage in the order of their codes, and where each code's positions begin: k + 1 numbers.  Workgroups of 16 waves
+// list a bucket of codes each, of a share of the positions.  One share, and one launch, up to 32,768 positions; more positions in shares, in two
+// launches, with as many codes per bucket as 16 waves can count in 60 KB of LDS.
+struct ListPlan {
+    int32_t width, buckets;
+    int32_t share, shares;
+};
+constexpr int kBucketMost = 960;
+inline ListPlan plan_lists(int64_t n, int32_t k) {
+    if (n <= 32768) {
+        const int32_t width = std::min<int32_t>(512, (k + 255) / 256);
+        return {width, (k + width - 1) / width, (int32_t)std::max<int64_t>(n, 1), 1};
+    }
+    const int32_t width = std::min<int32_t>(kBucketMost, k), buckets = (k + width - 1) / width;
+    // shares of 4096 positions or more, a few hundred workgroups, at most 256 shares
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / buckets)), share = std::max<int64_t>(4096, (n + most - 1) / most);
+    return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
+}
 // A code of more positions than this is summed in pieces of as many positions of the list, whose sums are joined afterwards.
 constexpr int kLongCode = 1024;
-inline int64_t embed_chunks(int64_t n) { return n > kLongCode ? (n + kLongCode - 1) / kLongCode : 0; }
-// Bytes of a call's workspace, in the order in which they lie there; each grows with each size.
+constexpr int64_t embed_edges(int64_t n) { return (n + kLongCode - 1) / kLongCode; }  // pieces of the list
+inline int64_t embed_chunks(int64_t n) { return n > kLongCode ? embed_edges(n) : 0; }
+// Bytes of a call's workspace, in the order in which they lie there; their sum grows with each size.
 struct EmbedWork {
-    int64_t start, rows, codes, partial, bytes;
+    int64_t start, rows, edges, counts, below, partial, bytes;
 };
 inline EmbedWork embed_work(int64_t n, int32_t k, int32_t dim, int32_t m) {
     const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+    // (shares times codes: no plan has more than 256 shares, nor more than 1024 of share and bucket)
+    const int64_t counts = n > 32768 ? std::min<int64_t>(256 * (int64_t)k, (int64_t)1024 * kBucketMost + k) : 0;
     EmbedWork w;
     w.start = 0;
     w.rows = up((int64_t)m * (k + 1) * 4);
-    w.codes = w.rows + up(m * n * 4);
-    w.partial = w.codes + up(m * n * 4);
+    w.edges = w.rows + up(m * n * 4);
+    w.counts = w.edges + up(m * embed_edges(n) * 4);
+    w.below = w.counts + up(m * counts * 4);
+    w.partial = w.below + up(n > 32768 ? m * 2048 * 4 : 0);
     w.bytes = w.partial + up(m * embed_chunks(n) * 2 * ((dim + 15) / 16 * 16) * 4);
     return w;
 }

@@ -62,17 +62,17 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
     VQ_TRY(admit(ctx, vq::check_code_embed(type, d_table, k, ld_table, dim, m, code_bytes, d_codes, n, code_stride, scale, out_type,
                                            d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
-    const int pieces = cdiv(dim, 16 / vq::type_bytes(type));
+    const int vectors = cdiv(dim, 16 / vq::type_bytes(type)), slices = vq::embed_slices(n, k, m, vectors), pieces = cdiv(vectors, slices);
     int shift = 0;
     while (shift < 8 && 1 << shift < pieces) ++shift;
     const unsigned across = cdiv(pieces, 1 << shift);
-    const int64_t slice = std::max<int64_t>(256, ((int64_t)1 << 31) / ((int64_t)across << shift));  // a grid has fewer than 2^32 lanes
+    const int64_t slice = std::max<int64_t>(256, ((int64_t)1 << 31) / ((int64_t)slices << shift));  // a grid has fewer than 2^32 lanes
     for (int64_t r = 0; r < n; r += slice) {
         const vq::EmbedArgs a{d_table, ld_table, k, dim, m, (const char *)d_codes + r * code_stride * code_bytes, code_bytes, std::min(slice, n - r),
                               code_stride, scale, (char *)d_out + r * ld_out * vq::type_bytes(out_type), ld_out};
         by_types(type, out_type, [&](auto t, auto o) {
-            hipLaunchKernelGGL((vq::k_code_embed<decltype(t), decltype(o)>), dim3((unsigned)cdiv64(a.n, 256 >> shift), across), dim3(256), 0,
-                               ctx->stream, a, shift);
+            hipLaunchKernelGGL((vq::k_code_embed<decltype(t), decltype(o)>), dim3((unsigned)cdiv64(a.n, 256 >> shift) * slices, across), dim3(256), 0,
+                               ctx->stream, a, shift, slices, pieces);
         });
         VQ_HIP(ctx, hipGetLastError());
     }
@@ -91,18 +91,44 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
     const vq::EmbedWork work = vq::embed_work(n, k, dim, m);
     VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)work.bytes));
     char *w = (char *)ctx->code_work.p;
-    const vq::ListArgs l{d_codes, code_bytes, code_stride, (int)n, k, vq::bucket_codes(k), (int32_t *)(w + work.start), (int32_t *)(w + work.rows),
-                         (int32_t *)(w + work.codes)};
-    hipLaunchKernelGGL(vq::k_code_lists<16>, dim3(cdiv(k, l.width), m), dim3(1024), 0, ctx->stream, l);
+    const vq::ListPlan plan = vq::plan_lists(n, k);
+    const vq::ListArgs l{d_codes, code_stride, (int)n, k, plan.width, plan.share, plan.shares, (int32_t *)(w + work.start),
+                         (int32_t *)(w + work.rows), (int32_t *)(w + work.edges), (int32_t *)(w + work.counts), (int32_t *)(w + work.below)};
+    const auto lists = [&](auto bytes) {
+        constexpr int BYTES = decltype(bytes)::value;
+        const dim3 grid(plan.buckets, plan.shares, m), wg(1024);
+        const int lds = 16 * plan.width * 4;
+        if (plan.shares == 1) {
+            hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, true, true>), grid, wg, lds, ctx->stream, l);
+        } else {
+            hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, true, false>), grid, wg, lds, ctx->stream, l);
+            hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, false, true>), grid, wg, lds, ctx->stream, l);
+        }
+    };
+    if (code_bytes == 1)
+        lists(std::integral_constant<int, 1>());
+    else if (code_bytes == 2)
+        lists(std::integral_constant<int, 2>());
+    else
+        lists(std::integral_constant<int, 4>());
     VQ_HIP(ctx, hipGetLastError());
-    const int keys = 4;
-    const vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, l.start, l.rows, l.row_codes, (float *)(w + work.partial),
-                        (int)vq::embed_chunks(n), (dim + 15) / 16 * 16, keys, (int)cdiv(k, 16 * keys)};
-    const unsigned columns = 16 * 16 / vq::type_bytes(type);
-    by_types(type, grad_type, [&](auto t, auto o) {
-        hipLaunchKernelGGL((vq::k_embed_sums<decltype(t), decltype(o)>), dim3(a.groups + a.chunks, cdiv(dim, columns), m), dim3(256), 0, ctx->stream, a);
-    });
-    VQ_HIP(ctx, hipGetLastError());
+    const int columns = 16 * 16 / vq::type_bytes(type), across = cdiv(dim, columns);
+    // codes of a workgroup: as many as leave 2048 workgroups, 16 to 128
+    const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(16, (int64_t)k * m * across / 2048 / 16 * 16));
+    vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, l.start, l.rows, l.edges, (float *)(w + work.partial),
+                  (int)vq::embed_chunks(n), (dim + 15) / 16 * 16, codes, (int)cdiv(k, codes), 0, 0};
+    // the columns of some workgroups side by side, the others' in launches of their own: a grid has fewer than 2^32 lanes
+    const int most = std::max(1, (1 << 23) / (a.groups + a.chunks));
+    for (a.first = 0; a.first < across; a.first += most) {
+        a.across = std::min(most, across - a.first);
+        // rows without members, all columns of them, behind the last columns' sums
+        const bool last = a.first + a.across == across;
+        const unsigned zeros = last && !accumulate ? cdiv(k, vq::kZeroCodes) * cdiv((int64_t)dim * vq::type_bytes(grad_type), vq::kZeroBytes) : 0;
+        by_types(type, grad_type, [&](auto t, auto o) {
+            hipLaunchKernelGGL((vq::k_embed_sums<decltype(t), decltype(o)>), dim3((a.groups + a.chunks) * a.across + zeros, 1, m), dim3(256), 0, ctx->stream, a);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+    }
     if (a.chunks) {
         by_type(grad_type, [&](auto o) {
             hipLaunchKernelGGL(vq::k_embed_join<decltype(o)>, dim3(a.chunks, cdiv(dim, 64), m), dim3(256), 0, ctx->stream, a);
