@@ -121,22 +121,25 @@ struct ListArgs {
 
 // A workgroup has a bucket of codes (blockIdx.x), a share of the positions (blockIdx.y) and a stage (blockIdx.z); it reads all codes of its
 // share, counts those below its bucket, whose number is where its part of the list begins, and those in it, by wave and code.  Each wave has a
-// run of the positions, so that the order within a code is that of the positions.  With one share it goes on and writes its part of the
-// list; of several shares the counts are added up first, by the launch after (PLACE).
+// run of the positions, so that the order within a code is that of the positions; the few of them that its bucket has it keeps in LDS, and
+// reads its run again only where they are more than fit there.  With one share the workgroup goes on and writes its part of the list; of several
+// shares the counts are added up first, by the launch after (PLACE).
+constexpr int kQueue = 512;
 template <int WAVES, int BYTES, bool COUNT, bool PLACE>
 __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
-    extern __shared__ int hist[];  // [wave][code of the bucket]
-    __shared__ int below_of[WAVES], total_of[WAVES];
+    extern __shared__ int hist[];  // [wave][code of the bucket], and (PLACE) [wave][kQueue]
+    __shared__ int below_of[WAVES], total_of[WAVES], sums_of[COUNT ? 1 : 2][COUNT ? 1 : 64 * WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), stage = blockIdx.z, share = blockIdx.y, buckets = gridDim.x;
     const int lo = blockIdx.x * a.width, width = min(a.width, a.k - lo);
     const int first = (int)min((int64_t)a.n, (int64_t)share * a.share), end = (int)min((int64_t)a.n, (int64_t)first + a.share);
     const int run = ((end - first) + 64 * WAVES - 1) / (64 * WAVES) * 64, from = min(end, first + wave * run), to = min(end, from + run);
     int *mine = hist + wave * a.width;
+    uint2 *queue = reinterpret_cast<uint2 *>(hist + ((WAVES * a.width + 1) & ~1)) + wave * kQueue;
     for (int i = tid; i < WAVES * a.width; i += 64 * WAVES) hist[i] = 0;
     __syncthreads();
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 16;
     const auto code_of = [&](int i) { return i < to ? (uint32_t)code_at(a.codes, BYTES, (int64_t)i * a.code_stride + stage) : 0xffffffffu; };
-    int below = 0;
+    int below = 0, queued = 0;
     for (int i = from + lane; i - lane < to; i += 64 * AHEAD) {
         uint32_t c[AHEAD];
 #pragma unroll
@@ -144,7 +147,15 @@ __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             below += c[j] < (uint32_t)lo;
-            if (c[j] - (uint32_t)lo < (uint32_t)width) atomicAdd(&mine[c[j] - lo], 1);
+            const uint32_t code = c[j] - (uint32_t)lo;
+            const unsigned long long who = __ballot(code < (uint32_t)width);
+            if (!who) continue;  // uniform
+            const int place = queued + __popcll(who & ((1ull << lane) - 1));
+            if (code < (uint32_t)width) {
+                atomicAdd(&mine[code], 1);
+                if (PLACE && place < kQueue) queue[place] = make_uint2(code, i + 64 * j);
+            }
+            queued += __popcll(who);
         }
     }
     below = (int)over_group<64>((uint32_t)below, 0u, [](uint32_t x, uint32_t y) { return x + y; });
@@ -154,11 +165,13 @@ __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
     if constexpr (!PLACE) {
         for (int i = tid; i < width; i += 64 * WAVES) {
             int sum = 0;
+#pragma unroll
             for (int w = 0; w < WAVES; ++w) sum += hist[w * a.width + i];
             counts[(int64_t)share * a.k + lo + i] = sum;
         }
         if (tid == 0) {
             int sum = 0;
+#pragma unroll
             for (int w = 0; w < WAVES; ++w) sum += below_of[w];
             belows[share * buckets + blockIdx.x] = sum;
         }
@@ -166,6 +179,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
     }
     int base = 0;
     if constexpr (COUNT) {
+#pragma unroll
         for (int w = 0; w < WAVES; ++w) base += below_of[w];
     } else {
         for (int s = tid; s < a.shares; s += 64 * WAVES) base += belows[s * buckets + blockIdx.x];
@@ -173,80 +187,97 @@ __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
         if (lane == 0) total_of[wave] = base;
         __syncthreads();
         base = 0;
+#pragma unroll
         for (int w = 0; w < WAVES; ++w) base += total_of[w];
         __syncthreads();
     }
-    // where each code's list begins, in it this share's part, and in that each wave's; a lane per code, 64 * WAVES codes at a time
+    // where each code's list begins, in it this share's part, and in that each wave's; a lane per code, and as many lanes more as there are
+    // for the counts of the shares
     int32_t *start = a.start + (int64_t)stage * (a.k + 1);
-    for (int c0 = 0; c0 < width; c0 += 64 * WAVES) {
-        const int c = c0 + tid;
-        int all = 0, ahead = 0;  // of the code: positions in all shares, in the shares before this one
-        if (c < width) {
-            if constexpr (COUNT) {
-                for (int w = 0; w < WAVES; ++w) all += hist[w * a.width + c];
-            } else {
-                for (int s = 0; s < a.shares; s += 16) {
-                    int here[16];
+    int all = 0, ahead = 0;  // of code tid: positions in all shares, in the shares before this one
+    if constexpr (COUNT) {
+        if (tid < width) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) here[j] = s + j < a.shares ? counts[(int64_t)(s + j) * a.k + lo + c] : 0;
+            for (int w = 0; w < WAVES; ++w) all += hist[w * a.width + tid];
+        }
+    } else {
+        const int sides = 64 * WAVES / width, side = tid / width, c = tid - side * width;
+        if (side < sides) {
+            for (int s = side; s < a.shares; s += 16 * sides) {
+                int here[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) all += here[j], ahead += s + j < share ? here[j] : 0;
-                }
+                for (int j = 0; j < 16; ++j) here[j] = s + j * sides < a.shares ? counts[(int64_t)(s + j * sides) * a.k + lo + c] : 0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) all += here[j], ahead += s + j * sides < share ? here[j] : 0;
             }
         }
-        int upto = all;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
-        }
-        if (lane == 63) total_of[wave] = upto;
+        sums_of[0][tid] = all;
+        sums_of[1][tid] = ahead;
         __syncthreads();
-        int at = base + upto - all, next = base;
-        for (int w = 0; w < WAVES; ++w) {
-            if (w < wave) at += total_of[w];
-            next += total_of[w];
-        }
-        if (c < width) {
-            if (share == 0) {
-                start[lo + c] = at;
-                if (lo + c == a.k - 1) start[a.k] = at + all;
-            }
-            at += ahead;
-            for (int w = 0; w < WAVES; ++w) {
-                const int here = hist[w * a.width + c];
-                hist[w * a.width + c] = at;
-                at += here;
-            }
-        }
-        base = next;
-        __syncthreads();
+        if (tid < width) {
+            for (int o = 1; o < sides; ++o) all += sums_of[0][o * width + tid], ahead += sums_of[1][o * width + tid];
+        } else
+            all = 0;
     }
+    int upto = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 63) total_of[wave] = upto;
+    __syncthreads();
+    int at = base + upto - all;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) at += w < wave ? total_of[w] : 0;
+    if (tid < width) {
+        if (share == 0) {
+            start[lo + tid] = at;
+            if (lo + tid == a.k - 1) start[a.k] = at + all;
+        }
+        at += ahead;
+        int here[WAVES];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) here[w] = hist[w * a.width + tid];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            hist[w * a.width + tid] = at;
+            at += here[w];
+        }
+    }
+    __syncthreads();
     int32_t *rows = a.rows + (int64_t)stage * a.n, *edges = a.edges + (int64_t)stage * embed_edges(a.n);
-    for (int i = from + lane; i - lane < to; i += 64 * AHEAD) {
-        uint32_t c[AHEAD];
+    // up to 64 positions in their order, those with `own` in the bucket
+    const auto put = [&](bool own, uint32_t code, int position) {
+        // the lanes with the same code: bit by bit of it
+        unsigned long long same = __ballot(own);
+        for (int bit = 1; bit < a.width; bit <<= 1) {
+            const unsigned long long set = __ballot((code & bit) != 0);
+            same &= code & bit ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int place = own ? mine[code] + rank : 0;
+        wave_sync();
+        if (own && rank == 0) mine[code] = place + __popcll(same);
+        wave_sync();
+        if (own) {
+            rows[place] = position;
+            if (place % kLongCode == 0) edges[place / kLongCode] = lo + (int)code;
+        }
+    };
+    if (queued <= kQueue) {  // uniform
+        for (int i = lane; i - lane < queued; i += 64) {
+            const uint2 o = queue[min(i, queued - 1)];
+            put(i < queued, o.x, (int)o.y);
+        }
+    } else {
+        for (int i = from + lane; i - lane < to; i += 64 * AHEAD) {
+            uint32_t c[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) c[j] = code_of(i + 64 * j) - (uint32_t)lo;
+            for (int j = 0; j < AHEAD; ++j) c[j] = code_of(i + 64 * j) - (uint32_t)lo;
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const bool own = c[j] < (uint32_t)width;
-            const unsigned long long who = __ballot(own);
-            if (!who) continue;  // uniform
-            // the lanes with the same code: bit by bit of it
-            unsigned long long same = who;
-            for (int bit = 1; bit < a.width; bit <<= 1) {
-                const unsigned long long set = __ballot((c[j] & bit) != 0);
-                same &= c[j] & bit ? set : ~set;
-            }
-            const int rank = __popcll(same & ((1ull << lane) - 1));
-            const int place = own ? mine[c[j]] + rank : 0;
-            wave_sync();
-            if (own && rank == 0) mine[c[j]] = place + __popcll(same);
-            wave_sync();
-            if (own) {
-                rows[place] = i + 64 * j;
-                if (place % kLongCode == 0) edges[place / kLongCode] = lo + (int)c[j];
-            }
+            for (int j = 0; j < AHEAD; ++j)
+                if (__ballot(c[j] < (uint32_t)width)) put(c[j] < (uint32_t)width, c[j], i + 64 * j);
         }
     }
 }

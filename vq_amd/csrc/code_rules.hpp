@@ -181,6 +181,8 @@ struct ListPlan {
     int32_t share, shares;
 };
 constexpr int kBucketMost = 960;
+// 16 waves' counts, and (to write the list) 512 positions and codes of each wave.
+constexpr int list_lds(int width, bool place) { return (16 * width + 1) / 2 * 8 + (place ? 16 * 512 * 8 : 0); }
 inline ListPlan plan_lists(int64_t n, int32_t k) {
     if (n <= 32768) {
         const int32_t width = std::min<int32_t>(512, (k + 255) / 256);

@@ -91,6 +91,7 @@ struct vq_ctx {
     DevBuf score_parts, score_packed;
     DevBuf code_work;            // lists of positions by code, parts of rows against a teacher or of drafts; kept like these two
     std::vector<void *> outgrown;
+    uint32_t list_lds_set = 0;    // the same granted to the lists of positions by code, a bit per instance
     uint32_t scores_lds_set = 0;  // dynamic-LDS limit granted to the tiles of scores, a bit per instance
     // optional per-kernel-class timing (HIP events on the stream)
     bool prof_on = false;

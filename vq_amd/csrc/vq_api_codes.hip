@@ -94,24 +94,32 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
     const vq::ListPlan plan = vq::plan_lists(n, k);
     const vq::ListArgs l{d_codes, code_stride, (int)n, k, plan.width, plan.share, plan.shares, (int32_t *)(w + work.start),
                          (int32_t *)(w + work.rows), (int32_t *)(w + work.edges), (int32_t *)(w + work.counts), (int32_t *)(w + work.below)};
-    const auto lists = [&](auto bytes) {
+    const auto lists = [&](auto bytes) -> int32_t {
         constexpr int BYTES = decltype(bytes)::value;
         const dim3 grid(plan.buckets, plan.shares, m), wg(1024);
-        const int lds = 16 * plan.width * 4;
+        const int lds = vq::list_lds(plan.width, true), count_lds = vq::list_lds(plan.width, false);
+        const int bit = 1 << (2 * (BYTES >> 1) + (plan.shares == 1));
+        if (!(ctx->list_lds_set & bit)) {  // more than 64 KB
+            const auto kernel = plan.shares == 1 ? vq::k_code_lists<16, BYTES, true, true> : vq::k_code_lists<16, BYTES, false, true>;
+            VQ_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                            vq::list_lds(vq::kBucketMost, true)));
+            ctx->list_lds_set |= bit;
+        }
         if (plan.shares == 1) {
             hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, true, true>), grid, wg, lds, ctx->stream, l);
         } else {
-            hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, true, false>), grid, wg, lds, ctx->stream, l);
+            hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, true, false>), grid, wg, count_lds, ctx->stream, l);
             hipLaunchKernelGGL((vq::k_code_lists<16, BYTES, false, true>), grid, wg, lds, ctx->stream, l);
         }
+        VQ_HIP(ctx, hipGetLastError());
+        return VQ_OK;
     };
     if (code_bytes == 1)
-        lists(std::integral_constant<int, 1>());
+        VQ_TRY(lists(std::integral_constant<int, 1>()));
     else if (code_bytes == 2)
-        lists(std::integral_constant<int, 2>());
+        VQ_TRY(lists(std::integral_constant<int, 2>()));
     else
-        lists(std::integral_constant<int, 4>());
-    VQ_HIP(ctx, hipGetLastError());
+        VQ_TRY(lists(std::integral_constant<int, 4>()));
     const int columns = 16 * 16 / vq::type_bytes(type), across = cdiv(dim, columns);
     // codes of a workgroup: as many as leave 2048 workgroups, 16 to 128
     const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(16, (int64_t)k * m * across / 2048 / 16 * 16));
