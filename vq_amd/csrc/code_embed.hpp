@@ -7,7 +7,8 @@
 
 namespace vq {
 
-// V values of a row from `s` on; `left` of them are the row's, the others 0.  (Held in words: an array of 16-bit values is loaded one by one.)
+// V values of a row from `s` on.  (Held in words: an array of 16-bit values is loaded one by one.)  A row's last piece, where it has no V values left,
+// is read from V before its end on and written value by value; rows shorter than that have V = 1.
 template <typename T, int V> struct Values {
     typedef typename T::Raw Raw;
     static constexpr int WORDS = V * (int)sizeof(Raw) / 4;
@@ -20,26 +21,10 @@ template <typename T, int V> struct Values {
                 return T::up((Raw)(v & 1 ? w[v >> 1] >> 16 : w[v >> 1] & 0xffffu));
         }
     };
-    static __device__ __forceinline__ Piece fetch(const Raw *s, int left) {
-        Piece p;
-        if (left >= V) {
-            p = *reinterpret_cast<const Piece *>(s);
-        } else {
-#pragma unroll
-            for (int q = 0; q < WORDS; ++q) p.w[q] = 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v < left) {
-                    if constexpr (sizeof(Raw) == 4)
-                        p.w[v] = __builtin_bit_cast(uint32_t, s[v]);
-                    else
-                        p.w[v >> 1] |= (uint32_t)s[v] << (v & 1) * 16;
-                }
-        }
-        return p;
-    }
-    static __device__ __forceinline__ void store(Raw *to, const float (&x)[V], int left) {
-        if (left >= V) {
+    static __device__ __forceinline__ Piece fetch(const Raw *s) { return *reinterpret_cast<const Piece *>(s); }
+    // values from number `skip` on
+    static __device__ __forceinline__ void store(Raw *to, const float (&x)[V], int skip = 0) {
+        if (skip == 0) {
             Piece p;
 #pragma unroll
             for (int q = 0; q < WORDS; ++q) {
@@ -52,10 +37,21 @@ template <typename T, int V> struct Values {
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (v < left) to[v] = T::down(x[v]);
+                if (v >= skip) to[v] = T::down(x[v]);
         }
     }
 };
+template <typename T> struct Values<T, 1> {
+    typedef typename T::Raw Raw;
+    struct Piece {
+        Raw value;
+        __device__ __forceinline__ float at(int) const { return T::up(value); }
+    };
+    static __device__ __forceinline__ Piece fetch(const Raw *s) { return {*s}; }
+    static __device__ __forceinline__ void store(Raw *to, const float (&x)[1], int = 0) { *to = T::down(x[0]); }
+};
+// Values of a lane: 16 bytes of the rows, or one where a row has fewer.
+template <typename T> constexpr int wide() { return 16 / (int)sizeof(typename T::Raw); }
 
 struct EmbedArgs {
     const void *table;
@@ -72,16 +68,16 @@ struct EmbedArgs {
 // out[i] = scale * sum over the stages s, in their order, of table[s * k + code].  The columns are cut into `slices` (of `pieces` vectors of 16 bytes of
 // the table each): workgroup b has slice b % slices, so that with eight of them every XCD reads its own eighth of the tables' columns,
 // which its L2 may hold.  1 << shift lanes of a row, rows side by side in a workgroup, a slice's further pieces by blockIdx.y.
-template <typename T, typename O>
+template <typename T, typename O, int V>
 __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift, int slices, int pieces) {
     typedef typename T::Raw Raw;
-    constexpr int V = 16 / (int)sizeof(Raw), AHEAD = 8;
+    constexpr int AHEAD = 8;
     typedef Values<T, V> In;
     const int slice = blockIdx.x % (unsigned)slices;
     const int64_t row = (int64_t)(blockIdx.x / (unsigned)slices) * (256 >> shift) + (threadIdx.x >> shift);
     const int piece = (blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1));
-    const int at = (slice * pieces + piece) * V, left = a.dim - at;
-    if (row >= a.n || left <= 0 || piece >= pieces) return;
+    const int place = (slice * pieces + piece) * V, at = min(place, a.dim - V);
+    if (row >= a.n || place >= a.dim || piece >= pieces) return;
     const Raw *table = (const Raw *)a.table + at;
     float sum[V];
 #pragma unroll
@@ -95,7 +91,7 @@ __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift, int 
             const int64_t code = s + j < a.m ? code_at(a.codes, a.code_bytes, row * a.code_stride + s + j) : -1;
             bad |= code >= a.k;
             has[j] = code >= 0 && code < a.k;
-            if (has[j]) p[j] = In::fetch(table + ((int64_t)(s + j) * a.k + code) * a.ld, left);
+            if (has[j]) p[j] = In::fetch(table + ((int64_t)(s + j) * a.k + code) * a.ld);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
@@ -106,7 +102,7 @@ __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift, int 
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[v] = bad ? __builtin_nanf("") : a.scale * sum[v];
-    Values<O, V>::store((typename O::Raw *)a.out + row * a.ld_out + at, sum, left);
+    Values<O, V>::store((typename O::Raw *)a.out + row * a.ld_out + at, sum, place - at);
 }
 
 // ---- the positions by code ---------------------------------------------------------------------------
@@ -291,17 +287,22 @@ struct SumArgs {
     int accumulate;
     void *grad;
     int64_t ld_grad;
+    const void *few_codes;  // (where the workgroups make their own lists)
+    int code_bytes;
+    int64_t code_stride;
     const int32_t *start, *rows, *edges;
     float *partial;  // [stage][chunk][2][padded dim]
     int chunks, padded, codes, groups, across, first;  // codes of a workgroup; workgroups of codes; of columns, and the first of these
 };
 
 constexpr int kGroupCodes = 128;  // codes of a workgroup at most
-constexpr int kOwnMembers = 32;  // a code of more positions is summed by the whole workgroup
+// A code of more positions than this is summed by the whole workgroup.  (Where a workgroup has few codes it sums one alone sooner than a group of
+// lanes sums 32 rows.)
+constexpr int kOwnMembers = 32, kFewMembers = 10;
 
 // Adds V columns of the members number a, a + step, ... below b of a list, in that order.
-template <typename T, int V>
-__device__ __forceinline__ void sum_members(const SumArgs &s, const int32_t *rows, int a, int b, int step, int at, int left, float (&sum)[V]) {
+template <typename T, int V, typename Rows>
+__device__ __forceinline__ void sum_members(const SumArgs &s, Rows rows, int a, int b, int step, int at, float (&sum)[V]) {
     typedef typename T::Raw Raw;
     typedef Values<T, V> In;
     constexpr int AHEAD = 8;
@@ -313,7 +314,7 @@ __device__ __forceinline__ void sum_members(const SumArgs &s, const int32_t *row
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld, left);
+        for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (p + j * step < b) {
@@ -329,7 +330,7 @@ __device__ __forceinline__ void sum_members(const SumArgs &s, const int32_t *row
 constexpr int kZeroCodes = 64, kZeroBytes = 16384;
 template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs &a, unsigned id, int stage, int *list, int *count) {
     typedef typename O::Raw Out;
-    constexpr int VO = 16 / (int)sizeof(Out), PIECE = kZeroBytes / (int)sizeof(Out);
+    constexpr int VO = wide<O>(), PIECE = kZeroBytes / (int)sizeof(Out);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned pieces = (unsigned)(a.dim + PIECE - 1) / PIECE;
     const int64_t code = (int64_t)(id / pieces) * kZeroCodes + tid;
@@ -350,8 +351,9 @@ template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs 
                 typedef uint32_t Four __attribute__((ext_vector_type(4)));
                 __builtin_nontemporal_store(Four{0, 0, 0, 0}, reinterpret_cast<Four *>(to + c));
             } else {
-                const float zeros[VO] = {};
-                Values<O, VO>::store(to + c, zeros, end - c);
+                #pragma unroll
+                for (int v = 0; v < VO; ++v)
+                    if (c + v < end) to[c + v] = O::down(0.0f);
             }
         }
     }
@@ -360,31 +362,58 @@ template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs 
 // Rows of the gradient: 16 lanes sum V columns each of a code's members.  The first a.groups workgroups take codes, those behind them the
 // chunks of the list that belong to codes of more than kLongCode members; a.across workgroups side by side have the columns,
 // 16 * V each; the last ones write the rows without members.  blockIdx.z: stages.
-template <typename T, typename O>
+// FEW: up to kFewPositions of them, which every workgroup lists for its own codes: one launch instead of two.
+template <typename T, typename O, int V, bool FEW>
 __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     typedef typename T::Raw Raw;
     typedef typename O::Raw Out;
-    constexpr int V = 16 / (int)sizeof(Raw), COLUMNS = 16 * V, VO = 16 / (int)sizeof(Out);
+    constexpr int COLUMNS = 16 * V, VO = V == 1 ? 1 : wide<O>();
     __shared__ float red[16][COLUMNS];
-    __shared__ int begin[kGroupCodes], behind[kGroupCodes], count[2];
-    __shared__ uint8_t which[2][kGroupCodes];
-    const int tid = threadIdx.x, sub = tid >> 4, column = (a.first + blockIdx.x % (unsigned)a.across) * COLUMNS, at = column + (tid & 15) * V, left = a.dim - at, stage = blockIdx.z;
-    if (blockIdx.x >= (unsigned)(a.groups + a.chunks) * (unsigned)a.across) {
+    __shared__ int begin[kGroupCodes], behind[kGroupCodes], count[3];
+    __shared__ uint8_t which[3][kGroupCodes];
+    __shared__ int few[FEW ? kFewPositions : 1], queue[FEW ? kFewPositions + 8 : 1], queued[4];
+    const int tid = threadIdx.x, sub = tid >> 4, column = (a.first + blockIdx.x % (unsigned)a.across) * COLUMNS, place = column + (tid & 15) * V, at = min(place, a.dim - V), stage = blockIdx.z;
+    const bool used = place < a.dim;  // this lane has columns
+    if (!FEW && blockIdx.x >= (unsigned)(a.groups + a.chunks) * (unsigned)a.across) {
         write_zeros<O>(a, blockIdx.x - (unsigned)(a.groups + a.chunks) * (unsigned)a.across, stage, begin, &count[0]);
         return;
     }
     const int group = blockIdx.x / (unsigned)a.across;
     const int32_t *start = a.start + (int64_t)stage * (a.k + 1), *rows = a.rows + (int64_t)stage * a.n;
+    const auto list = [&] {
+        if constexpr (FEW)
+            return (const int *)few;
+        else
+            return rows;
+    }();
     Out *grad = (Out *)a.grad + (int64_t)stage * a.k * a.ld_grad;
     float sum[V];
+    // a lane's sums to their columns' places (the last piece of a row reaches back over columns of another)
+    const auto lay_out = [&] {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (at + v >= column) red[sub][at - column + v] = sum[v];
+    };
+    // results: scaled, added to what is there
+    const auto put = [&](Out *to, float (&y)[VO], int skip) {
+        if (a.accumulate) {
+            const typename Values<O, VO>::Piece old = Values<O, VO>::fetch(to);
+#pragma unroll
+            for (int v = 0; v < VO; ++v) y[v] = __builtin_fmaf(a.scale, y[v], old.at(v));
+        } else {
+#pragma unroll
+            for (int v = 0; v < VO; ++v) y[v] *= a.scale;
+        }
+        Values<O, VO>::store(to, y, skip);
+    };
+    const auto put_one = [&](Out *to, float y) { *to = O::down(a.accumulate ? __builtin_fmaf(a.scale, y, O::up(*to)) : a.scale * y); };
     // all 16 groups of lanes sum members [from, to); the sums of COLUMNS columns are in the first lanes then
     const auto together = [&](int from, int to) {
-        if (left > 0) {
+        if (used) {
 #pragma unroll
             for (int v = 0; v < V; ++v) sum[v] = 0.0f;
-            sum_members<T, V>(a, rows, from + sub, to, 16, at, left, sum);
-#pragma unroll
-            for (int v = 0; v < V; ++v) red[sub][(tid & 15) * V + v] = sum[v];
+            sum_members<T, V>(a, list, from + sub, to, 16, at, sum);
+            lay_out();
         }
         __syncthreads();
         float total = 0.0f;
@@ -395,7 +424,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
         __syncthreads();
         return total;
     };
-    if (group >= a.groups) {
+    if (!FEW && group >= a.groups) {
         const int chunk = group - a.groups, all = start[a.k], first = chunk * kLongCode, last = min(all, first + kLongCode) - 1;
         if (first > last) return;
         // the codes of the chunk's first position and, where another one's list goes on behind the chunk, of that (no other list that
@@ -414,33 +443,96 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     }
     // the workgroup's codes by the number of their members: a group of lanes each, or the whole workgroup
     const int64_t from = (int64_t)group * a.codes;
-    if (tid < 2) count[tid] = 0;
+    if (tid < 3) count[tid] = 0;
+    int s0 = 0, s1 = 0;
+    if constexpr (FEW) {
+        // the positions of these codes, in their order, by wave; then each code's, a lane per code
+        const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        uint32_t code[kFewPositions / 256];
+#pragma unroll
+        for (int j = 0; j < kFewPositions / 256; ++j) {
+            const int i = wave * (kFewPositions / 4) + j * 64 + lane;
+            code[j] = i < a.n ? (uint32_t)(code_at(a.few_codes, a.code_bytes, (int64_t)i * a.code_stride + stage) - from) : 0xffffffffu;
+        }
+        const uint32_t codes = (uint32_t)min((int64_t)a.codes, a.k - from);
+        unsigned long long who[kFewPositions / 256];
+        int found = 0;
+#pragma unroll
+        for (int j = 0; j < kFewPositions / 256; ++j) {
+            who[j] = __ballot(code[j] < codes);
+            found += __popcll(who[j]);
+        }
+        if (lane == 0) queued[wave] = found;
+        __syncthreads();
+        int at = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            at += w < wave ? queued[w] : 0;
+            total += queued[w];
+        }
+#pragma unroll
+        for (int j = 0; j < kFewPositions / 256; ++j) {
+            if (code[j] < codes) queue[at + __popcll(who[j] & ((1ull << lane) - 1))] = (wave * (kFewPositions / 4) + j * 64 + lane) * kGroupCodes + (int)code[j];
+            at += __popcll(who[j]);
+        }
+        if (tid < 8) queue[total + tid] = -1;  // up to a whole eight: none of these codes (there are fewer than kGroupCodes)
+        __syncthreads();
+        if (tid < kFewCodes) {
+            int members = 0;
+            for (int i = 0; i < total; i += 8) {
+                int o[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) o[u] = queue[i + u];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) members += (o[u] & (kGroupCodes - 1)) == tid;
+            }
+            int upto = members;
+#pragma unroll
+            for (int d = 1; d < kFewCodes; d <<= 1) {
+                const int o = __shfl_up(upto, d);
+                if (lane >= d) upto += o;
+            }
+            s0 = upto - members;
+            s1 = s0;
+            for (int i = 0; i < total; i += 8) {
+                int o[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) o[u] = queue[i + u];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if ((o[u] & (kGroupCodes - 1)) == tid) few[s1++] = o[u] / kGroupCodes;
+            }
+        }
+    } else if (tid < a.codes && from + tid < a.k) {
+        s0 = start[from + tid];
+        s1 = start[from + tid + 1];
+    }
     __syncthreads();
     if (tid < a.codes && from + tid < a.k) {
-        const int s0 = start[from + tid], s1 = start[from + tid + 1], members = s1 - s0;
+        const int members = s1 - s0;
         begin[tid] = s0;
         behind[tid] = s1;
-        if (members > 0 && members <= kLongCode) {
-            const int kind = members <= kOwnMembers ? 0 : 1;
+        if (members <= kLongCode) {
+            const int kind = members == 0 ? 2 : members <= (FEW ? kFewMembers : kOwnMembers) ? 0 : 1;
             which[kind][atomicAdd(&count[kind], 1)] = (uint8_t)tid;  // (in whatever order: each is a sum of its own)
         }
     }
     __syncthreads();
     // codes of few members, a group of lanes each: the first two members of four codes at a time, since most have no more
     constexpr int SIDE = 4, EARLY = 2;
-    for (int i = sub; i < count[0]; i += 16 * SIDE) {
+    for (int i = sub; i < count[0]; i += 16 * SIDE) {  // (lanes without columns of the row go along)
         typename Values<T, V>::Piece x[SIDE][EARLY];
         int row[SIDE][EARLY];
 #pragma unroll
         for (int u = 0; u < SIDE; ++u) {  // (beyond the last code or member the last one again)
             const int j = which[0][min(i + 16 * u, count[0] - 1)], s0 = begin[j], s1 = behind[j];
 #pragma unroll
-            for (int e = 0; e < EARLY; ++e) row[u][e] = rows[min(s0 + e, s1 - 1)];
+            for (int e = 0; e < EARLY; ++e) row[u][e] = list[min(s0 + e, s1 - 1)];
         }
 #pragma unroll
         for (int u = 0; u < SIDE; ++u)
 #pragma unroll
-            for (int e = 0; e < EARLY; ++e) x[u][e] = Values<T, V>::fetch((const Raw *)a.g + at + (int64_t)row[u][e] * a.ld, left);
+            for (int e = 0; e < EARLY; ++e) x[u][e] = Values<T, V>::fetch((const Raw *)a.g + at + (int64_t)row[u][e] * a.ld);
 #pragma unroll
         for (int u = 0; u < SIDE; ++u) {
             if (i + 16 * u >= count[0]) break;
@@ -451,37 +543,28 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) sum[v] += x[u][1].at(v);
             }
-            if (s0 + EARLY < s1 && left > 0) sum_members<T, V>(a, rows, s0 + EARLY, s1, 1, at, left, sum);
-            // the lanes' 16 bytes of results side by side
-            Out *to = grad + (from + j) * a.ld_grad + column;
-            const auto finish = [&](float (&y)[VO], int col) {
-                const int rest = a.dim - column - col;
-                if (rest <= 0) return;
-                if (a.accumulate) {
-                    const typename Values<O, VO>::Piece old = Values<O, VO>::fetch(to + col, rest);
-#pragma unroll
-                    for (int v = 0; v < VO; ++v) y[v] = __builtin_fmaf(a.scale, y[v], old.at(v));
-                } else {
-#pragma unroll
-                    for (int v = 0; v < VO; ++v) y[v] *= a.scale;
-                }
-                Values<O, VO>::store(to + col, y, rest);
-            };
+            if (s0 + EARLY < s1) sum_members<T, V>(a, list, s0 + EARLY, s1, 1, at, sum);
+            Out *to = grad + (from + j) * a.ld_grad;
             if constexpr (VO == V) {
-                finish(sum, (tid & 15) * V);
-            } else {
+                if (used) put(to + at, sum, place - at);
+            } else {  // the lanes' 16 bytes of results side by side
                 wave_sync();
-#pragma unroll
-                for (int v = 0; v < V; ++v) red[sub][(tid & 15) * V + v] = sum[v];
+                if (used) lay_out();
                 wave_sync();
 #pragma unroll
                 for (int c = 0; c < COLUMNS; c += 16 * VO) {
-                    const int col = c + (tid & 15) * VO;
-                    if (col < COLUMNS) {
-                        float y[VO];
+                    const int col = c + (tid & 15) * VO, rest = a.dim - column - col;
+                    float y[VO];
+                    if (col < COLUMNS && rest > 0) {
 #pragma unroll
                         for (int v = 0; v < VO; ++v) y[v] = red[sub][col + v];
-                        finish(y, col);
+                        if (rest >= VO) {
+                            put(to + column + col, y, 0);
+                        } else {
+#pragma unroll
+                            for (int v = 0; v < VO; ++v)
+                                if (v < rest) put_one(to + column + col + v, y[v]);
+                        }
                     }
                 }
             }
@@ -492,9 +575,12 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     for (int i = 0; i < n_longer; ++i) {
         const int j = which[1][i];
         const float total = together(begin[j], behind[j]);
-        if (tid < COLUMNS && column + tid < a.dim) {
-            Out *to = grad + (from + j) * a.ld_grad + column + tid;
-            *to = O::down(a.accumulate ? __builtin_fmaf(a.scale, total, O::up(*to)) : a.scale * total);
+        if (tid < COLUMNS && column + tid < a.dim) put_one(grad + (from + j) * a.ld_grad + column + tid, total);
+    }
+    if (FEW && !a.accumulate) {
+        for (int i = sub; i < count[2]; i += 16) {
+            Out *to = grad + (from + which[2][i]) * a.ld_grad;
+            for (int c = column + (tid & 15); c < min(a.dim, column + COLUMNS); c += 16) to[c] = O::down(0.0f);
         }
     }
 }

@@ -193,6 +193,11 @@ inline ListPlan plan_lists(int64_t n, int32_t k) {
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / buckets)), share = std::max<int64_t>(4096, (n + most - 1) / most);
     return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
 }
+// Up to so many positions the workgroups that sum make their lists themselves, where no more than 512 of them read all codes (333 x 100 f32, 1001
+// codes: 10.0 us in two launches, ZZ so).
+constexpr int kFewPositions = 1024;
+constexpr int kFewCodes = 16;  // codes of such a workgroup
+inline bool embed_few(int64_t n, int32_t k, int32_t m, int64_t across) { return n <= kFewPositions && (k + kFewCodes - 1) / kFewCodes * m * across <= 512; }
 // A code of more positions than this is summed in pieces of as many positions of the list, whose sums are joined afterwards.
 constexpr int kLongCode = 1024;
 constexpr int64_t embed_edges(int64_t n) { return (n + kLongCode - 1) / kLongCode; }  // pieces of the list

@@ -14,6 +14,14 @@ template <typename F> void by_types(int32_t type, int32_t other, F f) {
     by_type(type, [&](auto t) { by_type(other, [&](auto o) { f(t, o); }); });
 }
 
+// Sums by code: 16 bytes of a row per lane, or a value where a row has fewer.
+template <typename T, typename O, bool FEW> void embed_sums(vq_ctx *ctx, const vq::SumArgs &a, unsigned groups, int m) {
+    if (a.dim < vq::wide<T>())
+        hipLaunchKernelGGL((vq::k_embed_sums<T, O, 1, FEW>), dim3(groups, 1, m), dim3(256), 0, ctx->stream, a);
+    else
+        hipLaunchKernelGGL((vq::k_embed_sums<T, O, vq::wide<T>(), FEW>), dim3(groups, 1, m), dim3(256), 0, ctx->stream, a);
+}
+
 // The alternatives' rows of a launch, from row r on.
 vq::DistillArgs distill_slice(const vq::DistillArgs &a, int64_t r, int64_t rows, int e) {
     vq::DistillArgs s = a;
@@ -62,7 +70,7 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
     VQ_TRY(admit(ctx, vq::check_code_embed(type, d_table, k, ld_table, dim, m, code_bytes, d_codes, n, code_stride, scale, out_type,
                                            d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
-    const int vectors = cdiv(dim, 16 / vq::type_bytes(type)), slices = vq::embed_slices(n, k, m, vectors), pieces = cdiv(vectors, slices);
+    const int wide = 16 / vq::type_bytes(type), vectors = dim < wide ? dim : cdiv(dim, wide), slices = vq::embed_slices(n, k, m, vectors), pieces = cdiv(vectors, slices);
     int shift = 0;
     while (shift < 8 && 1 << shift < pieces) ++shift;
     const unsigned across = cdiv(pieces, 1 << shift);
@@ -71,8 +79,13 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
         const vq::EmbedArgs a{d_table, ld_table, k, dim, m, (const char *)d_codes + r * code_stride * code_bytes, code_bytes, std::min(slice, n - r),
                               code_stride, scale, (char *)d_out + r * ld_out * vq::type_bytes(out_type), ld_out};
         by_types(type, out_type, [&](auto t, auto o) {
-            hipLaunchKernelGGL((vq::k_code_embed<decltype(t), decltype(o)>), dim3((unsigned)cdiv64(a.n, 256 >> shift) * slices, across), dim3(256), 0,
-                               ctx->stream, a, shift, slices, pieces);
+            typedef decltype(t) T;
+            typedef decltype(o) O;
+            const dim3 grid((unsigned)cdiv64(a.n, 256 >> shift) * slices, across);
+            if (dim < vq::wide<T>())
+                hipLaunchKernelGGL((vq::k_code_embed<T, O, 1>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+            else
+                hipLaunchKernelGGL((vq::k_code_embed<T, O, vq::wide<T>()>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
         });
         VQ_HIP(ctx, hipGetLastError());
     }
@@ -88,6 +101,16 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
     VQ_TRY(admit(ctx, vq::check_code_embed_grad(type, d_g, n, ld_g, dim, m, code_bytes, d_codes, code_stride, scale, k, accumulate,
                                                 grad_type, d_grad, ld_grad), accumulate ? n : 1, &go));
     if (!go) return VQ_OK;
+    const int wide = 16 / vq::type_bytes(type), columns = 16 * (dim < wide ? 1 : wide), across = cdiv(dim, columns);
+    if (vq::embed_few(n, k, m, across)) {
+        vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, d_codes, code_bytes, code_stride, nullptr, nullptr, nullptr, nullptr,
+                      0, 0, vq::kFewCodes, (int)cdiv(k, vq::kFewCodes), across, 0};
+        by_types(type, grad_type, [&](auto t, auto o) {
+            embed_sums<decltype(t), decltype(o), true>(ctx, a, a.groups * across, m);
+        });
+        VQ_HIP(ctx, hipGetLastError());
+        return VQ_OK;
+    }
     const vq::EmbedWork work = vq::embed_work(n, k, dim, m);
     VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)work.bytes));
     char *w = (char *)ctx->code_work.p;
@@ -120,10 +143,9 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
         VQ_TRY(lists(std::integral_constant<int, 2>()));
     else
         VQ_TRY(lists(std::integral_constant<int, 4>()));
-    const int columns = 16 * 16 / vq::type_bytes(type), across = cdiv(dim, columns);
     // codes of a workgroup: as many as leave 2048 workgroups, 16 to 128
     const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(16, (int64_t)k * m * across / 2048 / 16 * 16));
-    vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, l.start, l.rows, l.edges, (float *)(w + work.partial),
+    vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, nullptr, 0, 0, l.start, l.rows, l.edges, (float *)(w + work.partial),
                   (int)vq::embed_chunks(n), (dim + 15) / 16 * 16, codes, (int)cdiv(k, codes), 0, 0};
     // the columns of some workgroups side by side, the others' in launches of their own: a grid has fewer than 2^32 lanes
     const int most = std::max(1, (1 << 23) / (a.groups + a.chunks));
@@ -133,7 +155,7 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
         const bool last = a.first + a.across == across;
         const unsigned zeros = last && !accumulate ? cdiv(k, vq::kZeroCodes) * cdiv((int64_t)dim * vq::type_bytes(grad_type), vq::kZeroBytes) : 0;
         by_types(type, grad_type, [&](auto t, auto o) {
-            hipLaunchKernelGGL((vq::k_embed_sums<decltype(t), decltype(o)>), dim3((a.groups + a.chunks) * a.across + zeros, 1, m), dim3(256), 0, ctx->stream, a);
+            embed_sums<decltype(t), decltype(o), false>(ctx, a, (a.groups + a.chunks) * a.across + zeros, m);
         });
         VQ_HIP(ctx, hipGetLastError());
     }
