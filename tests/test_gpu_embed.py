@@ -69,7 +69,7 @@ SHAPES = [  # n, m, k, dim
 
 
 @pytest.mark.parametrize("kind,out", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
-@pytest.mark.parametrize("n,m,k,dim", SHAPES)
+@pytest.mark.parametrize("n,m,k,dim", SHAPES + [(20000, 5, 300, 200), (20001, 4, 700, 1030), (3000, 13, 512, 1000)])  # two pieces a lane; columns by XCD
 def test_embed(ctx, n, m, k, dim, kind, out):
     rng = np.random.default_rng(n + dim)
     table = R.pack(rng.standard_normal((m * k, dim)), kind)

@@ -68,41 +68,85 @@ struct EmbedArgs {
 // out[i] = scale * sum over the stages s, in their order, of table[s * k + code].  The columns are cut into `slices` (of `pieces` vectors of 16 bytes of
 // the table each): workgroup b has slice b % slices, so that with eight of them every XCD reads its own eighth of the tables' columns,
 // which its L2 may hold.  1 << shift lanes of a row, rows side by side in a workgroup, a slice's further pieces by blockIdx.y.
-template <typename T, typename O, int V>
+// Where a row is the sum of many the additions count: two instructions per value, so that what else a row costs is kept small: offsets of
+// 32 bits (Place) where a stage's table is below 4 GiB and its rows below 16 MiB apart, no conditions where all codes of a wave are codes.
+template <typename T, typename O, int V, int NV, int BYTES, typename Place>
 __global__ void __launch_bounds__(256) k_code_embed(EmbedArgs a, int shift, int slices, int pieces) {
     typedef typename T::Raw Raw;
-    constexpr int AHEAD = 8;
     typedef Values<T, V> In;
     const int slice = blockIdx.x % (unsigned)slices;
     const int64_t row = (int64_t)(blockIdx.x / (unsigned)slices) * (256 >> shift) + (threadIdx.x >> shift);
-    const int piece = (blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1));
-    const int place = (slice * pieces + piece) * V, at = min(place, a.dim - V);
-    if (row >= a.n || place >= a.dim || piece >= pieces) return;
-    const Raw *table = (const Raw *)a.table + at;
-    float sum[V];
+    // NV pieces of a lane, as far apart as its row has lanes
+    const int piece = (blockIdx.y * NV << shift) + (threadIdx.x & ((1 << shift) - 1)), end = min(pieces, (a.dim + V - 1) / V - slice * pieces);
+    if (row >= a.n || piece >= end) return;
+    const Place step = (Place)a.ld * (Place)sizeof(Raw), stage = (Place)a.k * step;
+    const int64_t code0 = row * a.code_stride;
+    float sum[NV][V];
+    Place from[NV];
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] = 0.0f;
-    bool bad = false;
-    for (int s = 0; s < a.m; s += AHEAD) {
-        typename In::Piece p[AHEAD];
-        bool has[AHEAD];
+    for (int u = 0; u < NV; ++u) {
+        from[u] = (Place)min((slice * pieces + min(piece + (u << shift), end - 1)) * V, a.dim - V) * (Place)sizeof(Raw);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int64_t code = s + j < a.m ? code_at(a.codes, a.code_bytes, row * a.code_stride + s + j) : -1;
-            bad |= code >= a.k;
-            has[j] = code >= 0 && code < a.k;
-            if (has[j]) p[j] = In::fetch(table + ((int64_t)(s + j) * a.k + code) * a.ld);
-        }
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (has[j]) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) sum[v] += p[j].at(v);
-            }
+        for (int v = 0; v < V; ++v) sum[u][v] = 0.0f;
     }
+    bool bad = false;
+    const char *table = (const char *)a.table;  // of the stage
+    const auto row_at = [&](uint32_t code) {
+        if constexpr (sizeof(Place) == 4)
+            return __umul24(code, step);  // (one instruction)
+        else
+            return (Place)code * step;
+    };
+    int s = 0;
+    const auto stages = [&](auto count) {
+        constexpr int S = decltype(count)::value;
+        uint32_t code[S];  // (a negative one is above all others)
+        bool fine = true;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] = bad ? __builtin_nanf("") : a.scale * sum[v];
-    Values<O, V>::store((typename O::Raw *)a.out + row * a.ld_out + at, sum, place - at);
+        for (int j = 0; j < S; ++j) code[j] = (uint32_t)code_at(a.codes, BYTES, code0 + s + j);
+#pragma unroll
+        for (int j = 0; j < S; ++j) fine = fine && code[j] < (uint32_t)a.k;
+        const auto fetch = [&](int j, int u) { return In::fetch(reinterpret_cast<const Raw *>(table + (int64_t)j * stage + (Place)(from[u] + row_at(code[j])))); };
+        if (__ballot(!fine) == 0) {
+            typename In::Piece p[S][NV];
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int u = 0; u < NV; ++u) p[j][u] = fetch(j, u);
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int u = 0; u < NV; ++u)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) sum[u][v] += p[j][u].at(v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (code[j] < (uint32_t)a.k) {
+#pragma unroll
+                    for (int u = 0; u < NV; ++u) {
+                        const typename In::Piece p = fetch(j, u);
+#pragma unroll
+                        for (int v = 0; v < V; ++v) sum[u][v] += p.at(v);
+                    }
+                } else if ((int32_t)code[j] >= 0)
+                    bad = true;
+        }
+        s += S;
+        table += (int64_t)S * stage;
+    };
+    while (s + 8 <= a.m) stages(std::integral_constant<int, 8>());
+    if (a.m & 4) stages(std::integral_constant<int, 4>());
+    if (a.m & 2) stages(std::integral_constant<int, 2>());
+    if (a.m & 1) stages(std::integral_constant<int, 1>());
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        if (u > 0 && piece + (u << shift) >= end) break;
+        const int place = (slice * pieces + piece + (u << shift)) * V, at = min(place, a.dim - V);
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[u][v] = bad ? __builtin_nanf("") : a.scale * sum[u][v];
+        Values<O, V>::store((typename O::Raw *)a.out + row * a.ld_out + at, sum[u], place - at);
+    }
 }
 
 // ---- the positions by code ---------------------------------------------------------------------------
@@ -325,8 +369,8 @@ __device__ __forceinline__ void sum_members(const SumArgs &s, Rows rows, int a, 
 }
 
 // Rows without members, most of a large table's, of 64 codes and up to 16 KB of their columns: whole lines that pass the caches.  These
-// workgroups come last: zeros written beside the reads of the sums made both slower (16,384 x 1280 bf16 to 65,536 f32 rows 100 us, apart
-// ZZ us).
+// workgroups come last: zeros written beside the reads of the sums made both slower (16,384 x 1280 bf16 to 65,536 f32 rows 101 us, apart
+// 77).
 constexpr int kZeroCodes = 64, kZeroBytes = 16384;
 template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs &a, unsigned id, int stage, int *list, int *count) {
     typedef typename O::Raw Out;

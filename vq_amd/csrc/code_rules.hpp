@@ -172,6 +172,10 @@ inline Refusal check_code_verify(int32_t type, const void *target, int64_t ld_ta
 // 128 bytes of a row or more; otherwise one.
 inline int embed_slices(int64_t n, int32_t k, int32_t m, int vectors) { return n >= 2 * (int64_t)k && vectors >= 64 && (int64_t)k * m * vectors * 16 > 2 << 20 ? 8 : 1; }
 
+// Pieces of 16 bytes of a row that a lane has: two where the additions of several stages count more than the number of waves (65,536 x 8 stages
+// of 1024 bf16 62 us with one, 59 with two).
+inline int embed_pieces(int64_t n, int32_t m, int pieces) { return m >= 4 && pieces >= 16 && n * pieces >= 1 << 18 ? 2 : 1; }
+
 // ---- sums by code ------------------------------------------------------------------------------------
 // The positions of each stage in the order of their codes, and where each code's positions begin: k + 1 numbers.  Workgroups of 16 waves
 // list a bucket of codes each, of a share of the positions.  One share, and one launch, up to 32,768 positions; more positions in shares, in two
@@ -194,7 +198,7 @@ inline ListPlan plan_lists(int64_t n, int32_t k) {
     return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
 }
 // Up to so many positions the workgroups that sum make their lists themselves, where no more than 512 of them read all codes (333 x 100 f32, 1001
-// codes: 10.0 us in two launches, ZZ so).
+// codes: 9.8 us in two launches, 7.4 so).
 constexpr int kFewPositions = 1024;
 constexpr int kFewCodes = 16;  // codes of such a workgroup
 inline bool embed_few(int64_t n, int32_t k, int32_t m, int64_t across) { return n <= kFewPositions && (k + kFewCodes - 1) / kFewCodes * m * across <= 512; }

@@ -14,6 +14,16 @@ template <typename F> void by_types(int32_t type, int32_t other, F f) {
     by_type(type, [&](auto t) { by_type(other, [&](auto o) { f(t, o); }); });
 }
 
+// f(integral constant) with the bytes of a code
+template <typename F> void by_bytes(int32_t bytes, F f) {
+    if (bytes == 1)
+        f(std::integral_constant<int, 1>());
+    else if (bytes == 2)
+        f(std::integral_constant<int, 2>());
+    else
+        f(std::integral_constant<int, 4>());
+}
+
 // Sums by code: 16 bytes of a row per lane, or a value where a row has fewer.
 template <typename T, typename O, bool FEW> void embed_sums(vq_ctx *ctx, const vq::SumArgs &a, unsigned groups, int m) {
     if (a.dim < vq::wide<T>())
@@ -71,9 +81,11 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
                                            d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
     const int wide = 16 / vq::type_bytes(type), vectors = dim < wide ? dim : cdiv(dim, wide), slices = vq::embed_slices(n, k, m, vectors), pieces = cdiv(vectors, slices);
+    const bool near = k <= 0xffffffffll / ld_table / vq::type_bytes(type) && ld_table * vq::type_bytes(type) < 1 << 24;  // (places in bytes of a stage's table fit 32 bits)
+    const int each = near ? vq::embed_pieces(n, m, pieces) : 1;
     int shift = 0;
-    while (shift < 8 && 1 << shift < pieces) ++shift;
-    const unsigned across = cdiv(pieces, 1 << shift);
+    while (shift < 8 && each << shift < pieces) ++shift;
+    const unsigned across = cdiv(pieces, each << shift);
     const int64_t slice = std::max<int64_t>(256, ((int64_t)1 << 31) / ((int64_t)slices << shift));  // a grid has fewer than 2^32 lanes
     for (int64_t r = 0; r < n; r += slice) {
         const vq::EmbedArgs a{d_table, ld_table, k, dim, m, (const char *)d_codes + r * code_stride * code_bytes, code_bytes, std::min(slice, n - r),
@@ -82,10 +94,18 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
             typedef decltype(t) T;
             typedef decltype(o) O;
             const dim3 grid((unsigned)cdiv64(a.n, 256 >> shift) * slices, across);
-            if (dim < vq::wide<T>())
-                hipLaunchKernelGGL((vq::k_code_embed<T, O, 1>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
-            else
-                hipLaunchKernelGGL((vq::k_code_embed<T, O, vq::wide<T>()>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+            const auto go = [&](auto bytes) {
+                constexpr int BYTES = decltype(bytes)::value;
+                if (dim < vq::wide<T>())
+                    hipLaunchKernelGGL((vq::k_code_embed<T, O, 1, 1, BYTES, int64_t>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+                else if (near && each == 2)
+                    hipLaunchKernelGGL((vq::k_code_embed<T, O, vq::wide<T>(), 2, BYTES, uint32_t>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+                else if (near)
+                    hipLaunchKernelGGL((vq::k_code_embed<T, O, vq::wide<T>(), 1, BYTES, uint32_t>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+                else
+                    hipLaunchKernelGGL((vq::k_code_embed<T, O, vq::wide<T>(), 1, BYTES, int64_t>), grid, dim3(256), 0, ctx->stream, a, shift, slices, pieces);
+            };
+            by_bytes(code_bytes, go);
         });
         VQ_HIP(ctx, hipGetLastError());
     }
@@ -137,12 +157,9 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
         VQ_HIP(ctx, hipGetLastError());
         return VQ_OK;
     };
-    if (code_bytes == 1)
-        VQ_TRY(lists(std::integral_constant<int, 1>()));
-    else if (code_bytes == 2)
-        VQ_TRY(lists(std::integral_constant<int, 2>()));
-    else
-        VQ_TRY(lists(std::integral_constant<int, 4>()));
+    int32_t rc = VQ_OK;
+    by_bytes(code_bytes, [&](auto bytes) { rc = lists(bytes); });
+    VQ_TRY(rc);
     // codes of a workgroup: as many as leave 2048 workgroups, 16 to 128
     const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(16, (int64_t)k * m * across / 2048 / 16 * 16));
     vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, nullptr, 0, 0, l.start, l.rows, l.edges, (float *)(w + work.partial),
