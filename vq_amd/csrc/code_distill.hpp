@@ -61,7 +61,7 @@ struct Teacher {
         // probabilities in 64 bits: what they leave of one may be small
         float most = 0.0f, l = has ? log_q : kNegInf;
         if (!a.rest) most = group_max<64>(l);
-        const double e = has && !bad ? exp2_wide(fmax(((double)l - (double)most) * kLog2e64, -2000.0)) : 0.0;
+        const double e = has && !bad ? exp2_wide(((double)l - (double)most) * kLog2e64) : 0.0;
         double sum = wave_sum(e);
         if (a.rest) {
             q = (float)e;

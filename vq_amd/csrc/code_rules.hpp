@@ -256,7 +256,7 @@ inline int64_t distill_work(int64_t n, int32_t k) {
 // Rows of scores are cut into parts of 4096 codes; a sequence has draft + 1 rows of its own and as many of its drafts'.
 constexpr int kVerifyPart = 4096;
 inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyPart; }
-// Per row and part a maximum and a sum in 64 bits; per sequence and part a sum more.
+// Per row and part a sum and a maximum (in 64 bits and 32; 16 bytes); per sequence and part a sum more.
 inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8); }
 static_assert(kMaxRowCodes / kVerifyPart * ((2 * kMaxDraft + 1) * 16 + 8) <= kPartBytes * 4, "one sequence fits");
 inline int64_t verify_sequences_of_a_launch(int32_t draft, int32_t k) {

@@ -25,10 +25,12 @@ struct VerifyArgs {
     int64_t ld_uniform;
     int32_t *accepted, *out;
     int64_t ld_out;
-    // per part of a row its largest score (as 64 bits: -inf for none, NaN where it holds one) and the sum of 2^((s - largest) c); the rows of the
+    // per part of a row its largest score (-inf for none, NaN where it holds one) and the sum of 2^((s - largest) c); the rows of the
     // targets, then of the drafts.  Without scores of the drafts a drafted code is left out of its row.
-    double *most, *sum;
+    float *most;
+    double *sum;
     double *left;  // per sequence and part: the sum of max(p - q, 0)
+    int left_parts;  // parts of a workgroup that makes these sums
     int64_t first_draft() const { return (int64_t)n * (draft + 1); }
 };
 
@@ -52,10 +54,11 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     const bool draft = row >= targets;
     const int64_t seq = draft ? (row - targets) / a.draft : row / (a.draft + 1);
     const int pos = (int)(draft ? (row - targets) % a.draft : row % (a.draft + 1));
-    int64_t code;
-    const int length = drafted(a, seq, lane, &code);
-    if (pos >= length + (draft ? 0 : 1)) return;  // uniform: a row that nothing is drafted for
     H x;
+    int64_t code;
+    int length = a.draft;
+    if (a.code_bytes == 4 || !a.drafts) length = drafted(a, seq, lane, &code);  // (unsigned codes end no draft)
+    if (pos >= length + (draft ? 0 : 1)) return;  // uniform: a row that nothing is drafted for
     x.load(draft ? (const Raw *)a.drafts + (row - targets) * a.ld_draft : (const Raw *)a.target + row * a.ld_target, lo, hi, tid);
     if (!a.drafts && pos < length) {  // the row without its drafted code
         const int64_t c = (int64_t)__shfl((int)code, pos) - lo;
@@ -83,11 +86,11 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     m = larger_or_nan(larger_or_nan(most_of[0], most_of[1]), larger_or_nan(most_of[2], most_of[3]));
     double sum = 0.0;
     if (m > kNegInf && m < __builtin_inff()) {  // uniform
-        const double c = draft ? a.c_draft : a.c_target, from = m;  // (the difference first: of scores of 1e38 a rounded product leaves too much)
+        const double c = draft ? a.c_draft : a.c_target, from = m, least = -1000.0 / c;  // (the difference first: of scores of 1e38 a rounded product leaves too much)
 #pragma unroll
         for (int u = 0; u < kVerifyEach / H::VEC; ++u)
 #pragma unroll
-            for (int v = 0; v < H::VEC; ++v) sum += exp2_wide(fmax(((double)x.at(u, v) - from) * c, -2000.0));
+            for (int v = 0; v < H::VEC; ++v) sum += exp2_of(fmax((double)x.at(u, v) - from, least), c);
     }
     sum = wave_sum(sum);
     if (lane == 0) sum_of[wave] = sum;
@@ -95,71 +98,114 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     if (tid == 0) a.most[blockIdx.x] = m, a.sum[blockIdx.x] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
 }
 
-// What the drafts of a sequence come to, in every lane of a wave.
+// What the drafts of a sequence come to.
 struct Verdict {
     int accepted, length;
     int refused;          // the first drafted code that does not stay, -1 for none
     bool bad;             // the position behind the accepted codes cannot be answered
     double mp, Sp, mq, Sq;  // its rows' largest scores and sums; of a refused draft without scores its code is left out of Sp
-    int64_t code;         // lane d: drafted code d
+};
+struct VerdictLds {
+    double m[2][kMaxDraft + 1], S[2][kMaxDraft + 1];
+    Verdict out;
 };
 
-// The largest score and the sum of a row from its parts.
-__device__ __forceinline__ void row_of_parts(const VerifyArgs &a, int64_t row, double c, double *m, double *S) {
-    double most = -__builtin_inf(), sum = 0.0;
-    bool bad = false;
-    for (int p = 0; p < a.parts; ++p) {
-        const double v = a.most[row * a.parts + p];
-        bad |= v != v;
-        most = fmax(most, v);
-    }
-    for (int p = 0; p < a.parts; ++p) {
-        const double v = a.most[row * a.parts + p];
-        if (v > -__builtin_inf()) sum += a.sum[row * a.parts + p] * exp2_wide(fmax((v - most) * c, -2000.0));
-    }
-    *m = most;
-    *S = bad || most == __builtin_inf() ? __builtin_nan("") : sum;
-}
-
-template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArgs &a, int64_t seq, int lane) {
+// By a workgroup of four waves: each joins the parts of every fourth row, the first decides.  code: a lane of the first wave's drafted code.
+template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArgs &a, int64_t seq, VerdictLds &l, int64_t *code) {
     typedef typename T::Raw Raw;
-    Verdict o;
-    o.length = drafted(a, seq, lane, &o.code);
-    const int64_t row = seq * (a.draft + 1) + lane;
-    const bool here = lane <= o.length, asked = lane < o.length, known = asked && o.code < a.k;
-    double mp = 0.0, Sp = 0.0, mq = 0.0, Sq = 1.0, p = 0.0, q = 1.0;
-    bool fine = here;
-    if (here) {
-        row_of_parts(a, row, a.c_target, &mp, &Sp);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int length = drafted(a, seq, lane, code), rows = length + 1 + (a.drafts ? length : 0);
+    const bool here = lane <= length, asked = lane < length, known = asked && *code < a.k;
+    float s = 0.0f, t = 0.0f, u = 0.0f;  // lane d: the scores of drafted code d, its random number
+    if (wave == 0 && asked) {
+        u = a.uniform[seq * a.ld_uniform + lane];
         if (known) {
-            const double s = (double)T::up(((const Raw *)a.target)[row * a.ld_target + o.code]);
-            if (!a.drafts) {
-                // the row's code was left out of its sums
-                const bool sound = s < __builtin_inf() && Sp == Sp;
-                const double most = sound ? fmax(mp, s) : mp;
-                const double e = s == -__builtin_inf() ? 0.0 : exp2_wide(fmax((s - most) * a.c_target, -2000.0));
-                const double others = mp == -__builtin_inf() ? 0.0 : Sp * exp2_wide(fmax((mp - most) * a.c_target, -2000.0));
-                p = sound ? e / (e + others) : __builtin_nan("");
-                fine = p == p;
-            } else {
-                const int64_t draft = seq * a.draft + lane;
-                row_of_parts(a, (int64_t)a.n * (a.draft + 1) + draft, a.c_draft, &mq, &Sq);
-                p = exp2_wide(fmax((s - mp) * a.c_target, -2000.0)) / Sp;
-                q = exp2_wide(fmax(((double)T::up(((const Raw *)a.drafts)[draft * a.ld_draft + o.code]) - mq) * a.c_draft, -2000.0)) / Sq;
-                fine = Sp > 0.0 && Sq > 0.0;
-            }
-        } else
-            fine = !asked && Sp > 0.0;
+            s = T::up(((const Raw *)a.target)[(seq * (a.draft + 1) + lane) * a.ld_target + *code]);
+            if (a.drafts) t = T::up(((const Raw *)a.drafts)[(seq * a.draft + lane) * a.ld_draft + *code]);
+        }
     }
-    const bool stays = asked && fine && (double)a.uniform[seq * a.ld_uniform + lane] * q < p;
-    o.accepted = __ffsll(__ballot(!stays)) - 1;
-    o.bad = !(__ballot(fine) >> o.accepted & 1);
-    o.refused = o.accepted < o.length ? __shfl((int)o.code, o.accepted) : -1;
-    o.mp = __shfl(mp, o.accepted);
-    o.Sp = __shfl(Sp, o.accepted);
-    o.mq = __shfl(mq, o.accepted);
-    o.Sq = __shfl(Sq, o.accepted);
-    return o;
+    constexpr int AHEAD = 4;
+    for (int r0 = wave; r0 < rows; r0 += 4 * AHEAD) {
+        float most[AHEAD];
+        double sum[AHEAD];
+        const auto row_of = [&](int i) {
+            const int r = min(r0 + 4 * i, rows - 1);
+            return r <= length ? seq * (a.draft + 1) + r : (int64_t)a.n * (a.draft + 1) + seq * a.draft + (r - length - 1);
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int64_t at = row_of(i) * a.parts + min(lane, a.parts - 1);
+            most[i] = lane < a.parts ? a.most[at] : kNegInf;
+            sum[i] = lane < a.parts ? a.sum[at] : 0.0;
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int r = r0 + 4 * i;
+            if (r >= rows) break;  // uniform
+            const bool draft = r > length;
+            const double c = draft ? a.c_draft : a.c_target;
+            float m = most[i];
+            bool bad = __ballot(m != m) != 0;
+            m = group_max<64>(m);
+            const auto scaled = [&](float pm, double ps) { return pm > kNegInf ? ps * exp2_wide(((double)pm - (double)m) * c) : 0.0; };
+            double S;
+            if (a.parts <= 64) {
+                S = wave_sum(scaled(most[i], sum[i]));
+            } else {  // the other parts, 64 at a time
+                const int64_t at = row_of(i) * a.parts;
+                for (int p = lane + 64; p - lane < a.parts; p += 64) {
+                    const float o = p < a.parts ? a.most[at + p] : kNegInf;
+                    bad = bad || __ballot(o != o) != 0;
+                    m = larger(m, group_max<64>(o));
+                }
+                double mine = scaled(most[i], sum[i]);
+                for (int p = lane + 64; p < a.parts; p += 64) mine += scaled(a.most[at + p], a.sum[at + p]);
+                S = wave_sum(mine);
+            }
+            if (lane == 0) {
+                const int d = draft ? r - length - 1 : r;
+                l.m[draft][d] = m;
+                l.S[draft][d] = bad || m == __builtin_inff() ? __builtin_nan("") : S;
+            }
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        double p = 0.0, q = 1.0;
+        bool fine = here;
+        const double mp = here ? l.m[0][lane] : 0.0, Sp = here ? l.S[0][lane] : 0.0;
+        const bool scored = known && a.drafts;
+        const double mq = scored ? l.m[1][lane] : 0.0, Sq = scored ? l.S[1][lane] : 1.0;
+        if (known && !a.drafts) {
+            // the row's code was left out of its sums
+            const bool sound = s < __builtin_inff() && Sp == Sp;
+            const double most = sound ? fmax(mp, (double)s) : 0.0;
+            const double e = s == kNegInf || !sound ? 0.0 : exp2_wide(((double)s - most) * a.c_target);
+            const double others = mp == -__builtin_inf() || !sound ? 0.0 : Sp * exp2_wide((mp - most) * a.c_target);
+            p = sound ? e / (e + others) : __builtin_nan("");
+            fine = p == p;
+        } else if (scored) {
+            fine = Sp > 0.0 && Sq > 0.0;
+            if (fine) {
+                p = exp2_wide(((double)s - mp) * a.c_target) / Sp;
+                q = exp2_wide(((double)t - mq) * a.c_draft) / Sq;
+            }
+        } else if (here)
+            fine = !asked && Sp > 0.0;
+        const bool stays = asked && fine && (double)u * q < p;
+        Verdict o;
+        o.length = length;
+        o.accepted = __ffsll(__ballot(!stays)) - 1;
+        o.refused = o.accepted < length ? __shfl((int)*code, o.accepted) : -1;
+        o.bad = !(__ballot(fine) >> o.accepted & 1);
+        o.mp = __shfl(mp, o.accepted);
+        o.Sp = __shfl(Sp, o.accepted);
+        o.mq = __shfl(mq, o.accepted);
+        o.Sq = __shfl(Sq, o.accepted);
+        if (lane == 0) l.out = o;
+    }
+    __syncthreads();
+    return l.out;
 }
 
 // The weights of the codes of the position behind the accepted ones.
@@ -168,9 +214,9 @@ struct Weights {
     int code;   // this one has none
     bool minus;  // max(p - q, 0), otherwise p
     __device__ __forceinline__ double operator()(float s, float t) const {
-        const double p = exp2_wide(fmax(((double)s - mp) * c_target, -2000.0)) * by_p;
+        const double p = exp2_wide(((double)s - mp) * c_target) * by_p;
         if (!minus) return p;
-        return fmax(p - exp2_wide(fmax(((double)t - mq) * c_draft, -2000.0)) * by_q, 0.0);
+        return fmax(p - exp2_wide(((double)t - mq) * c_draft) * by_q, 0.0);
     }
 };
 __device__ __forceinline__ Weights weights(const VerifyArgs &a, const Verdict &o) {
@@ -206,27 +252,26 @@ template <typename T> __device__ __forceinline__ void lane_weights(const VerifyA
 // Sums of max(p - q, 0) where a draft with scores was refused.
 template <typename T>
 __global__ void __launch_bounds__(256) k_verify_left(VerifyArgs a) {
-    __shared__ Verdict shared;
+    __shared__ VerdictLds lds;
     __shared__ double sum_of[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t seq = blockIdx.x / (unsigned)a.parts;
-    const int part = (int)(blockIdx.x % (unsigned)a.parts);
-    if (wave == 0) {
-        const Verdict o = verdict<T>(a, seq, lane);
-        if (lane == 0) shared = o;
-    }
-    __syncthreads();
-    const Verdict o = shared;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), groups = (a.parts + a.left_parts - 1) / a.left_parts;
+    const int64_t seq = blockIdx.x / (unsigned)groups;
+    const int first = (int)(blockIdx.x % (unsigned)groups) * a.left_parts;
+    int64_t code;
+    const Verdict o = verdict<T>(a, seq, lds, &code);
     if (o.bad || o.accepted == o.length) return;  // uniform
     const Weights w = weights(a, o);
-    double y[kVerifyEach], sum = 0.0;
-    lane_weights<T>(a, w, seq, o.accepted, part * kVerifyPart + tid * kVerifyEach, y);
+    for (int part = first; part < min(a.parts, first + a.left_parts); ++part) {
+        double y[kVerifyEach], sum = 0.0;
+        lane_weights<T>(a, w, seq, o.accepted, part * kVerifyPart + tid * kVerifyEach, y);
 #pragma unroll
-    for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
-    sum = wave_sum(sum);
-    if (lane == 0) sum_of[wave] = sum;
-    __syncthreads();
-    if (tid == 0) a.left[blockIdx.x] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
+        for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
+        sum = wave_sum(sum);
+        __syncthreads();
+        if (lane == 0) sum_of[wave] = sum;
+        __syncthreads();
+        if (tid == 0) a.left[seq * a.parts + part] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
+    }
 }
 
 // The outcome of a sequence: how many drafts stay, and the codes: these, the next one, -1 behind it.
@@ -234,17 +279,11 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
     __shared__ double part_of[256], sum_of[4];
     __shared__ int found[4];
-    __shared__ Verdict shared;
+    __shared__ VerdictLds lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t seq = blockIdx.x;
-    int64_t code = -1;
-    if (wave == 0) {
-        const Verdict o = verdict<T>(a, seq, lane);
-        code = o.code;
-        if (lane == 0) shared = o;
-    }
-    __syncthreads();
-    const Verdict o = shared;
+    int64_t code;
+    const Verdict o = verdict<T>(a, seq, lds, &code);
     int next = -1;
     if (!o.bad) {  // uniform
         Weights w = weights(a, o);
@@ -255,8 +294,8 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
                 if (w.minus)
                     mine = a.left[seq * a.parts + tid];
                 else {
-                    const double m = a.most[row * a.parts + tid];
-                    mine = m > -__builtin_inf() ? a.sum[row * a.parts + tid] * exp2_wide(fmax((m - o.mp) * a.c_target, -2000.0)) : 0.0;
+                    const float m = a.most[row * a.parts + tid];
+                    mine = m > kNegInf ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
                 }
             }
             // sums of the parts up to each

@@ -275,15 +275,17 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
     const void *drafts = draft > 0 ? d_draft : nullptr;
     for (int64_t b = 0; b < n; b += slice) {
         const int64_t here = std::min(slice, n - b), rows = here * (draft + 1 + (drafts ? draft : 0));
-        double *most = (double *)ctx->code_work.p, *sum = most + rows * parts;
+        double *sum = (double *)ctx->code_work.p, *left = sum + rows * parts;
+        float *most = (float *)(left + here * parts);
+        const int left_parts = here * parts >= 1024 ? 4 : 1;
         const vq::VerifyArgs a{(const char *)d_target + b * (draft + 1) * ld_target * e, drafts ? (const char *)drafts + b * draft * ld_draft * e : nullptr,
                                ld_target, ld_draft, beta * vq::kLog2e64, beta_draft * vq::kLog2e64, (int)here, draft, k, parts,
                                draft ? (const char *)d_codes + b * code_stride * code_bytes : nullptr, code_bytes, code_stride,
-                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, sum + rows * parts};
+                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, left, left_parts};
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
             hipLaunchKernelGGL(vq::k_verify_part<T>, dim3((unsigned)(rows * parts)), dim3(256), 0, ctx->stream, a);
-            if (drafts) hipLaunchKernelGGL(vq::k_verify_left<T>, dim3((unsigned)(here * parts)), dim3(256), 0, ctx->stream, a);
+            if (drafts) hipLaunchKernelGGL(vq::k_verify_left<T>, dim3((unsigned)(here * cdiv(parts, left_parts))), dim3(256), 0, ctx->stream, a);
             hipLaunchKernelGGL(vq::k_verify_pick<T>, dim3((unsigned)here), dim3(256), 0, ctx->stream, a);
         });
         VQ_HIP(ctx, hipGetLastError());
