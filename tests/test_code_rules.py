@@ -157,7 +157,7 @@ def test_drafts_fit_their_launches(lib):
             most = lib.verify_rows(d, k)
             assert most >= 1 and most * (2 * d + 1) * lib.verify_parts(k) * 256 < 1 << 32
             for n in (1, 5, 1000, 1 << 30):
-                assert lib.verify_bytes(n, d, k) >= min(n, most) * lib.verify_parts(k) * ((2 * d + 1) * 16 + 8)
+                assert lib.verify_bytes(n, d, k) >= min(n, most) * (lib.verify_parts(k) * ((2 * d + 1) * 16 + 8) + 64)
 
 
 def test_workspaces_grow_with_every_size(lib):

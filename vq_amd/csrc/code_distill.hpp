@@ -180,6 +180,7 @@ template <typename T, int LANES, int NV>
 __device__ __forceinline__ void write_grad(const DistillArgs &a, const Held<T, LANES, NV> &x, const RowGrad &row, typename T::Raw *to, int lo, int hi, int lane) {
     typedef Held<T, LANES, NV> H;
     const float c = a.beta * kLog2e;
+    const bool past = ((uintptr_t)a.grad & 127) == 0 && a.ld_grad % (128 / (int)sizeof(typename T::Raw)) == 0;  // whole lines pass the caches
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
         const int at = lo + (u * LANES + lane) * H::VEC;
@@ -196,7 +197,10 @@ __device__ __forceinline__ void write_grad(const DistillArgs &a, const Held<T, L
                 else
                     o.w[q] = (uint32_t)T::down(y[2 * q]) | (uint32_t)T::down(y[2 * q + 1]) << 16;
             }
-            *reinterpret_cast<typename H::Piece *>(to + at) = o;
+            if (past)
+                __builtin_nontemporal_store(__builtin_bit_cast(AnyWords, o), reinterpret_cast<AnyWords *>(to + at));
+            else
+                *reinterpret_cast<typename H::Piece *>(to + at) = o;
         } else {
 #pragma unroll
             for (int v = 0; v < H::VEC; ++v)
@@ -205,26 +209,31 @@ __device__ __forceinline__ void write_grad(const DistillArgs &a, const Held<T, L
     }
 }
 
-// The largest score and the sum of a wave's codes, or (split) of those that are no alternative.
+// The largest score and the sum of a wave's codes, or (split) of those that are no alternative: these are dropped.  The scores stay as they are
+// stored and are converted twice: 64 of them as floats beside would not fit the registers of a row of sixteen waves.
 template <typename T, int LANES, int NV>
-__device__ __forceinline__ Sums code_sums(const DistillArgs &a, const Held<T, LANES, NV> &x, const Marks<T, LANES, NV> &marks, int lane) {
+__device__ __forceinline__ Sums code_sums(const DistillArgs &a, Held<T, LANES, NV> &x, const Marks<T, LANES, NV> &marks, int lane) {
     typedef Held<T, LANES, NV> H;
-    float y[H::E], m = kNegInf;
+    float m = kNegInf;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-#pragma unroll
-        for (int v = 0; v < H::VEC; ++v) y[u * H::VEC + v] = x.at(u, v);
         if (a.split) {
             const uint32_t some = marks.of(u, lane);
             if (some) {
 #pragma unroll
-                for (int v = 0; v < H::VEC; ++v) y[u * H::VEC + v] = some >> v & 1 ? kNegInf : y[u * H::VEC + v];
+                for (int v = 0; v < H::VEC; ++v)
+                    if (some >> v & 1) x.drop(u, v);
             }
         }
 #pragma unroll
-        for (int v = 0; v < H::VEC; ++v) m = larger(m, y[u * H::VEC + v]);
+        for (int v = 0; v < H::VEC; v += 2) m = larger(larger(x.at(u, v), x.at(u, v + 1)), m);
     }
-    Sums s(y, group_max<64>(m), a.beta * kLog2e);
+    Sums s(group_max<64>(m), a.beta * kLog2e, [&](auto add) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int v = 0; v < H::VEC; ++v) add(x.at(u, v));
+    });
     s.S = group_sum<64>(s.S);
     s.away();
     return s;
@@ -238,7 +247,9 @@ __device__ __forceinline__ void join_rest(const DistillArgs &a, float pm, float 
     *Sr = group_sum<64>(mine ? f * pS : 0.0f);
 }
 
-// Rows that WAVES waves hold: the loss, and the gradient from the same registers where it is asked for.  One wave keeps the row's teacher.
+// Rows that WAVES waves hold: the loss, and the gradient from the same registers where it is asked for, so that the row is read once.  One wave
+// keeps the row's teacher.  Bound by memory: 8192 rows of 65,536 bf16 with 20 alternatives, loss and gradient, 432 us = 4.97 TB/s (with reads that
+// pass the caches, too, 451; with the scores as floats beside their stored form, which does not fit the registers, 624).
 template <typename T, int WAVES, int NV>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) k_distill_row(DistillArgs a) {
     typedef typename T::Raw Raw;
@@ -339,7 +350,8 @@ __global__ void __launch_bounds__(256) k_distill_join(DistillArgs a) {
     if (lane == 0) write_loss(a, row, o);
 }
 
-// The gradient alone, from m, L and log R as the loss's call left them: a row, or (blockIdx.y) a piece of one, per WAVES waves.
+// The gradient alone, from m, L and log R as the loss's call left them: a row, or (blockIdx.y) a piece of one, per WAVES waves.  Bound by memory:
+// 2048 rows of 65,536 f32 199 us = 5.4 TB/s with reads and whole lines that pass the caches (210 without).
 template <typename T, int WAVES, int NV>
 __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
     typedef typename T::Raw Raw;
@@ -353,7 +365,7 @@ __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
     Raw *to = (Raw *)a.grad + row * a.ld_grad;
     const int size = LANES * Held<T, LANES, NV>::E, lo = blockIdx.y * size, hi = min(a.k, lo + size);
     Held<T, LANES, NV> x;
-    x.load(s, lo, hi, place);
+    x.template load<true>(s, lo, hi, place);
     RowGrad grad;
     Teacher t;
     float value = 0.0f;

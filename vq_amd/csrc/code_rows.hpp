@@ -17,10 +17,17 @@ template <typename T, int LANES, int NV> struct Held {
     };
     Piece raw[NV];
 
-    __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
+    // ONCE: nobody is expected to read the row after this; it passes the caches
+    template <bool ONCE = false> static __device__ __forceinline__ Piece fetch(const Raw *s) {
+        if constexpr (ONCE)
+            return __builtin_bit_cast(Piece, __builtin_nontemporal_load(reinterpret_cast<const AnyWords *>(s)));
+        else
+            return *reinterpret_cast<const Piece *>(s);
+    }
+    template <bool ONCE = false> __device__ __forceinline__ void load(const Raw *s, int lo, int hi, int lane) {
         if (lo + LANES * E <= hi) {  // uniform: whole vectors all of them
 #pragma unroll
-            for (int u = 0; u < NV; ++u) raw[u] = *reinterpret_cast<const Piece *>(s + lo + (u * LANES + lane) * VEC);
+            for (int u = 0; u < NV; ++u) raw[u] = fetch<ONCE>(s + lo + (u * LANES + lane) * VEC);
             return;
         }
 #pragma unroll
@@ -28,7 +35,7 @@ template <typename T, int LANES, int NV> struct Held {
             const int at = lo + (u * LANES + lane) * VEC;
 #pragma unroll
             for (int q = 0; q < 4; ++q) raw[u].w[q] = NONE;
-            if (at + VEC <= hi) raw[u] = *reinterpret_cast<const Piece *>(s + at);
+            if (at + VEC <= hi) raw[u] = fetch<ONCE>(s + at);
         }
         // the vector that the row's end cuts
         const int tail = (hi - lo) / VEC, rest = (hi - lo) % VEC;

@@ -253,12 +253,14 @@ inline int64_t distill_work(int64_t n, int32_t k) {
 }
 
 // ---- drafts --------------------------------------------------------------------------------------------
-// Rows of scores are cut into parts of 4096 codes; a sequence has draft + 1 rows of its own and as many of its drafts'.
+// Rows of scores are cut into parts of 4096 codes, a workgroup each, or four to a workgroup where those are enough; a sequence has draft + 1 rows of its
+// own and as many as drafts of its drafts'.
 constexpr int kVerifyPart = 4096;
 inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyPart; }
-// Per row and part a sum and a maximum (in 64 bits and 32; 16 bytes); per sequence and part a sum more.
-inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8); }
-static_assert(kMaxRowCodes / kVerifyPart * ((2 * kMaxDraft + 1) * 16 + 8) <= kPartBytes * 4, "one sequence fits");
+inline bool verify_wide(int64_t rows, int32_t k) { return k > kVerifyPart && rows * ((k + 4 * kVerifyPart - 1) / (4 * kVerifyPart)) >= 2048; }
+// Per row and part a sum and a maximum (in 64 bits and 32; 16 bytes); per sequence and part a sum more, and 64 bytes for what its drafts come to.
+inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8) + 64; }
+static_assert(kMaxRowCodes / kVerifyPart * ((2 * kMaxDraft + 1) * 16 + 8) + 64 <= kPartBytes * 4, "one sequence fits");
 inline int64_t verify_sequences_of_a_launch(int32_t draft, int32_t k) {
     return std::max<int64_t>(1, std::min((kPartBytes * 4) / verify_bytes_of_a_sequence(draft, k), ((int64_t)1 << 23) / (verify_parts(k) * (2 * draft + 1))));
 }

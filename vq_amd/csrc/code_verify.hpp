@@ -17,7 +17,7 @@ struct VerifyArgs {
     const void *target, *drafts;
     int64_t ld_target, ld_draft;
     double c_target, c_draft;  // beta * log2 e
-    int n, draft, k, parts;
+    int n, draft, k, parts;  // parts of kVerifyPart codes
     const void *codes;
     int code_bytes;
     int64_t code_stride;
@@ -30,7 +30,7 @@ struct VerifyArgs {
     float *most;
     double *sum;
     double *left;  // per sequence and part: the sum of max(p - q, 0)
-    int left_parts;  // parts of a workgroup that makes these sums
+    struct Verdict *verdicts;  // per sequence, where those sums are made
     int64_t first_draft() const { return (int64_t)n * (draft + 1); }
 };
 
@@ -40,63 +40,88 @@ __device__ __forceinline__ int drafted(const VerifyArgs &a, int64_t seq, int lan
     return __ffsll(__ballot(*code < 0)) - 1;  // (lane 63 has none)
 }
 
-constexpr int kVerifyEach = kVerifyPart / 256;  // codes of a lane
-
-template <typename T>
+// EACH / 16 parts of a row per workgroup, their sums relative to the largest score of all of them.  Bound by the vector pipe: 18 instructions per code,
+// 13 of them in 64 bits, and some 180 per wave, which is why a lane has 64 codes where there are enough workgroups (128 sequences of 11
+// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).
+template <typename T, int EACH>
 __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     typedef typename T::Raw Raw;
-    typedef Held<T, 256, kVerifyEach * (int)sizeof(Raw) / 16> H;
-    __shared__ float most_of[4];
-    __shared__ double sum_of[4];
+    typedef Held<T, 256, EACH * (int)sizeof(Raw) / 16> H;
+    constexpr int PARTS = EACH / 16, PIECES = EACH / H::VEC / PARTS;  // vectors of a lane in a part
+    __shared__ float most_of[4][PARTS];
+    __shared__ double sum_of[4][PARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t row = blockIdx.x / (unsigned)a.parts, targets = (int64_t)a.n * (a.draft + 1);
-    const int part = (int)(blockIdx.x % (unsigned)a.parts), lo = part * kVerifyPart, hi = min(a.k, lo + kVerifyPart);
+    const uint32_t groups = (uint32_t)(a.parts + PARTS - 1) / PARTS;
+    const uint32_t row = blockIdx.x / groups, targets = (uint32_t)a.n * (uint32_t)(a.draft + 1);  // (a launch has fewer than 2^23)
+    const int first = (int)(blockIdx.x - row * groups) * PARTS, lo = first * kVerifyPart, hi = min(a.k, lo + PARTS * kVerifyPart);
     const bool draft = row >= targets;
-    const int64_t seq = draft ? (row - targets) / a.draft : row / (a.draft + 1);
-    const int pos = (int)(draft ? (row - targets) % a.draft : row % (a.draft + 1));
+    const uint32_t of = draft ? row - targets : row, each = draft ? a.draft : a.draft + 1, seq = of / each;
+    const int pos = (int)(of - seq * each);
     H x;
     int64_t code;
     int length = a.draft;
     if (a.code_bytes == 4 || !a.drafts) length = drafted(a, seq, lane, &code);  // (unsigned codes end no draft)
     if (pos >= length + (draft ? 0 : 1)) return;  // uniform: a row that nothing is drafted for
-    x.load(draft ? (const Raw *)a.drafts + (row - targets) * a.ld_draft : (const Raw *)a.target + row * a.ld_target, lo, hi, tid);
+    x.load(draft ? (const Raw *)a.drafts + (int64_t)of * a.ld_draft : (const Raw *)a.target + (int64_t)of * a.ld_target, lo, hi, tid);
     if (!a.drafts && pos < length) {  // the row without its drafted code
         const int64_t c = (int64_t)__shfl((int)code, pos) - lo;
         if (c >= 0 && c < hi - lo) {
             const int place = (int)c / H::VEC;
             if (place % 256 == tid) {
 #pragma unroll
-                for (int u = 0; u < kVerifyEach / H::VEC; ++u)
+                for (int u = 0; u < EACH / H::VEC; ++u)
 #pragma unroll
                     for (int v = 0; v < H::VEC; ++v)
                         if (u == place / 256 && v == (int)c % H::VEC) x.drop(u, v);
             }
         }
     }
-    float m = kNegInf;
+    float m = kNegInf, most[PARTS];
 #pragma unroll
-    for (int u = 0; u < kVerifyEach / H::VEC; ++u)
+    for (int p = 0; p < PARTS; ++p) {
+        most[p] = kNegInf;
 #pragma unroll
-        for (int v = 0; v < H::VEC; ++v) m = larger_or_nan(m, x.at(u, v));
-    m = __uint_as_float(over_group<64>(__float_as_uint(m), __float_as_uint(kNegInf), [](uint32_t p, uint32_t q) {
-        return __float_as_uint(larger_or_nan(__uint_as_float(p), __uint_as_float(q)));
-    }));
-    if (lane == 0) most_of[wave] = m;
-    __syncthreads();
-    m = larger_or_nan(larger_or_nan(most_of[0], most_of[1]), larger_or_nan(most_of[2], most_of[3]));
-    double sum = 0.0;
-    if (m > kNegInf && m < __builtin_inff()) {  // uniform
-        const double c = draft ? a.c_draft : a.c_target, from = m, least = -1000.0 / c;  // (the difference first: of scores of 1e38 a rounded product leaves too much)
+        for (int u = 0; u < PIECES; ++u)
 #pragma unroll
-        for (int u = 0; u < kVerifyEach / H::VEC; ++u)
-#pragma unroll
-            for (int v = 0; v < H::VEC; ++v) sum += exp2_of(fmax((double)x.at(u, v) - from, least), c);
+            for (int v = 0; v < H::VEC; v += 2) most[p] = larger_or_nan(larger_or_nan(x.at(p * PIECES + u, v), x.at(p * PIECES + u, v + 1)), most[p]);
+        most[p] = __uint_as_float(over_group<64>(__float_as_uint(most[p]), __float_as_uint(kNegInf), [](uint32_t p, uint32_t q) {
+            return __float_as_uint(larger_or_nan(__uint_as_float(p), __uint_as_float(q)));
+        }));
+        if (lane == 0) most_of[wave][p] = most[p];
     }
-    sum = wave_sum(sum);
-    if (lane == 0) sum_of[wave] = sum;
     __syncthreads();
-    if (tid == 0) a.most[blockIdx.x] = m, a.sum[blockIdx.x] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        most[p] = larger_or_nan(larger_or_nan(most_of[0][p], most_of[1][p]), larger_or_nan(most_of[2][p], most_of[3][p]));
+        m = larger_or_nan(m, most[p]);
+    }
+    const bool sound = m > kNegInf && m < __builtin_inff();  // uniform
+    const double c = draft ? a.c_draft : a.c_target, from = sound ? m : 0.0f, least = -1000.0 / c;  // (the difference first: of scores of 1e38 a rounded product leaves too much)
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        double sum = 0.0;
+        if (sound) {
+#pragma unroll
+            for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+                for (int v = 0; v < H::VEC; ++v) sum += exp2_of(fmax((double)x.at(p * PIECES + u, v) - from, least), c);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) sum_of[wave][p] = sum;
+    }
+    __syncthreads();
+    if (tid >= PARTS || first + tid >= a.parts) return;
+    float own = most[0];
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) own = tid == p ? most[p] : own;
+    // a part without a weight: its codes are too far below, or none can be
+    const bool none = sound && !((double)own - from >= least);
+    const int64_t at = (int64_t)row * a.parts + first + tid;
+    a.most[at] = none ? kNegInf : m;
+    a.sum[at] = none ? 0.0 : sum_of[0][tid] + sum_of[1][tid] + sum_of[2][tid] + sum_of[3][tid];
 }
+
+constexpr int kVerifyEach = kVerifyPart / 256;  // codes of a lane where weights are summed
 
 // What the drafts of a sequence come to.
 struct Verdict {
@@ -110,7 +135,7 @@ struct VerdictLds {
     Verdict out;
 };
 
-// By a workgroup of four waves: each joins the parts of every fourth row, the first decides.  code: a lane of the first wave's drafted code.
+// By a workgroup of four waves: each joins the parts of every fourth row, the first decides.  code: a lane's drafted code.
 template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArgs &a, int64_t seq, VerdictLds &l, int64_t *code) {
     typedef typename T::Raw Raw;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -124,12 +149,12 @@ template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArg
             if (a.drafts) t = T::up(((const Raw *)a.drafts)[(seq * a.draft + lane) * a.ld_draft + *code]);
         }
     }
-    constexpr int AHEAD = 4;
-    for (int r0 = wave; r0 < rows; r0 += 4 * AHEAD) {
+    constexpr int WAVES = 4, AHEAD = 4;
+    for (int r0 = wave; r0 < rows; r0 += WAVES * AHEAD) {
         float most[AHEAD];
         double sum[AHEAD];
         const auto row_of = [&](int i) {
-            const int r = min(r0 + 4 * i, rows - 1);
+            const int r = min(r0 + WAVES * i, rows - 1);
             return r <= length ? seq * (a.draft + 1) + r : (int64_t)a.n * (a.draft + 1) + seq * a.draft + (r - length - 1);
         };
 #pragma unroll
@@ -140,7 +165,7 @@ template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArg
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int r = r0 + 4 * i;
+            const int r = r0 + WAVES * i;
             if (r >= rows) break;  // uniform
             const bool draft = r > length;
             const double c = draft ? a.c_draft : a.c_target;
@@ -210,18 +235,20 @@ template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArg
 
 // The weights of the codes of the position behind the accepted ones.
 struct Weights {
-    double c_target, c_draft, mp, mq, by_p, by_q;
+    double c_target, c_draft, least_p, least_q, mp, mq, by_p, by_q;
     int code;   // this one has none
     bool minus;  // max(p - q, 0), otherwise p
     __device__ __forceinline__ double operator()(float s, float t) const {
-        const double p = exp2_wide(((double)s - mp) * c_target) * by_p;
-        if (!minus) return p;
-        return fmax(p - exp2_wide(((double)t - mq) * c_draft) * by_q, 0.0);
+        const double y = (double)s - mp;
+        double w = exp2_of(fmax(y, least_p), c_target) * by_p;
+        if (minus) w = fmax(w - exp2_of(fmax((double)t - mq, least_q), c_draft) * by_q, 0.0);
+        return y < least_p ? 0.0 : w;
     }
 };
 __device__ __forceinline__ Weights weights(const VerifyArgs &a, const Verdict &o) {
     const bool minus = o.accepted < o.length && a.drafts;
-    return {a.c_target, a.c_draft, o.mp, o.mq, minus ? 1.0 / o.Sp : 1.0, minus ? 1.0 / o.Sq : 0.0, minus ? -1 : o.refused, minus};
+    return {a.c_target, a.c_draft, -1000.0 / a.c_target, minus ? -1000.0 / a.c_draft : 0.0, o.mp, o.mq, minus ? 1.0 / o.Sp : 1.0, minus ? 1.0 / o.Sq : 0.0,
+            minus ? -1 : o.refused, minus};
 }
 
 // 16 codes of a lane one after another, from a part of a row on.
@@ -249,98 +276,127 @@ template <typename T> __device__ __forceinline__ void lane_weights(const VerifyA
     }
 }
 
-// Sums of max(p - q, 0) where a draft with scores was refused.
-template <typename T>
-__global__ void __launch_bounds__(256) k_verify_left(VerifyArgs a) {
+template <typename T> __global__ void __launch_bounds__(256) k_verify_verdict(VerifyArgs a) {
     __shared__ VerdictLds lds;
-    __shared__ double sum_of[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), groups = (a.parts + a.left_parts - 1) / a.left_parts;
-    const int64_t seq = blockIdx.x / (unsigned)groups;
-    const int first = (int)(blockIdx.x % (unsigned)groups) * a.left_parts;
     int64_t code;
-    const Verdict o = verdict<T>(a, seq, lds, &code);
+    const Verdict o = verdict<T>(a, blockIdx.x, lds, &code);
+    if (threadIdx.x == 0) a.verdicts[blockIdx.x] = o;
+}
+
+// Sums of max(p - q, 0) by parts where a draft with scores was refused.  READY: the verdicts are there; else every workgroup comes to its
+// sequence's, which takes it 4 us, a launch less, and the first one writes it.
+template <typename T, bool READY>
+__global__ void __launch_bounds__(256) k_verify_left(VerifyArgs a) {
+    __shared__ double sum_of[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t seq = blockIdx.x / (uint32_t)a.parts;
+    const int part = (int)(blockIdx.x - seq * (uint32_t)a.parts);
+    Verdict o;
+    if constexpr (READY) {
+        o = a.verdicts[seq];
+    } else {
+        __shared__ VerdictLds lds;
+        int64_t code;
+        o = verdict<T>(a, seq, lds, &code);
+        if (part == 0 && tid == 0) a.verdicts[seq] = o;
+    }
     if (o.bad || o.accepted == o.length) return;  // uniform
     const Weights w = weights(a, o);
-    for (int part = first; part < min(a.parts, first + a.left_parts); ++part) {
-        double y[kVerifyEach], sum = 0.0;
-        lane_weights<T>(a, w, seq, o.accepted, part * kVerifyPart + tid * kVerifyEach, y);
+    float s[kVerifyEach], t[kVerifyEach];
+    const int at = part * kVerifyPart + tid * kVerifyEach;
+    lane_codes<T>(a.target, (int64_t)seq * (a.draft + 1) + o.accepted, a.ld_target, at, a.k, s);
+    lane_codes<T>(a.drafts, (int64_t)seq * a.draft + o.accepted, a.ld_draft, at, a.k, t);
+    double sum = 0.0;
 #pragma unroll
-        for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
-        sum = wave_sum(sum);
-        __syncthreads();
-        if (lane == 0) sum_of[wave] = sum;
-        __syncthreads();
-        if (tid == 0) a.left[seq * a.parts + part] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
-    }
+    for (int e = 0; e < kVerifyEach; ++e) sum += w(s[e], t[e]);
+    sum = wave_sum(sum);
+    if (lane == 0) sum_of[wave] = sum;
+    __syncthreads();
+    if (tid == 0) a.left[blockIdx.x] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
 }
 
 // The outcome of a sequence: how many drafts stay, and the codes: these, the next one, -1 behind it.
-template <typename T>
+// READY: what the drafts come to is there.
+template <typename T, bool READY>
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
-    __shared__ double part_of[256], sum_of[4];
-    __shared__ int found[4];
-    __shared__ VerdictLds lds;
+    constexpr int WAVES = 4, NOT = 1024;
+    __shared__ double part_of[64 * WAVES], sum_of[WAVES];
+    __shared__ int found[WAVES], next_of;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t seq = blockIdx.x;
     int64_t code;
-    const Verdict o = verdict<T>(a, seq, lds, &code);
-    int next = -1;
+    Verdict o;
+    const float v = a.uniform[seq * a.ld_uniform + a.draft];
+    if constexpr (READY) {
+        o = a.verdicts[seq];
+        code = lane < o.accepted ? code_at(a.codes, a.code_bytes, seq * a.code_stride + lane) : -1;
+    } else {
+        __shared__ VerdictLds lds;
+        o = verdict<T>(a, seq, lds, &code);
+    }
+    // sums over the workgroup up to each lane, `from` on; the sum of all
+    double total;
+    const auto scan = [&](double mine, double from) {
+        const double upto = wave_scan(mine, lane);
+        __syncthreads();
+        if (lane == 63) sum_of[wave] = upto;
+        __syncthreads();
+        total = 0.0;
+        double before = from;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            before += i < wave ? sum_of[i] : 0.0;
+            total += sum_of[i];
+        }
+        return before + upto;
+    };
+    double goal = 0.0;
+    // the first lane whose sum reaches the goal; NOT + the last that has any weight, if none does; -1: none has
+    const auto choose = [&](bool has, double upto) {
+        const unsigned long long hit = __ballot(has && upto > goal), any = __ballot(has);
+        if (lane == 0) found[wave] = hit ? wave * 64 + __ffsll(hit) - 1 : any ? NOT + wave * 64 + 63 - __clzll(any) : -1;
+        __syncthreads();
+        int at = -1, last = -1;
+#pragma unroll
+        for (int i = WAVES - 1; i >= 0; --i) {
+            at = found[i] >= 0 && found[i] < NOT ? found[i] : at;
+            last = last < 0 && found[i] >= NOT ? found[i] : last;
+        }
+        __syncthreads();
+        return at >= 0 ? at : last;
+    };
+    if (tid == 0) next_of = -1;
     if (!o.bad) {  // uniform
         Weights w = weights(a, o);
         const int64_t row = seq * (a.draft + 1) + o.accepted;
-        double total = 0.0, mine = 0.0, before = 0.0;
+        double mine, upto;
         for (;;) {  // (a second time where nothing is left of p - q)
-            if (tid < a.parts) {
-                if (w.minus)
-                    mine = a.left[seq * a.parts + tid];
-                else {
-                    const float m = a.most[row * a.parts + tid];
-                    mine = m > kNegInf ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
-                }
+            mine = 0.0;
+            if (tid < a.parts && w.minus) {
+                mine = a.left[seq * a.parts + tid];
+            } else if (tid < a.parts) {
+                const float m = a.most[row * a.parts + tid];
+                mine = m > kNegInf ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
             }
-            // sums of the parts up to each
-            double scan = wave_scan(mine, lane);
-            __syncthreads();
-            if (lane == 63) sum_of[wave] = scan;
-            __syncthreads();
-            before = 0.0;
-            for (int i = 0; i < wave; ++i) before += sum_of[i];
-            scan += before;
-            part_of[tid] = scan;
-            total = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
+            upto = scan(mine, 0.0);
             if (total > 0.0 || !w.minus) break;
             w.minus = false;
             w.by_p = 1.0;
         }
-        const double goal = (double)a.uniform[seq * a.ld_uniform + a.draft] * total;
-        // the first part that reaches the goal, or the last that has any weight
-        const auto choose = [&](bool has, double upto) {
-            const unsigned long long hit = __ballot(has && upto > goal), any = __ballot(has);
-            if (lane == 0) found[wave] = hit ? wave * 64 + __ffsll(hit) - 1 : any ? 1024 + wave * 64 + 63 - __clzll(any) : -1;
-            __syncthreads();
-            int at = -1;
-            for (int i = 3; i >= 0; --i) at = found[i] >= 0 && found[i] < 1024 ? found[i] : at;
-            if (at < 0)
-                for (int i = 0; i < 4; ++i) at = found[i] >= 0 ? found[i] - 1024 : at;
-            __syncthreads();
-            return at;
-        };
-        const int part = choose(mine > 0.0, part_of[tid]);
+        part_of[tid] = upto;
+        goal = (double)v * total;
+        int part = choose(mine > 0.0, upto);
         if (part >= 0) {  // uniform
-            const double base = part ? part_of[part - 1] : 0.0;
+            part &= NOT - 1;
             const int at = part * kVerifyPart + tid * kVerifyEach;
             double y[kVerifyEach], sum = 0.0;
             lane_weights<T>(a, w, seq, o.accepted, at, y);
 #pragma unroll
             for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
-            double scan = wave_scan(sum, lane);
-            if (lane == 63) sum_of[wave] = scan;
-            __syncthreads();
-            double from = base;
-            for (int i = 0; i < wave; ++i) from += sum_of[i];
-            const int who = choose(sum > 0.0, from + scan);
-            if (tid == who) {
-                double so_far = from + (scan - sum);
+            upto = scan(sum, part ? part_of[part - 1] : 0.0);
+            const int who = choose(sum > 0.0, upto);
+            if (who >= 0 && tid == (who & (NOT - 1))) {
+                double so_far = upto - sum;
                 int last = -1, first = -1;
 #pragma unroll
                 for (int e = 0; e < kVerifyEach; ++e) {
@@ -350,15 +406,14 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
                         if (first < 0 && so_far > goal) first = e;
                     }
                 }
-                found[0] = at + (first >= 0 ? first : last);
+                next_of = at + (first >= 0 ? first : last);
             }
-            __syncthreads();
-            if (who >= 0) next = found[0];
         }
     }
+    __syncthreads();
     if (wave) return;
     if (lane == 0) a.accepted[seq] = o.accepted;
-    if (lane <= a.draft) a.out[seq * a.ld_out + lane] = lane < o.accepted ? (int32_t)code : lane == o.accepted ? next : -1;
+    if (lane <= a.draft) a.out[seq * a.ld_out + lane] = lane < o.accepted ? (int32_t)code : lane == o.accepted ? next_of : -1;
 }
 
 }  // namespace vq

@@ -269,24 +269,38 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
     VQ_TRY(admit(ctx, vq::check_code_verify(type, d_target, ld_target, beta, d_draft, ld_draft, beta_draft, n, draft, k, code_bytes,
                                             d_codes, code_stride, d_uniform, ld_uniform, d_accepted, d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
-    const int e = vq::type_bytes(type), parts = vq::verify_parts(k);
+    static_assert(sizeof(vq::Verdict) <= 64, "as the workspace counts it");
+    const int e = vq::type_bytes(type);
     const int64_t slice = vq::verify_sequences_of_a_launch(draft, k);
     VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
     const void *drafts = draft > 0 ? d_draft : nullptr;
     for (int64_t b = 0; b < n; b += slice) {
         const int64_t here = std::min(slice, n - b), rows = here * (draft + 1 + (drafts ? draft : 0));
+        const bool wide = vq::verify_wide(rows, k);
+        const int parts = vq::verify_parts(k);
         double *sum = (double *)ctx->code_work.p, *left = sum + rows * parts;
-        float *most = (float *)(left + here * parts);
-        const int left_parts = here * parts >= 1024 ? 4 : 1;
+        vq::Verdict *verdicts = (vq::Verdict *)(left + here * parts);
+        float *most = (float *)(verdicts + here);
         const vq::VerifyArgs a{(const char *)d_target + b * (draft + 1) * ld_target * e, drafts ? (const char *)drafts + b * draft * ld_draft * e : nullptr,
                                ld_target, ld_draft, beta * vq::kLog2e64, beta_draft * vq::kLog2e64, (int)here, draft, k, parts,
                                draft ? (const char *)d_codes + b * code_stride * code_bytes : nullptr, code_bytes, code_stride,
-                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, left, left_parts};
+                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, left, verdicts};
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
-            hipLaunchKernelGGL(vq::k_verify_part<T>, dim3((unsigned)(rows * parts)), dim3(256), 0, ctx->stream, a);
-            if (drafts) hipLaunchKernelGGL(vq::k_verify_left<T>, dim3((unsigned)(here * cdiv(parts, left_parts))), dim3(256), 0, ctx->stream, a);
-            hipLaunchKernelGGL(vq::k_verify_pick<T>, dim3((unsigned)here), dim3(256), 0, ctx->stream, a);
+            const dim3 all((unsigned)(rows * (wide ? cdiv(parts, 4) : parts))), some((unsigned)(here * parts)), each((unsigned)here), wg(256);
+            if (wide) {
+                hipLaunchKernelGGL((vq::k_verify_part<T, 64>), all, wg, 0, ctx->stream, a);
+                hipLaunchKernelGGL(vq::k_verify_verdict<T>, each, wg, 0, ctx->stream, a);
+                if (drafts) hipLaunchKernelGGL((vq::k_verify_left<T, true>), some, wg, 0, ctx->stream, a);
+                hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
+            } else {
+                hipLaunchKernelGGL((vq::k_verify_part<T, 16>), all, wg, 0, ctx->stream, a);
+                if (drafts) {
+                    hipLaunchKernelGGL((vq::k_verify_left<T, false>), some, wg, 0, ctx->stream, a);
+                    hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
+                } else
+                    hipLaunchKernelGGL((vq::k_verify_pick<T, false>), each, wg, 0, ctx->stream, a);
+            }
         });
         VQ_HIP(ctx, hipGetLastError());
     }
