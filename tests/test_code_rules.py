@@ -24,8 +24,9 @@ int back(int type, i64 s, i64 n, i64 ld, int k, float beta, int top, i64 lp, i64
 int verify(int type, i64 t, i64 ldt, float beta, i64 q, i64 ldq, float bq, i64 n, int d, int k, int cb, i64 c, i64 cs, i64 u, i64 ldu, i64 a, i64 o, i64 ldo) {
     return vq::check_code_verify(type, P(t), ldt, beta, P(q), ldq, bq, n, d, k, cb, P(c), cs, P(u), ldu, P(a), P(o), ldo).status; }
 i64 embed_bytes(i64 n, int k, int dim, int m) { return vq::embed_work(n, k, dim, m).bytes; }
-int lists(i64 n, int k, i64 *out) { const vq::ListPlan p = vq::plan_lists(n, k); out[0] = p.width, out[1] = p.buckets, out[2] = p.share, out[3] = p.shares;
-    const vq::EmbedWork w = vq::embed_work(n, k, 100, 1); out[4] = w.below - w.counts, out[5] = w.partial - w.below, out[6] = w.counts - w.edges; return 0; }
+int lists(i64 n, int k, int m, i64 *out) { const vq::ListPlan p = vq::plan_lists(n, k, m); out[0] = p.width, out[1] = p.buckets, out[2] = p.share, out[3] = p.shares;
+    const vq::EmbedWork w = vq::embed_work(n, k, 100, m); out[4] = w.below - w.counts, out[5] = w.partial - w.below, out[6] = w.counts - w.edges;
+    out[7] = vq::list_lds(p.width, true); return 0; }
 int plan(i64 n, int k, int grad, i64 *out) { const vq::DistillPlan p = vq::plan_distill(n, k, grad); out[0] = p.waves, out[1] = p.per_lane, out[2] = p.parts;
     out[3] = vq::distill_rows_of_a_launch(p); return 0; }
 i64 distill_bytes(i64 n, int k) { return vq::distill_work(n, k); }
@@ -120,17 +121,20 @@ SIZES = [1, 2, 3, 15, 16, 17, 255, 256, 257, 511, 512, 513, 1024, 1025, 2048, 20
 
 
 def test_buckets_and_shares_hold_every_code_and_position(lib):
-    lib.lists.argtypes = [C.c_longlong, C.c_int, C.c_void_p]
-    out = (C.c_longlong * 7)()
+    lib.lists.argtypes = [C.c_longlong, C.c_int, C.c_int, C.c_void_p]
+    out = (C.c_longlong * 8)()
     for k in SIZES:
         for n in (0, 1, 63, 1024, 1025, 4096, 32768, 32769, 50000, 100_000, 1_000_000, 16_777_216, 1 << 30):
-            lib.lists(n, k, out)
-            width, buckets, share, shares, counts, below, edges = out
-            assert 1 <= width <= 1024 and (buckets - 1) * width < k <= buckets * width and 16 * width * 4 <= 61440  # (and the waves' totals, below 64 KB)
-            assert share * shares >= n and (shares == 1 or (shares - 1) * share < n) and shares <= 256 and share < 1 << 31
-            if shares > 1:
-                assert counts >= 4 * shares * k and below >= 4 * shares * buckets
-            assert edges >= 4 * -(-n // 1024)
+            for m in (1, 4, 64):
+                if n * m > 1 << 30:
+                    continue
+                lib.lists(n, k, m, out)
+                width, buckets, share, shares, counts, below, edges, lds = out
+                assert 1 <= width <= 512 and (buckets - 1) * width < k <= buckets * width and buckets * 1024 < 1 << 32 and lds <= 65536
+                assert share * shares >= n and (shares == 1 or (shares - 1) * share < n) and shares <= 256 and share < 1 << 31
+                if shares > 1:
+                    assert counts >= 4 * m * shares * k and below >= 4 * m * shares * buckets
+                assert edges >= 4 * m * -(-n // 1024)
 
 
 def test_every_code_of_a_row_has_a_lane(lib):

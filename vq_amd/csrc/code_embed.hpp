@@ -164,7 +164,7 @@ struct ListArgs {
 // run of the positions, so that the order within a code is that of the positions; the few of them that its bucket has it keeps in LDS, and
 // reads its run again only where they are more than fit there.  With one share the workgroup goes on and writes its part of the list; of several
 // shares the counts are added up first, by the launch after (PLACE).
-constexpr int kQueue = 512;
+constexpr int kQueue = kListQueue;
 template <int WAVES, int BYTES, bool COUNT, bool PLACE>
 __global__ void __launch_bounds__(64 * WAVES) k_code_lists(ListArgs a) {
     extern __shared__ int hist[];  // [wave][code of the bucket], and (PLACE) [wave][kQueue]
@@ -372,6 +372,16 @@ __device__ __forceinline__ void sum_members(const SumArgs &s, Rows rows, int a, 
 // workgroups come last: zeros written beside the reads of the sums made both slower (16,384 x 1280 bf16 to 65,536 f32 rows 101 us, apart
 // 77).
 constexpr int kZeroCodes = 64, kZeroBytes = 16384;
+template <typename O, int VO> __device__ __forceinline__ void zero_piece(typename O::Raw *to, int c, int end) {  // [c, c + VO) below end
+    const float zeros[VO] = {};
+    if (c + VO <= end) {
+        Values<O, VO>::store(to + c, zeros);
+    } else {
+#pragma unroll
+        for (int v = 0; v < VO; ++v)
+            if (c + v < end) to[c + v] = O::down(0.0f);
+    }
+}
 template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs &a, unsigned id, int stage, int *list, int *count) {
     typedef typename O::Raw Out;
     constexpr int VO = wide<O>(), PIECE = kZeroBytes / (int)sizeof(Out);
@@ -395,9 +405,7 @@ template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs 
                 typedef uint32_t Four __attribute__((ext_vector_type(4)));
                 __builtin_nontemporal_store(Four{0, 0, 0, 0}, reinterpret_cast<Four *>(to + c));
             } else {
-                #pragma unroll
-                for (int v = 0; v < VO; ++v)
-                    if (c + v < end) to[c + v] = O::down(0.0f);
+                zero_piece<O, VO>(to, c, end);
             }
         }
     }
@@ -413,7 +421,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     typedef typename O::Raw Out;
     constexpr int COLUMNS = 16 * V, VO = V == 1 ? 1 : wide<O>();
     __shared__ float red[16][COLUMNS];
-    __shared__ int begin[kGroupCodes], behind[kGroupCodes], count[3];
+    __shared__ int begin[kGroupCodes], behind[kGroupCodes], count[4];
     __shared__ uint8_t which[3][kGroupCodes];
     __shared__ int few[FEW ? kFewPositions : 1], queue[FEW ? kFewPositions + 8 : 1], queued[4];
     const int tid = threadIdx.x, sub = tid >> 4, column = (a.first + blockIdx.x % (unsigned)a.across) * COLUMNS, place = column + (tid & 15) * V, at = min(place, a.dim - V), stage = blockIdx.z;
@@ -487,7 +495,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     }
     // the workgroup's codes by the number of their members: a group of lanes each, or the whole workgroup
     const int64_t from = (int64_t)group * a.codes;
-    if (tid < 3) count[tid] = 0;
+    if (tid < 4) count[tid] = 0;
     int s0 = 0, s1 = 0;
     if constexpr (FEW) {
         // the positions of these codes, in their order, by wave; then each code's, a lane per code
@@ -552,12 +560,17 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
         s1 = start[from + tid + 1];
     }
     __syncthreads();
-    if (tid < a.codes && from + tid < a.k) {
-        const int members = s1 - s0;
+    const bool has = tid < a.codes && from + tid < a.k;
+    const int members = s1 - s0;
+    if (has && members > (FEW ? kFewMembers : kOwnMembers) && members <= kLongCode) atomicAdd(&count[3], 1);
+    __syncthreads();
+    if (has) {
+        // (16 codes side by side take the time of the longest, each by all lanes that of their sum: the more there are, the longer they may be)
+        const int own = (FEW ? kFewMembers : kOwnMembers) * max(1, count[3]);
         begin[tid] = s0;
         behind[tid] = s1;
         if (members <= kLongCode) {
-            const int kind = members == 0 ? 2 : members <= (FEW ? kFewMembers : kOwnMembers) ? 0 : 1;
+            const int kind = members == 0 ? 2 : members <= own ? 0 : 1;
             which[kind][atomicAdd(&count[kind], 1)] = (uint8_t)tid;  // (in whatever order: each is a sum of its own)
         }
     }
@@ -624,7 +637,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     if (FEW && !a.accumulate) {
         for (int i = sub; i < count[2]; i += 16) {
             Out *to = grad + (from + which[2][i]) * a.ld_grad;
-            for (int c = column + (tid & 15); c < min(a.dim, column + COLUMNS); c += 16) to[c] = O::down(0.0f);
+            for (int c = column + (tid & 15) * VO; c < min(a.dim, column + COLUMNS); c += 16 * VO) zero_piece<O, VO>(to, c, min(a.dim, column + COLUMNS));
         }
     }
 }

@@ -179,22 +179,24 @@ inline int embed_pieces(int64_t n, int32_t m, int pieces) { return m >= 4 && pie
 // ---- sums by code ------------------------------------------------------------------------------------
 // The positions of each stage in the order of their codes, and where each code's positions begin: k + 1 numbers.  Workgroups of 16 waves
 // list a bucket of codes each, of a share of the positions.  One share, and one launch, up to 32,768 positions; more positions in shares, in two
-// launches, with as many codes per bucket as 16 waves can count in 60 KB of LDS.
+// launches, so that there are about 1024 workgroups, two to a compute unit by their 60 KB of LDS (363,313 x 4 codes of 8379: 3204 workgroups, one to a
+// compute unit, 31 + 174 us, so ZZ).
 struct ListPlan {
     int32_t width, buckets;
     int32_t share, shares;
 };
-constexpr int kBucketMost = 960;
-// 16 waves' counts, and (to write the list) 512 positions and codes of each wave.
-constexpr int list_lds(int width, bool place) { return (16 * width + 1) / 2 * 8 + (place ? 16 * 512 * 8 : 0); }
-inline ListPlan plan_lists(int64_t n, int32_t k) {
+constexpr int kBucketMost = 480, kOneShareMost = 512;  // codes of a bucket
+constexpr int kListQueue = 256;                        // positions of a bucket that a wave keeps
+// 16 waves' counts, and (to write the list) positions and codes of each wave.
+constexpr int list_lds(int width, bool place) { return (16 * width + 1) / 2 * 8 + (place ? 16 * kListQueue * 8 : 0); }
+inline ListPlan plan_lists(int64_t n, int32_t k, int32_t m) {
     if (n <= 32768) {
-        const int32_t width = std::min<int32_t>(512, (k + 255) / 256);
+        const int32_t width = std::min<int32_t>(kOneShareMost, (k + 255) / 256);
         return {width, (k + width - 1) / width, (int32_t)std::max<int64_t>(n, 1), 1};
     }
     const int32_t width = std::min<int32_t>(kBucketMost, k), buckets = (k + width - 1) / width;
-    // shares of 4096 positions or more, a few hundred workgroups, at most 256 shares
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / buckets)), share = std::max<int64_t>(4096, (n + most - 1) / most);
+    // shares of 4096 positions or more, at most 256 of them
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / ((int64_t)buckets * m))), share = std::max<int64_t>(4096, (n + most - 1) / most);
     return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
 }
 // Up to so many positions the workgroups that sum make their lists themselves, where no more than 512 of them read all codes (333 x 100 f32, 1001
@@ -213,14 +215,14 @@ struct EmbedWork {
 inline EmbedWork embed_work(int64_t n, int32_t k, int32_t dim, int32_t m) {
     const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
     // (shares times codes: no plan has more than 256 shares, nor more than 1024 of share and bucket)
-    const int64_t counts = n > 32768 ? std::min<int64_t>(256 * (int64_t)k, (int64_t)1024 * kBucketMost + k) : 0;
+    const int64_t counts = n > 32768 ? std::min<int64_t>(256 * (int64_t)k, (int64_t)1024 * kBucketMost + k) : 0, belows = n > 32768 ? 4096 : 0;
     EmbedWork w;
     w.start = 0;
     w.rows = up((int64_t)m * (k + 1) * 4);
     w.edges = w.rows + up(m * n * 4);
     w.counts = w.edges + up(m * embed_edges(n) * 4);
     w.below = w.counts + up(m * counts * 4);
-    w.partial = w.below + up(n > 32768 ? m * 2048 * 4 : 0);
+    w.partial = w.below + up(m * belows * 4);
     w.bytes = w.partial + up(m * embed_chunks(n) * 2 * ((dim + 15) / 16 * 16) * 4);
     return w;
 }

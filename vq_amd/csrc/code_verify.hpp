@@ -42,14 +42,15 @@ __device__ __forceinline__ int drafted(const VerifyArgs &a, int64_t seq, int lan
 
 // EACH / 16 parts of a row per workgroup, their sums relative to the largest score of all of them.  Bound by the vector pipe: 18 instructions per code,
 // 13 of them in 64 bits, and some 180 per wave, which is why a lane has 64 codes where there are enough workgroups (128 sequences of 11
-// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).
-template <typename T, int EACH>
-__global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
+// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).  Rows of up to 2048 codes have a wave each (WAVES = 1, one part; 395
+// sequences of 17 rows of 1600 codes 25 us with a workgroup each, ZZ).
+template <typename T, int EACH, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) k_verify_part(VerifyArgs a) {
     typedef typename T::Raw Raw;
-    typedef Held<T, 256, EACH * (int)sizeof(Raw) / 16> H;
-    constexpr int PARTS = EACH / 16, PIECES = EACH / H::VEC / PARTS;  // vectors of a lane in a part
-    __shared__ float most_of[4][PARTS];
-    __shared__ double sum_of[4][PARTS];
+    typedef Held<T, 64 * WAVES, EACH * (int)sizeof(Raw) / 16> H;
+    constexpr int PARTS = WAVES == 1 ? 1 : EACH / 16, PIECES = EACH / H::VEC / PARTS;  // vectors of a lane in a part
+    __shared__ float most_of[WAVES][PARTS];
+    __shared__ double sum_of[WAVES][PARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t groups = (uint32_t)(a.parts + PARTS - 1) / PARTS;
     const uint32_t row = blockIdx.x / groups, targets = (uint32_t)a.n * (uint32_t)(a.draft + 1);  // (a launch has fewer than 2^23)
@@ -67,12 +68,12 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
         const int64_t c = (int64_t)__shfl((int)code, pos) - lo;
         if (c >= 0 && c < hi - lo) {
             const int place = (int)c / H::VEC;
-            if (place % 256 == tid) {
+            if (place % (64 * WAVES) == tid) {
 #pragma unroll
                 for (int u = 0; u < EACH / H::VEC; ++u)
 #pragma unroll
                     for (int v = 0; v < H::VEC; ++v)
-                        if (u == place / 256 && v == (int)c % H::VEC) x.drop(u, v);
+                        if (u == place / (64 * WAVES) && v == (int)c % H::VEC) x.drop(u, v);
             }
         }
     }
@@ -92,7 +93,8 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     __syncthreads();
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
-        most[p] = larger_or_nan(larger_or_nan(most_of[0][p], most_of[1][p]), larger_or_nan(most_of[2][p], most_of[3][p]));
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) most[p] = larger_or_nan(most[p], most_of[w][p]);
         m = larger_or_nan(m, most[p]);
     }
     const bool sound = m > kNegInf && m < __builtin_inff();  // uniform
@@ -118,7 +120,10 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     const bool none = sound && !((double)own - from >= least);
     const int64_t at = (int64_t)row * a.parts + first + tid;
     a.most[at] = none ? kNegInf : m;
-    a.sum[at] = none ? 0.0 : sum_of[0][tid] + sum_of[1][tid] + sum_of[2][tid] + sum_of[3][tid];
+    double sum = sum_of[0][tid];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum += sum_of[w][tid];
+    a.sum[at] = none ? 0.0 : sum;
 }
 
 constexpr int kVerifyEach = kVerifyPart / 256;  // codes of a lane where weights are summed

@@ -134,7 +134,7 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
     const vq::EmbedWork work = vq::embed_work(n, k, dim, m);
     VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)work.bytes));
     char *w = (char *)ctx->code_work.p;
-    const vq::ListPlan plan = vq::plan_lists(n, k);
+    const vq::ListPlan plan = vq::plan_lists(n, k, m);
     const vq::ListArgs l{d_codes, code_stride, (int)n, k, plan.width, plan.share, plan.shares, (int32_t *)(w + work.start),
                          (int32_t *)(w + work.rows), (int32_t *)(w + work.edges), (int32_t *)(w + work.counts), (int32_t *)(w + work.below)};
     const auto lists = [&](auto bytes) -> int32_t {
@@ -145,7 +145,7 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
         if (!(ctx->list_lds_set & bit)) {  // more than 64 KB
             const auto kernel = plan.shares == 1 ? vq::k_code_lists<16, BYTES, true, true> : vq::k_code_lists<16, BYTES, false, true>;
             VQ_HIP(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                            vq::list_lds(vq::kBucketMost, true)));
+                                            vq::list_lds(vq::kOneShareMost, true)));
             ctx->list_lds_set |= bit;
         }
         if (plan.shares == 1) {
@@ -160,8 +160,8 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
     int32_t rc = VQ_OK;
     by_bytes(code_bytes, [&](auto bytes) { rc = lists(bytes); });
     VQ_TRY(rc);
-    // codes of a workgroup: as many as leave 2048 workgroups, 16 to 128
-    const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(16, (int64_t)k * m * across / 2048 / 16 * 16));
+    // codes of a workgroup: as many as leave 2048 workgroups, at most 128
+    const int codes = (int)std::min<int64_t>(128, std::max<int64_t>(1, (int64_t)k * m * across / 2048));
     vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, nullptr, 0, 0, l.start, l.rows, l.edges, (float *)(w + work.partial),
                   (int)vq::embed_chunks(n), (dim + 15) / 16 * 16, codes, (int)cdiv(k, codes), 0, 0};
     // the columns of some workgroups side by side, the others' in launches of their own: a grid has fewer than 2^32 lanes
@@ -289,12 +289,15 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
             typedef decltype(t) T;
             const dim3 all((unsigned)(rows * (wide ? cdiv(parts, 4) : parts))), some((unsigned)(here * parts)), each((unsigned)here), wg(256);
             if (wide) {
-                hipLaunchKernelGGL((vq::k_verify_part<T, 64>), all, wg, 0, ctx->stream, a);
+                hipLaunchKernelGGL((vq::k_verify_part<T, 64, 4>), all, wg, 0, ctx->stream, a);
                 hipLaunchKernelGGL(vq::k_verify_verdict<T>, each, wg, 0, ctx->stream, a);
                 if (drafts) hipLaunchKernelGGL((vq::k_verify_left<T, true>), some, wg, 0, ctx->stream, a);
                 hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
             } else {
-                hipLaunchKernelGGL((vq::k_verify_part<T, 16>), all, wg, 0, ctx->stream, a);
+                if (k <= 2048)
+                    hipLaunchKernelGGL((vq::k_verify_part<T, 32, 1>), all, dim3(64), 0, ctx->stream, a);
+                else
+                    hipLaunchKernelGGL((vq::k_verify_part<T, 16, 4>), all, wg, 0, ctx->stream, a);
                 if (drafts) {
                     hipLaunchKernelGGL((vq::k_verify_left<T, false>), some, wg, 0, ctx->stream, a);
                     hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
