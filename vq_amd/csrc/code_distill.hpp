@@ -36,6 +36,7 @@ struct DistillArgs {
 };
 
 // A row's alternatives, one per lane of a wave.
+constexpr int kSlots = 4096;
 struct Teacher {
     int code = -1;
     bool has = false, first = false;  // an alternative; the first with its code
@@ -53,7 +54,8 @@ struct Teacher {
         has = code >= 0 && l != kNegInf;
         log_q = l;
     }
-    __device__ __forceinline__ void read(const DistillArgs &a, int64_t row, int lane) {
+    // slots: the wave's own, with anything in them
+    __device__ __forceinline__ void read(const DistillArgs &a, int64_t row, int lane, uint8_t *slots) {
         names(a, row, lane);
         const unsigned long long who = __ballot(has);
         some = who != 0;
@@ -67,11 +69,18 @@ struct Teacher {
             q = (float)e;
             Q = sum;
         } else if (some) {
-            q = (float)(e / sum);
+            q = (float)e * __builtin_amdgcn_rcpf((float)sum);
             log_q = l - most - __builtin_amdgcn_logf((float)sum) * kLn2;
             Q = 1.0;
         }
         first = has;
+        q_code = has ? q : 0.0f;
+        // The same code twice is rare: where every alternative finds its own mark in the slot of its code's lowest bits there is none.  (Else the
+        // sums of the probabilities with this code, in the order of the list.)
+        if (has) slots[code & (kSlots - 1)] = (uint8_t)lane;
+        wave_sync();
+        if (__ballot(has && slots[code & (kSlots - 1)] != lane) == 0) return;
+        if (has) q_code = 0.0f;
         for (int t = 0; t < a.top; ++t) {
             if (!(who >> t & 1)) continue;  // uniform
             const int other = __builtin_amdgcn_readlane(code, t);
@@ -255,6 +264,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) k_distill_row(D
     typedef typename T::Raw Raw;
     constexpr int LANES = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
     __shared__ Marks<T, LANES, NV> marks_of[ROWS];
+    __shared__ uint8_t slots_of[ROWS][kSlots];
     __shared__ float joined[2][16];
     __shared__ RowGrad common;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, place = WAVES == 1 ? lane : threadIdx.x;
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) k_distill_row(D
     Teacher t;
     float score = kNegInf, value = 0.0f;
     if (leads) {
-        t.read(a, row, lane);
+        t.read(a, row, lane, slots_of[WAVES == 1 ? wave : 0]);
         if (t.has && t.code < a.k) score = T::up(s[t.code]);
     }
     if (a.split) {  // uniform
@@ -336,13 +346,14 @@ __global__ void __launch_bounds__(256) k_distill_part(DistillArgs a) {
 // A wave joins the parts of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) k_distill_join(DistillArgs a) {
+    __shared__ uint8_t slots_of[4][kSlots];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.n) return;
     const float *sums = a.sums + (row * a.parts + min(lane, a.parts - 1)) * 2;
     const float pm = sums[0], pS = sums[1];
     Teacher t;
-    t.read(a, row, lane);
+    t.read(a, row, lane, slots_of[wave]);
     const float score = t.has && t.code < a.k ? T::up(((const typename T::Raw *)a.s)[row * a.ld + t.code]) : kNegInf;
     float mr, Sr;
     join_rest(a, pm, pS, lane < a.parts, &mr, &Sr);
@@ -356,6 +367,7 @@ template <typename T, int WAVES, int NV>
 __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
     typedef typename T::Raw Raw;
     constexpr int LANES = 64 * WAVES, ROWS = 4 / WAVES;
+    __shared__ uint8_t slots_of[ROWS][kSlots];
     __shared__ RowGrad common;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, place = WAVES == 1 ? lane : threadIdx.x;
     const int64_t row = (int64_t)blockIdx.x * ROWS + (WAVES == 1 ? wave : 0);
@@ -370,7 +382,7 @@ __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
     Teacher t;
     float value = 0.0f;
     if (leads) {
-        t.read(a, row, lane);
+        t.read(a, row, lane, slots_of[WAVES == 1 ? wave : 0]);
         const float score = t.has && t.code >= lo && t.code < hi ? T::up(s[t.code]) : kNegInf;
         grad = row_grad(a, row, t, a.max[row], a.logsum[row], a.rest ? a.logrest[row] : kNegInf, score, &value);
         if constexpr (WAVES > 1)
