@@ -167,3 +167,30 @@ def test_more_sequences_than_a_launch_takes(ctx):
     ctx.code_verify("f32", dt, k, 1.0, dd, k, 1.0, n, 1, k, 4, dc, 1, du, 2, da, do, 2)
     wa, wo = Q.verify(t, 1.0, d, 1.0, codes, u.astype(np.float64))
     assert np.array_equal(da.download(), tile(wa)) and np.array_equal(do.download(), tile(wo))
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("scored", [True, False])
+@pytest.mark.parametrize("k", [2047, 2048, 2049, 30])
+def test_around_the_lines_between_the_ways(ctx, k, kind, scored):
+    """Rows of one workgroup per sequence and of parts; many drafts of few and of many sequences."""
+    rng = np.random.default_rng(k)
+    for n, draft in ((3, 16), (3, 17), (512, 17 if k < 100 else 3)):
+        t, d, codes, u = case(rng, n, draft, k, kind, 1.0, 1.0, scored, noise=0.3)
+        u[:, :draft] *= 0.5
+        run(ctx, t, d, codes, u, kind, 1.0, 1.0, pad=k % 3, offset=1)
+
+
+def test_enough_rows_for_four_parts_to_a_workgroup(ctx):
+    """Masked codes, whole parts among them, where a workgroup makes the sums of four parts of a row."""
+    rng = np.random.default_rng(8)
+    for kind, k in (("bf16", 17000), ("f32", 40000), ("f16", 5000)):
+        n, draft = (2100 if k == 5000 else 700 if k == 17000 else 240), 1
+        t, d, codes, u = case(rng, n, draft, k, kind, 1.0, 1.0, spread=1.0)
+        t[::3, :, :4096] = -np.inf
+        t[1::5, :, 4096:] = -np.inf
+        t[5, 0], t[6, 1], t[7, 0, 4500], t[8, 1, 2] = -np.inf, -np.inf, np.nan, np.inf
+        u[::4, :draft] = 0.999
+        u[9], u[10] = 0.0, 1.0
+        run(ctx, t, d, codes, u, kind, 1.0, 1.0)
+        run(ctx, t, None, codes, u, kind, 1.0, 1.0)

@@ -180,7 +180,7 @@ inline int embed_pieces(int64_t n, int32_t m, int pieces) { return m >= 4 && pie
 // The positions of each stage in the order of their codes, and where each code's positions begin: k + 1 numbers.  Workgroups of 16 waves
 // list a bucket of codes each, of a share of the positions.  One share, and one launch, up to 32,768 positions; more positions in shares, in two
 // launches, so that there are about 1024 workgroups, two to a compute unit by their 60 KB of LDS (363,313 x 4 codes of 8379: 3204 workgroups, one to a
-// compute unit, 31 + 174 us, so ZZ).
+// compute unit, 31 + 174 us, so 19 + 50).
 struct ListPlan {
     int32_t width, buckets;
     int32_t share, shares;
@@ -259,6 +259,8 @@ inline int64_t distill_work(int64_t n, int32_t k) {
 // own and as many as drafts of its drafts'.
 constexpr int kVerifyPart = 4096;
 inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyPart; }
+// Rows of up to 2048 codes: a workgroup per sequence does everything, unless a few sequences have many rows each.
+inline bool verify_few(int64_t n, int32_t draft, int32_t k) { return k <= 2048 && (draft <= 16 || n >= 512); }
 inline bool verify_wide(int64_t rows, int32_t k) { return k > kVerifyPart && rows * ((k + 4 * kVerifyPart - 1) / (4 * kVerifyPart)) >= 2048; }
 // Per row and part a sum and a maximum (in 64 bits and 32; 16 bytes); per sequence and part a sum more, and 64 bytes for what its drafts come to.
 inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8) + 64; }

@@ -42,13 +42,12 @@ __device__ __forceinline__ int drafted(const VerifyArgs &a, int64_t seq, int lan
 
 // EACH / 16 parts of a row per workgroup, their sums relative to the largest score of all of them.  Bound by the vector pipe: 18 instructions per code,
 // 13 of them in 64 bits, and some 180 per wave, which is why a lane has 64 codes where there are enough workgroups (128 sequences of 11
-// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).  Rows of up to 2048 codes have a wave each (WAVES = 1, one part; 395
-// sequences of 17 rows of 1600 codes 25 us with a workgroup each, ZZ).
-template <typename T, int EACH, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) k_verify_part(VerifyArgs a) {
+// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).
+template <typename T, int EACH>
+__global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     typedef typename T::Raw Raw;
-    typedef Held<T, 64 * WAVES, EACH * (int)sizeof(Raw) / 16> H;
-    constexpr int PARTS = WAVES == 1 ? 1 : EACH / 16, PIECES = EACH / H::VEC / PARTS;  // vectors of a lane in a part
+    typedef Held<T, 256, EACH * (int)sizeof(Raw) / 16> H;
+    constexpr int WAVES = 4, PARTS = EACH / 16, PIECES = EACH / H::VEC / PARTS;  // vectors of a lane in a part
     __shared__ float most_of[WAVES][PARTS];
     __shared__ double sum_of[WAVES][PARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -140,20 +139,9 @@ struct VerdictLds {
     Verdict out;
 };
 
-// By a workgroup of four waves: each joins the parts of every fourth row, the first decides.  code: a lane's drafted code.
-template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArgs &a, int64_t seq, VerdictLds &l, int64_t *code) {
-    typedef typename T::Raw Raw;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int length = drafted(a, seq, lane, code), rows = length + 1 + (a.drafts ? length : 0);
-    const bool here = lane <= length, asked = lane < length, known = asked && *code < a.k;
-    float s = 0.0f, t = 0.0f, u = 0.0f;  // lane d: the scores of drafted code d, its random number
-    if (wave == 0 && asked) {
-        u = a.uniform[seq * a.ld_uniform + lane];
-        if (known) {
-            s = T::up(((const Raw *)a.target)[(seq * (a.draft + 1) + lane) * a.ld_target + *code]);
-            if (a.drafts) t = T::up(((const Raw *)a.drafts)[(seq * a.draft + lane) * a.ld_draft + *code]);
-        }
-    }
+// The sums of a sequence's rows from those of their parts: the target's of each position up to `length`, then the drafts'.
+__device__ __forceinline__ void join_parts(const VerifyArgs &a, int64_t seq, int length, VerdictLds &l) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = length + 1 + (a.drafts ? length : 0);
     constexpr int WAVES = 4, AHEAD = 4;
     for (int r0 = wave; r0 < rows; r0 += WAVES * AHEAD) {
         float most[AHEAD];
@@ -199,6 +187,24 @@ template <typename T> __device__ __forceinline__ Verdict verdict(const VerifyArg
             }
         }
     }
+}
+
+// By a workgroup of four waves: each makes or joins the sums of every fourth row, row_sums(l, length), and the first decides.  code: a lane's
+// drafted code.
+template <typename T, typename F> __device__ __forceinline__ Verdict verdict(const VerifyArgs &a, int64_t seq, VerdictLds &l, int64_t *code, F row_sums) {
+    typedef typename T::Raw Raw;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int length = drafted(a, seq, lane, code);
+    const bool here = lane <= length, asked = lane < length, known = asked && *code < a.k;
+    float s = 0.0f, t = 0.0f, u = 0.0f;  // lane d: the scores of drafted code d, its random number
+    if (wave == 0 && asked) {
+        u = a.uniform[seq * a.ld_uniform + lane];
+        if (known) {
+            s = T::up(((const Raw *)a.target)[(seq * (a.draft + 1) + lane) * a.ld_target + *code]);
+            if (a.drafts) t = T::up(((const Raw *)a.drafts)[(seq * a.draft + lane) * a.ld_draft + *code]);
+        }
+    }
+    row_sums(length);
     __syncthreads();
     if (wave == 0) {
         double p = 0.0, q = 1.0;
@@ -284,7 +290,7 @@ template <typename T> __device__ __forceinline__ void lane_weights(const VerifyA
 template <typename T> __global__ void __launch_bounds__(256) k_verify_verdict(VerifyArgs a) {
     __shared__ VerdictLds lds;
     int64_t code;
-    const Verdict o = verdict<T>(a, blockIdx.x, lds, &code);
+    const Verdict o = verdict<T>(a, blockIdx.x, lds, &code, [&](int length) { join_parts(a, blockIdx.x, length, lds); });
     if (threadIdx.x == 0) a.verdicts[blockIdx.x] = o;
 }
 
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(256) k_verify_left(VerifyArgs a) {
     } else {
         __shared__ VerdictLds lds;
         int64_t code;
-        o = verdict<T>(a, seq, lds, &code);
+        o = verdict<T>(a, seq, lds, &code, [&](int length) { join_parts(a, seq, length, lds); });
         if (part == 0 && tid == 0) a.verdicts[seq] = o;
     }
     if (o.bad || o.accepted == o.length) return;  // uniform
@@ -320,13 +326,70 @@ __global__ void __launch_bounds__(256) k_verify_left(VerifyArgs a) {
     if (tid == 0) a.left[blockIdx.x] = sum_of[0] + sum_of[1] + sum_of[2] + sum_of[3];
 }
 
+// Sums over a workgroup of four waves, and the lane that a sum belongs to.
+struct Choice {
+    double sum[4];
+    int found[4];
+};
+struct Chooser {
+    Choice &l;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __device__ __forceinline__ explicit Chooser(Choice &c) : l(c) {}
+    // the sum up to each lane, from `from` on, and of all
+    __device__ __forceinline__ double scan(double mine, double from, double *total) {
+        const double upto = wave_scan(mine, lane);
+        __syncthreads();
+        if (lane == 63) l.sum[wave] = upto;
+        __syncthreads();
+        *total = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            from += i < wave ? l.sum[i] : 0.0;
+            *total += l.sum[i];
+        }
+        return from + upto;
+    }
+    // the first lane whose sum is above the goal, or else the last that has any weight; -1: none has
+    __device__ __forceinline__ int choose(bool has, double upto, double goal) {
+        constexpr int NOT = 1024;
+        const unsigned long long hit = __ballot(has && upto > goal), any = __ballot(has);
+        if (lane == 0) l.found[wave] = hit ? wave * 64 + __ffsll(hit) - 1 : any ? NOT + wave * 64 + 63 - __clzll(any) : -1;
+        __syncthreads();
+        int at = -1, last = -1;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            at = l.found[i] >= 0 && l.found[i] < NOT ? l.found[i] : at;
+            last = last < 0 && l.found[i] >= NOT ? l.found[i] - NOT : last;
+        }
+        __syncthreads();
+        return at >= 0 ? at : last;
+    }
+};
+// The same among a lane's codes.
+__device__ __forceinline__ int among(const double (&y)[kVerifyEach], double so_far, double goal) {
+    int last = -1, first = -1;
+#pragma unroll
+    for (int e = 0; e < kVerifyEach; ++e) {
+        so_far += y[e];
+        if (y[e] > 0.0) {
+            last = e;
+            if (first < 0 && so_far > goal) first = e;
+        }
+    }
+    return first >= 0 ? first : last;
+}
+__device__ __forceinline__ void write_outcome(const VerifyArgs &a, int64_t seq, const Verdict &o, int64_t code, int next, int lane) {
+    if (lane == 0) a.accepted[seq] = o.accepted;
+    if (lane <= a.draft) a.out[seq * a.ld_out + lane] = lane < o.accepted ? (int32_t)code : lane == o.accepted ? next : -1;
+}
+
 // The outcome of a sequence: how many drafts stay, and the codes: these, the next one, -1 behind it.
 // READY: what the drafts come to is there.
 template <typename T, bool READY>
 __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
-    constexpr int WAVES = 4, NOT = 1024;
-    __shared__ double part_of[64 * WAVES], sum_of[WAVES];
-    __shared__ int found[WAVES], next_of;
+    __shared__ double part_of[256];
+    __shared__ Choice choice;
+    __shared__ int next_of;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t seq = blockIdx.x;
     int64_t code;
@@ -337,39 +400,10 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
         code = lane < o.accepted ? code_at(a.codes, a.code_bytes, seq * a.code_stride + lane) : -1;
     } else {
         __shared__ VerdictLds lds;
-        o = verdict<T>(a, seq, lds, &code);
+        o = verdict<T>(a, seq, lds, &code, [&](int length) { join_parts(a, seq, length, lds); });
     }
-    // sums over the workgroup up to each lane, `from` on; the sum of all
+    Chooser chooser(choice);
     double total;
-    const auto scan = [&](double mine, double from) {
-        const double upto = wave_scan(mine, lane);
-        __syncthreads();
-        if (lane == 63) sum_of[wave] = upto;
-        __syncthreads();
-        total = 0.0;
-        double before = from;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            before += i < wave ? sum_of[i] : 0.0;
-            total += sum_of[i];
-        }
-        return before + upto;
-    };
-    double goal = 0.0;
-    // the first lane whose sum reaches the goal; NOT + the last that has any weight, if none does; -1: none has
-    const auto choose = [&](bool has, double upto) {
-        const unsigned long long hit = __ballot(has && upto > goal), any = __ballot(has);
-        if (lane == 0) found[wave] = hit ? wave * 64 + __ffsll(hit) - 1 : any ? NOT + wave * 64 + 63 - __clzll(any) : -1;
-        __syncthreads();
-        int at = -1, last = -1;
-#pragma unroll
-        for (int i = WAVES - 1; i >= 0; --i) {
-            at = found[i] >= 0 && found[i] < NOT ? found[i] : at;
-            last = last < 0 && found[i] >= NOT ? found[i] : last;
-        }
-        __syncthreads();
-        return at >= 0 ? at : last;
-    };
     if (tid == 0) next_of = -1;
     if (!o.bad) {  // uniform
         Weights w = weights(a, o);
@@ -383,42 +417,101 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
                 const float m = a.most[row * a.parts + tid];
                 mine = m > kNegInf ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
             }
-            upto = scan(mine, 0.0);
+            upto = chooser.scan(mine, 0.0, &total);
             if (total > 0.0 || !w.minus) break;
             w.minus = false;
             w.by_p = 1.0;
         }
         part_of[tid] = upto;
-        goal = (double)v * total;
-        int part = choose(mine > 0.0, upto);
+        const double goal = (double)v * total;
+        int part = chooser.choose(mine > 0.0, upto, goal);
         if (part >= 0) {  // uniform
-            part &= NOT - 1;
             const int at = part * kVerifyPart + tid * kVerifyEach;
             double y[kVerifyEach], sum = 0.0;
             lane_weights<T>(a, w, seq, o.accepted, at, y);
 #pragma unroll
             for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
-            upto = scan(sum, part ? part_of[part - 1] : 0.0);
-            const int who = choose(sum > 0.0, upto);
-            if (who >= 0 && tid == (who & (NOT - 1))) {
-                double so_far = upto - sum;
-                int last = -1, first = -1;
-#pragma unroll
-                for (int e = 0; e < kVerifyEach; ++e) {
-                    so_far += y[e];
-                    if (y[e] > 0.0) {
-                        last = e;
-                        if (first < 0 && so_far > goal) first = e;
-                    }
-                }
-                next_of = at + (first >= 0 ? first : last);
-            }
+            upto = chooser.scan(sum, part ? part_of[part - 1] : 0.0, &total);
+            if (tid == chooser.choose(sum > 0.0, upto, goal)) next_of = at + among(y, upto - sum, goal);
         }
     }
     __syncthreads();
     if (wave) return;
-    if (lane == 0) a.accepted[seq] = o.accepted;
-    if (lane <= a.draft) a.out[seq * a.ld_out + lane] = lane < o.accepted ? (int32_t)code : lane == o.accepted ? next_of : -1;
+    write_outcome(a, seq, o, code, next_of, lane);
+}
+
+// Rows of up to 2048 codes: a workgroup does all of a sequence, a wave per row, in one launch (62 sequences of 17 rows of 237 codes 23 us in
+// three, 17 so).
+constexpr int kVerifyFew = 2048;
+template <typename T> __global__ void __launch_bounds__(256) k_verify_few(VerifyArgs a) {
+    typedef typename T::Raw Raw;
+    constexpr int EACH = kVerifyFew / 64;
+    typedef Held<T, 64, EACH * (int)sizeof(Raw) / 16> H;
+    __shared__ VerdictLds lds;
+    __shared__ Choice choice;
+    __shared__ int next_of;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t seq = blockIdx.x;
+    const float v = a.uniform[seq * a.ld_uniform + a.draft];
+    int64_t code;
+    const Verdict o = verdict<T>(a, seq, lds, &code, [&](int length) {
+        const int rows = length + 1 + (a.drafts ? length : 0);
+        for (int r = wave; r < rows; r += 4) {
+            const bool draft = r > length;
+            const int pos = draft ? r - length - 1 : r;
+            H x;
+            x.load(draft ? (const Raw *)a.drafts + (seq * a.draft + pos) * a.ld_draft : (const Raw *)a.target + (seq * (a.draft + 1) + pos) * a.ld_target, 0, a.k,
+                   lane);
+            const int out = !a.drafts && pos < length ? __shfl((int)code, pos) : -1;  // the row without its drafted code
+            float m = kNegInf;
+#pragma unroll
+            for (int u = 0; u < EACH / H::VEC; ++u)
+#pragma unroll
+                for (int v = 0; v < H::VEC; ++v) {
+                    if ((u * 64 + lane) * H::VEC + v == out) x.drop(u, v);
+                    m = larger_or_nan(m, x.at(u, v));
+                }
+            m = __uint_as_float(over_group<64>(__float_as_uint(m), __float_as_uint(kNegInf), [](uint32_t p, uint32_t q) {
+                return __float_as_uint(larger_or_nan(__uint_as_float(p), __uint_as_float(q)));
+            }));
+            const bool sound = m > kNegInf && m < __builtin_inff();  // uniform
+            const double c = draft ? a.c_draft : a.c_target, from = sound ? m : 0.0f, least = -1000.0 / c;
+            double sum = 0.0;
+            if (sound) {
+#pragma unroll
+                for (int u = 0; u < EACH / H::VEC; ++u) {
+                    if (u * 64 * H::VEC >= a.k) break;  // uniform
+#pragma unroll
+                    for (int v = 0; v < H::VEC; ++v) sum += exp2_of(fmax((double)x.at(u, v) - from, least), c);
+                }
+            }
+            sum = wave_sum(sum);
+            if (lane == 0) {
+                lds.m[draft][pos] = m;
+                lds.S[draft][pos] = m == kNegInf ? 0.0 : sound ? sum : __builtin_nan("");
+            }
+        }
+    });
+    Chooser chooser(choice);
+    if (tid == 0) next_of = -1;
+    if (!o.bad) {  // uniform
+        Weights w = weights(a, o);
+        double y[kVerifyEach], sum, upto, total;
+        for (;;) {  // (a second time where nothing is left of p - q)
+            lane_weights<T>(a, w, seq, o.accepted, tid * kVerifyEach, y);
+            sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < kVerifyEach; ++e) sum += y[e];
+            upto = chooser.scan(sum, 0.0, &total);
+            if (total > 0.0 || !w.minus) break;
+            w.minus = false;
+            w.by_p = 1.0;
+        }
+        const double goal = (double)v * total;
+        if (tid == chooser.choose(sum > 0.0, upto, goal)) next_of = tid * kVerifyEach + among(y, upto - sum, goal);
+    }
+    __syncthreads();
+    if (wave == 0) write_outcome(a, seq, o, code, next_of, lane);
 }
 
 }  // namespace vq

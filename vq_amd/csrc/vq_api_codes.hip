@@ -270,9 +270,11 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
                                             d_codes, code_stride, d_uniform, ld_uniform, d_accepted, d_out, ld_out), n, &go));
     if (!go) return VQ_OK;
     static_assert(sizeof(vq::Verdict) <= 64, "as the workspace counts it");
+    static_assert(vq::kVerifyFew <= 256 * vq::kVerifyEach, "a workgroup's lanes have all of a row's weights");
     const int e = vq::type_bytes(type);
     const int64_t slice = vq::verify_sequences_of_a_launch(draft, k);
-    VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
+    const bool few = vq::verify_few(n, draft, k);
+    if (!few) VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
     const void *drafts = draft > 0 ? d_draft : nullptr;
     for (int64_t b = 0; b < n; b += slice) {
         const int64_t here = std::min(slice, n - b), rows = here * (draft + 1 + (drafts ? draft : 0));
@@ -288,16 +290,15 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
             const dim3 all((unsigned)(rows * (wide ? cdiv(parts, 4) : parts))), some((unsigned)(here * parts)), each((unsigned)here), wg(256);
-            if (wide) {
-                hipLaunchKernelGGL((vq::k_verify_part<T, 64, 4>), all, wg, 0, ctx->stream, a);
+            if (few) {
+                hipLaunchKernelGGL(vq::k_verify_few<T>, each, wg, 0, ctx->stream, a);
+            } else if (wide) {
+                hipLaunchKernelGGL((vq::k_verify_part<T, 64>), all, wg, 0, ctx->stream, a);
                 hipLaunchKernelGGL(vq::k_verify_verdict<T>, each, wg, 0, ctx->stream, a);
                 if (drafts) hipLaunchKernelGGL((vq::k_verify_left<T, true>), some, wg, 0, ctx->stream, a);
                 hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
             } else {
-                if (k <= 2048)
-                    hipLaunchKernelGGL((vq::k_verify_part<T, 32, 1>), all, dim3(64), 0, ctx->stream, a);
-                else
-                    hipLaunchKernelGGL((vq::k_verify_part<T, 16, 4>), all, wg, 0, ctx->stream, a);
+                hipLaunchKernelGGL((vq::k_verify_part<T, 16>), all, wg, 0, ctx->stream, a);
                 if (drafts) {
                     hipLaunchKernelGGL((vq::k_verify_left<T, false>), some, wg, 0, ctx->stream, a);
                     hipLaunchKernelGGL((vq::k_verify_pick<T, true>), each, wg, 0, ctx->stream, a);
