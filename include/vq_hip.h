@@ -489,8 +489,8 @@ int32_t vq_code_logprobs_grad(vq_ctx *ctx, int32_t type, const void *d_scores, i
  * counterpart in the reference.  All are asynchronous and run on the context's stream; strides are in elements; any stride and any address
  * that is a multiple of the element's size will do; what lies between rows or behind the last one is left as it is.  vq_code_embed_grad,
  * vq_code_verify and, for rows above 16,384 codes, vq_code_distill use a buffer of the context, which grows with each of their sizes and is
- * kept until the context is destroyed: such a call may be captured into a graph where the same call, or one that is smaller in no size,
- * has run before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the capture goes on).  Graphs
+ * kept until the context is destroyed: such a call may be captured into a graph where the same call, or one of the same types that is smaller in
+ * no size, has run before on the context (else VQ_ERR_UNSUPPORTED where the buffer would have to grow, and the capture goes on).  Graphs
  * captured from one context share that buffer and are to run on its stream, one after another. */
 
 /* d_out[i] = scale * sum_s d_table[s * k + d_codes[i * code_stride + s]], n rows of dim from the m stages' tables of k rows each (m = 1: a
@@ -503,7 +503,7 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
 
 /* The gradient of the tables from that of the rows, d_g (n rows of dim):
  *   d_grad[s * k + j] = scale * (sum of d_g[i] over the positions i whose code of stage s is j)
- * or that added to what d_grad holds (accumulate = 1).  Sums are held in f32, in an order that depends on the codes alone: the same call gives
+ * or that added to what d_grad holds (accumulate = 1).  Sums are held in f32, in an order that codes and sizes decide: the same call gives
  * the same bits.  All m * k rows are written, codes without a position with zeros, except that with accumulate rows without a position
  * are not touched; n = 0 writes zeros, too.  A code that is negative, or k or above, takes no part.  n * m <= 2^30.
  * d_grad may not overlap an input. */
@@ -550,7 +550,7 @@ int32_t vq_code_distill_grad(vq_ctx *ctx, int32_t type, const void *d_scores, in
  * Drafted code c of position d stays where the ones before it do and d_uniform[d] * q_c < p_c.  Of the first that does not stay the position
  * gets a code drawn from max(p - q, 0) (from p, should nothing be left of that); where all stay the position behind the last gets one from p: the
  * first code at which the sum of the weights up to it is above d_uniform[draft] times the sum of all (the last code with a weight, should
- * there be none).  Exponentials and sums are held in f64.
+ * there be none).  Exponentials and sums are held in f64; a weight below 2^-1000 of the row's largest probability counts as none.
  *   d_accepted[b]                  how many drafted codes stay
  *   d_out[b * ld_out + 0..draft]   these, the next code, -1 behind it
  * A position whose row, or whose draft's row, has no score above -inf, a NaN or +inf, or whose drafted code is k or above, is answered

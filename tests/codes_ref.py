@@ -28,9 +28,9 @@ def embed(table, codes, scale):
 
 
 def depth(count):
-    """Additions behind one another on the way of a member of `count` to their sum: up to 32 in a row; a sixteenth of up to 1024 and sixteen
-    sums; beyond that as many again, and a sixteenth of the pieces of 1024 and sixteen."""
-    return np.minimum(count, 64 + 16 + count // 16384 + 18) + 1
+    """Additions behind one another on the way of a member of `count` to their sum: up to 1024 members in a row at the most; beyond that a
+    sixteenth of the 1024 of a piece and sixteen sums, then a sixteenth of the pieces and sixteen sums."""
+    return np.where(count <= 1024, count, 64 + 16 + count // 16384 + 18) + 1
 
 
 def embed_grad(g, codes, scale, k, old=None):

@@ -199,6 +199,50 @@ def test_a_smaller_call_after_a_larger_one():
         ctx.close()
 
 
+def test_fewer_rows_go_another_way():
+    """64 rows of 40,000 codes lie in registers, 63 go in parts; 512 sequences of many drafts go at once, 3 in three launches: the smaller calls are
+    captured after the larger ones alone."""
+    import vq_amd
+    rng = np.random.default_rng(11)
+    n, k, top = 64, 40000, 4
+    ctx = vq_amd.Context(0)
+    scores, grad, g = ctx.to_device(rng.standard_normal((n, k)).astype(np.float32)), ctx.empty((n, k), np.float32), ctx.to_device(rng.random(n).astype(np.float32))
+    lp, code = ctx.to_device(np.full((n, top), -1.5, np.float32)), ctx.to_device(rng.integers(0, k, (n, top)).astype(np.int32))
+    loss = ctx.empty(n, np.float32)
+
+    def call(rows):
+        ctx.code_distill("f32", scores, rows, k, k, 1.0, top, lp, code, top, True, loss, None, None, None, g, grad, k)
+    call(n)
+    ctx.sync()
+    graph = Captured(ctx, lambda: call(n - 1))
+    for _ in range(3):
+        graph.launch()
+        a = [loss.download()[:n - 1], grad.download()[:n - 1]]
+        call(n)
+        call(n - 1)
+        assert np.array_equal(a[0], loss.download()[:n - 1]) and np.array_equal(a[1], grad.download()[:n - 1])
+    graph.close()
+    ctx.close()
+    ctx = vq_amd.Context(0)
+    n, draft, k = 512, 20, 100
+    target, u = ctx.to_device(rng.standard_normal((n * (draft + 1), k)).astype(np.float32)), ctx.to_device(rng.random((n, draft + 1)).astype(np.float32))
+    codes, accepted, out = ctx.to_device(rng.integers(0, k, (n, draft)).astype(np.int32)), ctx.empty(n, np.int32), ctx.empty((n, draft + 1), np.int32)
+
+    def verify(count):
+        ctx.code_verify("f32", target, k, 1.0, None, k, 1.0, count, draft, k, 4, codes, draft, u, draft + 1, accepted, out, draft + 1)
+    verify(n)
+    ctx.sync()
+    want = out.download()
+    graph = Captured(ctx, lambda: verify(3))
+    for _ in range(3):
+        out.upload(np.zeros((n, draft + 1), np.int32))
+        graph.launch()
+        assert np.array_equal(out.download()[:3], want[:3]) and not out.download()[3:].any()
+        verify(n)
+    graph.close()
+    ctx.close()
+
+
 def test_two_contexts_side_by_side():
     """Calls of two contexts in turn, without waiting for one another: each has its own buffers and stream."""
     import vq_amd

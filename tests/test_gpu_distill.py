@@ -241,3 +241,25 @@ def test_gradient_against_differences(ctx, k):
             d = (Q.distill(x + e, 1.0, lp, code, rest)["loss"] - Q.distill(x - e, 1.0, lp, code, rest)["loss"]) / (2 * h)
             # the difference is off by h^2 / 6 of the third derivative, which is below 1, and by 1e-16 / h of the loss
             assert np.abs(d - y[:, j]).max() < 2e-9 + 1e-11 + 1e-6 * np.abs(d).max()
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+def test_most_codes(ctx, kind):
+    rng = np.random.default_rng(30)
+    x, lp, code = case(rng, 2, 1 << 20, 64, kind)
+    for rest, how in ((True, "same"), (False, "inplace")):
+        run(ctx, x, kind, 1.0, lp, code, rest, rng.standard_normal(2), how)
+
+
+def test_more_rows_than_a_launch_takes(ctx):
+    """Short rows, of which a launch takes 2^25."""
+    n, k = (1 << 25) + 5, 2
+    x = np.zeros((n, k), np.float32)
+    x[:, 1] = np.arange(n) % 7
+    lp, code = np.full((n, 1), -0.5, np.float32), np.ones((n, 1), np.int32)
+    loss = ctx.empty(n, np.float32)
+    ctx.code_distill("f32", ctx.to_device(x), n, k, k, 1.0, 1, ctx.to_device(lp), ctx.to_device(code), 1, False, loss, None, None, None)
+    want = Q.distill(x[:7].astype(np.float64), 1.0, lp[:7], code[:7], False)
+    got = loss.download()
+    for i in range(7):
+        assert (np.abs(got[i::7] - want["loss"][i]) <= want["tloss"][i]).all()

@@ -194,3 +194,14 @@ def test_enough_rows_for_four_parts_to_a_workgroup(ctx):
         u[9], u[10] = 0.0, 1.0
         run(ctx, t, d, codes, u, kind, 1.0, 1.0)
         run(ctx, t, None, codes, u, kind, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("scored", [True, False])
+def test_most_codes(ctx, scored):
+    """More than 64 parts of a row, up to as many as there may be."""
+    rng = np.random.default_rng(20)
+    for k, n in ((270_001, 3), (1 << 20, 2)):
+        t, d, codes, u = case(rng, n, 2, k, "bf16", 1.0, 1.0, scored, noise=0.3)
+        t[0, 0, :300_000] = -np.inf
+        t[0, 0, k - 1] = 2.0
+        run(ctx, t, d, codes, u, "bf16", 1.0, 1.0)

@@ -198,9 +198,9 @@ int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t
                         d_logrest, d_g_loss, d_grad, ld_grad, plan.parts, nullptr};
     float *stats = nullptr;
     const int64_t slice = vq::distill_rows_of_a_launch(plan);
+    VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::distill_work(n, k)));  // (also where fewer rows only would go in parts: they may follow in a capture)
     if (plan.waves == 0) {
         // the gradient of a row in parts is a call of its own, from the sums that the caller need not have asked for
-        VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::distill_work(n, k)));
         all.sums = (float *)ctx->code_work.p;
         stats = all.sums + std::min(slice, n) * plan.parts * 2;
     }
@@ -274,7 +274,7 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
     const int e = vq::type_bytes(type);
     const int64_t slice = vq::verify_sequences_of_a_launch(draft, k);
     const bool few = vq::verify_few(n, draft, k);
-    if (!few) VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
+    if (!vq::verify_few(1, draft, k)) VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::verify_work(n, draft, k)));
     const void *drafts = draft > 0 ? d_draft : nullptr;
     for (int64_t b = 0; b < n; b += slice) {
         const int64_t here = std::min(slice, n - b), rows = here * (draft + 1 + (drafts ? draft : 0));
