@@ -24,6 +24,7 @@ int back(int type, i64 s, i64 n, i64 ld, int k, float beta, int top, i64 lp, i64
 int verify(int type, i64 t, i64 ldt, float beta, i64 q, i64 ldq, float bq, i64 n, int d, int k, int cb, i64 c, i64 cs, i64 u, i64 ldu, i64 a, i64 o, i64 ldo) {
     return vq::check_code_verify(type, P(t), ldt, beta, P(q), ldq, bq, n, d, k, cb, P(c), cs, P(u), ldu, P(a), P(o), ldo).status; }
 i64 embed_bytes(i64 n, int k, int dim, int m) { return vq::embed_work(n, k, dim, m).bytes; }
+int few(i64 n, int k, int m, i64 across) { return vq::embed_few(n, k, m, across); }
 int lists(i64 n, int k, int m, i64 *out) { const vq::ListPlan p = vq::plan_lists(n, k, m); out[0] = p.width, out[1] = p.buckets, out[2] = p.share, out[3] = p.shares;
     const vq::EmbedWork w = vq::embed_work(n, k, 100, m); out[4] = w.below - w.counts, out[5] = w.partial - w.below, out[6] = w.counts - w.edges;
     out[7] = vq::list_lds(p.width, true); return 0; }
@@ -184,3 +185,19 @@ def test_a_missing_context_is_an_error():
     assert lib.vq_code_distill(None, 0, None, 0, 1, 1, 1.0, 1, None, None, 1, 0, None, None, None, None, None, None, 1) == INVALID
     assert lib.vq_code_distill_grad(None, 0, None, 0, 1, 1, 1.0, 1, None, None, 1, 0, None, None, None, None, None, 1) == INVALID
     assert lib.vq_code_verify(None, 0, None, 1, 1.0, None, 1, 1.0, 0, 0, 1, 4, None, 1, None, 1, None, None, 1) == INVALID
+
+
+def test_lists_of_their_own_stay_so_for_smaller_calls(lib):
+    """A call without a buffer is followed by none, smaller in every size, that needs one."""
+    lib.few.argtypes = [C.c_longlong, C.c_int, C.c_int, C.c_longlong]
+    for k in SIZES:
+        for m in (1, 2, 8, 64):
+            for across in (1, 2, 5, 40):
+                for n in (0, 1, 1000, 1024):
+                    codes = lib.few(n, k, m, across)
+                    assert codes in (0, 4, 16, 64)
+                    if codes:
+                        assert -(-k // codes) * m * across <= 1024
+                        assert all(lib.few(a, b, c, d) for a, b, c, d in ((n // 2, k, m, across), (n, max(1, k - 1), m, across), (n, k // 2 + 1, m, across), (n, k, max(1, m - 1), across),
+                                                                          (n, k, m, max(1, across - 1))))
+                assert not lib.few(1025, k, m, across)

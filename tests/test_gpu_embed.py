@@ -64,7 +64,7 @@ def near(got, want, tol):
 
 SHAPES = [  # n, m, k, dim
     (1, 1, 1, 1), (1, 1, 16, 5), (3, 1, 300, 8), (7, 2, 5, 9), (16, 1, 1000, 1280), (65, 4, 33, 100), (257, 8, 256, 24), (1000, 1, 70000, 17), (33, 3, 64, 2049),
-    (5, 64, 20, 40), (4099, 5, 777, 130), (2, 1, 40, 5000),
+    (5, 64, 20, 40), (4099, 5, 777, 130), (2, 1, 40, 5000), (759, 2, 12388, 75), (1024, 1, 20000, 33), (900, 1, 30011, 3),
 ]
 
 

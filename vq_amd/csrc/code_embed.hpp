@@ -398,9 +398,12 @@ template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs 
     }
     __syncthreads();
     const bool past = ((uintptr_t)a.grad & 15) == 0 && a.ld_grad % VO == 0 && a.dim % VO == 0;  // whole pieces of 16 aligned bytes
-    for (int i = wave; i < *count; i += 4) {
+    // 1 << shift lanes of a row, so that rows of a few bytes lie side by side in a wave
+    int shift = 0;
+    while (shift < 6 && VO << shift < end - column) ++shift;
+    for (int i = tid >> shift; i < *count; i += 256 >> shift) {
         Out *to = (Out *)a.grad + ((int64_t)stage * a.k + list[i]) * a.ld_grad;
-        for (int c = column + lane * VO; c < end; c += 64 * VO) {
+        for (int c = column + (tid & ((1 << shift) - 1)) * VO; c < end; c += VO << shift) {
             if (past) {
                 typedef uint32_t Four __attribute__((ext_vector_type(4)));
                 __builtin_nontemporal_store(Four{0, 0, 0, 0}, reinterpret_cast<Four *>(to + c));

@@ -199,11 +199,14 @@ inline ListPlan plan_lists(int64_t n, int32_t k, int32_t m) {
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 1024 / ((int64_t)buckets * m))), share = std::max<int64_t>(4096, (n + most - 1) / most);
     return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
 }
-// Up to so many positions the workgroups that sum make their lists themselves, where no more than 512 of them read all codes (333 x 100 f32, 1001
-// codes: 9.8 us in two launches, 7.4 so).
-constexpr int kFewPositions = 1024;
-constexpr int kFewCodes = 16;  // codes of such a workgroup
-inline bool embed_few(int64_t n, int32_t k, int32_t m, int64_t across) { return n <= kFewPositions && (k + kFewCodes - 1) / kFewCodes * m * across <= 512; }
+// Up to so many positions the workgroups that sum make their lists themselves, for 4 codes each, or 16 or 64 where that would be more workgroups than
+// 512 to read all codes, 1024 at most (333 x 100 f32, 1001 codes: 9.8 us in two launches, 7.4 so; 759 x 2 stages of 175 f16, 12,388 codes 24
+// and 9).  0: the lists come first.
+constexpr int kFewPositions = 1024, kFewCodes = 64;
+inline int embed_few(int64_t n, int32_t k, int32_t m, int64_t across) {
+    const auto groups = [&](int codes) { return (k + codes - 1) / codes * (int64_t)m * across; };
+    return n > kFewPositions ? 0 : groups(4) <= 512 ? 4 : groups(16) <= 512 ? 16 : groups(kFewCodes) <= 1024 ? kFewCodes : 0;
+}
 // A code of more positions than this is summed in pieces of as many positions of the list, whose sums are joined afterwards.
 constexpr int kLongCode = 1024;
 constexpr int64_t embed_edges(int64_t n) { return (n + kLongCode - 1) / kLongCode; }  // pieces of the list

@@ -122,9 +122,9 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
                                                 grad_type, d_grad, ld_grad), accumulate ? n : 1, &go));
     if (!go) return VQ_OK;
     const int wide = 16 / vq::type_bytes(type), columns = 16 * (dim < wide ? 1 : wide), across = cdiv(dim, columns);
-    if (vq::embed_few(n, k, m, across)) {
+    if (const int few = vq::embed_few(n, k, m, across)) {
         vq::SumArgs a{d_g, ld_g, (int)n, dim, k, scale, accumulate, d_grad, ld_grad, d_codes, code_bytes, code_stride, nullptr, nullptr, nullptr, nullptr,
-                      0, 0, vq::kFewCodes, (int)cdiv(k, vq::kFewCodes), across, 0};
+                      0, 0, few, (int)cdiv(k, few), across, 0};
         by_types(type, grad_type, [&](auto t, auto o) {
             embed_sums<decltype(t), decltype(o), true>(ctx, a, a.groups * across, m);
         });
