@@ -237,12 +237,22 @@ __device__ __forceinline__ Sums code_sums(const DistillArgs &a, Held<T, LANES, N
 #pragma unroll
         for (int v = 0; v < H::VEC; v += 2) m = larger(larger(x.at(u, v), x.at(u, v + 1)), m);
     }
-    Sums s(group_max<64>(m), a.beta * kLog2e, [&](auto add) {
+    // as the sums of a row in floats are made (Sums)
+    Sums s(group_max<64>(m), 0.0f, 0.0f);
+    const float c = a.beta * kLog2e, from = Sums::is_bad(s.m) || s.m == kNegInf ? 0.0f : s.m, M = from * c;
+    const bool far = fabsf(M) >= 1e6f;  // uniform
+    s.r = far ? 0.0f : __builtin_fmaf(from, c, -M);
+    if (!far) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
 #pragma unroll
-            for (int v = 0; v < H::VEC; ++v) add(x.at(u, v));
-    });
+            for (int v = 0; v < H::VEC; ++v) s.add(__builtin_fmaf(x.at(u, v), c, -M));
+    } else {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int v = 0; v < H::VEC; ++v) s.add((x.at(u, v) - from) * c);
+    }
     s.S = group_sum<64>(s.S);
     s.away();
     return s;

@@ -200,7 +200,7 @@ inline ListPlan plan_lists(int64_t n, int32_t k, int32_t m) {
     return {width, buckets, (int32_t)share, (int32_t)((n + share - 1) / share)};
 }
 // Up to so many positions the workgroups that sum make their lists themselves, for 4 codes each, or 16 or 64 where that would be more workgroups than
-// 512 to read all codes, 1024 at most (333 x 100 f32, 1001 codes: 9.8 us in two launches, 7.4 so; 759 x 2 stages of 175 f16, 12,388 codes 24
+// 512 to read all codes, 1024 at most (333 x 100 f32, 1001 codes: 9.8 us in two launches, 6.8 so; 759 x 2 stages of 175 f16, 12,388 codes 24
 // and 9).  0: the lists come first.
 constexpr int kFewPositions = 1024, kFewCodes = 64;
 inline int embed_few(int64_t n, int32_t k, int32_t m, int64_t across) {

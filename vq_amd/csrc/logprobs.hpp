@@ -155,22 +155,18 @@ template <int G> __device__ __forceinline__ int group_min(int v) {
 // them, and taken out of the joined sums (away).  Below |M| = 10^6 r is at most 1/32; from there on exponents are formed from x - m.
 struct Sums {
     float m, S = 0.0f, W = 0.0f, r = 0.0f;
-    template <int E> __device__ __forceinline__ Sums(const float (&x)[E], float most, float c)
-        : Sums(most, c, [&](auto add) {
-#pragma unroll
-              for (int e = 0; e < E; ++e) add(x[e]);
-          }) {}
-    // of the scores that each(add) hands to `add`
-    template <typename F> __device__ __forceinline__ Sums(float most, float c, F each) : m(most) {
+    template <int E> __device__ __forceinline__ Sums(const float (&x)[E], float most, float c) : m(most) {
         const float from = is_bad(m) || m == kNegInf ? 0.0f : m, M = from * c;  // (such rows' sums are not looked at)
         if (__ballot(fabsf(M) >= 1e6f) == 0) {
             r = __builtin_fmaf(from, c, -M);
-            each([&](float x) { add(__builtin_fmaf(x, c, -M)); });
+#pragma unroll
+            for (int e = 0; e < E; ++e) add(__builtin_fmaf(x[e], c, -M));
         } else {  // each row of the wave in its own way, so that its bits do not depend on what the others hold
             const bool far = fabsf(M) >= 1e6f;
             const float off = far ? from : 0.0f, by = far ? 0.0f : M;
             r = far ? 0.0f : __builtin_fmaf(from, c, -M);
-            each([&](float x) { add(__builtin_fmaf(x - off, c, -by)); });
+#pragma unroll
+            for (int e = 0; e < E; ++e) add(__builtin_fmaf(x[e] - off, c, -by));
         }
     }
     __device__ __forceinline__ Sums(float most, float sum, float weighted) : m(most), S(sum), W(weighted) {}
