@@ -263,3 +263,58 @@ def test_more_rows_than_a_launch_takes(ctx):
     got = loss.download()
     for i in range(7):
         assert (np.abs(got[i::7] - want["loss"][i]) <= want["tloss"][i]).all()
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("k", [300, 900, 3000, 6000, 20001, 65537])
+def test_alternatives_that_hold_next_to_nothing(ctx, k, kind):
+    """log R, next to zero, and what the other codes' gradients have in common, a difference of two small shares, to the number's own
+    accuracy: both come of the alternatives' own sum."""
+    rng = np.random.default_rng(k)
+    n, top, u = 70, 3, 2.0 ** -24
+    x = R.unpack(R.pack(rng.standard_normal((n, k)), kind), kind)
+    code = np.stack([rng.permutation(k)[:top] for _ in range(n)]).astype(np.int32)
+    rows = np.arange(n)[:, None]
+    x[rows, code] = R.unpack(R.pack(rng.uniform(-4, -2, (n, top)), kind), kind)
+    d = x - x.max(axis=1, keepdims=True)
+    e = np.exp(d)
+    S = e.sum(axis=1)
+    share = e[rows, code].sum(axis=1) / S
+    lp = np.log(e[rows, code] / S[:, None] * rng.uniform(2, 3, (n, top))).astype(np.float32)
+    g = (rng.random(n) + 0.5).astype(np.float32)
+    for how in ("same", "apart"):
+        got = run(ctx, x, kind, 1.0, lp, code, True, g, how)
+        lr, y = got[3][:n].astype(np.float64), R.unpack(got[4], kind)
+        want = np.log1p(-share)
+        # a term: the product's, the factor's and the difference's rounding times its exponent, and the power's; two sums, of three and (tL) of k
+        # terms, a reciprocal, a product; log1p makes at most 1.5 times as much of that and adds two steps
+        tL = Q.distill(x, 1.0, lp, code, True)["tL"]
+        rel = 1.5 * ((3 * np.abs(d[rows, code]).max(axis=1) + 12) * u + tL) + 4 * u
+        assert (np.abs(lr - want) <= rel * np.abs(want)).all()
+        q = np.exp(lp.astype(np.float64)).sum(axis=1)
+        factor = q - share  # Q R - r, where Q + r are one
+        wy = g.astype(np.float64)[:, None] * factor[:, None] * e / (S * (1 - share))[:, None]
+        # the factor: of a log R that is off by rel, a power less one, a product, a rounded Q, a sum; the share: as in distill_grad
+        L = np.log(S)[:, None]
+        ep = (6 * np.abs(d) + 4 * np.abs(d - L) + 8 * L + 24) * u + 2 * tL[:, None]
+        err = 1.01 * np.abs(wy) * (((rel + 8 * u) * share + 8 * u * q)[:, None] / np.abs(factor)[:, None] + ep) + 2.0 ** -126
+        other = np.ones((n, k), bool)
+        other[rows, code] = False
+        near(np.where(other, y, 0.0), np.where(other, wy, 0.0), Q.rounded(wy, err, kind))
+
+
+def test_a_loss_of_next_to_nothing(ctx):
+    """Alternatives of a few billionths, and the teacher's of as little: r log r and r log R are small, and so is what they leave."""
+    k, n = 4096, 8
+    x = np.zeros((n, k))
+    x[:, 5] = -np.arange(8, 16)
+    code = np.full((n, 1), 5, np.int32)
+    share = np.exp(x[:, 5]) / (k - 1 + np.exp(x[:, 5]))
+    lp = np.log(3 * share).astype(np.float32)[:, None]
+    got = run(ctx, x, "f32", 1.0, lp, code, True, how="loss")
+    q = np.exp(lp[:, 0].astype(np.float64))
+    parts = q * (lp[:, 0] - np.log(share)), (1 - q) * (np.log1p(-q) - np.log1p(-share))
+    # log p_c: a product and a difference (exact here), L's rounding, theirs; the rest's two logarithms are relative to their own size: log R's
+    # share has the exponent's two roundings (15 at most), a power's, a sum's, a reciprocal's and a product's
+    err = q * 2.0 ** -24 * (4 * np.abs(np.log(share)) + 32) + 2.0 ** -24 * (48 * share + 8 * q)
+    assert (np.abs(got[0][:n] - sum(parts)) <= err).all()

@@ -9,7 +9,8 @@
 //   beta (Q R - r) p_j / R        of another code
 // So the other codes' gradients are one exponential each, by a factor and an offset that the row's codes have in common; the
 // alternatives', at most 64 numbers, are written over what that makes of their codes.  Where R is asked for, the sums of the two kinds are
-// kept apart from the start: it is never 1 minus something.
+// kept apart from the start; where the alternatives' is the smaller, log R is log1p of what they hold, and Q R - r is Q + (Q + r)(R - 1):
+// neither is a small difference of large numbers.
 #pragma once
 #include "code_rows.hpp"
 #include "code_rules.hpp"
@@ -123,7 +124,8 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs &a, int64_t row, c
     o.off = L * kLog2e;
     o.C = bg * total;
     if (open) {
-        o.C = bg * __builtin_fmaf(total, __builtin_amdgcn_exp2f(log_rest * kLog2e), -r);
+        o.C = bg * (log_rest > -0.5f ? __builtin_fmaf(total, expm1f(log_rest), (float)t.Q)
+                                     : __builtin_fmaf(total, __builtin_amdgcn_exp2f(log_rest * kLog2e), -r));
         o.off = fmaxf((L + log_rest) * kLog2e, -3e38f);
         if (mr != kNegInf) o.from = mr, o.off = __builtin_amdgcn_logf(Sr);
     }
@@ -142,19 +144,21 @@ __device__ __forceinline__ RowLoss row_loss(const DistillArgs &a, const Teacher 
     const float m = larger(group_max<64>(mine), mr);
     const float from = Sums::is_bad(m) || m == kNegInf ? 0.0f : m;
     const float e = __builtin_amdgcn_exp2f(larger_or_nan((mine - from) * c, -200.0f));
-    const float S = __builtin_fmaf(Sr, __builtin_amdgcn_exp2f(fmaxf((mr - from) * c, -200.0f)), group_sum<64>(e));
+    const float A = group_sum<64>(e), S = __builtin_fmaf(Sr, __builtin_amdgcn_exp2f(fmaxf((mr - from) * c, -200.0f)), A);
     const RowSums sums = row_sums(Sums(m, S, 0.0f));
     RowLoss o{sums.m, sums.L, kNegInf, 0.0f};
     const bool bad = sums.L != sums.L;
     if (bad)
         o.log_rest = sums.L;
+    else if (a.split && mr != kNegInf && A <= 0.5f * S)
+        o.log_rest = log1pf(-A * __builtin_amdgcn_rcpf(S));
     else if (a.split && mr != kNegInf)
         o.log_rest = fminf(2.0f * a.beta * __builtin_fmaf(0.5f, mr, -0.5f * m) + (__builtin_amdgcn_logf(Sr) * kLn2 - sums.L), 0.0f);
     const float log_p = sums.m == kNegInf ? kNegInf : log_probability(a.beta, score, sums);
     float loss = group_sum<64>(t.q > 0.0f ? t.q * (t.log_q - log_p) : 0.0f);
     if (a.rest && o.log_rest != kNegInf) {
         const float r = (float)fmax(0.0, 1.0 - t.Q);
-        if (r > 0.0f) loss += r * (__builtin_amdgcn_logf(r) * kLn2 - o.log_rest);
+        if (r > 0.0f) loss += r * ((t.Q < 0.5 ? log1pf(-(float)t.Q) : __builtin_amdgcn_logf(r) * kLn2) - o.log_rest);
     }
     o.loss = !t.some ? 0.0f : t.bad || bad ? __builtin_nanf("") : loss;
     return o;
