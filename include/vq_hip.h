@@ -521,7 +521,8 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
  *   d_logrest         log R; -inf where no other code can be
  * An entry with a negative code, or with the log probability -inf, is no alternative; one whose probability is below 2^-149 counts as zero in
  * the loss.  Of entries with the same code each counts.  A row without any alternative: loss and gradient 0, whatever its scores.  An alternative of
- * k or above, or a log probability that is NaN or +inf: loss and gradient NaN.  Rows of -inf only, with a NaN or with +inf:
+ * k or above, or a log probability that is NaN or +inf: loss and gradient NaN.  A log probability above 0 is taken as it is; where its probability is
+ * beyond f32 (rest = 1, from 88.8 on) the loss and the entry's gradient are infinite or NaN.  Rows of -inf only, with a NaN or with +inf:
  * m and L as vq_code_logprobs has them, log R -inf or NaN, the loss +inf (against a teacher with alternatives) or NaN.
  * d_g_loss and d_grad, together or not at all: the gradient by the scores in the same call,
  *   d_grad[i][j] = d_g_loss[i] * beta * (Q p_j - q_j), or, for rest = 1 and codes that are no alternative, d_g_loss[i] * beta * (Q R - r) p_j / R

@@ -26,9 +26,9 @@ __device__ __forceinline__ double exp2_of(double y, double c) {
     bits.y += __builtin_bit_cast(Halves, t).x << 20;
     return __builtin_bit_cast(double, bits);
 }
-// 2^d for d below 1000, 0 below -1000; no NaN.
+// 2^d, from d = 1000 on 2^1000 (more than binary32 holds: from 1024 on the whole part would run over into the sign), 0 below -1000; no NaN.
 __device__ __forceinline__ double exp2_wide(double d) {
-    const double e = exp2_of(fmax(d, -1000.0), 1.0);
+    const double e = exp2_of(fmin(fmax(d, -1000.0), 1000.0), 1.0);
     return d < -1000.0 ? 0.0 : e;
 }
 
