@@ -518,7 +518,7 @@ int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n
  *   rest = 1   q_t = the probabilities as they are; what they leave, r = max(0, 1 - sum_t q_t), is one more class beside them, against
  *              R, the probability of all codes that are no alternative (no such term where no other code can be: its scores are all -inf)
  *   d_max, d_logsum   m and L as vq_code_logprobs writes them
- *   d_logrest         log R; -inf where no other code can be
+ *   d_logrest         log R; -inf where no other code can be, and only there: the lowest f32 stands for what lies below it
  * An entry with a negative code, or with the log probability -inf, is no alternative; one whose probability is below 2^-149 counts as zero in
  * the loss.  Of entries with the same code each counts.  A row without any alternative: loss and gradient 0, whatever its scores.  An alternative of
  * k or above, or a log probability that is NaN or +inf: loss and gradient NaN.  A log probability above 0 is taken as it is; where its probability is

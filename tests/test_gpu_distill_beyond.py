@@ -57,3 +57,80 @@ def test_log_probabilities_above_zero(ctx, k, n, own_call):
     loss, *_ = run(ctx, x, "f32", 1.0, lp, code, True, g, own_call)
     want = Q.distill(x, 1.0, lp, code, True)
     assert (np.abs(loss - want["loss"]) <= want["tloss"]).all()
+
+
+def masked_rows(rng, n, k, kind, far):
+    """Rows whose codes all have the score `far`, but for two of them, the teacher's alternatives, with 0.5 and 0.3."""
+    x = np.full((n, k), far)
+    code = np.stack([rng.permutation(k)[:2] for _ in range(n)]).astype(np.int32)
+    x[np.arange(n)[:, None], code] = R.unpack(R.pack(rng.uniform(-2, 2, (n, 2)), kind), kind)
+    lp = np.log(np.tile(np.array([[0.5, 0.3]]), (n, 1))).astype(np.float32)
+    return x, lp, code
+
+
+def formulas(x, beta, lp, code, g):
+    """(loss, log R, gradient) of rows with a rest that has far less than the alternatives: R is nothing beside them, shares of it are not."""
+    n, k = x.shape
+    rows = np.arange(n)[:, None]
+    named = np.zeros((n, k), bool)
+    named[rows, code] = True
+    q = np.exp(lp.astype(np.float64))
+    r = 1.0 - q.sum(axis=1)
+    z = beta * x[rows, code]
+    top = z.max(axis=1, keepdims=True)
+    logp = z - top - np.log(np.exp(z - top).sum(axis=1, keepdims=True))
+    L = np.log(np.exp(z - top).sum(axis=1))
+    other = np.where(named, -np.inf, beta * (x - x[rows, code].max(axis=1, keepdims=True)))
+    most = other.max(axis=1, keepdims=True)
+    e = np.exp(other - most)
+    logr = most[:, 0] + np.log(e.sum(axis=1)) - L
+    loss = (q * (lp - logp)).sum(axis=1) + r * (np.log(r) - logr)
+    y = -r[:, None] * e / e.sum(axis=1, keepdims=True)
+    y[rows, code] = np.exp(logp) - q
+    return loss, logr, y * (beta * g.astype(np.float64))[:, None]
+
+
+FAR = [("f32", 2.0, LOW["f32"]), ("f32", 1e6, LOW["f32"]), ("bf16", 1.5, LOW["bf16"]), ("bf16", 2.5, LOW["bf16"]), ("f32", 1e30, -1e9)]
+
+
+@pytest.mark.parametrize("kind,beta,far", FAR)
+@pytest.mark.parametrize("k,n", WAYS)
+def test_a_rest_below_binary32(ctx, k, n, kind, beta, far):
+    """All codes but the alternatives masked by the type's lowest value: log R is beyond binary32, and still they can be, so that the loss has the rest's
+    term and the gradient its class."""
+    rng = np.random.default_rng(k)
+    x, lp, code = masked_rows(rng, n, k, kind, far)
+    if beta == 1e30:  # (differences that beta leaves in the range)
+        x[np.arange(n), code[:, 0]], x[np.arange(n), code[:, 1]] = 0.0, -1e-30
+    beta = float(np.float32(beta))
+    g = (rng.random(n) / beta).astype(np.float32)
+    if beta == float(np.float32(1e6)):
+        x[np.arange(n)[:, None], code] /= 1e6
+        x = R.unpack(R.pack(x, kind), kind)
+    loss, m, L, lr, y = run(ctx, x, kind, beta, lp, code, True, g, False)
+    want, logr, wy = formulas(x, beta, lp, code, g)
+    assert (logr < LOW["f32"]).all() and (lr == LOW["f32"]).all()
+    # the rest's term is nearly all of the loss: r from two exponentials in f64, rounded once; the product and the sum, once each
+    fits = want < 3.4e38
+    assert np.isinf(loss[~fits]).all() and (loss[~fits] > 0).all()
+    assert (np.abs(loss - want)[fits] <= 8 * U * want[fits]).all()
+    rows = np.arange(n)[:, None]
+    # p: an exponent of at most 4 rounded four times, two steps of the power, four sums and products; q: rounded once
+    tol = beta * g.astype(np.float64)[:, None] * (64 * U)
+    near = np.abs(y - wy)[rows, code]
+    assert (near <= tol + 1.01 * R.HALF_STEP[kind] * np.abs(wy[rows, code]) + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("k,n", WAYS)
+def test_an_alternative_below_binary32(ctx, k, n, rest):
+    """An alternative whose score is masked by the lowest value: its log probability is beyond binary32, its share of the loss is not."""
+    rng = np.random.default_rng(k)
+    x = R.unpack(R.pack(rng.standard_normal((n, k)), "f32"), "f32")
+    code = np.stack([rng.permutation(k)[:2] for _ in range(n)]).astype(np.int32)
+    x[np.arange(n), code[:, 1]] = LOW["f32"]
+    lp = np.log(np.tile(np.array([[0.9, 0.1]]), (n, 1))).astype(np.float32)
+    loss, *_ = run(ctx, x, "f32", 4.0, lp, code, rest, np.ones(n, np.float32), False)
+    # q of 0.1: the exponential rounded once, over a sum (a reciprocal, a product), and its product
+    want = np.exp(lp[:, 1].astype(np.float64)) / (1.0 if rest else np.exp(lp.astype(np.float64)).sum(axis=1)) * 4.0 * -LOW["f32"]
+    assert (np.abs(loss - want) <= 8 * U * want).all()

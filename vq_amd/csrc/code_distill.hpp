@@ -135,11 +135,13 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs &a, int64_t row, c
 }
 
 // The sums of a row: from the largest score mr and the sum Sr of its codes, or (split) of those that are no alternative, and the scores at
-// the alternatives' codes.
+// the alternatives' codes.  Log R is -inf where no other code can be, and nowhere else: what lies below f32's lowest number is written as that.  A
+// term of the loss whose log probability lies there is formed in 64 bits, since the teacher's probability may bring it back.
 struct RowLoss {
     float m, L, log_rest, loss;
 };
 __device__ __forceinline__ RowLoss row_loss(const DistillArgs &a, const Teacher &t, float mr, float Sr, float score) {
+    constexpr float LOWEST = -3.402823466e38f;
     const float c = a.beta * kLog2e, mine = a.split && t.first ? score : kNegInf;
     const float m = larger(group_max<64>(mine), mr);
     const float from = Sums::is_bad(m) || m == kNegInf ? 0.0f : m;
@@ -147,18 +149,27 @@ __device__ __forceinline__ RowLoss row_loss(const DistillArgs &a, const Teacher 
     const float A = group_sum<64>(e), S = __builtin_fmaf(Sr, __builtin_amdgcn_exp2f(fmaxf((mr - from) * c, -200.0f)), A);
     const RowSums sums = row_sums(Sums(m, S, 0.0f));
     RowLoss o{sums.m, sums.L, kNegInf, 0.0f};
-    const bool bad = sums.L != sums.L;
+    const bool bad = sums.L != sums.L, others = a.split && mr != kNegInf;
+    const auto beyond = [&](float s, float rest) { return (double)a.beta * ((double)s - (double)m) + (double)rest; };  // a log probability in 64 bits
     if (bad)
         o.log_rest = sums.L;
-    else if (a.split && mr != kNegInf && A <= 0.5f * S)
+    else if (others && A <= 0.5f * S)
         o.log_rest = log1pf(-A * __builtin_amdgcn_rcpf(S));
-    else if (a.split && mr != kNegInf)
-        o.log_rest = fminf(2.0f * a.beta * __builtin_fmaf(0.5f, mr, -0.5f * m) + (__builtin_amdgcn_logf(Sr) * kLn2 - sums.L), 0.0f);
+    else if (others)
+        o.log_rest = fmaxf(fminf(2.0f * a.beta * __builtin_fmaf(0.5f, mr, -0.5f * m) + (__builtin_amdgcn_logf(Sr) * kLn2 - sums.L), 0.0f), LOWEST);
     const float log_p = sums.m == kNegInf ? kNegInf : log_probability(a.beta, score, sums);
-    float loss = group_sum<64>(t.q > 0.0f ? t.q * (t.log_q - log_p) : 0.0f);
+    float term = t.q > 0.0f ? t.q * (t.log_q - log_p) : 0.0f;
+    if (t.q > 0.0f && log_p == kNegInf && score > kNegInf) term = (float)((double)t.q * ((double)t.log_q - beyond(score, -sums.L)));
+    float loss = group_sum<64>(term);
     if (a.rest && o.log_rest != kNegInf) {
         const float r = (float)fmax(0.0, 1.0 - t.Q);
-        if (r > 0.0f) loss += r * ((t.Q < 0.5 ? log1pf(-(float)t.Q) : __builtin_amdgcn_logf(r) * kLn2) - o.log_rest);
+        if (r > 0.0f) {
+            const float log_r = t.Q < 0.5 ? log1pf(-(float)t.Q) : __builtin_amdgcn_logf(r) * kLn2;
+            if (o.log_rest > LOWEST)
+                loss += r * (log_r - o.log_rest);
+            else
+                loss += (float)((double)r * ((double)log_r - beyond(mr, __builtin_amdgcn_logf(Sr) * kLn2 - sums.L)));
+        }
     }
     o.loss = !t.some ? 0.0f : t.bad || bad ? __builtin_nanf("") : loss;
     return o;
