@@ -534,8 +534,9 @@ int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t
                         const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest, float *d_loss,
                         float *d_max, float *d_logsum, float *d_logrest, const float *d_g_loss, void *d_grad, int64_t ld_grad);
 
-/* That gradient alone, from what vq_code_distill left: d_max, d_logsum and, for rest = 1, d_logrest (else it may be NULL).  d_grad may be
- * d_scores itself (same stride); another overlap is refused. */
+/* That gradient alone, from what vq_code_distill left: d_max, d_logsum and, for rest = 1, d_logrest (else it may be NULL).  Shares of the rest, p_j / R,
+ * are taken from log p_j - log R here, and so are off by some six times 2^-24 * |log R| of themselves; where log R is below -2^20 they count as
+ * zero.  (With d_grad vq_code_distill has them from the scores.)  d_grad may be d_scores itself (same stride); another overlap is refused. */
 int32_t vq_code_distill_grad(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t n, int64_t ld, int32_t k, float beta, int32_t top,
                              const float *d_teacher_logprob, const int32_t *d_teacher_code, int64_t ld_teacher, int32_t rest,
                              const float *d_max, const float *d_logsum, const float *d_logrest, const float *d_g_loss, void *d_grad,

@@ -134,3 +134,43 @@ def test_an_alternative_below_binary32(ctx, k, n, rest):
     # q of 0.1: the exponential rounded once, over a sum (a reciprocal, a product), and its product
     want = np.exp(lp[:, 1].astype(np.float64)) / (1.0 if rest else np.exp(lp.astype(np.float64)).sum(axis=1)) * 4.0 * -LOW["f32"]
     assert (np.abs(loss - want) <= 8 * U * want).all()
+
+
+@pytest.mark.parametrize("kind,beta,far", FAR + [("f32", 1.0, -1e8), ("f32", 1.0, -1e5), ("bf16", 1.0, -1e6), ("f16", 1.0, -60000.0), ("f32", 0.5, -300.0)])
+@pytest.mark.parametrize("k,n", WAYS)
+def test_shares_of_a_far_rest(ctx, k, n, kind, beta, far):
+    """The rest's codes share its gradient, however little they have, where the gradient comes with the loss, in whatever way a row goes; in a call of
+    its own to log R's accuracy, and below -2^20 not at all."""
+    rng = np.random.default_rng(k + 1)
+    x, lp, code = masked_rows(rng, n, k, kind, far)
+    rows = np.arange(n)[:, None]
+    if beta > 100:
+        x[rows, code] /= beta
+    else:  # codes among the masked ones that have more of the rest than the others
+        odd = rng.random((n, k)) < 0.3
+        odd[rows, code] = False
+        x[odd] = R.unpack(R.pack(np.array([far * 0.999999]), kind), kind) if far > -1e30 else far
+    x = R.unpack(R.pack(x, kind), kind)
+    beta = float(np.float32(beta))
+    g = (rng.random(n) / beta).astype(np.float32)
+    _, logr, wy = formulas(x, beta, lp, code, g)
+    named = np.zeros((n, k), bool)
+    named[rows, code] = True
+    bg = beta * g.astype(np.float64)[:, None]
+    # an exponent relative to the rest's largest score, of a difference and a factor rounded once each, and the logarithm of a sum of k terms (each a power
+    # of two roundings' exponent), itself to a step of at most 20; the factor r from f64
+    d = np.where(named, 0.0, beta * np.abs(x - np.where(named, -np.inf, x).max(axis=1, keepdims=True)))
+    rel = (6 * d.max(axis=1, keepdims=True) + 3 * np.log2(k) + 64 + 16) * U
+    for own_call in (False, True):
+        y = run(ctx, x, kind, beta, lp, code, True, g, own_call)[4]
+        if own_call and (logr < -2.0 ** 20).all():
+            assert (y[~named] == 0).all()
+            continue
+        more = rel + (8 * U * np.abs(logr)[:, None] if own_call else 0.0)
+        want = np.where(named, 0.0, wy)
+        tol = more * np.abs(want) + 1.01 * R.HALF_STEP[kind] * np.abs(want) * (1 + more) + R.LEAST[kind] + bg * 2.0 ** -126
+        assert (np.abs(np.where(named, 0.0, y) - want) <= tol).all(), (np.abs(np.where(named, 0.0, y) - want) / np.where(want == 0, 1, np.abs(want))).max()
+        if not own_call or (logr > -2.0 ** 20).all():
+            # the rest's codes have minus r in all
+            total = np.where(named, 0.0, y).sum(axis=1)
+            assert (np.abs(total - want.sum(axis=1)) <= tol.sum(axis=1)).all()

@@ -34,6 +34,7 @@ struct DistillArgs {
     int64_t ld_grad;
     int parts;
     float *sums;  // [row][part][2]: largest score of the codes that are no alternative, their sum
+    float *rest_max, *rest_sum;  // the same of a row, from its parts for its gradient
 };
 
 // A row's alternatives, one per lane of a wave.
@@ -104,10 +105,12 @@ struct RowGrad {
     }
 };
 // The gradient of a row, from m, L, the log of R and the scores at the alternatives' codes (a lane each): the common part, and value, a lane's
-// own.  The other codes' shares of the rest are relative to the rest's largest score mr and their sum Sr where the row is at hand (mr above
-// -inf), otherwise to m, L and log R.
+// own.  The other codes' shares of the rest are relative to the rest's largest score mr and their sum Sr where these are at hand (mr above
+// -inf), otherwise to m, L and log R, whose rounding they then have: some six steps of 2^-24 of log R, so that from FAR on, where that is more than a
+// third, nothing is known of them and their probability counts as the zero that it nearly is.
 __device__ __forceinline__ RowGrad row_grad(const DistillArgs &a, int64_t row, const Teacher &t, float m, float L, float log_rest, float score,
-                                            float *value, float mr = kNegInf, float Sr = 0.0f) {
+                                            float *value, float mr, float Sr) {
+    constexpr float FAR = -1048576.0f;
     RowGrad o{0.0f, 0.0f, 0.0f, 0.0f};
     *value = 0.0f;
     const bool none = m == kNegInf;
@@ -127,7 +130,10 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs &a, int64_t row, c
         o.C = bg * (log_rest > -0.5f ? __builtin_fmaf(total, expm1f(log_rest), (float)t.Q)
                                      : __builtin_fmaf(total, __builtin_amdgcn_exp2f(log_rest * kLog2e), -r));
         o.off = fmaxf((L + log_rest) * kLog2e, -3e38f);
-        if (mr != kNegInf) o.from = mr, o.off = __builtin_amdgcn_logf(Sr);
+        if (mr != kNegInf)
+            o.from = mr, o.off = __builtin_amdgcn_logf(Sr);
+        else if (log_rest < FAR)
+            o.C = 0.0f;
     }
     const float p = __builtin_amdgcn_exp2f(fmaxf(__builtin_fmaf(score - m, c, -L * kLog2e), -200.0f));
     *value = bg * __builtin_fmaf(total, p, -t.q_code);
@@ -384,9 +390,10 @@ __global__ void __launch_bounds__(256) k_distill_join(DistillArgs a) {
     join_rest(a, pm, pS, lane < a.parts, &mr, &Sr);
     const RowLoss o = row_loss(a, t, mr, Sr, score);
     if (lane == 0) write_loss(a, row, o);
+    if (lane == 0 && a.rest_max) a.rest_max[row] = mr, a.rest_sum[row] = Sr;
 }
 
-// The gradient alone, from m, L and log R as the loss's call left them: a row, or (blockIdx.y) a piece of one, per WAVES waves.  Bound by memory:
+// The gradient alone, from m, L and log R as the loss's call left them (in that call of rows in parts also from the rest's own sums): a row, or (blockIdx.y) a piece of one, per WAVES waves.  Bound by memory:
 // 2048 rows of 65,536 f32 199 us = 5.4 TB/s with reads and whole lines that pass the caches (210 without).
 template <typename T, int WAVES, int NV>
 __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
@@ -409,7 +416,8 @@ __global__ void __launch_bounds__(256) k_distill_grad(DistillArgs a) {
     if (leads) {
         t.read(a, row, lane, slots_of[WAVES == 1 ? wave : 0]);
         const float score = t.has && t.code >= lo && t.code < hi ? T::up(s[t.code]) : kNegInf;
-        grad = row_grad(a, row, t, a.max[row], a.logsum[row], a.rest ? a.logrest[row] : kNegInf, score, &value);
+        grad = row_grad(a, row, t, a.max[row], a.logsum[row], a.rest ? a.logrest[row] : kNegInf, score, &value, a.rest_max ? a.rest_max[row] : kNegInf,
+                        a.rest_max ? a.rest_sum[row] : 0.0f);
         if constexpr (WAVES > 1)
             if (lane == 0) common = grad;
     }

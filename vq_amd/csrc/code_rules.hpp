@@ -246,15 +246,15 @@ inline DistillPlan plan_distill(int64_t n, int32_t k, bool grad) {
     return {0, e, (k + 256 * e - 1) / (256 * e)};
 }
 // Rows of a launch (a grid has fewer than 2^32 lanes) and bytes of the parts' results, which lie beside one another for a launch's rows.
-// (and, behind them, three numbers per row for the gradient)
-constexpr int kDistillPartBytes = 8;
+// (and, behind them, five numbers per row for the gradient)
+constexpr int kDistillPartBytes = 8, kDistillRowBytes = 20;
 inline int64_t distill_rows_of_a_launch(const DistillPlan &p) {
     return p.waves == 1 ? (int64_t)1 << 25 : p.waves ? ((int64_t)1 << 24) / (p.waves * 2) : std::max<int64_t>(1, (kPartBytes / kDistillPartBytes) / p.parts);
 }
 inline int64_t distill_work(int64_t n, int32_t k) {
     if (k <= 16384) return 0;
-    const int64_t most = (k + 8191) / 8192;  // (no plan cuts a row into more)
-    return std::min<int64_t>(2 * kPartBytes, std::min(n, kPartBytes) * (most * kDistillPartBytes + 12));
+    const int64_t most = (k + 8191) / 8192;  // (no plan cuts a row into more, and none into fewer than two: a launch's rows have at most 2.25 kPartBytes)
+    return std::min<int64_t>(3 * kPartBytes, std::min(n, kPartBytes) * (most * kDistillPartBytes + kDistillRowBytes));
 }
 
 // ---- drafts --------------------------------------------------------------------------------------------

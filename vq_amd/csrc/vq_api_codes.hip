@@ -41,6 +41,7 @@ vq::DistillArgs distill_slice(const vq::DistillArgs &a, int64_t r, int64_t rows,
     s.lp = a.lp + r * a.ld_teacher;
     s.code = a.code + r * a.ld_teacher;
     s.loss = at(a.loss), s.max = at(a.max), s.logsum = at(a.logsum), s.logrest = at(a.logrest);
+    s.rest_max = at(a.rest_max), s.rest_sum = at(a.rest_sum);
     s.g = a.g ? a.g + r : nullptr;
     s.grad = a.grad ? (char *)a.grad + r * a.ld_grad * e : nullptr;
     return s;
@@ -195,7 +196,7 @@ int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t
     if (!go) return VQ_OK;
     const vq::DistillPlan plan = vq::plan_distill(n, k, d_grad != nullptr);
     vq::DistillArgs all{d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, rest || d_logrest, d_loss, d_max, d_logsum,
-                        d_logrest, d_g_loss, d_grad, ld_grad, plan.parts, nullptr};
+                        d_logrest, d_g_loss, d_grad, ld_grad, plan.parts, nullptr, nullptr, nullptr};
     float *stats = nullptr;
     const int64_t slice = vq::distill_rows_of_a_launch(plan);
     VQ_TRY(ensure_kept(ctx, ctx->code_work, (size_t)vq::distill_work(n, k)));  // (also where fewer rows only would go in parts: they may follow in a capture)
@@ -210,6 +211,7 @@ int32_t vq_code_distill(vq_ctx *ctx, int32_t type, const void *d_scores, int64_t
             if (!a.max) a.max = stats;
             if (!a.logsum) a.logsum = stats + std::min(slice, n);
             if (!a.logrest && rest) a.logrest = stats + 2 * std::min(slice, n);
+            if (rest) a.rest_max = stats + 3 * std::min(slice, n), a.rest_sum = stats + 4 * std::min(slice, n);
         }
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
@@ -256,7 +258,7 @@ int32_t vq_code_distill_grad(vq_ctx *ctx, int32_t type, const void *d_scores, in
                                                   rest, d_max, d_logsum, d_logrest, d_g_loss, d_grad, ld_grad), n, &go));
     if (!go) return VQ_OK;
     const vq::DistillArgs a{d_scores, n, ld, k, beta, top, d_teacher_logprob, d_teacher_code, ld_teacher, rest, rest, nullptr, const_cast<float *>(d_max),
-                            const_cast<float *>(d_logsum), const_cast<float *>(d_logrest), d_g_loss, d_grad, ld_grad, 1, nullptr};
+                            const_cast<float *>(d_logsum), const_cast<float *>(d_logrest), d_g_loss, d_grad, ld_grad, 1, nullptr, nullptr, nullptr};
     return distill_grad(ctx, type, a);
 }
 
