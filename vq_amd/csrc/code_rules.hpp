@@ -265,7 +265,7 @@ inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyP
 // Rows of up to 2048 codes: a workgroup per sequence does everything, unless a few sequences have many rows each.
 inline bool verify_few(int64_t n, int32_t draft, int32_t k) { return k <= 2048 && (draft <= 16 || n >= 512); }
 inline bool verify_wide(int64_t rows, int32_t k) { return k > kVerifyPart && rows * ((k + 4 * kVerifyPart - 1) / (4 * kVerifyPart)) >= 2048; }
-// Per row and part a sum and a maximum (in 64 bits and 32; 16 bytes); per sequence and part a sum more, and 64 bytes for what its drafts come to.
+// Per row and part a sum in 64 bits and two maxima in 32; per sequence and part a sum more, and 64 bytes for what its drafts come to.
 inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8) + 64; }
 static_assert(kMaxRowCodes / kVerifyPart * ((2 * kMaxDraft + 1) * 16 + 8) + 64 <= kPartBytes * 4, "one sequence fits");
 inline int64_t verify_sequences_of_a_launch(int32_t draft, int32_t k) {

@@ -29,6 +29,7 @@ struct VerifyArgs {
     // targets, then of the drafts.  Without scores of the drafts a drafted code is left out of its row.
     float *most;
     double *sum;
+    float *own;    // the largest score of the part alone, where `most` is that of the parts that a workgroup summed with it
     double *left;  // per sequence and part: the sum of max(p - q, 0)
     struct Verdict *verdicts;  // per sequence, where those sums are made
     int64_t first_draft() const { return (int64_t)n * (draft + 1); }
@@ -119,6 +120,7 @@ __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     const bool none = sound && !((double)own - from >= least);
     const int64_t at = (int64_t)row * a.parts + first + tid;
     a.most[at] = none ? kNegInf : m;
+    a.own[at] = own;
     double sum = sum_of[0][tid];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) sum += sum_of[w][tid];
@@ -414,8 +416,9 @@ __global__ void __launch_bounds__(256) k_verify_pick(VerifyArgs a) {
             if (tid < a.parts && w.minus) {
                 mine = a.left[seq * a.parts + tid];
             } else if (tid < a.parts) {
-                const float m = a.most[row * a.parts + tid];
-                mine = m > kNegInf ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
+                // a part has a weight where its largest score has one, by the same rule: its sum times a power may be a number where no code's weight is
+                const float m = a.most[row * a.parts + tid], own = a.own[row * a.parts + tid];
+                mine = m > kNegInf && (double)own - o.mp >= w.least_p ? a.sum[row * a.parts + tid] * exp2_wide(((double)m - o.mp) * a.c_target) : 0.0;
             }
             upto = chooser.scan(mine, 0.0, &total);
             if (total > 0.0 || !w.minus) break;

@@ -284,11 +284,11 @@ int32_t vq_code_verify(vq_ctx *ctx, int32_t type, const void *d_target, int64_t 
         const int parts = vq::verify_parts(k);
         double *sum = (double *)ctx->code_work.p, *left = sum + rows * parts;
         vq::Verdict *verdicts = (vq::Verdict *)(left + here * parts);
-        float *most = (float *)(verdicts + here);
+        float *most = (float *)(verdicts + here), *own = most + rows * parts;
         const vq::VerifyArgs a{(const char *)d_target + b * (draft + 1) * ld_target * e, drafts ? (const char *)drafts + b * draft * ld_draft * e : nullptr,
                                ld_target, ld_draft, beta * vq::kLog2e64, beta_draft * vq::kLog2e64, (int)here, draft, k, parts,
                                draft ? (const char *)d_codes + b * code_stride * code_bytes : nullptr, code_bytes, code_stride,
-                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, left, verdicts};
+                               d_uniform + b * ld_uniform, ld_uniform, d_accepted + b, d_out + b * ld_out, ld_out, most, sum, own, left, verdicts};
         by_type(type, [&](auto t) {
             typedef decltype(t) T;
             const dim3 all((unsigned)(rows * (wide ? cdiv(parts, 4) : parts))), some((unsigned)(here * parts)), each((unsigned)here), wg(256);
