@@ -344,27 +344,35 @@ constexpr int kGroupCodes = 128;  // codes of a workgroup at most
 // lanes sums 32 rows.)
 constexpr int kOwnMembers = 32, kFewMembers = 10;
 
-// Adds V columns of the members number a, a + step, ... below b of a list, in that order.
+// Adds V columns of the members number a, a + step, ... below b of a list, in that order, by blocks of 32 whose sums are added: a rounding for each of
+// 1024 members behind one another would lose ten of the 24 bits.
 template <typename T, int V, typename Rows>
 __device__ __forceinline__ void sum_members(const SumArgs &s, Rows rows, int a, int b, int step, int at, float (&sum)[V]) {
     typedef typename T::Raw Raw;
     typedef Values<T, V> In;
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 8, BLOCK = 32;
     const Raw *g = (const Raw *)s.g + at;
-    for (int p = a; p < b; p += AHEAD * step) {
-        // (behind the last member the last one again, which is not added: loads under a condition would wait for one another)
-        int row[AHEAD];
-        typename In::Piece x[AHEAD];
+    for (int p = a; p < b;) {
+        float block[V];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
+        for (int v = 0; v < V; ++v) block[v] = 0.0f;
+        for (const int end = min(b, p + BLOCK * step); p < end; p += AHEAD * step) {
+            // (behind the last member the last one again, which is not added: loads under a condition would wait for one another)
+            int row[AHEAD];
+            typename In::Piece x[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld);
+            for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (p + j * step < b) {
+            for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld);
 #pragma unroll
-                for (int v = 0; v < V; ++v) sum[v] += x[j].at(v);
-            }
+            for (int j = 0; j < AHEAD; ++j)
+                if (p + j * step < b) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) block[v] += x[j].at(v);
+                }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] += block[v];
     }
 }
 
@@ -646,11 +654,11 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
 }
 
 // The sums of the chunks of a code of more than kLongCode members, by the workgroup of the chunk in which the code's list begins:
-// 64 columns (blockIdx.y), 16 groups of 16 lanes that share the chunks.
+// 64 columns (blockIdx.y), 16 groups of 16 lanes that share the chunks, a million of them where all positions have one code: summed in 64 bits.
 template <typename O>
 __global__ void __launch_bounds__(256) k_embed_join(SumArgs a) {
     typedef typename O::Raw Out;
-    __shared__ float red[16][64];
+    __shared__ double red[16][64];
     const int tid = threadIdx.x, sub = tid >> 4, column = blockIdx.y * 64, at = column + (tid & 15) * 4, stage = blockIdx.z, chunk = blockIdx.x;
     const int32_t *start = a.start + (int64_t)stage * (a.k + 1), *edges = a.edges + (int64_t)stage * embed_edges(a.n);
     const int all = start[a.k], first = chunk * kLongCode, last = first + kLongCode - 1;
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(256) k_embed_join(SumArgs a) {
     if (s1 - s0 <= kLongCode || s0 < first || s0 > last) return;
     const int end = (s1 - 1) / kLongCode;  // the last chunk with members of this code
     const float *partial = a.partial + (int64_t)stage * a.chunks * 2 * a.padded;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
     if (at < a.dim) {
         for (int c = chunk + sub; c <= end; c += 16) {
             const int slot = c == chunk && s0 != first ? 1 : 0;
@@ -671,9 +679,10 @@ __global__ void __launch_bounds__(256) k_embed_join(SumArgs a) {
     for (int v = 0; v < 4; ++v) red[sub][(tid & 15) * 4 + v] = sum[v];
     __syncthreads();
     if (tid >= 64 || column + tid >= a.dim) return;
-    float total = 0.0f;
+    double all_of = 0.0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) total += red[j][tid];
+    for (int j = 0; j < 16; ++j) all_of += red[j][tid];
+    const float total = (float)all_of;
     Out *to = (Out *)a.grad + ((int64_t)stage * a.k + code) * a.ld_grad + column + tid;
     *to = O::down(a.accumulate ? __builtin_fmaf(a.scale, total, O::up(*to)) : a.scale * total);
 }
