@@ -6,9 +6,10 @@ import scores_ref as R
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
-# Additions behind one another on the way of a member to the sum of its code: 32 and a 32nd of the members for a group of lanes (1024 members at
-# most) or for each of sixteen that share 1024, sixteen of these; then, in 64 bits, the pieces.
-DEPTH = 2 + 32 + 32 + 16 + 2
+# Additions behind one another on the way of a member to the sum of its code: for a group of lanes, which has 512 members at most, the first two, 64
+# eights, three within an eight, seven that are no eight.  Sixteen groups that share 1024 have fewer: eight eights each, and sixteen sums; then, in
+# 64 bits, the pieces.
+DEPTH = 2 + 64 + 3 + 7
 
 
 @pytest.fixture(scope="module")

@@ -341,38 +341,40 @@ struct SumArgs {
 
 constexpr int kGroupCodes = 128;  // codes of a workgroup at most
 // A code of more positions than this is summed by the whole workgroup.  (Where a workgroup has few codes it sums one alone sooner than a group of
-// lanes sums 32 rows.)
-constexpr int kOwnMembers = 32, kFewMembers = 10;
+// lanes sums 32 rows.)  16,384 x 1280 bf16 of 65,536 uneven codes 96 us, with 16 instead of 32 members 115; 100,000 x 128 of 1024 uneven codes 35, with 64 78;
+// 1000 x 100 of 50 codes in one launch 12.9, with 5 instead of 10 15.6, with 20 12.8.
+// kOwnMost: no group of lanes sums more, however many such codes a workgroup has, so that no sum is of more than 76 roundings behind one another
+// (uncapped 1024 and more; the cap and eights: 100,000 x 64 bf16 of 1000 uneven codes 32.4 -> 28.6 us).
+constexpr int kOwnMembers = 32, kFewMembers = 10, kOwnMost = 512;
 
-// Adds V columns of the members number a, a + step, ... below b of a list, in that order, by blocks of 32 whose sums are added: a rounding for each of
-// 1024 members behind one another would lose ten of the 24 bits.
+// Adds V columns of the members number a, a + step, ... below b of a list, in that order, eight at a time whose sum is added: a rounding for each of
+// 512 members behind one another would lose nine of the 24 bits.
 template <typename T, int V, typename Rows>
 __device__ __forceinline__ void sum_members(const SumArgs &s, Rows rows, int a, int b, int step, int at, float (&sum)[V]) {
     typedef typename T::Raw Raw;
     typedef Values<T, V> In;
-    constexpr int AHEAD = 8, BLOCK = 32;
+    constexpr int AHEAD = 8;
     const Raw *g = (const Raw *)s.g + at;
-    for (int p = a; p < b;) {
-        float block[V];
+    for (int p = a; p < b; p += AHEAD * step) {
+        // (behind the last member the last one again, which is not added: loads under a condition would wait for one another)
+        int row[AHEAD];
+        typename In::Piece x[AHEAD];
 #pragma unroll
-        for (int v = 0; v < V; ++v) block[v] = 0.0f;
-        for (const int end = min(b, p + BLOCK * step); p < end; p += AHEAD * step) {
-            // (behind the last member the last one again, which is not added: loads under a condition would wait for one another)
-            int row[AHEAD];
-            typename In::Piece x[AHEAD];
+        for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) row[j] = rows[min(p + j * step, b - 1)];
+        for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld);
+        if (p + (AHEAD - 1) * step < b) {
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) x[j] = In::fetch(g + (int64_t)row[j] * s.ld);
+            for (int v = 0; v < V; ++v)
+                sum[v] += ((x[0].at(v) + x[1].at(v)) + (x[2].at(v) + x[3].at(v))) + ((x[4].at(v) + x[5].at(v)) + (x[6].at(v) + x[7].at(v)));
+        } else {
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j)
+            for (int j = 0; j < AHEAD - 1; ++j)
                 if (p + j * step < b) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) block[v] += x[j].at(v);
+                    for (int v = 0; v < V; ++v) sum[v] += x[j].at(v);
                 }
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += block[v];
     }
 }
 
@@ -426,8 +428,9 @@ template <typename O> __device__ __forceinline__ void write_zeros(const SumArgs 
 // chunks of the list that belong to codes of more than kLongCode members; a.across workgroups side by side have the columns,
 // 16 * V each; the last ones write the rows without members.  blockIdx.z: stages.
 // FEW: up to kFewPositions of them, which every workgroup lists for its own codes: one launch instead of two.
+// Five waves to a SIMD, which 96 registers allow; sums of 16-bit rows to f32, which would spill, four (FEW spills three registers for them).
 template <typename T, typename O, int V, bool FEW>
-__global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
+__global__ void __launch_bounds__(256, FEW || sizeof(typename T::Raw) == 4 || sizeof(typename O::Raw) == 2 ? 5 : 4) k_embed_sums(SumArgs a) {
     typedef typename T::Raw Raw;
     typedef typename O::Raw Out;
     constexpr int COLUMNS = 16 * V, VO = V == 1 ? 1 : wide<O>();
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(256) k_embed_sums(SumArgs a) {
     __syncthreads();
     if (has) {
         // (16 codes side by side take the time of the longest, each by all lanes that of their sum: the more there are, the longer they may be)
-        const int own = (FEW ? kFewMembers : kOwnMembers) * max(1, count[3]);
+        const int own = min(kOwnMost, (FEW ? kFewMembers : kOwnMembers) * max(1, count[3]));
         begin[tid] = s0;
         behind[tid] = s1;
         if (members <= kLongCode) {
