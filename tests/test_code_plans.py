@@ -13,6 +13,8 @@ typedef long long i64;
 extern "C" {
 int plan(i64 n, int k, int grad, i64 *out) { const vq::DistillPlan p = vq::plan_distill(n, k, grad); out[0] = p.waves, out[1] = p.parts;
     out[2] = vq::distill_rows_of_a_launch(p); return 0; }
+int lists(i64 n, int k, int m, i64 *out) { const vq::ListPlan p = vq::plan_lists(n, k, m); out[0] = p.buckets, out[1] = p.shares,
+    out[2] = vq::list_lds(p.width, true), out[3] = vq::list_lds(p.width, false), out[4] = vq::kListBeside; return 0; }
 i64 distill_bytes(i64 n, int k) { return vq::distill_work(n, k); }
 }
 """
@@ -41,3 +43,17 @@ def test_rows_in_parts_have_their_sums_and_five_numbers(lib):
                 if waves == 0:
                     assert parts >= 2 and rows <= 1 << 22
                     assert lib.distill_bytes(n, k) >= min(n, rows) * (parts * 8 + 20)
+
+
+def test_two_workgroups_that_list_positions_fit_a_compute_unit(lib):
+    """By all of their LDS, the 160 KB of a compute unit: what a launch asks for and what the kernel has beside.  Shares are cut where that makes at
+    most 1024 workgroups."""
+    lib.lists.argtypes = [C.c_longlong, C.c_int, C.c_int, C.c_void_p]
+    out = (C.c_longlong * 5)()
+    for n in (0, 1, 1024, 32768, 32769, 100_000, 1_000_000, 1 << 24):
+        for k in (1, 2, 255, 256, 257, 480, 481, 8379, 65536, 262_144, 1 << 20):
+            for m in (1, 4, 8, 64):
+                lib.lists(n, k, m, out)
+                buckets, shares, lds, count_lds, beside = out
+                assert lds + beside <= 80 * 1024 and count_lds + beside <= 80 * 1024
+                assert shares == 1 or buckets * m * shares <= 1024

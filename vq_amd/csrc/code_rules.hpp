@@ -173,19 +173,24 @@ inline Refusal check_code_verify(int32_t type, const void *target, int64_t ld_ta
 inline int embed_slices(int64_t n, int32_t k, int32_t m, int vectors) { return n >= 2 * (int64_t)k && vectors >= 64 && (int64_t)k * m * vectors * 16 > 2 << 20 ? 8 : 1; }
 
 // Pieces of 16 bytes of a row that a lane has: two where the additions of several stages count more than the number of waves (65,536 x 8 stages
-// of 1024 bf16 62 us with one, 59 with two).
+// of 1024 bf16 54 us with one, 49 with two; 4 stages 38 and 33; 16,384 x 8 stages 14.9 and 14.5).
 inline int embed_pieces(int64_t n, int32_t m, int pieces) { return m >= 4 && pieces >= 16 && n * pieces >= 1 << 18 ? 2 : 1; }
 
 // ---- sums by code ------------------------------------------------------------------------------------
 // The positions of each stage in the order of their codes, and where each code's positions begin: k + 1 numbers.  Workgroups of 16 waves
 // list a bucket of codes each, of a share of the positions.  One share, and one launch, up to 32,768 positions; more positions in shares, in two
-// launches, so that there are about 1024 workgroups, two to a compute unit by their 60 KB of LDS (363,313 x 4 codes of 8379: 3204 workgroups, one to a
-// compute unit, 31 + 174 us, so 19 + 50).
+// launches, of at most 1024 workgroups, two to a compute unit by their 62 KB of LDS and 8 beside (363,313 x 4 codes of 8379: 3204 workgroups, one to a
+// compute unit, 31 + 174 us, so 19 + 50).  Where the buckets of all stages are more than 512 already there is one share again, and a workgroup per bucket.
+// The line, of whole gradients of 32 columns: 256 codes, 16,000 positions 11.5 us in one share, 18.8 in several; 48,000 16.9 and 20.4; 130,000 29.6 and
+// 24.6.  It is low for many codes: 65,536 codes, 32,000 20 and 48; 130,000 37 and 69.
+// Every bucket's workgroup reads all codes of its share, n * m * k / 480 of them in all: next to nothing for 256 codes or for the 65,536 of a batch, but 1M
+// positions of 262,144 codes take 0.27 ms for the list alone, of 2^20 codes 0.72, and 8 stages of 262,144 codes 7.6, where the sums take 0.05, 0.1 and 0.4.
 struct ListPlan {
     int32_t width, buckets;
     int32_t share, shares;
 };
 constexpr int kBucketMost = 480, kOneShareMost = 512;  // codes of a bucket
+constexpr int kListBeside = 2 * 16 * 4 + 2 * 1024 * 4; // LDS of a workgroup beside list_lds
 constexpr int kListQueue = 256;                        // positions of a bucket that a wave keeps
 // 16 waves' counts, and (to write the list) positions and codes of each wave.
 constexpr int list_lds(int width, bool place) { return (16 * width + 1) / 2 * 8 + (place ? 16 * kListQueue * 8 : 0); }
@@ -237,6 +242,8 @@ struct DistillPlan {
     int waves, per_lane;
     int32_t parts;
 };
+// Where the gradient comes along 64 rows or more have sixteen waves each: 65,536 bf16, 256 rows 16.8 us, 29.3 in parts; 64 rows 12.0 and 16.2.  The line is
+// high: 48 rows 11.8 and 15.5, 16 rows 11.3 and 14.0, 8 rows 11.1 and 11.4; of 20,000 codes 8 rows 7.2 and 11.2.
 inline DistillPlan plan_distill(int64_t n, int32_t k, bool grad) {
     if (k <= 4096) return {1, k <= 512 ? 8 : k <= 1024 ? 16 : k <= 2048 ? 32 : 64, 1};
     if (k <= 16384) return {4, k <= 8192 ? 32 : 64, 1};
@@ -264,6 +271,8 @@ constexpr int kVerifyPart = 4096;
 inline int32_t verify_parts(int32_t k) { return (k + kVerifyPart - 1) / kVerifyPart; }
 // Rows of up to 2048 codes: a workgroup per sequence does everything, unless a few sequences have many rows each.
 inline bool verify_few(int64_t n, int32_t draft, int32_t k) { return k <= 2048 && (draft <= 16 || n >= 512); }
+// Four parts to a workgroup, 11 rows a sequence: 65,536 bf16, 32 sequences 36.1 us and 33.8 a part each; 64 52.6 and 53.9; 256 160 and 174.  Of 4097 to
+// 8192 codes half of such a workgroup's lanes have none: 256 sequences 49 and 34.
 inline bool verify_wide(int64_t rows, int32_t k) { return k > kVerifyPart && rows * ((k + 4 * kVerifyPart - 1) / (4 * kVerifyPart)) >= 2048; }
 // Per row and part a sum in 64 bits and two maxima in 32; per sequence and part a sum more, and 64 bytes for what its drafts come to.
 inline int64_t verify_bytes_of_a_sequence(int32_t draft, int32_t k) { return (int64_t)verify_parts(k) * ((2 * draft + 1) * 16 + 8) + 64; }

@@ -32,7 +32,6 @@ struct VerifyArgs {
     float *own;    // the largest score of the part alone, where `most` is that of the parts that a workgroup summed with it
     double *left;  // per sequence and part: the sum of max(p - q, 0)
     struct Verdict *verdicts;  // per sequence, where those sums are made
-    int64_t first_draft() const { return (int64_t)n * (draft + 1); }
 };
 
 // The drafted codes of a sequence: lane d has code d; returns how many there are before the first that is none.
@@ -41,9 +40,9 @@ __device__ __forceinline__ int drafted(const VerifyArgs &a, int64_t seq, int lan
     return __ffsll(__ballot(*code < 0)) - 1;  // (lane 63 has none)
 }
 
-// EACH / 16 parts of a row per workgroup, their sums relative to the largest score of all of them.  Bound by the vector pipe: 18 instructions per code,
-// 13 of them in 64 bits, and some 180 per wave, which is why a lane has 64 codes where there are enough workgroups (128 sequences of 11
-// rows of 65,536 bf16: 16 codes per lane 77 us, 64 70).
+// EACH / 16 parts of a row per workgroup, their sums relative to the largest score of all of them.  Bound by the vector pipe: 15 instructions in 64 bits
+// per code (conversion, difference, limit, three for the whole part and the rest, eight of the polynomial, the sum), which go at 580 x 10^9 a second and wave,
+// and some six others with those of a wave, at 1000.  128 sequences of 11 rows of 65,536 bf16: 21.6M and 9.4M, 37 + 9 of 61 us.
 template <typename T, int EACH>
 __global__ void __launch_bounds__(256) k_verify_part(VerifyArgs a) {
     typedef typename T::Raw Raw;
