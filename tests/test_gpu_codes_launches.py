@@ -70,3 +70,29 @@ def test_columns_of_a_gradient_in_two_launches(ctx):
             near(got.astype(np.float64), want, Q.rounded(want, 5 * 2.0 ** -24 * (np.abs(old) + np.abs(rows).sum(axis=0)), "f16"))
     finally:
         grad.free()
+
+
+def test_a_graph_of_rows_in_parts_with_their_gradient(ctx):
+    """Loss and gradient of fewer than 64 long rows, whose sums go from launch to launch through the context's buffer: captured, replayed between eager
+    calls of other sizes, every replay against the eager result."""
+    from test_gpu_scores_workspace import Captured
+    rng = np.random.default_rng(7)
+    n, k, top = 9, 40_003, 6
+    x = rng.standard_normal((n, k)).astype(np.float32)
+    lp, code = np.log(np.full((n, top), 0.15, np.float32)), np.stack([rng.permutation(k)[:top] for _ in range(n)]).astype(np.int32)
+    dx, dl, dc, dg = (ctx.to_device(a) for a in (x, lp, code, rng.random(n).astype(np.float32)))
+    out, grad = [ctx.empty(n, np.float32) for _ in range(4)], ctx.empty((n, k), np.float32)
+    call = lambda rows=n: ctx.code_distill("f32", dx, rows, k, k, 1.0, top, dl, dc, top, True, *out, dg, grad, k)
+    call()
+    ctx.sync()
+    graph = Captured(ctx, call)
+    for rep in range(4):
+        dx.upload(rng.standard_normal((n, k)).astype(np.float32) * (rep + 1))
+        grad.upload(np.zeros((n, k), np.float32))
+        graph.launch()
+        got = [a.download() for a in (*out, grad)]
+        call(3 + rep)
+        call()
+        ctx.sync()
+        for a, b in zip(got, (*out, grad)):
+            assert np.array_equal(a, b.download())
