@@ -506,7 +506,7 @@ int32_t vq_code_embed(vq_ctx *ctx, int32_t type, const void *d_table, int32_t k,
  * or that added to what d_grad holds (accumulate = 1).  Sums are held in f32, in an order that codes and sizes decide: the same call gives
  * the same bits.  All m * k rows are written, codes without a position with zeros, except that with accumulate rows without a position
  * are not touched; n = 0 writes zeros, too.  A code that is negative, or k or above, takes no part.  n * m <= 2^30.
- * d_grad may not overlap an input. */
+ * d_grad may not overlap an input.  Listing the positions reads n * m * k / 480 codes, which counts for tables of more than some 65,536 codes. */
 int32_t vq_code_embed_grad(vq_ctx *ctx, int32_t type, const void *d_g, int64_t n, int64_t ld_g, int32_t dim, int32_t m,
                            int32_t code_bytes, const void *d_codes, int64_t code_stride, float scale, int32_t k, int32_t accumulate,
                            int32_t grad_type, void *d_grad, int64_t ld_grad);
